@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define TQ_ABI_VERSION 12 /* what tq_abi_version() returns */
+#define TQ_ABI_VERSION 13 /* what tq_abi_version() returns */
 
 typedef struct ihipStream_t* tq_stream_t; /* == hipStream_t */
 
@@ -182,6 +182,90 @@ int tq_decode_partials_balanced(const void* q, int64_t q_stride_b, int64_t q_str
  */
 int tq_decode_balanced_rows(int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
                             int32_t padded_dim);
+
+/*
+ * Cache budget: attention that records what each cached entry receives, and
+ * eviction by that record (tq_track.hip, tq_evict.hip; no counterpart in the
+ * reference, whose cache only grows).  State beside the cache, owned by the
+ * caller and reached through the same page tables:
+ *   weights   fp32  [num_blocks, num_kv_heads, block_size]: attention weight
+ *             that the entry received, summed over the q heads of its kv head;
+ *             16-byte aligned
+ *   positions int32 [num_blocks, num_kv_heads, block_size]: the position in
+ *             its sequence that the entry came from
+ * num_indices is the length of `indices`; table entries at or behind it, and
+ * pages outside [0, num_blocks), count as empty: their tokens get no weight
+ * and are not written.  No two sequences of a call share a page (they would
+ * race for its weights and entries).  `ends` int32 [batch]: the number of
+ * tokens that each sequence has seen, evicted ones included.  batch <= 1024,
+ * num_kv_heads <= 4096, num_blocks * block_size < 2^31, the sum of seq_lens <
+ * 2^30.  A workspace serves one call at a time and holds nothing between calls.
+ */
+
+/*
+ * Decode attention of one new token per sequence whose K/V is in the cache
+ * already, as tq_decode_paged_balanced_rows (q and o rows of head_dim
+ * elements, any head_dim up to padded_dim; q strides in elements), which also
+ * adds each head's softmax weights to `weights`: of the newest entry (token
+ * seq_len - 1) the weight is set, not added to, and its position becomes
+ * ends - 1.  positions (and then ends) may be NULL.  o [batch, num_qo_heads,
+ * head_dim] contiguous; a sequence without tokens gets a row of zeros.
+ * The weights are fp32 sums of fp32 probabilities; equal inputs give equal bits.
+ */
+int64_t tq_decode_tracked_workspace_bytes(int32_t batch, int64_t num_indices,
+                                          int32_t num_qo_heads, int32_t num_kv_heads,
+                                          int32_t padded_dim, int32_t block_size);
+int tq_decode_paged_tracked(const void* q, int64_t q_stride_b, int64_t q_stride_h,
+                            int32_t q_dtype, const uint8_t* k_slab, const uint8_t* v_slab,
+                            const int32_t* indices, int64_t num_indices, const int32_t* indptr,
+                            const int32_t* seq_lens, int32_t batch, int32_t num_qo_heads,
+                            int32_t num_kv_heads, int32_t head_dim, int32_t padded_dim,
+                            int32_t block_size, int32_t ebs, int64_t num_blocks, float sm_scale,
+                            const float* signs, void* o, int32_t o_dtype, float* weights,
+                            int32_t* positions, const int32_t* ends, void* workspace,
+                            int64_t workspace_bytes, tq_stream_t stream);
+
+/*
+ * The same record from a prompt: rows query_start_loc[b] ..
+ * query_start_loc[b + 1] - 1 of q are the chunk of sequence b whose K/V make up
+ * its last cached tokens; the last min(window, chunk) of them are observed,
+ * each over the tokens up to its own.  Tokens cached before the chunk are
+ * added to, the chunk's own are set and get their positions (ends - seq_len +
+ * index); a sequence with an empty chunk keeps its weights.  q has num_rows
+ * rows; observed rows outside them count as missing.  window *
+ * num_qo_heads / num_kv_heads <= 1024.
+ */
+int64_t tq_track_window_workspace_bytes(int32_t batch, int32_t window, int32_t num_qo_heads,
+                                        int32_t num_kv_heads, int32_t padded_dim);
+int tq_track_window(const void* q, int64_t num_rows, int64_t q_stride_tok, int64_t q_stride_h,
+                    int32_t q_dtype, const int32_t* query_start_loc, int32_t window, const uint8_t* k_slab,
+                    const int32_t* indices, int64_t num_indices, const int32_t* indptr,
+                    const int32_t* seq_lens, int32_t batch, int32_t num_qo_heads,
+                    int32_t num_kv_heads, int32_t head_dim, int32_t padded_dim,
+                    int32_t block_size, int32_t ebs, int64_t num_blocks, float sm_scale,
+                    const float* signs, float* weights, int32_t* positions, const int32_t* ends,
+                    void* workspace, int64_t workspace_bytes, tq_stream_t stream);
+
+/*
+ * Cuts every sequence with more than `budget` tokens down to it, each kv head
+ * by itself: kept are the entries at positions < sink or >= ends - recent,
+ * then those with the largest weights (NaN counts as the smallest; equal ones:
+ * the lowest index).  The i-th kept entry at an index >= budget moves, with its
+ * weight and position, to the i-th index < budget that is not kept; nothing
+ * else is written, entries behind the budget included.  new_lens[b] (may be
+ * seq_lens itself) = min(seq_lens[b], budget).  recent + sink <= budget;
+ * positions and ends may be NULL if both are 0.  Attention does not depend on
+ * the order of the entries, so decode goes on with the new lengths.
+ */
+int64_t tq_evict_workspace_bytes(int32_t batch, int32_t num_kv_heads, int64_t num_indices,
+                                 int32_t block_size, int32_t budget);
+int tq_evict_paged(uint8_t* k_slab, uint8_t* v_slab, float* weights, int32_t* positions,
+                   const int32_t* indices, int64_t num_indices, const int32_t* indptr,
+                   const int32_t* seq_lens, const int32_t* ends, int32_t batch,
+                   int32_t num_kv_heads, int32_t padded_dim, int32_t block_size, int32_t ebs,
+                   int64_t num_blocks, int32_t budget, int32_t recent, int32_t sink,
+                   int32_t* new_lens, void* workspace, int64_t workspace_bytes,
+                   tq_stream_t stream);
 
 /*
  * The first kernel of tq_decode_paged_splitkv alone (the reference's v5 split

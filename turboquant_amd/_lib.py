@@ -84,10 +84,21 @@ SIGNATURES = {
     "tq_e2e_qk_norm_rope": (_I32, [_P, _I64, _P, _P, _P, _P, _I64, _P, _I64, _I32, _I32, _I32,
                                    _F32, _P, _P, _P]),
     "tq_e2e_silu_mul": (_I32, [_P, _P, _I64, _I32, _P]),
+    "tq_decode_tracked_workspace_bytes": (_I64, [_I32, _I64, _I32, _I32, _I32, _I32]),
+    "tq_decode_paged_tracked": (_I32, [_P, _I64, _I64, _I32, _P, _P, _P, _I64, _P, _P, _I32, _I32,
+                                       _I32, _I32, _I32, _I32, _I32, _I64, _F32, _P, _P, _I32, _P,
+                                       _P, _P, _P, _I64, _P]),
+    "tq_track_window_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32]),
+    "tq_track_window": (_I32, [_P, _I64, _I64, _I64, _I32, _P, _I32, _P, _P, _I64, _P, _P, _I32, _I32,
+                               _I32, _I32, _I32, _I32, _I32, _I64, _F32, _P, _P, _P, _P, _P, _I64,
+                               _P]),
+    "tq_evict_workspace_bytes": (_I64, [_I32, _I32, _I64, _I32, _I32]),
+    "tq_evict_paged": (_I32, [_P, _P, _P, _P, _P, _I64, _P, _P, _P, _I32, _I32, _I32, _I32, _I32,
+                              _I64, _I32, _I32, _I32, _P, _P, _I64, _P]),
     "tq_last_error": (ctypes.c_char_p, []),
     "tq_abi_version": (_I32, []),
 }
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 _lib = None
 

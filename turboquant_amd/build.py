@@ -18,7 +18,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtq_hip.so")
 TORCH_LIB = os.path.join(HERE, "_tq_torch.so")
 SOURCES = ["tq_write.hip", "tq_decode.hip", "tq_dequant.hip", "tq_prefill.hip", "tq_mse.hip",
-           "tq_qjl.hip", "tq_e2e.hip"]
+           "tq_qjl.hip", "tq_e2e.hip", "tq_track.hip", "tq_evict.hip"]
 ARCH = os.environ.get("TQ_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [

@@ -857,6 +857,206 @@ def _prod_dequantize_qjl(packed, norms, qjl_signs, residual_norms, dim, padded_d
 
 
 # --------------------------------------------------------------------------
+# cache budget: attention that records what each entry receives, and eviction
+# --------------------------------------------------------------------------
+
+def _cache_geometry(kv_cache, num_kv_heads, what):
+    if kv_cache.dim() != 5 or kv_cache.size(0) != 2 or not kv_cache.is_contiguous():
+        raise RuntimeError(f"{what}: kv_cache must be contiguous [2, num_blocks, block_size, H, "
+                           "ebs]")
+    _, nb, bs, hk, _ = kv_cache.shape
+    if hk != num_kv_heads:
+        raise RuntimeError(f"{what}: kv_cache has {hk} kv heads, num_kv_heads={num_kv_heads}")
+    return nb, bs, kv_cache.size(-1) * kv_cache.element_size()
+
+
+def _int32(t, n, name, what):
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < n:
+        raise RuntimeError(f"{what}: {name} must be a contiguous int32 tensor of at least {n} "
+                           "entries")
+
+
+def _check_tables(batch, indices, indptr, seq_lens, what):
+    _int32(indices, 0, "indices", what)
+    _int32(indptr, batch, "indptr", what)
+    _int32(seq_lens, batch, "seq_lens", what)
+
+
+def _check_record(kv_cache, weights, positions, ends, batch, what):
+    """weights / positions [num_blocks, H, block_size] beside the cache."""
+    _, nb, bs, h, _ = kv_cache.shape
+    if weights.dtype != torch.float32 or tuple(weights.shape) != (nb, h, bs) \
+            or not weights.is_contiguous():
+        raise RuntimeError(f"{what}: weights must be contiguous fp32 [num_blocks, H, block_size]")
+    if positions is None:
+        return
+    if positions.dtype != torch.int32 or tuple(positions.shape) != (nb, h, bs) \
+            or not positions.is_contiguous():
+        raise RuntimeError(f"{what}: positions must be contiguous int32 [num_blocks, H, "
+                           "block_size]")
+    if ends is None:
+        raise RuntimeError(f"{what}: positions need ends")
+    _int32(ends, batch, "ends", what)
+
+
+def _check_q(q, head_dim, num_kv_heads, padded_dim, what):
+    if q.dtype not in (torch.float16, torch.bfloat16) or q.dim() != 3 or q.size(2) != head_dim \
+            or (q.stride(2) != 1 and q.size(2) > 1):
+        raise RuntimeError(f"{what}: q must be fp16 or bf16 [rows, Hq, head_dim] with a "
+                           "contiguous last dim")
+    if num_kv_heads <= 0 or q.size(1) % num_kv_heads:
+        raise RuntimeError(f"{what}: {q.size(1)} q heads over {num_kv_heads} kv heads")
+
+
+def _signs_ptr(signs, padded_dim, q, what):
+    """(the tensor to keep alive, its address or 0)"""
+    if signs is None or signs.numel() == 0:
+        return None, 0
+    if signs.dtype != torch.float32 or signs.numel() < padded_dim:
+        raise RuntimeError(f"{what}: signs must be fp32 [padded_dim]")
+    _require_gpu(q, signs)
+    signs = signs.contiguous()
+    return signs, signs.data_ptr()
+
+
+def _workspace(nbytes, device, what):
+    """A call's workspace from torch's allocator (graph-safe)."""
+    if nbytes < 0:
+        _lib.check(int(nbytes), what)
+    return torch.empty(max(1, int(nbytes)), dtype=torch.uint8, device=device)
+
+
+def _opt_ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def decode_paged_tracked(q: torch.Tensor, kv_cache: torch.Tensor, indices: torch.Tensor,
+                         indptr: torch.Tensor, seq_lens: torch.Tensor, num_kv_heads: int,
+                         head_dim: int, padded_dim: int, sm_scale: float,
+                         signs: torch.Tensor | None, o: torch.Tensor, weights: torch.Tensor,
+                         positions: torch.Tensor | None = None,
+                         ends: torch.Tensor | None = None) -> torch.Tensor:
+    """Decode attention that records what each cached entry receives: q [B, Hq,
+    head_dim] (fp16 or bf16), one new token per sequence whose K/V is in the
+    cache already, -> o [B, Hq, head_dim] (fp16 or bf16), and to weights fp32
+    [num_blocks, H, block_size] the softmax weights are added, summed over the
+    q heads of each kv head.  The newest entry's weight is set instead, and its
+    position (positions int32, of the same shape) becomes ends - 1; ends int32
+    [B] counts the tokens each sequence has seen, evicted ones included.
+    Sequences must not share pages.  tq_decode_paged_tracked; equal inputs give
+    equal bits."""
+    what = "decode_paged_tracked"
+    _require_gpu(q, kv_cache, indices, indptr, seq_lens, o, weights,
+                 *(t for t in (positions, ends) if t is not None))
+    _check_q(q, head_dim, num_kv_heads, padded_dim, what)
+    nb, bs, ebs = _cache_geometry(kv_cache, num_kv_heads, what)
+    b, hq, _ = q.shape
+    _check_tables(b, indices, indptr, seq_lens, what)
+    _check_record(kv_cache, weights, positions, ends, b, what)
+    if o.dtype not in (torch.float16, torch.bfloat16) or tuple(o.shape) != tuple(q.shape) \
+            or not o.is_contiguous():
+        raise RuntimeError(f"{what}: o must be contiguous fp16 or bf16 [B, Hq, head_dim]")
+    signs, sp = _signs_ptr(signs, padded_dim, q, what)
+    if b == 0:
+        return o
+    lib = _lib.load()
+    base = kv_cache.data_ptr()
+    with torch.cuda.device(q.device):
+        ws = _workspace(lib.tq_decode_tracked_workspace_bytes(
+            b, indices.numel(), hq, int(num_kv_heads), int(padded_dim), bs), q.device, what)
+        rc = lib.tq_decode_paged_tracked(
+            q.data_ptr(), q.stride(0), q.stride(1), _DTYPES[q.dtype], base,
+            base + kv_cache.stride(0) * kv_cache.element_size(), indices.data_ptr(),
+            indices.numel(), indptr.data_ptr(), seq_lens.data_ptr(), b, hq, int(num_kv_heads),
+            int(head_dim), int(padded_dim), bs, ebs, nb, float(sm_scale), sp, o.data_ptr(),
+            _DTYPES[o.dtype], weights.data_ptr(), _opt_ptr(positions), _opt_ptr(ends),
+            ws.data_ptr(), ws.numel(), _stream_ptr(q.device))
+    _lib.check(rc, what)
+    return o
+
+
+def track_window(q: torch.Tensor, query_start_loc: torch.Tensor, window: int,
+                 kv_cache: torch.Tensor, indices: torch.Tensor, indptr: torch.Tensor,
+                 seq_lens: torch.Tensor, num_kv_heads: int, head_dim: int, padded_dim: int,
+                 sm_scale: float, signs: torch.Tensor | None, weights: torch.Tensor,
+                 positions: torch.Tensor | None = None,
+                 ends: torch.Tensor | None = None) -> None:
+    """The record of decode_paged_tracked from a prompt: rows query_start_loc[b]
+    .. query_start_loc[b + 1] - 1 of q [T, Hq, head_dim] are a chunk of sequence
+    b whose K/V are its last cached tokens; the last min(window, chunk) of them
+    are observed, each over the tokens up to its own.  Weights of tokens cached
+    before the chunk are added to, the chunk's own are set, with their
+    positions.  window * Hq / H <= 1024.  tq_track_window."""
+    what = "track_window"
+    _require_gpu(q, query_start_loc, kv_cache, indices, indptr, seq_lens, weights,
+                 *(t for t in (positions, ends) if t is not None))
+    _check_q(q, head_dim, num_kv_heads, padded_dim, what)
+    nb, bs, ebs = _cache_geometry(kv_cache, num_kv_heads, what)
+    b, hq = query_start_loc.numel() - 1, q.size(1)
+    if b < 0:
+        raise RuntimeError(f"{what}: query_start_loc must hold batch + 1 entries")
+    _int32(query_start_loc, b + 1, "query_start_loc", what)
+    _check_tables(b, indices, indptr, seq_lens, what)
+    _check_record(kv_cache, weights, positions, ends, b, what)
+    signs, sp = _signs_ptr(signs, padded_dim, q, what)
+    if b == 0 or q.size(0) == 0:
+        return
+    lib = _lib.load()
+    with torch.cuda.device(q.device):
+        ws = _workspace(lib.tq_track_window_workspace_bytes(b, int(window), hq, int(num_kv_heads),
+                                                            int(padded_dim)), q.device, what)
+        rc = lib.tq_track_window(
+            q.data_ptr(), q.size(0), q.stride(0), q.stride(1), _DTYPES[q.dtype],
+            query_start_loc.data_ptr(), int(window), kv_cache.data_ptr(), indices.data_ptr(),
+            indices.numel(), indptr.data_ptr(), seq_lens.data_ptr(), b, hq, int(num_kv_heads),
+            int(head_dim), int(padded_dim), bs, ebs, nb, float(sm_scale), sp, weights.data_ptr(),
+            _opt_ptr(positions), _opt_ptr(ends), ws.data_ptr(), ws.numel(),
+            _stream_ptr(q.device))
+    _lib.check(rc, what)
+
+
+def evict_paged(kv_cache: torch.Tensor, weights: torch.Tensor, positions: torch.Tensor | None,
+                indices: torch.Tensor, indptr: torch.Tensor, seq_lens: torch.Tensor,
+                ends: torch.Tensor | None, budget: int, recent: int, sink: int,
+                new_lens: torch.Tensor) -> torch.Tensor:
+    """Cuts sequences of more than `budget` cached tokens down to it, each kv
+    head by itself: kept are the entries at positions < sink or >= ends -
+    recent, then those with the largest weights (equal ones: the lowest index;
+    NaN counts as the smallest).  Kept entries behind the budget move, with
+    weight and position, into the places in front of it that are not kept, in
+    order; nothing else is written.  new_lens int32 [B] (may be seq_lens) =
+    min(seq_lens, budget).  positions and ends may be None if recent = sink =
+    0.  Sequences must not share pages.  tq_evict_paged."""
+    what = "evict_paged"
+    _require_gpu(kv_cache, weights, indices, indptr, seq_lens, new_lens,
+                 *(t for t in (positions, ends) if t is not None))
+    b = seq_lens.numel()
+    nb, bs, ebs = _cache_geometry(kv_cache, kv_cache.size(3) if kv_cache.dim() == 5 else 0, what)
+    _check_tables(b, indices, indptr, seq_lens, what)
+    _check_record(kv_cache, weights, positions, ends, b, what)
+    _int32(new_lens, b, "new_lens", what)
+    pd = {48: 64, 80: 128, 144: 256}.get(ebs)
+    if pd is None:
+        raise RuntimeError(f"{what}: kv_cache entries of {ebs} bytes")
+    if b == 0:
+        return new_lens
+    hkv = kv_cache.size(3)
+    lib = _lib.load()
+    base = kv_cache.data_ptr()
+    with torch.cuda.device(kv_cache.device):
+        ws = _workspace(lib.tq_evict_workspace_bytes(b, hkv, indices.numel(), bs, int(budget)),
+                        kv_cache.device, what)
+        rc = lib.tq_evict_paged(
+            base, base + kv_cache.stride(0) * kv_cache.element_size(), weights.data_ptr(),
+            _opt_ptr(positions), indices.data_ptr(), indices.numel(), indptr.data_ptr(),
+            seq_lens.data_ptr(), _opt_ptr(ends), b, hkv, pd, bs, ebs, nb, int(budget),
+            int(recent), int(sink), new_lens.data_ptr(), ws.data_ptr(), ws.numel(),
+            _stream_ptr(kv_cache.device))
+    _lib.check(rc, what)
+    return new_lens
+
+
+# --------------------------------------------------------------------------
 # torch.library registration under the reference's namespaces and schemas
 # --------------------------------------------------------------------------
 _registered = False
@@ -1018,6 +1218,12 @@ def _register_fakes() -> None:
     for name in ("decode_paged_balanced_ws", "decode_paged_balanced_rows_ws"):
         register_fake(f"turboquant_v5::{name}", _balanced_fake, lib=_libs[1])
 
+    def _budget_fake(*args):  # they write their arguments and return nothing
+        return None
+
+    for name in ("decode_paged_tracked", "track_window", "evict_paged"):
+        register_fake(f"turboquant_v5::{name}", _budget_fake, lib=_libs[1])
+
 
 def register_ops() -> None:
     """Define turboquant_write::* and turboquant_v5::* with the reference
@@ -1069,6 +1275,27 @@ def register_ops() -> None:
                  "int padded_dim, float sm_scale, Tensor hadamard_signs, Tensor(a!) o_ws, "
                  "Tensor(b!) partition_o_ws, Tensor(c!) partition_lse_ws, "
                  "Tensor(d!) split_indptr) -> ()")
+    # the cache-budget operators: attention that records, and eviction (every
+    # tensor that a call writes is declared)
+    def nothing(fn):
+        def call(*args):
+            fn(*args)
+        return call
+    table = "Tensor indices, Tensor indptr, Tensor seq_lens"
+    geometry = "int num_kv_heads, int head_dim, int padded_dim, float sm_scale, " \
+               "Tensor? hadamard_signs"
+    d.define(f"decode_paged_tracked(Tensor q, Tensor kv_cache, {table}, {geometry}, "
+             "Tensor(a!) o, Tensor(b!) weights, Tensor(c!)? positions, Tensor? ends) -> ()")
+    d.impl("decode_paged_tracked", nothing(decode_paged_tracked), "CUDA")
+    d.define("track_window(Tensor q, Tensor query_start_loc, int window, Tensor kv_cache, "
+             f"{table}, {geometry}, Tensor(a!) weights, Tensor(b!)? positions, Tensor? ends) "
+             "-> ()")
+    d.impl("track_window", nothing(track_window), "CUDA")
+    # (new_lens may be seq_lens)
+    d.define("evict_paged(Tensor(a!) kv_cache, Tensor(b!) weights, Tensor(c!)? positions, "
+             "Tensor indices, Tensor indptr, Tensor seq_lens, Tensor? ends, int budget, "
+             "int recent, int sink, Tensor(d!) new_lens) -> ()")
+    d.impl("evict_paged", nothing(evict_paged), "CUDA")
     _native()  # binds the write and the two balanced ops
     _libs.extend([w, d])
     _register_fakes()
