@@ -1,5 +1,6 @@
 // tq_plan.h -- what the kernels that stream a paged cache share: lane
-// exchanges without LDS, the balanced split plan, occupancy facts.
+// exchanges without LDS, the balanced split plan, table addresses, the packed
+// scores of two tiles, occupancy facts.
 #pragma once
 
 #include <math.h>
@@ -179,8 +180,8 @@ struct PlanSlot {
 // sequence 64 i + lane (0 past the batch) and `starts` likewise for the
 // page-table starts; nreg = ceil(B / 64).  Every lane of a wave runs it and
 // every field of the result is wave-uniform.  writer: this wave also stores
-// the row table (rows = rowmul * units) and U.
-template <typename LensFn, typename StartsFn>
+// the row table (rows = rowmul * units) and U.  U is a multiple of A tokens.
+template <int A = kPlanAlign, typename LensFn, typename StartsFn>
 __device__ __forceinline__ PlanSlot plan_slot(LensFn lens, StartsFn starts, int B, int nreg,
                                               int units, int u, int rowmul, int32_t* split_out,
                                               bool writer) {
@@ -195,7 +196,6 @@ __device__ __forceinline__ PlanSlot plan_slot(LensFn lens, StartsFn starts, int 
   tsum = __builtin_amdgcn_readfirstlane(wave_sum_i(tsum));
   mx = __builtin_amdgcn_readfirstlane(wave_max_i(mx));
   nz = __builtin_amdgcn_readfirstlane(wave_sum_i(nz));
-  constexpr int A = kPlanAlign;
   if (nreg == 1 && nz == B && (int64_t)mx * B == (int64_t)tsum) {
     // every sequence has the same length L: sum_b ceil(L / U) <= units is
     // ceil(L / U) <= k = floor(units / B), i.e. U >= L / k, so the plan has
@@ -292,6 +292,58 @@ __device__ __forceinline__ PlanSlot plan_slot(LensFn lens, StartsFn starts, int 
 // vmcnt[5:4] in [15:14]; expcnt and lgkmcnt left at their maximum).
 __host__ __device__ constexpr int vmcnt_imm(int n) {
   return (n & 15) | (7 << 4) | (15 << 8) | ((n >> 4) << 14);
+}
+
+// Table addresses from code bytes spread into 16-bit halves: lut_spread
+// puts bytes 2i and 2i + 1 of w into the low and high halves of one register
+// (v_perm), and lut_mad forms half * 2^SH + lanec in one v_mad_u32_u16
+// (op_sel picks the half), so a pair of lookups costs three instructions
+// instead of four.  lut_mad<SH, HI>(lut_spread(w, i), lanec) equals
+// lut_addr<SH>(w, 2 * i + HI, lanec).
+__device__ __forceinline__ uint32_t lut_spread(uint32_t w, int i) {
+  return __builtin_amdgcn_perm(0u, w, i ? 0x0c030c02u : 0x0c010c00u);
+}
+template <int SH, int HI>
+__device__ __forceinline__ uint32_t lut_mad(uint32_t h, uint32_t lanec) {
+  uint32_t a;
+#if defined(__HIP_DEVICE_COMPILE__)
+  if constexpr (HI)
+    asm("v_mad_u32_u16 %0, %1, %2, %3 op_sel:[1,0,0,0]" : "=v"(a) : "v"(h), "s"(1u << SH), "v"(lanec));
+  else
+    asm("v_mad_u32_u16 %0, %1, %2, %3" : "=v"(a) : "v"(h), "s"(1u << SH), "v"(lanec));
+#else
+  a = ((HI ? h >> 16 : h & 0xffffu) << SH) + lanec;
+#endif
+  return a;
+}
+
+// PACK 2 scores of two tiles from their unmerged QC accumulators: lanes n < 8
+// of each row get tile 0's hi + lo sums (lane n + 8 holds the lo part), lanes
+// n >= 8 tile 1's (lane n - 8 holds the hi part): two DPP adds per value
+// whose bank masks write one half of each row each.  The leading s_nops
+// cover the wait states between the MFMAs that wrote a0 / a1 and their DPP
+// read (inline assembly, so the compiler does not count them).
+__device__ __forceinline__ float4_t pack_merge(float4_t a0, float4_t a1) {
+  float4_t d;
+#if defined(__HIP_DEVICE_COMPILE__)
+  float d0, d1, d2, d3;
+  asm volatile("s_nop 7\n\ts_nop 7\n\t"
+               "v_add_f32_dpp %0, %4, %4 row_ror:8 row_mask:0xf bank_mask:0x3\n\t"
+               "v_add_f32_dpp %0, %8, %8 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+               "v_add_f32_dpp %1, %5, %5 row_ror:8 row_mask:0xf bank_mask:0x3\n\t"
+               "v_add_f32_dpp %1, %9, %9 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+               "v_add_f32_dpp %2, %6, %6 row_ror:8 row_mask:0xf bank_mask:0x3\n\t"
+               "v_add_f32_dpp %2, %10, %10 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+               "v_add_f32_dpp %3, %7, %7 row_ror:8 row_mask:0xf bank_mask:0x3\n\t"
+               "v_add_f32_dpp %3, %11, %11 row_ror:8 row_mask:0xf bank_mask:0xc"
+               : "=&v"(d0), "=&v"(d1), "=&v"(d2), "=&v"(d3)
+               : "v"(a0[0]), "v"(a0[1]), "v"(a0[2]), "v"(a0[3]), "v"(a1[0]), "v"(a1[1]),
+                 "v"(a1[2]), "v"(a1[3]));
+  d = float4_t{d0, d1, d2, d3};
+#else
+  d = a0 + a1;
+#endif
+  return d;
 }
 
 // Occupancy facts of one kernel on the current device: CUs and resident

@@ -74,9 +74,10 @@ struct TrackParams {
   const int32_t* seq_lens;
   int64_t entries;  // of the page table
   int num_blocks, B, Hq, Hkv, ratio, rp, block_size, HG, units;
-  const _Float16* qh;  // q' hi and lo parts [rows][PD], and 1 / their scale
-  const _Float16* ql;
-  const float* qs;
+  const void* q;
+  int64_t q_sb, q_sh;
+  int q_bf16, hd;
+  const float* signs;
   float csc;  // score constant (log2 units)
   float osc;  // output constant
   float* s;   // scores, log2 units [table tile][Hkv][ratio][16]
@@ -91,14 +92,15 @@ struct TrackParams {
 
 // The unit that workgroup `u` serves (plan_slot of tq_plan.h); st: at least
 // 8 KB of LDS, free again afterwards.
-__device__ __forceinline__ PlanSlot unit_of(const TrackParams& p, int* st, int u, bool writer) {
+template <int A, typename Params>
+__device__ __forceinline__ PlanSlot unit_of(const Params& p, int* st, int u, bool writer) {
   const int lane = threadIdx.x & 63;
   if (p.B <= 64) {
     const bool in = lane < p.B;
     const int len = in ? max(p.seq_lens[lane], 0) : 0;
     const int ip = in ? p.indptr[lane] : 0;
-    return plan_slot([&](int) { return len; }, [&](int) { return ip; }, p.B, 1, p.units, u, 1,
-                     p.split, writer);
+    return plan_slot<A>([&](int) { return len; }, [&](int) { return ip; }, p.B, 1, p.units, u, 1,
+                        p.split, writer);
   }
   for (int i = threadIdx.x; i < kPlanMost; i += blockDim.x) {
     st[i] = i < p.B ? max(p.seq_lens[i], 0) : 0;
@@ -106,9 +108,9 @@ __device__ __forceinline__ PlanSlot unit_of(const TrackParams& p, int* st, int u
   }
   __syncthreads();
   const PlanSlot r =
-      plan_slot([&](int i) { return st[64 * i + lane]; },
-                [&](int i) { return st[kPlanMost + 64 * i + lane]; }, p.B, (p.B + 63) >> 6,
-                p.units, u, 1, p.split, writer);
+      plan_slot<A>([&](int i) { return st[64 * i + lane]; },
+                   [&](int i) { return st[kPlanMost + 64 * i + lane]; }, p.B, (p.B + 63) >> 6,
+                   p.units, u, 1, p.split, writer);
   __syncthreads();
   return r;
 }
@@ -231,38 +233,48 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b) {
   return __builtin_bit_cast(uint32_t, half2_t{(_Float16)a, (_Float16)b});
 }
 
-// The key tables: code byte -> fp16 hi parts of its two levels (high nibble
-// first, as the dims go), and their lo parts, times kLevelScale; 16 copies of
-// each, lane l reads copy l mod 16.  Two tables of dwords: as pairs in one
-// table, each operand register would cost a move.
-__device__ __forceinline__ void init_key_table(uint32_t* hi, uint32_t* lo) {
+__device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The key table: code byte -> fp16 hi parts of its two levels (high nibble
+// first, as the dims go) in the low dword, their lo parts in the high one,
+// times kLevelScale; 16 copies, lane l reads copy l mod 16.  Two entries are a
+// whole MFMA operand (hi, lo, hi, lo of two dims each) against q' with every
+// pair of dims twice: with hi and lo parts in operands of their own each entry
+// would cost two moves.
+__device__ __forceinline__ void init_key_table(uint64_t* lut) {
   for (int e = threadIdx.x; e < 4096; e += blockDim.x) {
     const int byte = e >> 4;
     const float a = level(byte >> 4) * kLevelScale, b = level(byte & 15) * kLevelScale;
     const float ah = (float)(_Float16)a, bh = (float)(_Float16)b;
-    hi[e] = pack_half(ah, bh);
-    lo[e] = pack_half(a - ah, b - bh);
+    lut[e] = pack_half(ah, bh) | (uint64_t)pack_half(a - ah, b - bh) << 32;
   }
 }
-// the operands of 8 codes
-__device__ __forceinline__ void key_operands(uint32_t c, const uint32_t* hi, const uint32_t* lo,
-                                             half8_t& kh, half8_t& kl) {
-  uint32_t h[4], l[4];
+// the two operands of 8 codes; lanec = 8 * (lane mod 16)
+__device__ __forceinline__ void key_operands(uint32_t c, const uint64_t* lut, uint32_t lanec,
+                                             half8_t& k0, half8_t& k1) {
+  uint64_t e[4];
 #pragma unroll
-  for (int y = 0; y < 4; y++) {
-    const uint32_t at = ((c >> (8 * y)) & 0xffu) << 4;
-    h[y] = hi[at];
-    l[y] = lo[at];
+  for (int i = 0; i < 2; i++) {
+    const uint32_t h = lut_spread(c, i);
+    const uint8_t* const t = reinterpret_cast<const uint8_t*>(lut);
+    e[2 * i] = *reinterpret_cast<const uint64_t*>(t + lut_mad<7, 0>(h, lanec));
+    e[2 * i + 1] = *reinterpret_cast<const uint64_t*>(t + lut_mad<7, 1>(h, lanec));
   }
-  kh = __builtin_bit_cast(half8_t, u32x4{h[0], h[1], h[2], h[3]});
-  kl = __builtin_bit_cast(half8_t, u32x4{l[0], l[1], l[2], l[3]});
+  typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+  k0 = __builtin_bit_cast(half8_t, u64x2{e[0], e[1]});
+  k1 = __builtin_bit_cast(half8_t, u64x2{e[2], e[3]});
+}
+// q' of 8 dims with every pair of dims twice
+__device__ __forceinline__ void twice(half8_t q, half8_t& q0, half8_t& q1) {
+  const u32x4 v = __builtin_bit_cast(u32x4, q);
+  q0 = __builtin_bit_cast(half8_t, u32x4{v[0], v[0], v[1], v[1]});
+  q1 = __builtin_bit_cast(half8_t, u32x4{v[2], v[2], v[3], v[3]});
 }
 
-// the codes of one tile and the norm of token 4 * (l/16) + l%4, from LDS: one
-// block that ends with its own wait, as the compiler does not see these reads
-template <int PD, int G>
-__device__ __forceinline__ void read_key_tile(uint32_t row, uint32_t nrm, uint32_t* c,
-                                              uint32_t& n) {
+// the codes of a tile (or of two) and a norm, from LDS: one block that ends
+// with its own wait, as the compiler does not see these reads
+template <int PD>
+__device__ __forceinline__ void read_keys(uint32_t row, uint32_t nrm, uint32_t* c, uint32_t& n) {
 #if defined(__HIP_DEVICE_COMPILE__)
   if constexpr (PD == 64) {
     u32x2 a;
@@ -286,19 +298,126 @@ __device__ __forceinline__ void read_key_tile(uint32_t row, uint32_t nrm, uint32
   (void)row; (void)nrm; (void)c; n = 0;
 #endif
 }
+template <int PD>  // 64 or 128; STEP: bytes from the first tile to the second
+__device__ __forceinline__ void read_key_pair(uint32_t row0, uint32_t row1, uint32_t nrm,
+                                              uint32_t (*c)[PD / 32], uint32_t& n) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef typename std::conditional<PD == 128, u32x4, u32x2>::type KT;
+  KT a, b;
+  if constexpr (PD == 128)
+    asm volatile("ds_read_b128 %0, %3\n\tds_read_b128 %1, %4\n\tds_read_u16 %2, %5\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(a), "=&v"(b), "=&v"(n) : "v"(row0), "v"(row1), "v"(nrm) : "memory");
+  else
+    asm volatile("ds_read_b64 %0, %3\n\tds_read_b64 %1, %4\n\tds_read_u16 %2, %5\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(a), "=&v"(b), "=&v"(n) : "v"(row0), "v"(row1), "v"(nrm) : "memory");
+#pragma unroll
+  for (int k = 0; k < PD / 32; k++) {
+    c[0][k] = a[k];
+    c[1][k] = b[k];
+  }
+#else
+  (void)row0; (void)row1; (void)nrm; (void)c; n = 0;
+#endif
+}
+
+// the norms of tokens 4 * (l/16) .. + 3, each lane holding that of l % 4
+__device__ __forceinline__ void spread_norms(uint32_t n, uint32_t* v) {
+  v[0] = quad_bcast<0>(n);
+  v[1] = quad_bcast<1>(n);
+  v[2] = quad_bcast<2>(n);
+  v[3] = quad_bcast<3>(n);
+}
+
+// running maximum and sum of exp2 over four more scores
+__device__ __forceinline__ void add_scores(const float4_t& x, float& m, float& l) {
+  const float mx = vmax3(vmax3(m, x[0], x[1]), x[2], x[3]);
+  float e = 0.f;
+#pragma unroll
+  for (int r = 0; r < 4; r++) e += exp2_raw(x[r] - mx);
+  l = l * exp2_raw(m - mx) + e;
+  m = mx;
+}
+// two (maximum, sum) pairs
+__device__ __forceinline__ void join_stats(float om, float ol, float& m, float& l) {
+  const float mx = vmax(m, om);
+  l = l * exp2_raw(m - mx) + ol * exp2_raw(om - mx);
+  m = mx;
+}
+
+// FWHT over the 64 lanes' PD / 64 elements each (element lane * E + k)
+template <int E>
+__device__ __forceinline__ void fwht_wave(float* x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int h = 1; h < E; h <<= 1)
+#pragma unroll
+    for (int k = 0; k < E; k++)
+      if (!(k & h)) {
+        const float a = x[k], b = x[k + h];
+        x[k] = a + b;
+        x[k + h] = a - b;
+      }
+#pragma unroll
+  for (int h = 1; h < 64; h <<= 1)
+#pragma unroll
+    for (int k = 0; k < E; k++) {
+      const float o = xor_lane(x[k], h);
+      x[k] = lane & h ? o - x[k] : x[k] + o;
+    }
+}
+
+// A row of hd elements (fp16 or bf16): lane l holds dims l * E .. + E - 1, zero
+// past hd
+template <int E>
+__device__ __forceinline__ void load_row(const void* q, int64_t off, bool bf16, int hd, float* x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int k = 0; k < E; k++) {
+    const int d = lane * E + k;
+    const int64_t at = off + min(d, hd - 1);
+    const uint16_t v = static_cast<const uint16_t*>(q)[at];
+    const float f = bf16 ? __uint_as_float((uint32_t)v << 16)
+                         : (float)__builtin_bit_cast(_Float16, v);
+    x[k] = d < hd ? f : 0.f;
+  }
+}
+// ... and rotated: FWHT(s x)/sqrt(pd); without signs as it is
+template <int E>
+__device__ __forceinline__ void rotate_row(const float* signs, float* x) {
+  if (!signs) return;
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int k = 0; k < E; k++) x[k] *= signs[lane * E + k];
+  fwht_wave<E>(x);
+  const float isq = 1.0f / sqrtf((float)(64 * E));
+#pragma unroll
+  for (int k = 0; k < E; k++) x[k] *= isq;
+}
+// The power of two that brings a row's largest magnitude into [128, 256), as an
+// exponent: x * 2^e = hi + lo to 22 bits, the lo parts of the large elements
+// normal numbers.
+__device__ __forceinline__ int row_exponent(float mx) {
+  return mx > 0.f && mx < INFINITY ? max(-100, min(100, 7 - ilogbf(mx))) : 0;
+}
 
 // ---- the keys: scores, and the splits' maxima and sums ----------------------
 // MFMA 16x16x32: A = a tile's keys (row = token), B = q' (column = q head).
 // QC (at most 8 q heads per kv head): columns 0-7 hold the hi parts of q',
 // 8-15 the lo parts, so the products with the hi and the lo parts of the keys
-// add up all four terms in one accumulator.
+// add up all four terms in one accumulator.  PACK (then, where a wave has two
+// tiles a step): lanes n < 8 take on the scores of the first tile and n >= 8
+// those of the second, which halves the work per score.
 template <int PD, int G, bool QC>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4)))
 void track_scores_kernel(TrackParams p) {
   using R = Rows<PD, G>;
   constexpr int KB = PD / 32;
+  constexpr bool PACK = QC && PD <= 128 && R::NTW == 2;
+  constexpr int NS = PACK ? 1 : R::NTW;  // score sets
   struct __attribute__((aligned(16))) Lds {
-    uint32_t hi[4096], lo[4096];  // the key tables
+    uint64_t lut[4096];
     uint8_t ring[R::RING];
   };
   __shared__ Lds sm;
@@ -306,8 +425,8 @@ void track_scores_kernel(TrackParams p) {
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int q4 = lane >> 4, n = lane & 15;
   const int hg = blockIdx.x % p.HG;
-  const PlanSlot ps = unit_of(p, reinterpret_cast<int*>(sm.hi), blockIdx.x / p.HG,
-                              blockIdx.x == 0 && w == 0);
+  const PlanSlot ps = unit_of<kPlanAlign>(p, reinterpret_cast<int*>(sm.lut), blockIdx.x / p.HG,
+                                          blockIdx.x == 0 && w == 0);
   if (ps.b < 0) return;
   const int c0 = ps.j * ps.U, c1 = min(c0 + ps.U, ps.L);
   Stream<PD, G> st(p, ps, c0, c1, w, hg);
@@ -315,160 +434,264 @@ void track_scores_kernel(TrackParams p) {
 
   const int kvh = hg * G + w % G, sub = w / G;
   const int head = QC ? n & 7 : n;
-  half8_t qa[KB], qb[QC ? 1 : KB];
-  float csc = 0.f;
-  {
-    const int64_t row = (int64_t)ps.b * p.Hq + kvh * p.ratio + min(head, p.ratio - 1);
-    const bool real = head < p.ratio;
-    const _Float16* src = (QC && n >= 8 ? p.ql : p.qh) + row * PD + (PD / 4) * q4;
+  // q' of the workgroup's heads: each wave rotates every eighth row into LDS
+  // (where the table goes later), fp32 with the 16-byte pieces of a row in an
+  // order of its own (no bank conflicts between rows); then each lane takes its
+  // column's dims, scales them by the row's power of two and splits them.
+  constexpr int E = PD / 64, NB = 4;  // rows loaded at a time
+  const int rows = G * p.ratio;
+  float* const rot = reinterpret_cast<float*>(sm.lut);
+  const int64_t q_at = (int64_t)ps.b * p.q_sb + (int64_t)hg * rows * p.q_sh;
+  float x0[NB][E];
 #pragma unroll
-    for (int k = 0; k < KB; k++) {
-      const half8_t v = *reinterpret_cast<const half8_t*>(src + 8 * k);
-      qa[k] = real ? v : half8_t{};
-    }
-    if constexpr (!QC) {
-      const _Float16* lo = p.ql + row * PD + (PD / 4) * q4;
-#pragma unroll
-      for (int k = 0; k < KB; k++) {
-        const half8_t v = *reinterpret_cast<const half8_t*>(lo + 8 * k);
-        qb[k] = real ? v : half8_t{};
-      }
-    }
-    csc = real ? p.csc * p.qs[row] : 0.f;
-  }
+  for (int i = 0; i < NB; i++)
+    load_row<E>(p.q, q_at + min(w + kWaves * i, rows - 1) * p.q_sh, p.q_bf16, p.hd, x0[i]);
   uint8_t* const spare = sm.ring + 2 * R::SLOT;
   st.issue(0, sm.ring, spare);
   st.issue(1, sm.ring + R::SLOT, spare);
-  init_key_table(sm.hi, sm.lo);
+  for (int r0 = w; r0 < rows; r0 += NB * kWaves) {
+    if (r0 != w)
+#pragma unroll
+      for (int i = 0; i < NB; i++)
+        load_row<E>(p.q, q_at + min(r0 + kWaves * i, rows - 1) * p.q_sh, p.q_bf16, p.hd, x0[i]);
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+      const int r = r0 + kWaves * i;
+      if (r >= rows) break;
+      rotate_row<E>(p.signs, x0[i]);
+#pragma unroll
+      for (int k = 0; k < E; k++) {
+        const int d = lane * E + k;
+        rot[r * PD + (((d >> 2) ^ (r & 7)) << 2) + (d & 3)] = x0[i][k];
+      }
+    }
+  }
   lds_written();
-  // q' ends here, not at its first use inside the loop
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * R::NJ));
+  barrier();
+  half8_t qa[2 * KB], qb[QC ? 1 : 2 * KB];
+  float csc = 0.f;
+  {
+    const int r = w % G * p.ratio + min(head, p.ratio - 1);
+    float x[8 * KB], mx = 0.f;
+#pragma unroll
+    for (int k = 0; k < 2 * KB; k++) {
+      const int piece = (PD / 16) * q4 + k;
+      const float4_t v =
+          *reinterpret_cast<const float4_t*>(rot + r * PD + ((piece ^ (r & 7)) << 2));
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        x[4 * k + j] = v[j];
+        mx = fmaxf(mx, fabsf(v[j]));
+      }
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 16));
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    const int ex = row_exponent(mx);
+    const bool real = head < p.ratio;
+    csc = real ? ldexpf(p.csc, -ex) : 0.f;
+#pragma unroll
+    for (int k = 0; k < KB; k++) {
+      half8_t hi, lo;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float v = real ? ldexpf(x[8 * k + j], ex) : 0.f;
+        hi[j] = (_Float16)v;
+        lo[j] = (_Float16)(v - (float)hi[j]);
+      }
+      if constexpr (QC) {
+        twice(n < 8 ? hi : lo, qa[2 * k], qa[2 * k + 1]);
+      } else {
+        twice(hi, qa[2 * k], qa[2 * k + 1]);
+        twice(lo, qb[2 * k], qb[2 * k + 1]);
+      }
+    }
+  }
+  lds_written();
+  barrier();  // every wave has its q'
+  init_key_table(sm.lut);
+  lds_written();
 
+  const int mine = PACK && n >= 8 ? R::SUB : 0;  // this lane's tile behind the wave's first
   const uint32_t ring = lds_addr(sm.ring);
-  const uint32_t o_row = n * R::ROWB + w % G * R::EBS + q4 * (PD / 8);
-  const uint32_t o_nrm = (4 * q4 + (lane & 3)) * R::ROWB + w % G * R::EBS + PD / 2;
-  const uint32_t *const hi_t = sm.hi + n, *const lo_t = sm.lo + n;
-  const int64_t tile_base = (int64_t)ps.ip * st.tpp + st.tile0;  // of the unit, in the table
-  const int64_t max_tile = p.entries * st.tpp;
+  const uint32_t o_row = sub * R::TILEB + n * R::ROWB + w % G * R::EBS + q4 * (PD / 8);
+  const uint32_t o_nrm = (sub + mine) * R::TILEB + (4 * q4 + (lane & 3)) * R::ROWB +
+                         w % G * R::EBS + PD / 2;
+  const uint32_t lanec = 8 * n;
+  // where this lane's scores of step s go: s * TPS tiles further
+  const int64_t tile_floats = (int64_t)p.Hq * kTile;
+  float* const s_at = p.s + ((int64_t)ps.ip * st.tpp + st.tile0 + sub + mine) * tile_floats +
+                      (kvh * p.ratio + head) * kTile + 4 * q4;
   float m = kNone, l = 0.f;
-  float4_t sc[R::NTW];
+  float4_t sc[NS];
+  bool keep[NS];
 
   auto store = [&](int s) {  // the scores of step s
 #pragma unroll
-    for (int i = 0; i < R::NTW; i++) {
-      const int t = s * R::TPS + sub + R::SUB * i;
-      const int64_t gt = tile_base + t;
-      if (t < st.tiles && gt >= 0 && gt < max_tile && n < p.ratio)
-        *reinterpret_cast<float4_t*>(p.s + ((gt * p.Hkv + kvh) * p.ratio + n) * kTile + 4 * q4) =
+    for (int i = 0; i < NS; i++)
+      if (keep[i])
+        *reinterpret_cast<float4_t*>(s_at + (int64_t)(s * R::TPS + R::SUB * i) * tile_floats) =
             sc[i];
-    }
   };
+  const bool store_lane = head < p.ratio && (PACK || n < p.ratio);
 
   for (int s = 0; s < steps; s++) {
     st.advance(s);
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(R::NJ));
     barrier();  // the copies of step s have landed (and the table is there)
-    uint32_t c[R::NTW][PD / 32], nr[R::NTW];
+    uint32_t c[R::NTW][PD / 32], nr[NS];
+    const uint32_t at = ring + (s & 1) * R::SLOT;
+    if constexpr (PACK) {
+      read_key_pair<PD>(at + o_row, at + o_row + R::SUB * R::TILEB, at + o_nrm, c, nr[0]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < R::NTW; i++) {
-      const uint32_t at = ring + (s & 1) * R::SLOT + (sub + R::SUB * i) * R::TILEB;
-      read_key_tile<PD, G>(at + o_row, at + o_nrm, c[i], nr[i]);
+      for (int i = 0; i < R::NTW; i++)
+        read_keys<PD>(at + o_row + R::SUB * R::TILEB * i, at + o_nrm + R::SUB * R::TILEB * i, c[i],
+                      nr[i]);
     }
     if (s) store(s - 1);
     barrier();  // every wave has read the slot
     st.issue(s + 2, sm.ring + (s & 1) * R::SLOT, spare);
+    float4_t acc[R::NTW];
 #pragma unroll
     for (int i = 0; i < R::NTW; i++) {
-      float4_t acc = {0.f, 0.f, 0.f, 0.f};
+      acc[i] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < KB; k++) {
-        half8_t hi, lo;
-        key_operands(c[i][k], hi_t, lo_t, hi, lo);
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, qa[k], acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, qa[k], acc, 0, 0, 0);
-        if constexpr (!QC) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, qb[k], acc, 0, 0, 0);
+        half8_t k0, k1;
+        key_operands(c[i][k], sm.lut, lanec, k0, k1);
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qa[2 * k], acc[i], 0, 0, 0);
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qa[2 * k + 1], acc[i], 0, 0, 0);
+        if constexpr (!QC) {
+          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qb[2 * k], acc[i], 0, 0, 0);
+          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qb[2 * k + 1], acc[i], 0, 0, 0);
+        }
       }
-      const int t = s * R::TPS + sub + R::SUB * i;
-      const bool ok = st.place(t) >= 0;
-      const int left = c1 - (st.tile0 + t) * kTile - 4 * q4;  // tokens of this lane's four
-      const uint32_t nv[4] = {quad_bcast<0>(nr[i]), quad_bcast<1>(nr[i]), quad_bcast<2>(nr[i]),
-                              quad_bcast<3>(nr[i])};
-      float mx = m;
+    }
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        float x = acc[r];
-        if constexpr (QC) x += ror8(x);
-        x = x * lo_half(nv[r]) * csc;
-        sc[i][r] = ok && r < left ? x : -INFINITY;
-        mx = fmaxf(mx, sc[i][r]);
+    for (int i = 0; i < NS; i++) {
+      const int t0 = s * R::TPS + sub + R::SUB * i;
+      float4_t x;
+      if constexpr (PACK) {
+        x = pack_merge(acc[0], acc[R::NTW - 1]);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; r++) x[r] = QC ? acc[i][r] + ror8(acc[i][r]) : acc[i][r];
       }
-      l *= exp2f(m - mx);
-      m = mx;
+      uint32_t nv[4];
+      spread_norms(nr[i], nv);
 #pragma unroll
-      for (int r = 0; r < 4; r++) l += exp2f(sc[i][r] - m);
+      for (int r = 0; r < 4; r++) x[r] = mul_lo_half(x[r], nv[r]) * csc;
+      // all tokens of the tiles are there (uniform); else masks
+      const int tl = PACK ? t0 + R::SUB : t0;  // the last tile
+      const int p0 = st.place(t0), p1 = PACK ? st.place(tl) : p0;
+      keep[i] = store_lane;
+      if (p0 < 0 || p1 < 0 || (st.tile0 + tl + 1) * kTile > c1) {
+        const bool there = (mine ? p1 : p0) >= 0;
+        const int left = c1 - (st.tile0 + t0 + mine) * kTile - 4 * q4;
+        keep[i] = keep[i] && there;
+#pragma unroll
+        for (int r = 0; r < 4; r++) x[r] = there && r < left ? x[r] : -INFINITY;
+      }
+      sc[i] = x;
+      add_scores(x, m, l);
     }
   }
   store(steps - 1);
   // no copy may land after the workgroup's LDS is given away
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-  // a head's lanes n, n + 16, n + 32, n + 48 meet
-  const float mx = fmaxf(fmaxf(m, __shfl_xor(m, 16)),
-                         fmaxf(__shfl_xor(m, 32), __shfl_xor(m, 48)));
-  l *= exp2f(m - mx);
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
+  // a head's lanes meet: its other tile's, then the token groups
+  if constexpr (PACK) join_stats(ror8(m), ror8(l), m, l);
+  join_stats(__shfl_xor(m, 16), __shfl_xor(l, 16), m, l);
+  join_stats(__shfl_xor(m, 32), __shfl_xor(l, 32), m, l);
   if (lane < p.rp)
     p.stats[((int64_t)kvh * p.stat_rows + (int64_t)(ps.Pb + ps.j) * R::SUB + sub) * p.rp + lane] =
-        lane < p.ratio ? make_float2(mx, l) : make_float2(kNone, 0.f);
+        lane < p.ratio ? make_float2(m, l) : make_float2(kNone, 0.f);
 }
 
-// V codes of tokens 4 * (l/16) .. + 3 (PD / 32 bytes each) and one norm
-template <int PD, int G>
-__device__ __forceinline__ void read_value_tile(uint32_t row, uint32_t nrm, uint32_t (*c)[4],
-                                                uint32_t& n) {
+// V codes of tokens 4 * (l/16) .. + 3 (PD / 32 bytes each) of NT tiles and one
+// norm
+template <int PD, int G, int NT>
+__device__ __forceinline__ void read_values(uint32_t row0, uint32_t row1, uint32_t nrm,
+                                            uint32_t (*c)[PD == 256 ? 2 : 1][4], uint32_t& n) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int S = Rows<PD, G>::ROWB;
+#define TQ_V8(OP)                                                                               \
+  OP " %0, %9\n\t" OP " %1, %9 offset:%12\n\t" OP " %2, %9 offset:%13\n\t"                     \
+  OP " %3, %9 offset:%14\n\t" OP " %4, %10\n\t" OP " %5, %10 offset:%12\n\t"                   \
+  OP " %6, %10 offset:%13\n\t" OP " %7, %10 offset:%14\n\tds_read_u16 %8, %11\n\t"             \
+     "s_waitcnt lgkmcnt(0)"
 #define TQ_V4(OP)                                                                              \
-  OP " %0, %5\n\t" OP " %1, %5 offset:%7\n\t" OP " %2, %5 offset:%8\n\t" OP " %3, %5 offset:%9\n\t" \
-     "ds_read_u16 %4, %6\n\ts_waitcnt lgkmcnt(0)"
-  if constexpr (PD == 64) {
-    asm volatile(TQ_V4("ds_read_u16")
-                 : "=&v"(c[0][0]), "=&v"(c[0][1]), "=&v"(c[0][2]), "=&v"(c[0][3]), "=&v"(n)
-                 : "v"(row), "v"(nrm), "i"(S), "i"(2 * S), "i"(3 * S) : "memory");
-  } else if constexpr (PD == 128) {
-    asm volatile(TQ_V4("ds_read_b32")
-                 : "=&v"(c[0][0]), "=&v"(c[0][1]), "=&v"(c[0][2]), "=&v"(c[0][3]), "=&v"(n)
-                 : "v"(row), "v"(nrm), "i"(S), "i"(2 * S), "i"(3 * S) : "memory");
-  } else {
+  OP " %0, %5\n\t" OP " %1, %5 offset:%7\n\t" OP " %2, %5 offset:%8\n\t"                       \
+  OP " %3, %5 offset:%9\n\tds_read_u16 %4, %6\n\ts_waitcnt lgkmcnt(0)"
+  if constexpr (PD == 256) {
+    static_assert(NT == 1, "one tile at a time");
     u32x2 a[4];
     asm volatile(TQ_V4("ds_read_b64")
                  : "=&v"(a[0]), "=&v"(a[1]), "=&v"(a[2]), "=&v"(a[3]), "=&v"(n)
-                 : "v"(row), "v"(nrm), "i"(S), "i"(2 * S), "i"(3 * S) : "memory");
+                 : "v"(row0), "v"(nrm), "i"(S), "i"(2 * S), "i"(3 * S) : "memory");
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      c[0][j] = a[j][0];
-      c[1][j] = a[j][1];
+      c[0][0][j] = a[j][0];
+      c[0][1][j] = a[j][1];
     }
+  } else if constexpr (NT == 2) {
+#define TQ_PAIR(OP)                                                                              \
+  asm volatile(TQ_V8(OP)                                                                         \
+               : "=&v"(c[0][0][0]), "=&v"(c[0][0][1]), "=&v"(c[0][0][2]), "=&v"(c[0][0][3]),     \
+                 "=&v"(c[1][0][0]), "=&v"(c[1][0][1]), "=&v"(c[1][0][2]), "=&v"(c[1][0][3]),     \
+                 "=&v"(n)                                                                        \
+               : "v"(row0), "v"(row1), "v"(nrm), "i"(S), "i"(2 * S), "i"(3 * S) : "memory")
+    if constexpr (PD == 64) TQ_PAIR("ds_read_u16");
+    else TQ_PAIR("ds_read_b32");
+#undef TQ_PAIR
+  } else {
+#define TQ_ONE(OP)                                                                               \
+  asm volatile(TQ_V4(OP)                                                                         \
+               : "=&v"(c[0][0][0]), "=&v"(c[0][0][1]), "=&v"(c[0][0][2]), "=&v"(c[0][0][3]),     \
+                 "=&v"(n)                                                                        \
+               : "v"(row0), "v"(nrm), "i"(S), "i"(2 * S), "i"(3 * S) : "memory")
+    if constexpr (PD == 64) TQ_ONE("ds_read_u16");
+    else TQ_ONE("ds_read_b32");
+#undef TQ_ONE
   }
+#undef TQ_V8
 #undef TQ_V4
 #else
-  (void)row; (void)nrm; (void)c; n = 0;
+  (void)row0; (void)row1; (void)nrm; (void)c; n = 0;
 #endif
 }
 
 constexpr float kValueScale = 1.4809800386428833f;  // levels near fp16 grid points (8.7e-5)
 
+// fp16 pair, towards zero (a hi part: the lo part takes up the rest)
+__device__ __forceinline__ uint32_t pack_rtz(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+}
+// nibble pairs of two tokens' code dwords: byte k indexes the levels (first
+// token's nibble low) of dim 2k (even) and 2k + 1 (odd)
+__device__ __forceinline__ void nibble_pairs(uint32_t a, uint32_t b, uint32_t& even,
+                                             uint32_t& odd) {
+  const uint32_t m4 = 0x0f0f0f0fu;
+  odd = (a & m4) | ((b << 4) & ~m4);
+  even = ((a >> 4) & m4) | (b & ~m4);
+}
+
 // ---- the values: output partials and the weights ----------------------------
-// MFMA 16x16x16: A = V^T (row = dim slot, k = tokens 4 * (l/16) ..), B = the
-// probabilities, whose layout is that of the scores' tile.  Dim of (row r,
-// product i) is r * (PD/16) + i.  QC: columns 0-7 hold the hi parts of
-// p * norm, 8-15 the lo parts.
+// MFMA with A = V^T (row = dim slot), B = the probabilities in the layout of
+// the scores' tile (16x16x16), or of a pair of tiles (PACK: 16x16x32, whose 8
+// k-values of a lane are tokens 4 * (l/16) .. + 3 of either tile).  Dim of (row
+// r, product i) is r * (PD/16) + i.  QC: columns 0-7 hold the hi parts of p *
+// norm, 8-15 the lo parts.  Probabilities are relative to the sequence's
+// maximum in the product and normalised at the end.
 template <int PD, int G, bool QC>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(PD == 256 ? 2 : 4)))
 void track_values_kernel(TrackParams p) {
   using R = Rows<PD, G>;
   constexpr int NO = PD / 16;           // products per tile
   constexpr int VW = PD == 256 ? 2 : 1;  // code dwords per token and lane
+  constexpr bool PACK = QC && PD <= 128 && R::NTW == 2;
+  constexpr int NS = PACK ? 1 : R::NTW;  // score sets
+  constexpr int NT = PACK ? 2 : 1;       // tiles of a set
   struct __attribute__((aligned(16))) Lds {
     uint32_t lut[8192];  // code byte -> levels of its low and high nibble, 32 copies
     uint8_t ring[R::RING];
@@ -478,7 +701,8 @@ void track_values_kernel(TrackParams p) {
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int q4 = lane >> 4, n = lane & 15;
   const int hg = blockIdx.x % p.HG;
-  const PlanSlot ps = unit_of(p, reinterpret_cast<int*>(sm.lut), blockIdx.x / p.HG, false);
+  const PlanSlot ps =
+      unit_of<kPlanAlign>(p, reinterpret_cast<int*>(sm.lut), blockIdx.x / p.HG, false);
   if (ps.b < 0) return;
   const int c0 = ps.j * ps.U, c1 = min(c0 + ps.U, ps.L);
   Stream<PD, G> st(p, ps, c0, c1, w, hg);
@@ -488,66 +712,72 @@ void track_values_kernel(TrackParams p) {
   st.issue(1, sm.ring + R::SLOT, spare);
   const int kvh = hg * G + w % G, sub = w / G;
   const int head = QC ? n & 7 : n;
+  const bool real = head < p.ratio;
 
   // the maximum and the sum of this lane's head over the sequence
   float M = kNone, den = 0.f;
   {
     const int64_t rows = (int64_t)((ps.L + ps.U - 1) / ps.U) * R::SUB;
     const float2* src = p.stats + ((int64_t)kvh * p.stat_rows + (int64_t)ps.Pb * R::SUB) * p.rp;
+#pragma unroll 4
     for (int64_t i = lane; i < rows * p.rp; i += 64) {
       const float2 x = src[i];
-      const float mx = fmaxf(M, x.x);
-      den = den * exp2f(M - mx) + x.y * exp2f(x.x - mx);
-      M = mx;
+      join_stats(x.x, x.y, M, den);
     }
-    for (int d = p.rp; d < 64; d <<= 1) {
-      const float om = __shfl_xor(M, d), od = __shfl_xor(den, d);
-      const float mx = fmaxf(M, om);
-      den = den * exp2f(M - mx) + od * exp2f(om - mx);
-      M = mx;
-    }
+    for (int d = p.rp; d < 64; d <<= 1) join_stats(__shfl_xor(M, d), __shfl_xor(den, d), M, den);
   }
-  const float inv = head < p.ratio && den != 0.f ? 1.0f / den : 0.f;
-  {
-    for (int e = threadIdx.x; e < 8192; e += kThreads) {
-      const int byte = e >> 5;
-      sm.lut[e] = pack_half(level(byte & 15) * kValueScale, level(byte >> 4) * kValueScale);
-    }
-    lds_written();
+  const float inv = real && den != 0.f ? 1.0f / den : 0.f;
+  if (!real) M = INFINITY;  // lanes of no head: probabilities of zero
+  for (int e = threadIdx.x; e < 8192; e += kThreads) {
+    const int byte = e >> 5;
+    sm.lut[e] = pack_half(level(byte & 15) * kValueScale, level(byte >> 4) * kValueScale);
   }
+  lds_written();
 
+  const int mine = PACK && n >= 8 ? R::SUB : 0;  // this lane's tile behind the wave's first
   const uint32_t ring = lds_addr(sm.ring);
-  const uint32_t o_row = 4 * q4 * R::ROWB + w % G * R::EBS + n * (PD / 32);
-  const uint32_t o_nrm = (4 * q4 + (lane & 3)) * R::ROWB + w % G * R::EBS + PD / 2;
-  const uint32_t* const lut = sm.lut + (lane & 31);
-  const int64_t tile_base = (int64_t)ps.ip * st.tpp + st.tile0;
+  const uint32_t o_row = sub * R::TILEB + 4 * q4 * R::ROWB + w % G * R::EBS + n * (PD / 32);
+  const uint32_t o_nrm = (sub + mine) * R::TILEB + (4 * q4 + (lane & 3)) * R::ROWB +
+                         w % G * R::EBS + PD / 2;
+  const uint32_t lanec = 4 * (lane & 31);
+  const int64_t tile_floats = (int64_t)p.Hq * kTile;
+  const float* const s_at = p.s +
+                            ((int64_t)ps.ip * st.tpp + st.tile0 + sub + mine) * tile_floats +
+                            (kvh * p.ratio + min(head, p.ratio - 1)) * kTile + 4 * q4;
   float4_t O[NO];
 #pragma unroll
   for (int i = 0; i < NO; i++) O[i] = float4_t{0.f, 0.f, 0.f, 0.f};
 
-  // scores and weights of step s, loaded one step ahead of their use; tiles
-  // outside the unit or the cache read an address inside the arrays and are
+  // scores and weights of step s, loaded one step ahead of their use; lanes
+  // whose tile is outside the unit or the cache read the arrays' start and are
   // masked
   struct Ahead {
-    float4_t sc[R::NTW], wt[R::NTW];
-    int64_t at[R::NTW];  // of the weights, -1: none
+    float4_t sc[NS], wt[NS];
+    int64_t at[NS];  // of the weights, -1: none
   } nx, cu;
   auto load = [&](int s, Ahead& a) {
 #pragma unroll
-    for (int i = 0; i < R::NTW; i++) {
-      const int t = s * R::TPS + sub + R::SUB * i;
-      const bool ok = st.place(t) >= 0;
-      const int64_t gt = ok ? tile_base + t : 0;
-      a.at[i] = ok ? st.weight_at(t, kvh) : -1;
+    for (int i = 0; i < NS; i++) {
+      const int t0 = s * R::TPS + sub + R::SUB * i;
+      const bool ok0 = st.place(t0) >= 0;
+      const int64_t w0 = ok0 ? st.weight_at(t0, kvh) : -1;
+      int64_t at = w0;
+      if constexpr (PACK) {
+        const bool ok1 = st.place(t0 + R::SUB) >= 0;
+        const int64_t w1 = ok1 ? st.weight_at(t0 + R::SUB, kvh) : -1;
+        at = mine ? w1 : w0;
+      }
+      a.at[i] = at;
       a.sc[i] = *reinterpret_cast<const float4_t*>(
-          p.s + ((gt * p.Hkv + kvh) * p.ratio + min(head, p.ratio - 1)) * kTile + 4 * q4);
-      a.wt[i] = *reinterpret_cast<const float4_t*>(p.weights + max(a.at[i], (int64_t)0) + 4 * q4);
+          at >= 0 ? s_at + (int64_t)(s * R::TPS + R::SUB * i) * tile_floats : p.s);
+      a.wt[i] = *reinterpret_cast<const float4_t*>(p.weights + (at >= 0 ? at : 0) + 4 * q4);
     }
   };
+  const bool store_lane = PACK ? (n & 7) == 0 : n == 0;
   auto store = [&](const Ahead& a) {  // the weights of a step
 #pragma unroll
-    for (int i = 0; i < R::NTW; i++)
-      if (a.at[i] >= 0 && n == 0)
+    for (int i = 0; i < NS; i++)
+      if (a.at[i] >= 0 && store_lane)
         *reinterpret_cast<float4_t*>(p.weights + a.at[i] + 4 * q4) = a.wt[i];
   };
   load(0, cu);
@@ -556,12 +786,13 @@ void track_values_kernel(TrackParams p) {
     st.advance(s);
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(R::NJ));
     barrier();
-    uint32_t c[R::NTW][VW][4], nr[R::NTW];
+    uint32_t c[R::NTW][VW][4], nr[NS];
+    const uint32_t at = ring + (s & 1) * R::SLOT;
 #pragma unroll
-    for (int i = 0; i < R::NTW; i++) {
-      const uint32_t at = ring + (s & 1) * R::SLOT + (sub + R::SUB * i) * R::TILEB;
-      read_value_tile<PD, G>(at + o_row, at + o_nrm, c[i], nr[i]);
-    }
+    for (int i = 0; i < NS; i++)
+      read_values<PD, G, NT>(at + o_row + R::SUB * R::TILEB * i,
+                             at + o_row + R::SUB * R::TILEB * (i + 1),
+                             at + o_nrm + R::SUB * R::TILEB * i, c + i, nr[i]);
     if (s) {
       store(cu);
       cu = nx;
@@ -570,51 +801,112 @@ void track_values_kernel(TrackParams p) {
     barrier();
     st.issue(s + 2, sm.ring + (s & 1) * R::SLOT, spare);
 #pragma unroll
-    for (int i = 0; i < R::NTW; i++) {
-      const int t = s * R::TPS + sub + R::SUB * i;
-      const int left = cu.at[i] >= 0 ? c1 - (st.tile0 + t) * kTile - 4 * q4 : 0;
-      const int last = ps.L - 1 - (st.tile0 + t) * kTile - 4 * q4;
-      const uint32_t nv[4] = {quad_bcast<0>(nr[i]), quad_bcast<1>(nr[i]), quad_bcast<2>(nr[i]),
-                              quad_bcast<3>(nr[i])};
-      float x[4];
+    for (int i = 0; i < NS; i++) {
+      const int t0 = s * R::TPS + sub + R::SUB * i, tl = PACK ? t0 + R::SUB : t0;
+      uint32_t nv[4];
+      spread_norms(nr[i], nv);
+      float rel[4], g[4], x[4];
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const float rel = r < left && head < p.ratio ? exp2f(cu.sc[i][r] - M) : 0.f;
-        float g = rel * inv;  // this head's weight; summed over the group's heads
-        g += xor_lane(g, 1);
-        g += xor_lane(g, 2);
-        g += xor_lane(g, 4);
-        if constexpr (!QC) g += xor_lane(g, 8);
-        if (r < left) cu.wt[i][r] = r == last ? g : cu.wt[i][r] + g;
-        x[r] = r < left ? rel * lo_half(nv[r]) : 0.f;
-        if constexpr (QC) {
-          const float h = (float)(_Float16)x[r];
-          x[r] = n < 8 ? h : x[r] - h;
+        rel[r] = exp2_raw(cu.sc[i][r] - M);
+        x[r] = mul_lo_half(rel[r], nv[r]);
+      }
+      // tiles with tokens that are not there, or with the newest one (uniform)
+      const int first = (st.tile0 + t0 + mine) * kTile + 4 * q4;
+      const bool whole = st.place(t0) >= 0 && st.place(tl) >= 0 &&
+                         (st.tile0 + tl + 1) * kTile < ps.L;
+      if (!whole) {
+        const int left = cu.at[i] >= 0 ? c1 - first : 0;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          rel[r] = r < left ? rel[r] : 0.f;
+          x[r] = r < left ? x[r] : 0.f;
         }
       }
-      const half4_t pb = {(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
-      // nibble pairs of tokens (0, 1) and (2, 3): byte k of ev / od indexes the
-      // levels of dims 2k + 1 / 2k
+      // this head's weights, summed over the group's heads
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        g[r] = rel[r] * inv;
+        g[r] += xor_lane(g[r], 1);
+        g[r] += xor_lane(g[r], 2);
+        // (row_half_mirror: the other four of eight lanes, alike by now)
+        g[r] += __int_as_float(
+            __builtin_amdgcn_mov_dpp(__float_as_int(g[r]), 0x141, 0xf, 0xf, false));
+        if constexpr (!QC) g[r] += ror8(g[r]);
+      }
+      if (whole) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) cu.wt[i][r] += g[r];
+      } else {
+        const int left = c1 - first, last = ps.L - 1 - first;
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          if (r < left) cu.wt[i][r] = r == last ? g[r] : cu.wt[i][r] + g[r];
+      }
+      // B operand
+      uint32_t pb[4];
+      if constexpr (QC) {
+        uint32_t hi[2], lo[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          hi[j] = pack_rtz(x[2 * j], x[2 * j + 1]);
+          lo[j] = pack_rtz(x[2 * j] - lo_half(hi[j]), x[2 * j + 1] - hi_half(hi[j]));
+        }
+        if constexpr (PACK) {
+          // lanes n < 8 hold the first tile's, n >= 8 the second's: swap lo
+          // parts against hi parts
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            const uint32_t in = (uint32_t)__builtin_amdgcn_mov_dpp(
+                (int)(mine ? hi[j] : lo[j]), 0x128, 0xf, 0xf, false);
+            pb[j] = mine ? in : hi[j];
+            pb[2 + j] = mine ? lo[j] : in;
+          }
+        } else {
+          pb[0] = n < 8 ? hi[0] : lo[0];
+          pb[1] = n < 8 ? hi[1] : lo[1];
+        }
+      } else {
+        pb[0] = pack_half(x[0], x[1]);
+        pb[1] = pack_half(x[2], x[3]);
+      }
 #pragma unroll
       for (int v = 0; v < VW; v++) {
-        const uint32_t m4 = 0x0f0f0f0fu;
-        const uint32_t* cc = c[i][v];
-        const uint32_t lo01 = (cc[0] & m4) | ((cc[1] & m4) << 4);
-        const uint32_t hi01 = ((cc[0] >> 4) & m4) | (cc[1] & ~m4);
-        const uint32_t lo23 = (cc[2] & m4) | ((cc[3] & m4) << 4);
-        const uint32_t hi23 = ((cc[2] >> 4) & m4) | (cc[3] & ~m4);
-        constexpr int BY = PD == 64 ? 2 : 4;
+        uint32_t ev[NT][2], od[NT][2];
 #pragma unroll
-        for (int k = 0; k < BY; k++) {
-          const uint32_t a0 = lut[((hi01 >> (8 * k)) & 0xffu) << 5];
-          const uint32_t a1 = lut[((hi23 >> (8 * k)) & 0xffu) << 5];
-          const uint32_t b0 = lut[((lo01 >> (8 * k)) & 0xffu) << 5];
-          const uint32_t b1 = lut[((lo23 >> (8 * k)) & 0xffu) << 5];
-          const int d = 8 * v + 2 * k;
-          O[d] = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(half4_t, u32x2{a0, a1}),
-                                                       pb, O[d], 0, 0, 0);
-          O[d + 1] = __builtin_amdgcn_mfma_f32_16x16x16f16(
-              __builtin_bit_cast(half4_t, u32x2{b0, b1}), pb, O[d + 1], 0, 0, 0);
+        for (int t = 0; t < NT; t++) {
+          nibble_pairs(c[i + t][v][0], c[i + t][v][1], ev[t][0], od[t][0]);
+          nibble_pairs(c[i + t][v][2], c[i + t][v][3], ev[t][1], od[t][1]);
+        }
+        constexpr int BY = PD == 64 ? 2 : 4;
+        const uint8_t* const lut = reinterpret_cast<const uint8_t*>(sm.lut);
+        auto entry = [&](uint32_t a) { return *reinterpret_cast<const uint32_t*>(lut + a); };
+#pragma unroll
+        for (int k = 0; k < BY; k += 2) {
+          uint32_t a[4][2 * NT];  // dims 2k, 2k + 1, 2k + 2, 2k + 3
+#pragma unroll
+          for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+              const uint32_t he = lut_spread(ev[t][j], k / 2), ho = lut_spread(od[t][j], k / 2);
+              a[0][2 * t + j] = entry(lut_mad<7, 0>(he, lanec));
+              a[1][2 * t + j] = entry(lut_mad<7, 0>(ho, lanec));
+              a[2][2 * t + j] = entry(lut_mad<7, 1>(he, lanec));
+              a[3][2 * t + j] = entry(lut_mad<7, 1>(ho, lanec));
+            }
+#pragma unroll
+          for (int d = 0; d < 4; d++) {
+            float4_t& acc = O[8 * v + 2 * k + d];
+            if constexpr (PACK)
+              acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                  __builtin_bit_cast(half8_t, u32x4{a[d][0], a[d][1], a[d][2 * NT - 2],
+                                                    a[d][2 * NT - 1]}),
+                  __builtin_bit_cast(half8_t, u32x4{pb[0], pb[1], pb[2], pb[3]}), acc, 0, 0, 0);
+            else
+              acc = __builtin_amdgcn_mfma_f32_16x16x16f16(
+                  __builtin_bit_cast(half4_t, u32x2{a[d][0], a[d][1]}),
+                  __builtin_bit_cast(half4_t, u32x2{pb[0], pb[1]}), acc, 0, 0, 0);
+          }
         }
       }
     }
@@ -649,87 +941,28 @@ void track_values_kernel(TrackParams p) {
   }
 }
 
-// FWHT over the 64 lanes' PD / 64 elements each (element lane * E + k)
-template <int E>
-__device__ __forceinline__ void fwht_wave(float* x) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int h = 1; h < E; h <<= 1)
-#pragma unroll
-    for (int k = 0; k < E; k++)
-      if (!(k & h)) {
-        const float a = x[k], b = x[k + h];
-        x[k] = a + b;
-        x[k + h] = a - b;
-      }
-#pragma unroll
-  for (int h = 1; h < 64; h <<= 1)
-#pragma unroll
-    for (int k = 0; k < E; k++) {
-      const float o = xor_lane(x[k], h);
-      x[k] = lane & h ? o - x[k] : x[k] + o;
-    }
-}
-
-// One row of hd elements (fp16 or bf16) rotated, scaled by a power of two to
-// a maximum in [128, 256) and split: x * scale = hi + lo to 22 bits, lo parts
-// of the large elements normal numbers.  Returns 1 / scale.
+// One row of hd elements rotated, scaled and split: x * scale = hi + lo.
+// Returns 1 / scale.
 template <int PD>
 __device__ __forceinline__ float split_row(const void* q, int64_t off, bool bf16, int hd,
                                            const float* signs, _Float16* hi, _Float16* lo) {
   constexpr int E = PD / 64;
-  const int lane = threadIdx.x & 63;
   float x[E];
-#pragma unroll
-  for (int k = 0; k < E; k++) {
-    const int d = lane * E + k;
-    x[k] = 0.f;
-    if (d < hd)
-      x[k] = bf16 ? (float)static_cast<const __bf16*>(q)[off + d]
-                  : (float)static_cast<const _Float16*>(q)[off + d];
-    if (signs) x[k] *= signs[d];
-  }
-  if (signs) {
-    fwht_wave<E>(x);
-    const float isq = 1.0f / sqrtf((float)PD);
-#pragma unroll
-    for (int k = 0; k < E; k++) x[k] *= isq;
-  }
+  load_row<E>(q, off, bf16, hd, x);
+  rotate_row<E>(signs, x);
   float mx = 0.f;
 #pragma unroll
   for (int k = 0; k < E; k++) mx = fmaxf(mx, fabsf(x[k]));
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) mx = fmaxf(mx, xor_lane(mx, d));
-  int ex = 0;
-  if (mx > 0.f && mx < INFINITY) ex = max(-100, min(100, 8 - (ilogbf(mx) + 1)));
-  const float sc = ldexpf(1.0f, ex);
+  const int ex = row_exponent(mx);
 #pragma unroll
   for (int k = 0; k < E; k++) {
-    const float v = x[k] * sc;
+    const float v = ldexpf(x[k], ex);
     hi[k] = (_Float16)v;
     lo[k] = (_Float16)(v - (float)hi[k]);
   }
   return ldexpf(1.0f, -ex);
-}
-
-template <int PD>
-__global__ __launch_bounds__(256) void rotate_q_kernel(const void* __restrict__ q, int64_t q_sb,
-                                                       int64_t q_sh, int bf16, int hd, int Hq,
-                                                       int rows, const float* __restrict__ signs,
-                                                       _Float16* __restrict__ qh,
-                                                       _Float16* __restrict__ ql,
-                                                       float* __restrict__ qs) {
-  constexpr int E = PD / 64;
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (row >= rows) return;
-  _Float16 hi[E], lo[E];
-  const float inv = split_row<PD>(q, row / Hq * q_sb + row % Hq * q_sh, bf16, hd, signs, hi, lo);
-#pragma unroll
-  for (int k = 0; k < E; k++) {
-    qh[(int64_t)row * PD + lane * E + k] = hi[k];
-    ql[(int64_t)row * PD + lane * E + k] = lo[k];
-  }
-  if (lane == 0) qs[row] = inv;
 }
 
 // o = s FWHT(sum of the partial rows)/sqrt(pd): one workgroup per (sequence,
@@ -841,48 +1074,98 @@ __global__ __launch_bounds__(256) void rotate_window_kernel(
   if (lane == 0) qs[row] = inv;
 }
 
+// hi and lo operands of 8 codes, in registers of their own
+__device__ __forceinline__ void key_parts(uint32_t c, const uint64_t* lut, uint32_t lanec,
+                                          half8_t& hi, half8_t& lo) {
+  half8_t k0, k1;
+  key_operands(c, lut, lanec, k0, k1);
+  const u32x4 a = __builtin_bit_cast(u32x4, k0), b = __builtin_bit_cast(u32x4, k1);
+  hi = __builtin_bit_cast(half8_t, u32x4{a[0], a[2], b[0], b[2]});
+  lo = __builtin_bit_cast(half8_t, u32x4{a[1], a[3], b[1], b[3]});
+}
+
+// operands of two steps of a row tile, hi and lo, from LDS (1 KB each)
+__device__ __forceinline__ void read_operands(uint32_t at, half8_t* f) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  u32x4 a, b, c, d;
+  asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:1024\n\t"
+               "ds_read_b128 %2, %4 offset:2048\n\tds_read_b128 %3, %4 offset:3072\n\t"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d) : "v"(at) : "memory");
+  f[0] = __builtin_bit_cast(half8_t, a);
+  f[1] = __builtin_bit_cast(half8_t, b);
+  f[2] = __builtin_bit_cast(half8_t, c);
+  f[3] = __builtin_bit_cast(half8_t, d);
+#else
+  (void)at; (void)f;
+#endif
+}
+
 // One pass of the keys over the rows.  SUM false: each row's maximum and sum
 // over the unit's tokens; true: each token's sum of weights over the rows,
 // added to (or, for the chunk's own tokens, set as) its weight.
+//
+// A workgroup's four waves hold 32 MT keys each as operands and walk the row
+// tiles together: a tile's operands (PD * 128 bytes) come into LDS one ahead
+// of their use, by direct-to-LDS copies that the four waves share.
 template <int PD, int MT, bool SUM>
-__global__ __launch_bounds__(256) void window_kernel(WindowParams p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+void window_kernel(WindowParams p) {
   constexpr int KS = PD / 16;
   constexpr int EBS = Rows<PD, 1>::EBS;
+  constexpr int QT = PD * 128;  // bytes of a row tile's operands
+  constexpr int TOK = 4 * 32 * MT;
+  typedef float float16_t __attribute__((ext_vector_type(16)));
   struct __attribute__((aligned(16))) Lds {
-    uint32_t hi[4096], lo[4096];
-    float2 st[SUM ? 1 : 4][SUM ? 1 : 1024];  // per wave: a row's running (max, sum)
+    union {
+      uint64_t lut[4096];
+      uint8_t q[2][QT];
+    };
+    float2 wave[SUM ? 1 : 4][32];    // a row tile's (max, sum) of each wave
+    float2 rows[SUM ? 1 : 1024];     // running (max, sum) of the unit
   };
   __shared__ Lds sm;
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kvh = blockIdx.x / p.units, u = blockIdx.x % p.units;
-  TrackParams tp = {};
-  tp.B = p.B;
-  tp.units = p.units;
-  tp.seq_lens = p.seq_lens;
-  tp.indptr = p.indptr;
-  tp.split = p.split;
-  const PlanSlot ps = unit_of(tp, reinterpret_cast<int*>(sm.hi), u,
-                              !SUM && blockIdx.x == 0 && w == 0);
+  const PlanSlot ps = unit_of<TOK>(p, reinterpret_cast<int*>(sm.lut), u,
+                                   !SUM && blockIdx.x == 0 && w == 0);
   if (ps.b < 0) return;
   const int q_len = p.q_start[ps.b + 1] - p.q_start[ps.b];
   if (SUM && q_len <= 0) return;  // no queries: the weights stay
-  init_key_table(sm.hi, sm.lo);
   const int c0 = ps.j * ps.U, c1 = min(c0 + ps.U, ps.L);
   const int64_t bh = (int64_t)ps.b * p.Hkv + kvh;
-  const half8_t* const qf = p.qf + bh * p.tiles * KS * 2 * 64;
+  const uint8_t* const qf =
+      reinterpret_cast<const uint8_t*>(p.qf) + bh * p.tiles * (int64_t)QT;
   const float* const qs = p.qs + bh * p.tiles * 32;
   const float* const lse = SUM ? p.lse + bh * p.tiles * 32 : nullptr;
   if constexpr (!SUM)
-    for (int i = lane; i < p.tiles * 32; i += 64) sm.st[w][i] = make_float2(kNone, 0.f);
-  __syncthreads();
-  const uint32_t *const hi_t = sm.hi + (lane & 15), *const lo_t = sm.lo + (lane & 15);
+    for (int i = threadIdx.x; i < p.tiles * 32; i += 256) sm.rows[i] = make_float2(kNone, 0.f);
+  const uint32_t lanec = 8 * (lane & 15);
 
-  for (int t0 = c0 + w * 32 * MT; t0 < c1; t0 += 4 * 32 * MT) {
-    // the keys of tokens t0 + 32 m + col, as operands; their norms by row of
-    // the product's layout (row 8 * (i / 4) + 4 * half + i % 4)
+  // copies of row tile rt into buffer rt & 1
+  auto issue = [&](int rt) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)(qf + (int64_t)rt * QT), (short)0, QT, 0x00020000);
+#pragma unroll
+    for (int j = 0; j < QT / 4096; j++)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (void*)(sm.q[rt & 1] + (4 * j + w) * 1024), 16,
+                                               (uint32_t)((4 * j + w) * 1024 + lane * 16), 0, 0, 0);
+#else
+    (void)rt;
+#endif
+  };
+
+  for (int cb = c0; cb < c1; cb += TOK) {
+    const int t0 = cb + w * 32 * MT;
+    __syncthreads();  // the last chunk's operands are no longer read
+    init_key_table(sm.lut);
+    __syncthreads();
+    // the keys of tokens t0 + 32 m + col, as operands; their norms (fp16) by row
+    // of the product's layout: row 8 * (i / 4) + 4 * half + i % 4
     half8_t kh[MT][KS], kl[MT][KS];
-    float kn[MT][16];
+    uint32_t kn[MT][8];
     uint32_t okm[MT];
     int64_t place[MT];  // index of this lane's token in weights, -1: none
 #pragma unroll
@@ -901,7 +1184,7 @@ __global__ __launch_bounds__(256) void window_kernel(WindowParams p) {
       }
       okm[m] = (uint32_t)__ballot(place[m] >= 0);
       const uint32_t* src = reinterpret_cast<const uint32_t*>(p.slab + at + half * (PD / 4));
-      const float norm = lo_half(*reinterpret_cast<const uint32_t*>(p.slab + at + PD / 2));
+      const uint32_t norm = *reinterpret_cast<const uint32_t*>(p.slab + at + PD / 2) & 0xffffu;
       uint32_t c[KS];
 #pragma unroll
       for (int k = 0; k < KS; k += 4) {
@@ -909,68 +1192,117 @@ __global__ __launch_bounds__(256) void window_kernel(WindowParams p) {
         c[k] = v[0]; c[k + 1] = v[1]; c[k + 2] = v[2]; c[k + 3] = v[3];
       }
 #pragma unroll
-      for (int k = 0; k < KS; k++) key_operands(c[k], hi_t, lo_t, kh[m][k], kl[m][k]);
+      for (int k = 0; k < KS; k++) key_parts(c[k], sm.lut, lanec, kh[m][k], kl[m][k]);
 #pragma unroll
-      for (int i = 0; i < 16; i++) kn[m][i] = __shfl(norm, 8 * (i / 4) + 4 * half + i % 4);
+      for (int i = 0; i < 8; i++) {
+        const int r = 8 * (i / 2) + 4 * half + 2 * (i % 2);
+        kn[m][i] = (uint32_t)__shfl((int)norm, r) | (uint32_t)__shfl((int)norm, r + 1) << 16;
+      }
     }
-    float got[MT][16];
+    float got[SUM ? MT : 1][16];
+    if constexpr (SUM) {
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+      for (int m = 0; m < MT; m++)
 #pragma unroll
-      for (int i = 0; i < 16; i++) got[m][i] = 0.f;
+        for (int i = 0; i < 16; i++) got[m][i] = 0.f;
+    }
+    bool all = t0 + 32 * MT <= c1;  // every token of the wave is there
+#pragma unroll
+    for (int m = 0; m < MT; m++) all = all && okm[m] == 0xffffffffu;
+    __syncthreads();  // the table is no longer read
+    issue(0);
 
     for (int rt = 0; rt < p.tiles; rt++) {
-      typedef float float16_t __attribute__((ext_vector_type(16)));
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+      barrier();  // tile rt is there, and nobody reads the other buffer
+      if (rt + 1 < p.tiles) issue(rt + 1);
+      const int row = rt * 32 + col;
+      const float cq = qs[row] * p.csc;
+      const float ls = SUM ? lse[row] : 0.f;
       float16_t acc[MT];
 #pragma unroll
       for (int m = 0; m < MT; m++)
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[m][i] = 0.f;
-      const half8_t* f = qf + (int64_t)rt * KS * 2 * 64 + lane;
+      const uint32_t at = lds_addr(sm.q[rt & 1]) + lane * 16;
 #pragma unroll
-      for (int k = 0; k < KS; k++) {
-        const half8_t bh8 = f[k * 128], bl8 = f[k * 128 + 64];
+      for (int k = 0; k < KS; k += 2) {
+        half8_t f[4];
+        read_operands(at + k * 2048, f);
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
-          acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[m][k], bh8, acc[m], 0, 0, 0);
-          acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl[m][k], bh8, acc[m], 0, 0, 0);
-          acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[m][k], bl8, acc[m], 0, 0, 0);
-        }
-      }
-      const int row = rt * 32 + col;
-      const float cq = qs[row] * p.csc;
-      // the last token that this row's query sees
-      const int see = ps.L - p.window + row / p.ratio;
-      if constexpr (SUM) {
-        const float ls = lse[row];
+        for (int y = 0; y < 2; y++)
 #pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const int tr = 8 * (i / 4) + 4 * half + i % 4;
-            const float x = exp2f(acc[m][i] * kn[m][i] * cq - ls);
-            got[m][i] += t0 + 32 * m + tr <= see ? x : 0.f;
+          for (int m = 0; m < MT; m++) {
+            acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[m][k + y], f[2 * y], acc[m], 0, 0, 0);
+            acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl[m][k + y], f[2 * y], acc[m], 0, 0, 0);
+            acc[m] =
+                __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[m][k + y], f[2 * y + 1], acc[m], 0, 0, 0);
           }
+      }
+      // the last token that this row's query sees; the tile's first row sees least
+      const int see = ps.L - p.window + row / p.ratio;
+      const bool clear = all && t0 + 32 * MT - 1 <= ps.L - p.window + rt * 32 / p.ratio;
+#pragma unroll
+      for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          acc[m][i] = mul_lo_half(acc[m][i], kn[m][i / 2]);
+          acc[m][i + 1] = mul_lo_half(acc[m][i + 1], kn[m][i / 2] >> 16);
+        }
+      if constexpr (SUM) {
+        if (clear) {
+#pragma unroll
+          for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) got[m][i] += exp2_raw(fmaf(acc[m][i], cq, -ls));
+        } else {
+#pragma unroll
+          for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              const int t = t0 + 32 * m + 8 * (i / 4) + 4 * half + i % 4;
+              got[m][i] += t <= see ? exp2_raw(fmaf(acc[m][i], cq, -ls)) : 0.f;
+            }
+        }
       } else {
         float mx = kNone, l = 0.f;
+        if (!clear) {
+#pragma unroll
+          for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              const int tr = 8 * (i / 4) + 4 * half + i % 4;
+              const bool ok = ((okm[m] >> tr) & 1) && t0 + 32 * m + tr <= see;
+              acc[m][i] = ok ? acc[m][i] * cq : -INFINITY;
+              mx = vmax(mx, acc[m][i]);
+            }
+        } else {
+#pragma unroll
+          for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              acc[m][i] *= cq;
+              mx = vmax(mx, acc[m][i]);
+            }
+        }
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const int tr = 8 * (i / 4) + 4 * half + i % 4;
-            const bool ok = ((okm[m] >> tr) & 1) && t0 + 32 * m + tr <= see;
-            acc[m][i] = ok ? acc[m][i] * kn[m][i] * cq : -INFINITY;
-            mx = fmaxf(mx, acc[m][i]);
+          for (int i = 0; i < 16; i++) l += exp2_raw(acc[m][i] - mx);
+        join_stats(__shfl_xor(mx, 32), __shfl_xor(l, 32), mx, l);
+        if (half == 0) sm.wave[w][col] = make_float2(mx, l);
+        lds_written();
+        barrier();
+        if (w == 0 && half == 0) {
+          float2 a = sm.rows[row];
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const float2 b = sm.wave[k][col];
+            join_stats(b.x, b.y, a.x, a.y);
           }
-#pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-          for (int i = 0; i < 16; i++) l += exp2f(acc[m][i] - mx);
-        const float om = __shfl_xor(mx, 32), ol = __shfl_xor(l, 32);
-        const float2 old = sm.st[w][row];
-        const float top = fmaxf(fmaxf(mx, om), old.x);
-        l = l * exp2f(mx - top) + ol * exp2f(om - top) + old.y * exp2f(old.x - top);
-        if (half == 0) sm.st[w][row] = make_float2(top, l);
+          sm.rows[row] = a;
+          lds_written();
+        }
       }
     }
     if constexpr (SUM) {
@@ -983,8 +1315,8 @@ __global__ __launch_bounds__(256) void window_kernel(WindowParams p) {
           g += xor_lane(g, 1);
           g += xor_lane(g, 2);
           g += xor_lane(g, 4);
-          g += xor_lane(g, 8);
-          g += __shfl_xor(g, 16);
+          g += ror8(g);
+          g = xor16_sum(g);
           const float other = __shfl_xor(g, 32);
           const int r0 = 8 * (i / 4) + i % 4;  // half 0's row; half 1's is 4 further
           if (col == r0) mine = half ? other : g;
@@ -1005,44 +1337,44 @@ __global__ __launch_bounds__(256) void window_kernel(WindowParams p) {
   if constexpr (!SUM) {
     __syncthreads();
     float2* const out = p.stats + ((int64_t)kvh * p.units + u) * p.tiles * 32;
-    for (int i = threadIdx.x; i < p.tiles * 32; i += 256) {
-      float2 a = sm.st[0][i];
-#pragma unroll
-      for (int k = 1; k < 4; k++) {
-        const float2 b = sm.st[k][i];
-        const float top = fmaxf(a.x, b.x);
-        a = make_float2(top, a.y * exp2f(a.x - top) + b.y * exp2f(b.x - top));
-      }
-      out[i] = a;
-    }
+    for (int i = threadIdx.x; i < p.tiles * 32; i += 256) out[i] = sm.rows[i];
   }
 }
 
-// the normalisers of a sequence's rows from its units' maxima and sums
+// The normalisers of a sequence's rows from its units' maxima and sums: a
+// workgroup takes 32 rows, thread (r, g) their units g, g + 8, ...
 __global__ __launch_bounds__(256) void window_lse_kernel(WindowParams p) {
-  const int R = p.tiles * 32;
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= (int64_t)p.B * p.Hkv * R) return;
-  const int row = (int)(at % R);
-  const int64_t bh = at / R;
+  __shared__ float2 part[8][32];
+  const int R = p.tiles * 32, r = threadIdx.x & 31, g = threadIdx.x >> 5;
+  const int tile = blockIdx.x % p.tiles;
+  const int64_t bh = blockIdx.x / p.tiles;
   const int kvh = (int)(bh % p.Hkv), b = (int)(bh / p.Hkv);
+  const int row = tile * 32 + r;
+  const int u0 = p.split[b], u1 = p.split[b + 1];
+  const float2* const src = p.stats + (int64_t)kvh * p.units * R + row;
   float m = kNone, l = 0.f;
 #pragma unroll 4
-  for (int u = p.split[b]; u < p.split[b + 1]; u++) {
-    const float2 x = p.stats[((int64_t)kvh * p.units + u) * R + row];
-    const float top = fmaxf(m, x.x);
-    l = l * exp2f(m - top) + x.y * exp2f(x.x - top);
-    m = top;
+  for (int u = u0 + g; u < u1; u += 8) {
+    const float2 x = src[(int64_t)u * R];
+    join_stats(x.x, x.y, m, l);
   }
+  part[g][r] = make_float2(m, l);
+  __syncthreads();
+  if (g) return;
+#pragma unroll
+  for (int k = 1; k < 8; k++) join_stats(part[k][r].x, part[k][r].y, m, l);
   // rows past the window or before the chunk's first query add nothing
+  const int64_t at = bh * R + row;
   p.lse[at] = p.qs[at] != 0.f && l != 0.f ? m + log2f(l) : INFINITY;
 }
 
 // ---- host ------------------------------------------------------------------
 
-int group_of(int pd, int hkv) {
+// Kv heads of a workgroup: the largest of 8, 4, 2, 1 (at most 4 at head size
+// 256) that divides their number and whose q' fit the 32 KB of the table.
+int group_of(int pd, int hkv, int ratio) {
   int g = pd == 256 ? 4 : 8;
-  while (hkv % g) g >>= 1;
+  while (hkv % g || g * ratio * pd * 4 > 32768) g >>= 1;
   return g;
 }
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
@@ -1109,7 +1441,7 @@ int track_units(int batch, int pd, int g, int hg, bool qc) {
 
 // A tracked decode's workspace
 struct TrackWs {
-  size_t qh, ql, qs, stats, split, s, po, total;
+  size_t stats, split, s, po, total;
 };
 TrackWs track_ws(int batch, int64_t entries, int hq, int hkv, int pd, int bs, int units, int sub) {
   const int ratio = hq / hkv;
@@ -1122,10 +1454,6 @@ TrackWs track_ws(int batch, int64_t entries, int hq, int hkv, int pd, int bs, in
     at += up256(n);
     return r;
   };
-  const size_t rows = (size_t)batch * hq;
-  w.qh = take(rows * pd * 2);
-  w.ql = take(rows * pd * 2);
-  w.qs = take(rows * 4);
   w.stats = take((size_t)hkv * units * sub * rp * 8);
   w.split = take((size_t)(batch + 2) * 4);
   // (a tile at least: tiles outside the table read the first one)
@@ -1207,9 +1535,8 @@ extern "C" int64_t tq_decode_tracked_workspace_bytes(int32_t batch, int64_t num_
                              padded_dim, block_size);
   if (rc) return rc;
   if (batch == 0) return 0;
-  const int g = group_of(padded_dim, num_kv_heads);
-  const int units =
-      track_units(batch, padded_dim, g, num_kv_heads / g, num_qo_heads / num_kv_heads <= 8);
+  const int ratio = num_qo_heads / num_kv_heads, g = group_of(padded_dim, num_kv_heads, ratio);
+  const int units = track_units(batch, padded_dim, g, num_kv_heads / g, ratio <= 8);
   if (units <= 0) {
     set_error("decode_tracked: occupancy query failed");
     return kEinval;
@@ -1240,8 +1567,8 @@ extern "C" int tq_decode_paged_tracked(
     set_error("%s: o must be fp16 or bf16", who);
     return kEinval;
   }
-  const int pd = padded_dim, g = group_of(pd, num_kv_heads), sub = kWaves / g;
-  const int ratio = num_qo_heads / num_kv_heads;
+  const int pd = padded_dim, ratio = num_qo_heads / num_kv_heads;
+  const int g = group_of(pd, num_kv_heads, ratio), sub = kWaves / g;
   const bool qc = ratio <= 8;
   const int units = track_units(batch, pd, g, num_kv_heads / g, qc);
   if (units <= 0) {
@@ -1256,9 +1583,6 @@ extern "C" int tq_decode_paged_tracked(
     return kEinval;
   }
   uint8_t* const base = static_cast<uint8_t*>(workspace);
-  _Float16* qh = reinterpret_cast<_Float16*>(base + ws.qh);
-  _Float16* ql = reinterpret_cast<_Float16*>(base + ws.ql);
-  float* qs = reinterpret_cast<float*>(base + ws.qs);
   TrackParams p = {};
   p.slab = k_slab;
   p.indices = indices;
@@ -1275,9 +1599,12 @@ extern "C" int tq_decode_paged_tracked(
   p.block_size = block_size;
   p.HG = num_kv_heads / g;
   p.units = units;
-  p.qh = qh;
-  p.ql = ql;
-  p.qs = qs;
+  p.q = q;
+  p.q_sb = q_stride_b;
+  p.q_sh = q_stride_h;
+  p.q_bf16 = q_dtype == TQ_BF16;
+  p.hd = head_dim;
+  p.signs = signs;
   const float isq = 1.0f / sqrtf((float)pd);
   p.csc = sm_scale * 1.4426950408889634f * isq / kLevelScale;
   p.osc = isq / kValueScale;
@@ -1289,17 +1616,7 @@ extern "C" int tq_decode_paged_tracked(
   p.weights = weights;
   p.positions = positions;
   p.ends = ends;
-  const int rows = batch * num_qo_heads;
-  int bf = q_dtype == TQ_BF16, hq = num_qo_heads, hd = head_dim;
-  {
-    void* args[] = {&q, &q_stride_b, &q_stride_h, &bf, &hd, &hq, (void*)&rows, &signs, &qh, &ql,
-                    &qs};
-    const void* fn = pd == 64    ? reinterpret_cast<const void*>(&rotate_q_kernel<64>)
-                     : pd == 128 ? reinterpret_cast<const void*>(&rotate_q_kernel<128>)
-                                 : reinterpret_cast<const void*>(&rotate_q_kernel<256>);
-    rc = launch(who, fn, (rows + 3) / 4, 256, args, stream);
-    if (rc) return rc;
-  }
+  int hq = num_qo_heads, hd = head_dim;
   void* targs[] = {&p};
   rc = launch(who, reinterpret_cast<const void*>(track_fn<false>(pd, g, qc)),
               (int64_t)units * p.HG, kThreads, targs, stream);
@@ -1316,7 +1633,7 @@ extern "C" int tq_decode_paged_tracked(
     const void* fn = pd == 64    ? reinterpret_cast<const void*>(&track_join_kernel<64>)
                      : pd == 128 ? reinterpret_cast<const void*>(&track_join_kernel<128>)
                                  : reinterpret_cast<const void*>(&track_join_kernel<256>);
-    return launch(who, fn, rows, 256, args, stream);
+    return launch(who, fn, (int64_t)batch * hq, 256, args, stream);
   }
 }
 
@@ -1327,12 +1644,12 @@ struct WindowWs {
   size_t qf, qs, stats, lse, split, total;
   int tiles, units;
 };
-// units of a window call: what the first pass keeps resident per kv head, at
-// least one per sequence
+// units of a window call: two workgroups a CU over the kv heads, at least one
+// per sequence
 WindowWs window_ws(int batch, int window, int ratio, int hkv, int pd, int cus) {
   WindowWs w;
   w.tiles = (window * ratio + 31) / 32;
-  w.units = max(batch, 4 * cus / hkv);
+  w.units = max(batch, 2 * cus / hkv);
   size_t at = 0;
   auto take = [&](size_t n) {
     const size_t r = at;
@@ -1462,8 +1779,8 @@ extern "C" int tq_track_window(const void* q, int64_t num_rows, int64_t q_stride
   void* args[] = {&p};
   rc = launch(who, f0, (int64_t)ws.units * num_kv_heads, 256, args, stream);
   if (rc) return rc;
-  rc = launch(who, reinterpret_cast<const void*>(&window_lse_kernel), (rows + 255) / 256, 256,
-              args, stream);
+  rc = launch(who, reinterpret_cast<const void*>(&window_lse_kernel), rows / 32, 256, args,
+              stream);
   if (rc) return rc;
   return launch(who, f1, (int64_t)ws.units * num_kv_heads, 256, args, stream);
 }
