@@ -11,10 +11,10 @@
 // rewrite the whole cache.
 //
 // select_kernel: one workgroup per (sequence, kv head) reads weights and
-// positions once into keys in LDS (32 bits that order like the rule above),
-// finds the budget-th largest by three radix passes (11 + 11 + 10 bits) and
-// lists sources and destinations in index order by ballots.  move_kernel
-// copies the listed entries, all (sequence, head) pairs at once.
+// positions once into keys (32 bits that order like the rule above), which stay
+// in LDS up to 32768 tokens, finds the budget-th largest by three radix passes
+// (12 + 10 + 10 bits) and lists sources and destinations in index order by
+// ballots.  move_kernel copies the listed entries, all sequences at once.
 #include "tq_common.h"
 
 namespace tq {
@@ -23,8 +23,12 @@ namespace {
 
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / 64;
-constexpr int kLdsKeys = 32768;
-constexpr int kBins = 2048;
+constexpr int kQuads = 8;  // quads of tokens of a thread and chunk
+constexpr int kChunk = 4 * kQuads * kSelThreads;  // tokens whose keys LDS holds
+// 12 bits first: weights crowd into a few binades, and bins of 1/8 binade keep
+// the lanes of a wave from meeting in one LDS counter
+constexpr int kBins = 4096;
+constexpr uint32_t kList = kBins - 1024;  // keys of one such bin kept aside
 
 struct EvictParams {
   const int32_t* indices;
@@ -37,7 +41,7 @@ struct EvictParams {
   int64_t cap;  // moves per (sequence, head) at most
   float* weights;
   int32_t* positions;
-  uint32_t* keys;  // [Hkv][entries * block_size], for sequences longer than kLdsKeys
+  uint32_t* keys;  // [Hkv][entries * block_size], for sequences longer than kChunk
   int32_t* dst;    // [B * Hkv][cap] entry slots (page * block_size + place, -1: none)
   int32_t* src;
   int32_t* moves;  // [B * Hkv]
@@ -60,28 +64,49 @@ __device__ __forceinline__ int64_t state_at(const EvictParams& p, int slot, int 
   return ((int64_t)pg * p.Hkv + h) * p.block_size + (slot - pg * p.block_size);
 }
 
-// Larger key, kept sooner: 0 no entry, 1 NaN, then the weights in order
-// (-0 as 0), all ones: protected.
-__device__ __forceinline__ uint32_t key_of(const EvictParams& p, int ip, int i, int h,
-                                           int64_t from) {
-  const int slot = slot_of(p, ip, i);
-  if (slot < 0) return 0;
-  const int64_t at = state_at(p, slot, h);
-  const float w = p.weights[at];
-  if (p.positions) {
-    const int pos = p.positions[at];
-    if (pos < p.sink || pos >= from) return 0xffffffffu;
-  }
-  if (w != w) return 1;
-  const uint32_t u = w == 0.f ? 0u : __float_as_uint(w);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+// Larger key, kept sooner: 0 no entry (set elsewhere), 1 NaN, then the weights
+// in order (-0 as 0: kZero), all ones: protected, at a position outside [sink,
+// sink + span).
+constexpr uint32_t kZero = 0x80000000u, kHeld = 0xffffffffu;
+__device__ __forceinline__ uint32_t key_of(float w, int pos, int sink, uint32_t span) {
+  const uint32_t u = __float_as_uint(w + 0.f);  // (-0 + 0 = 0)
+  const uint32_t k = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+  return (uint32_t)pos - (uint32_t)sink >= span ? kHeld : (w != w ? 1u : k);
 }
 
+// inclusive sums over the 64 lanes, by DPP: shifts inside rows of 16, then the
+// rows' totals
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+#define TQ_STEP(CTRL, ROWS) \
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false)
+  TQ_STEP(0x111, 0xf);  // row_shr:1, 2, 4, 8
+  TQ_STEP(0x112, 0xf);
+  TQ_STEP(0x114, 0xf);
+  TQ_STEP(0x118, 0xf);
+  TQ_STEP(0x142, 0xa);  // row_bcast:15 into rows 1 and 3
+  TQ_STEP(0x143, 0xc);  // row_bcast:31 into rows 2 and 3
+#undef TQ_STEP
+  return v;
+}
+
+// base + the lanes before this one in mask
+__device__ __forceinline__ uint32_t lanes_below(uint64_t mask, uint32_t base) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
+                                   __builtin_amdgcn_mbcnt_lo((uint32_t)mask, base));
+}
+
+// (Loops over a chunk's quads stay loops: unrolled, with the keys in registers,
+// the kernel was 42 KB of code, and fetching it cost a small call more than its
+// work.)
 __global__ __launch_bounds__(kSelThreads) void select_kernel(EvictParams p) {
-  __shared__ uint32_t lds_keys[kLdsKeys];
-  __shared__ uint32_t hist[kBins];
-  __shared__ uint32_t tot[2][kSelWaves];
+  __shared__ uint4 keys[kQuads * kSelThreads];
+  __shared__ __attribute__((aligned(16))) uint32_t hist[kBins];
+  uint32_t* const list = hist + 1024;  // (the second and third passes have 1024 bins)
+  __shared__ int tiles[kChunk / kTile];  // entry slots of a chunk's tiles, -1: none
+  __shared__ uint32_t tot[2][kQuads * kSelWaves];
+  __shared__ uint32_t part[kSelWaves];
   __shared__ uint32_t found[3];  // bin, still needed inside it, its count
+  __shared__ uint32_t many[3];   // protected ones, zeros, keys listed
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int b = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv;
@@ -94,148 +119,369 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(EvictParams p) {
     if (tid == 0) p.moves[blockIdx.x] = 0;
     return;
   }
-  const bool in_lds = n <= kLdsKeys;
-  uint32_t* const far = p.keys + (int64_t)h * room + first;
-  auto key = [&](int i) -> uint32_t { return in_lds ? lds_keys[i] : far[i]; };
-  const int64_t from =
-      p.positions && p.ends ? (int64_t)p.ends[b] - p.recent : (int64_t)0x7fffffffffffffff;
-  for (int i = tid; i < n; i += kSelThreads) {  // (n < 2^31 - 2^10: room is)
-    const uint32_t k = key_of(p, ip, i, h, from);
-    if (in_lds)
-      lds_keys[i] = k;
-    else
-      far[i] = k;
+  // free: positions in [sink, ends - recent); none without positions
+  const int sink = p.positions ? p.sink : 0;
+  const int64_t free_to = p.positions ? (int64_t)p.ends[b] - p.recent : 0;
+  const uint32_t span = p.positions ? (uint32_t)max(free_to - sink, (int64_t)0) : 1u;
+  const int chunks = (n + kChunk - 1) / kChunk;  // (n < 2^31 - 2^16: the table's room is)
+  uint4* const far = reinterpret_cast<uint4*>(p.keys + (int64_t)h * room + first);
+
+  // Quad j of thread t is tokens 4 * (t + 1024 j) .. + 3 of a chunk (a quad lies in
+  // one page).  Tokens behind the sequence get key 0, like those without an
+  // entry: they stand behind every other one of that key and are never needed.
+  // run(ch, j): first token of this wave's 256; runs behind the sequence are
+  // left out everywhere.
+  const auto run = [&](int ch, int j) { return ch * kChunk + 4 * (j * kSelThreads + 64 * w); };
+  // a quad's keys, from LDS or, where there are more chunks than one, from the
+  // workspace (a thread reads back what it wrote itself)
+  const auto get = [&](int ch, int j) -> uint4 {
+    if (chunks == 1) return keys[j * kSelThreads + tid];
+    return run(ch, j) + 4 * lane < n ? far[(run(ch, j) >> 2) + lane] : make_uint4(0, 0, 0, 0);
+  };
+  const auto put = [&](int ch, int j, uint4 k) {
+    if (chunks == 1)
+      keys[j * kSelThreads + tid] = k;
+    else if (run(ch, j) + 4 * lane < n)
+      far[(run(ch, j) >> 2) + lane] = k;
+  };
+  // the chunk's tile slots into LDS, one round trip for all of them; slot(): of a
+  // quad's first token
+  const auto load_tiles = [&](int ch) {
+    __syncthreads();
+    for (int t = tid; t < kChunk / kTile && ch * kChunk + t * kTile < n; t += kSelThreads)
+      tiles[t] = slot_of(p, ip, ch * kChunk + t * kTile);
+    __syncthreads();
+  };
+  const auto slot_in = [&](int j) {
+    const int q = j * kSelThreads + tid, s = tiles[q >> 2];
+    return s < 0 ? -1 : s + 4 * (q & 3);
+  };
+  if (tid < 3) many[tid] = 0;
+#pragma unroll 1
+  for (int ch = 0; ch < chunks; ch++) {
+    constexpr int H = 4;  // quads in flight
+    load_tiles(ch);
+#pragma unroll 1
+    for (int j0 = 0; j0 < kQuads && run(ch, j0) < n; j0 += H) {
+      int slot[H];
+      float4 wt[H];
+      int4 ps[H];
+#pragma unroll
+      for (int j = 0; j < H; j++) {
+        const int i = run(ch, j0 + j) + 4 * lane;
+        slot[j] = i < n ? slot_in(j0 + j) : -1;
+      }
+#pragma unroll
+      for (int j = 0; j < H; j++) {
+        const int64_t at = state_at(p, max(slot[j], 0), h);
+        wt[j] = *reinterpret_cast<const float4*>(p.weights + at);
+        ps[j] = p.positions ? *reinterpret_cast<const int4*>(p.positions + at)
+                            : make_int4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < H; j++) {
+        const int left = slot[j] >= 0 ? n - run(ch, j0 + j) - 4 * lane : 0;
+        put(ch, j0 + j,
+            make_uint4(0 < left ? key_of(wt[j].x, ps[j].x, sink, span) : 0u,
+                       1 < left ? key_of(wt[j].y, ps[j].y, sink, span) : 0u,
+                       2 < left ? key_of(wt[j].z, ps[j].z, sink, span) : 0u,
+                       3 < left ? key_of(wt[j].w, ps[j].w, sink, span) : 0u));
+      }
+    }
   }
 
-  // the budget-th largest key, 11 + 11 + 10 bits at a time
+  // The budget-th largest key, 12 + 10 + 10 bits at a time.  Protected ones and
+  // zeros are many: counted in registers, not in one LDS counter each.
   uint32_t need = (uint32_t)p.budget, prefix = 0, equal = 0;
-  int shift = 21;
-#pragma unroll
+  uint32_t listed = 0;  // keys of the first pass's bin in `list`, 0: not listed
+#pragma unroll 1
   for (int pass = 0; pass < 3; pass++) {
-    const int bits = pass == 2 ? 10 : 11;
-    for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+    const int bits = pass == 0 ? 12 : 10, shift = 20 - 10 * pass;
+    const int bins = 1 << bits;
+    for (int i = tid; i < bins / 4; i += kSelThreads)
+      reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    for (int i = tid; i < n; i += kSelThreads) {
-      const uint32_t k = key(i);
-      if (pass == 0 || (k >> (shift + bits)) == prefix)
-        atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+    if (pass == 0) {
+      uint32_t held = 0, zeros = 0;
+#pragma unroll 1
+      for (int ch = 0; ch < chunks; ch++)
+#pragma unroll 1
+        for (int j = 0; j < kQuads && run(ch, j) < n; j++) {
+          const uint4 q = get(ch, j);
+          const uint32_t k[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            held += k[e] == kHeld;
+            zeros += k[e] == kZero;
+            if (k[e] != kHeld && k[e] != kZero) atomicAdd(&hist[k[e] >> 20], 1u);
+          }
+        }
+      held = wave_scan(held);
+      zeros = wave_scan(zeros);
+      if (lane == 63 && held + zeros) {
+        atomicAdd(&hist[kHeld >> 20], held);
+        atomicAdd(&hist[kZero >> 20], zeros);
+        atomicAdd(&many[0], held);
+        atomicAdd(&many[1], zeros);
+      }
+    } else if (listed) {
+      for (uint32_t i = tid; i < listed; i += kSelThreads) {
+        const uint32_t k = list[i];
+        if (k >> (shift + 10) == prefix) atomicAdd(&hist[k >> shift & 1023], 1u);
+      }
+    } else {
+#pragma unroll 1
+      for (int ch = 0; ch < chunks; ch++)
+#pragma unroll 1
+        for (int j = 0; j < kQuads && run(ch, j) < n; j++) {
+          const uint4 q = get(ch, j);
+          const uint32_t k[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (k[e] >> (shift + 10) == prefix) atomicAdd(&hist[k[e] >> shift & 1023], 1u);
+        }
     }
     __syncthreads();
-    // bins from the top, two per thread: the one where the count reaches need
-    const uint32_t c0 = hist[kBins - 1 - 2 * tid], c1 = hist[kBins - 2 - 2 * tid];
-    uint32_t incl = c0 + c1;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t y = __shfl_up(incl, d);
-      if (lane >= d) incl += y;
-    }
-    if (lane == 63) tot[0][w] = incl;
+    // bins from the top, four a thread: the one where the count reaches need
+    const bool mine = tid < bins / 4;
+    const int top = bins - 4 - 4 * tid;  // the lowest of this thread's bins
+    const uint4 hv = *reinterpret_cast<const uint4*>(hist + (mine ? top : 0));
+    const uint32_t c[4] = {mine ? hv.w : 0u, mine ? hv.z : 0u, mine ? hv.y : 0u,
+                           mine ? hv.x : 0u};
+    const uint32_t own = c[0] + c[1] + c[2] + c[3];
+    const uint32_t incl = wave_scan(own);
+    if (lane == 63) part[w] = incl;
     __syncthreads();
-    uint32_t before = incl - c0 - c1;
+    uint32_t before = incl - own;
 #pragma unroll
-    for (int k = 0; k < kSelWaves; k++) before += k < w ? tot[0][k] : 0;
-    if (before < need && need <= before + c0) {
-      found[0] = kBins - 1 - 2 * tid;
-      found[1] = need - before;
-      found[2] = c0;
-    } else if (before + c0 < need && need <= before + c0 + c1) {
-      found[0] = kBins - 2 - 2 * tid;
-      found[1] = need - before - c0;
-      found[2] = c1;
+    for (int k = 0; k < kSelWaves; k++) before += k < w ? part[k] : 0;
+    if (before < need && need <= before + own) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if (before < need && need <= before + c[i]) {
+          found[0] = top + 3 - i;
+          found[1] = need - before;
+          found[2] = c[i];
+        }
+        before += c[i];
+      }
     }
     __syncthreads();
     prefix = (prefix << bits) | found[0];
     need = found[1];
     equal = found[2];
-    shift -= pass == 1 ? 10 : 11;
-    __syncthreads();
+    if (pass == 0) {
+      // the cut is a protected key, or zero with no other key in its bin
+      if (prefix == kHeld >> 20 && need <= many[0]) {
+        prefix = kHeld;
+        equal = many[0];
+        break;
+      }
+      if (prefix == kZero >> 20 && equal == many[1]) {
+        prefix = kZero;
+        break;
+      }
+      // the bin's keys, if they fit the list, so that the other passes need not
+      // look at all of them (in any order: they are only counted)
+      if (equal <= kList) {
+#pragma unroll 1
+        for (int ch = 0; ch < chunks; ch++)
+#pragma unroll 1
+          for (int j = 0; j < kQuads && run(ch, j) < n; j++) {
+            const uint4 q = get(ch, j);
+            const uint32_t k[4] = {q.x, q.y, q.z, q.w};
+            uint32_t m = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) m += k[e] >> 20 == prefix;
+            if (!__any(m)) continue;
+            const uint32_t sum = wave_scan(m);
+            uint32_t at = 0;
+            if (lane == 63) at = atomicAdd(&many[2], sum);
+            at = __builtin_amdgcn_readlane(at, 63) + sum - m;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              if (k[e] >> 20 == prefix) list[at++] = k[e];
+          }
+        listed = equal;
+      }
+    }
   }
   const uint32_t cut = prefix;
 
-  // each wave takes a run of indices, so that ranks are counts of the waves
-  // before plus counts of the lanes below
-  const int seg = ((n + kSelThreads - 1) / kSelThreads) * 64;
-  const int i0 = min(w * seg, n), i1 = min(i0 + seg, n);
-  const uint64_t below = lane ? ~0ull >> (64 - lane) : 0ull;
-  uint32_t eq0 = 0;  // keys equal to the cut before this wave's run
-  if (equal != need) {
-    uint32_t c = 0;
-    for (int i = i0; i < i1; i += 64)
-      c += __popcll(__ballot(i + lane < i1 && key(min(i + lane, n - 1)) == cut));
-    if (lane == 0) tot[0][w] = c;
+  // Kept: keys from the cut on; of those equal to it only the first `need`,
+  // which are made larger than the cut, and the others smaller, if need is not
+  // all of them.  Ranks are counts of the (chunk, j, wave) runs before, and of
+  // the tokens before in the run.
+  // exclusive sums of v[0 .. kQuads * kSelWaves) on top of `base`, by wave 0;
+  // returns the total
+  const auto scan = [&](uint32_t* v, uint32_t base) -> uint32_t {
     __syncthreads();
-    for (int k = 0; k < w; k++) eq0 += tot[0][k];
+    if (w == 0) {
+      const uint32_t a0 = v[2 * lane], a1 = v[2 * lane + 1];
+      const uint32_t incl = wave_scan(a0 + a1);
+      v[2 * lane] = base + incl - a0 - a1;
+      v[2 * lane + 1] = base + incl - a1;
+      if (lane == 63) part[0] = base + incl;
+    }
     __syncthreads();
-  }
-  // kept: above the cut, or one of the first `need` equal to it
-  auto kept = [&](int i, uint32_t& eq) -> bool {
-    const bool in = i + lane < i1;
-    const uint32_t k = in ? key(i + lane) : 0u;
-    bool keep = in && k > cut;
-    const uint64_t same = __ballot(in && k == cut);
-    if (in && k == cut) keep = eq + __popcll(same & below) < need;
-    eq += __popcll(same);
-    return keep;
+    return part[0];
   };
-  uint32_t holes = 0, more = 0, eq = eq0;
-  for (int i = i0; i < i1; i += 64) {
-    const bool keep = kept(i, eq), in = i + lane < i1, front = i + lane < p.budget;
-    holes += __popcll(__ballot(in && !keep && front));
-    more += __popcll(__ballot(in && keep && !front));
-  }
-  if (lane == 0) {
-    tot[0][w] = holes;
-    tot[1][w] = more;
-  }
-  __syncthreads();
-  uint32_t hole0 = 0, more0 = 0;
-  for (int k = 0; k < w; k++) {
-    hole0 += tot[0][k];
-    more0 += tot[1][k];
-  }
+  static_assert(kQuads * kSelWaves == 128, "scan() takes two counts a lane");
   int32_t* const dst = p.dst + (int64_t)blockIdx.x * p.cap;
   int32_t* const src = p.src + (int64_t)blockIdx.x * p.cap;
-  eq = eq0;
-  for (int i = i0; i < i1; i += 64) {
-    const bool keep = kept(i, eq), in = i + lane < i1, front = i + lane < p.budget;
-    const uint64_t hm = __ballot(in && !keep && front), mm = __ballot(in && keep && !front);
-    if (in && !keep && front) dst[hole0 + __popcll(hm & below)] = slot_of(p, ip, i + lane);
-    if (in && keep && !front) src[more0 + __popcll(mm & below)] = slot_of(p, ip, i + lane);
-    hole0 += __popcll(hm);
-    more0 += __popcll(mm);
+  const bool ties = equal != need;
+  const uint32_t from = ties && cut != kHeld ? cut + 1 : cut;  // kept: keys >= from
+  uint32_t eq_base = 0, hole_base = 0, more_base = 0;
+#pragma unroll 1
+  for (int ch = 0; ch < chunks; ch++) {
+    if (ties) {
+#pragma unroll 1
+      for (int j = 0; j < kQuads; j++) {
+        uint32_t c = 0;
+        if (run(ch, j) < n) {
+          const uint4 q = get(ch, j);
+          const uint32_t k[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int e = 0; e < 4; e++) c += __popcll(__ballot(k[e] == cut));
+        }
+        if (lane == 0) tot[0][j * kSelWaves + w] = c;
+      }
+      const uint32_t next = scan(tot[0], eq_base);
+#pragma unroll 1
+      for (int j = 0; j < kQuads && run(ch, j) < n; j++) {
+        const uint4 q = get(ch, j);
+        uint32_t k[4] = {q.x, q.y, q.z, q.w};
+        uint32_t rank = tot[0][j * kSelWaves + w];
+#pragma unroll
+        for (int e = 0; e < 4; e++) rank = lanes_below(__ballot(k[e] == cut), rank);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const bool same = k[e] == cut;
+          k[e] = same ? (rank < need ? kHeld : 0u) : k[e];
+          rank += same;
+        }
+        put(ch, j, make_uint4(k[0], k[1], k[2], k[3]));
+      }
+      eq_base = next;
+      __syncthreads();  // tot[0] is read
+    }
+    // holes in front of the budget, kept ones behind it
+#pragma unroll 1
+    for (int j = 0; j < kQuads; j++) {
+      const int i0 = run(ch, j), i = i0 + 4 * lane;
+      uint32_t a = 0, c = 0;
+      if (i0 < n) {
+        const uint4 q = get(ch, j);
+        const uint32_t k[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const uint64_t in = __ballot(k[e] >= from), front = __ballot(i + e < p.budget);
+          a += __popcll(~in & front);
+          c += __popcll(in & ~front);
+        }
+      }
+      if (lane == 0) {
+        tot[0][j * kSelWaves + w] = a;
+        tot[1][j * kSelWaves + w] = c;
+      }
+    }
+    const uint32_t hole_next = scan(tot[0], hole_base);
+    const uint32_t more_next = scan(tot[1], more_base);
+    if (chunks > 1) load_tiles(ch);  // (no loads below: they would wait for the stores)
+#pragma unroll 1
+    for (int j = 0; j < kQuads && run(ch, j) < n; j++) {
+      const int i = run(ch, j) + 4 * lane, slot = i < n ? slot_in(j) : -1;
+      const uint4 q = get(ch, j);
+      const uint32_t k[4] = {q.x, q.y, q.z, q.w};
+      // (both sides only in the run that the budget falls into)
+#pragma unroll 1
+      for (int back = 0; back < 2; back++) {
+        if (back ? run(ch, j) + 256 <= p.budget : run(ch, j) >= p.budget) continue;  // (uniform)
+        int32_t* const to = back ? src : dst;
+        uint32_t rank = tot[back][j * kSelWaves + w];
+        bool mark[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          mark[e] = (k[e] >= from) == (bool)back && (i + e >= p.budget) == (bool)back;
+          rank = lanes_below(__ballot(mark[e]), rank);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (mark[e]) to[rank++] = slot < 0 ? -1 : slot + e;
+      }
+    }
+    hole_base = hole_next;
+    more_base = more_next;
+    __syncthreads();  // tot is read
   }
   // exactly budget entries are kept, so there are as many holes as sources
-  if (w == kSelWaves - 1 && lane == 0) p.moves[blockIdx.x] = (int32_t)more0;
+  if (tid == 0) p.moves[blockIdx.x] = (int32_t)more_base;
 }
 
-// Entry moves: each takes 2 EBS / 16 lanes for the codes and norms of K and V
-// and one for weight and position.
+// Entry moves: a move takes 2 EBS / 16 lanes for the codes and norms of K and V
+// and one for weight and position.  A workgroup takes runs of move numbers for
+// up to eight heads of a sequence: the i-th holes of the heads lie close
+// together, and so do the pieces of cache lines that they share.
+constexpr int kMoveHeads = 8;
 template <int EBS>
 __global__ __launch_bounds__(256) void move_kernel(EvictParams p) {
-  constexpr int E = EBS / 16, C = 2 * E + 1;
-  const int bh = blockIdx.y, h = bh % p.Hkv;
-  if (h == 0 && blockIdx.x == 0 && threadIdx.x == 0) {
-    const int b = bh / p.Hkv;
+  constexpr int E = EBS / 16, C = 2 * E + 1, NI = 4, PAIRS = 256 * NI / C;
+  __shared__ int to_s[PAIRS], of_s[PAIRS];
+  const int groups = (p.Hkv + kMoveHeads - 1) / kMoveHeads;
+  const int b = blockIdx.y / groups, h0 = blockIdx.y % groups * kMoveHeads;
+  const int heads = min(kMoveHeads, p.Hkv - h0);
+  if (h0 == 0 && blockIdx.x == 0 && threadIdx.x == 0)
     p.new_lens[b] = min(p.seq_lens[b], p.budget);
-  }
-  const int64_t items = (int64_t)p.moves[bh] * C;
-  const int32_t* const dst = p.dst + bh * p.cap;
-  const int32_t* const src = p.src + bh * p.cap;
-  for (int64_t f = (int64_t)blockIdx.x * 256 + threadIdx.x; f < items;
-       f += (int64_t)gridDim.x * 256) {
-    const int64_t m = f / C;
-    const int c = (int)(f - m * C);
-    const int to = dst[m], of = src[m];
-    if (to < 0 || of < 0) continue;  // on no page of the cache
-    if (c < 2 * E) {
-      uint8_t* const slab = c < E ? p.ks : p.vs;
-      const int o = (c < E ? c : c - E) * 16;
-      *reinterpret_cast<uint4*>(slab + ((int64_t)to * p.Hkv + h) * EBS + o) =
-          *reinterpret_cast<const uint4*>(slab + ((int64_t)of * p.Hkv + h) * EBS + o);
-    } else {
-      const int64_t a = state_at(p, to, h), z = state_at(p, of, h);
-      p.weights[a] = p.weights[z];
-      if (p.positions) p.positions[a] = p.positions[z];
+  const int32_t* const moves = p.moves + b * p.Hkv + h0;
+  int most = 0;
+#pragma unroll
+  for (int i = 0; i < kMoveHeads; i++) most = max(most, moves[min(i, heads - 1)]);
+  const int per = PAIRS / heads, pairs = per * heads;  // move numbers a round
+  for (int64_t m0 = (int64_t)blockIdx.x * per; m0 < most; m0 += (int64_t)gridDim.x * per) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < pairs; i += 256) {
+      const int h = i % heads;
+      const int64_t m = m0 + i / heads;
+      const int64_t at = (int64_t)(b * p.Hkv + h0 + h) * p.cap + m;
+      const bool ok = m < moves[h];
+      const int to = ok ? p.dst[at] : -1, of = ok ? p.src[at] : -1;
+      to_s[i] = to >= 0 && of >= 0 ? to : -1;  // none, or on no page of the cache
+      of_s[i] = of;
+    }
+    __syncthreads();
+    uint4 v[NI];
+    int64_t at[NI];
+    int c[NI];
+#pragma unroll
+    for (int j = 0; j < NI; j++) {
+      const int f = threadIdx.x + 256 * j, i = f / C;
+      c[j] = f - i * C;
+      const int to = i < pairs ? to_s[i] : -1;
+      if (to < 0) {
+        c[j] = C;
+        continue;
+      }
+      const int of = of_s[i], h = h0 + i % heads;
+      if (c[j] < 2 * E) {
+        const int o = (c[j] < E ? c[j] : c[j] - E) * 16;
+        const uint8_t* const slab = c[j] < E ? p.ks : p.vs;
+        at[j] = ((int64_t)to * p.Hkv + h) * EBS + o;
+        v[j] = *reinterpret_cast<const uint4*>(slab + ((int64_t)of * p.Hkv + h) * EBS + o);
+      } else {
+        const int64_t z = state_at(p, of, h);
+        at[j] = state_at(p, to, h);
+        v[j].x = __float_as_uint(p.weights[z]);
+        v[j].y = p.positions ? (uint32_t)p.positions[z] : 0u;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NI; j++) {
+      if (c[j] < 2 * E) {
+        *reinterpret_cast<uint4*>((c[j] < E ? p.ks : p.vs) + at[j]) = v[j];
+      } else if (c[j] == 2 * E) {
+        p.weights[at[j]] = __uint_as_float(v[j].x);
+        if (p.positions) p.positions[at[j]] = (int32_t)v[j].y;
+      }
     }
   }
 }
@@ -259,7 +505,7 @@ EvictWs evict_ws(int batch, int hkv, int64_t entries, int bs, int budget) {
   w.dst = take((size_t)batch * hkv * w.cap * 4);
   w.src = take((size_t)batch * hkv * w.cap * 4);
   w.moves = take((size_t)batch * hkv * 4);
-  w.keys = take(room > kLdsKeys ? (size_t)room * hkv * 4 : 0);
+  w.keys = take(room > kChunk ? (size_t)room * hkv * 4 : 0);
   w.total = at;
   return w;
 }
@@ -330,8 +576,9 @@ extern "C" int tq_evict_paged(uint8_t* k_slab, uint8_t* v_slab, float* weights, 
     set_error("evict: null pointer");
     return kEinval;
   }
-  if ((uintptr_t)k_slab % 16 || (uintptr_t)v_slab % 16) {
-    set_error("evict: cache slabs must be 16-byte aligned");
+  if ((uintptr_t)k_slab % 16 || (uintptr_t)v_slab % 16 || (uintptr_t)weights % 16 ||
+      (uintptr_t)positions % 16) {
+    set_error("evict: cache slabs, weights and positions must be 16-byte aligned");
     return kEinval;
   }
   const EvictWs ws = evict_ws(batch, num_kv_heads, num_indices, block_size, budget);
@@ -358,7 +605,7 @@ extern "C" int tq_evict_paged(uint8_t* k_slab, uint8_t* v_slab, float* weights, 
   p.cap = ws.cap;
   p.weights = weights;
   p.positions = positions;
-  p.keys = num_indices * block_size > kLdsKeys ? reinterpret_cast<uint32_t*>(base + ws.keys)
+  p.keys = num_indices * block_size > kChunk ? reinterpret_cast<uint32_t*>(base + ws.keys)
                                                : nullptr;
   p.dst = reinterpret_cast<int32_t*>(base + ws.dst);
   p.src = reinterpret_cast<int32_t*>(base + ws.src);
@@ -371,13 +618,14 @@ extern "C" int tq_evict_paged(uint8_t* k_slab, uint8_t* v_slab, float* weights, 
   hipLaunchKernelGGL(select_kernel, dim3((unsigned)bh), dim3(kSelThreads), 0, st, p);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess) {
-    // up to four items a thread, and no more workgroups than keep the GPU busy
-    const int64_t c = 2 * ebs / 16 + 1;
-    int64_t gx = (ws.cap * c + 1023) / 1024;
-    gx = gx < 1 ? 1 : gx;
-    const int64_t most = 4096 / bh > 1 ? 4096 / bh : 1;
-    gx = gx < most ? gx : most;
-    const dim3 grid((unsigned)gx, (unsigned)bh);
+    // one round each, and no more workgroups than keep the GPU busy
+    const int64_t y = (int64_t)batch * ((num_kv_heads + kMoveHeads - 1) / kMoveHeads);
+    const int per = 1024 / (2 * ebs / 16 + 1) /
+                    (num_kv_heads < kMoveHeads ? num_kv_heads : kMoveHeads);
+    int64_t gx = (ws.cap + per - 1) / per;
+    const int64_t most = 4096 / y > 1 ? 4096 / y : 1;
+    gx = gx < 1 ? 1 : (gx < most ? gx : most);
+    const dim3 grid((unsigned)gx, (unsigned)y);
     if (ebs == 48)
       hipLaunchKernelGGL(move_kernel<48>, grid, dim3(256), 0, st, p);
     else if (ebs == 80)

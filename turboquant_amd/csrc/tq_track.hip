@@ -242,12 +242,15 @@ __device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp
 // pair of dims twice: with hi and lo parts in operands of their own each entry
 // would cost two moves.
 __device__ __forceinline__ void init_key_table(uint64_t* lut) {
-  for (int e = threadIdx.x; e < 4096; e += blockDim.x) {
-    const int byte = e >> 4;
-    const float a = level(byte >> 4) * kLevelScale, b = level(byte & 15) * kLevelScale;
-    const float ah = (float)(_Float16)a, bh = (float)(_Float16)b;
-    lut[e] = pack_half(ah, bh) | (uint64_t)pack_half(a - ah, b - bh) << 32;
-  }
+  // a byte's copies are shared by blockDim.x / 256 threads, two copies a store
+  const int per = 16 * 256 / blockDim.x, byte = threadIdx.x * 256 / blockDim.x;
+  const float a = level(byte >> 4) * kLevelScale, b = level(byte & 15) * kLevelScale;
+  const float ah = (float)(_Float16)a, bh = (float)(_Float16)b;
+  const uint32_t hi = pack_half(ah, bh), lo = pack_half(a - ah, b - bh);
+  u32x4* const to = reinterpret_cast<u32x4*>(lut + threadIdx.x * per);
+#pragma unroll
+  for (int i = 0; i < 16; i += 2)
+    if (i < per) to[i / 2] = u32x4{hi, lo, hi, lo};
 }
 // the two operands of 8 codes; lanec = 8 * (lane mod 16)
 __device__ __forceinline__ void key_operands(uint32_t c, const uint64_t* lut, uint32_t lanec,
@@ -728,9 +731,13 @@ void track_values_kernel(TrackParams p) {
   }
   const float inv = real && den != 0.f ? 1.0f / den : 0.f;
   if (!real) M = INFINITY;  // lanes of no head: probabilities of zero
-  for (int e = threadIdx.x; e < 8192; e += kThreads) {
-    const int byte = e >> 5;
-    sm.lut[e] = pack_half(level(byte & 15) * kValueScale, level(byte >> 4) * kValueScale);
+  {
+    const int byte = threadIdx.x >> 1;  // two threads a byte, four copies a store
+    const uint32_t e =
+        pack_half(level(byte & 15) * kValueScale, level(byte >> 4) * kValueScale);
+    u32x4* const to = reinterpret_cast<u32x4*>(sm.lut + threadIdx.x * 16);
+#pragma unroll
+    for (int i = 0; i < 4; i++) to[i] = u32x4{e, e, e, e};
   }
   lds_written();
 
