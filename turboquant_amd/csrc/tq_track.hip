@@ -81,10 +81,9 @@ struct TrackParams {
   float csc;  // score constant (log2 units)
   float osc;  // output constant
   float* s;   // scores, log2 units [table tile][Hkv][ratio][16]
-  float2* stats;  // (max, sum) [Hkv][stat_rows][rp]
-  int64_t stat_rows;
+  float2* stats;  // (max, sum) [Hkv][units][rp]
   int32_t* split;
-  float* po;  // partial outputs [unit * SUB + sub][Hq][PD]
+  float* po;  // partial outputs [unit][Hq][PD]
   float* weights;
   int32_t* positions;
   const int32_t* ends;
@@ -234,6 +233,12 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b) {
 }
 
 __device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
+// x times the fp16 value in the low half of n.  Not the assembly of
+// mul_lo_half: its operands here come straight from an MFMA or an exp2, whose
+// wait states the compiler counts for its own instructions only.
+__device__ __forceinline__ float by_half(float x, uint32_t n) {
+  return __builtin_fmaf(x, lo_half(n), 0.f);
+}
 
 // The key table: code byte -> fp16 hi parts of its two levels (high nibble
 // first, as the dims go) in the low dword, their lo parts in the high one,
@@ -386,13 +391,19 @@ __device__ __forceinline__ void load_row(const void* q, int64_t off, bool bf16, 
     x[k] = d < hd ? f : 0.f;
   }
 }
-// ... and rotated: FWHT(s x)/sqrt(pd); without signs as it is
+// this lane's rotation signs (1 without them)
 template <int E>
-__device__ __forceinline__ void rotate_row(const float* signs, float* x) {
-  if (!signs) return;
+__device__ __forceinline__ void load_signs(const float* signs, float* s) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
-  for (int k = 0; k < E; k++) x[k] *= signs[lane * E + k];
+  for (int k = 0; k < E; k++) s[k] = signs ? signs[lane * E + k] : 1.f;
+}
+// ... and rotated: FWHT(s x)/sqrt(pd); without signs (rotate false) as it is
+template <int E>
+__device__ __forceinline__ void rotate_row(bool rotate, const float* s, float* x) {
+  if (!rotate) return;
+#pragma unroll
+  for (int k = 0; k < E; k++) x[k] *= s[k];
   fwht_wave<E>(x);
   const float isq = 1.0f / sqrtf((float)(64 * E));
 #pragma unroll
@@ -413,7 +424,8 @@ __device__ __forceinline__ int row_exponent(float mx) {
 // tiles a step): lanes n < 8 take on the scores of the first tile and n >= 8
 // those of the second, which halves the work per score.
 template <int PD, int G, bool QC>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4)))
+__global__ __launch_bounds__(kThreads)
+__attribute__((amdgpu_waves_per_eu(PD == 256 && !QC ? 2 : 4)))
 void track_scores_kernel(TrackParams p) {
   using R = Rows<PD, G>;
   constexpr int KB = PD / 32;
@@ -445,7 +457,10 @@ void track_scores_kernel(TrackParams p) {
   const int rows = G * p.ratio;
   float* const rot = reinterpret_cast<float*>(sm.lut);
   const int64_t q_at = (int64_t)ps.b * p.q_sb + (int64_t)hg * rows * p.q_sh;
-  float x0[NB][E];
+  // (every load of the prologue goes out in front of the copies: a later one
+  // would wait for them)
+  float x0[NB][E], sg[E];
+  load_signs<E>(p.signs, sg);
 #pragma unroll
   for (int i = 0; i < NB; i++)
     load_row<E>(p.q, q_at + min(w + kWaves * i, rows - 1) * p.q_sh, p.q_bf16, p.hd, x0[i]);
@@ -461,7 +476,7 @@ void track_scores_kernel(TrackParams p) {
     for (int i = 0; i < NB; i++) {
       const int r = r0 + kWaves * i;
       if (r >= rows) break;
-      rotate_row<E>(p.signs, x0[i]);
+      rotate_row<E>(p.signs != nullptr, sg, x0[i]);
 #pragma unroll
       for (int k = 0; k < E; k++) {
         const int d = lane * E + k;
@@ -583,7 +598,7 @@ void track_scores_kernel(TrackParams p) {
       uint32_t nv[4];
       spread_norms(nr[i], nv);
 #pragma unroll
-      for (int r = 0; r < 4; r++) x[r] = mul_lo_half(x[r], nv[r]) * csc;
+      for (int r = 0; r < 4; r++) x[r] = by_half(x[r], nv[r]) * csc;
       // all tokens of the tiles are there (uniform); else masks
       const int tl = PACK ? t0 + R::SUB : t0;  // the last tile
       const int p0 = st.place(t0), p1 = PACK ? st.place(tl) : p0;
@@ -606,8 +621,21 @@ void track_scores_kernel(TrackParams p) {
   if constexpr (PACK) join_stats(ror8(m), ror8(l), m, l);
   join_stats(__shfl_xor(m, 16), __shfl_xor(l, 16), m, l);
   join_stats(__shfl_xor(m, 32), __shfl_xor(l, 32), m, l);
-  if (lane < p.rp)
-    p.stats[((int64_t)kvh * p.stat_rows + (int64_t)(ps.Pb + ps.j) * R::SUB + sub) * p.rp + lane] =
+  if constexpr (R::SUB > 1) {  // the waves of a head, in LDS that nobody reads any more
+    float2* const all = reinterpret_cast<float2*>(sm.ring);
+    barrier();
+    if (lane < 16) all[w * 16 + lane] = make_float2(m, l);
+    lds_written();
+    barrier();
+    if (sub == 0)
+#pragma unroll
+      for (int i = 1; i < R::SUB; i++) {
+        const float2 o = all[(w + i * G) * 16 + (lane & 15)];
+        join_stats(o.x, o.y, m, l);
+      }
+  }
+  if (sub == 0 && lane < p.rp)
+    p.stats[((int64_t)kvh * p.units + ps.Pb + ps.j) * p.rp + lane] =
         lane < p.ratio ? make_float2(m, l) : make_float2(kNone, 0.f);
 }
 
@@ -710,25 +738,28 @@ void track_values_kernel(TrackParams p) {
   const int c0 = ps.j * ps.U, c1 = min(c0 + ps.U, ps.L);
   Stream<PD, G> st(p, ps, c0, c1, w, hg);
   const int steps = (st.tiles + R::TPS - 1) / R::TPS;
-  uint8_t* const spare = sm.ring + 2 * R::SLOT;
-  st.issue(0, sm.ring, spare);
-  st.issue(1, sm.ring + R::SLOT, spare);
   const int kvh = hg * G + w % G, sub = w / G;
   const int head = QC ? n & 7 : n;
   const bool real = head < p.ratio;
 
-  // the maximum and the sum of this lane's head over the sequence
+  // the maximum and the sum of this lane's head over the sequence (the loads go
+  // out in front of the copies, up to NP of them: a later one waits for the
+  // copies)
+  constexpr int NP = 8;
   float M = kNone, den = 0.f;
-  {
-    const int64_t rows = (int64_t)((ps.L + ps.U - 1) / ps.U) * R::SUB;
-    const float2* src = p.stats + ((int64_t)kvh * p.stat_rows + (int64_t)ps.Pb * R::SUB) * p.rp;
-#pragma unroll 4
-    for (int64_t i = lane; i < rows * p.rp; i += 64) {
-      const float2 x = src[i];
-      join_stats(x.x, x.y, M, den);
-    }
-    for (int d = p.rp; d < 64; d <<= 1) join_stats(__shfl_xor(M, d), __shfl_xor(den, d), M, den);
-  }
+  const int parts = (ps.L + ps.U - 1) / ps.U * p.rp;
+  const float2* const src = p.stats + ((int64_t)kvh * p.units + ps.Pb) * p.rp;
+  float2 part[NP];
+#pragma unroll
+  for (int i = 0; i < NP; i++) part[i] = src[min(lane + 64 * i, parts - 1)];
+  uint8_t* const spare = sm.ring + 2 * R::SLOT;
+  st.issue(0, sm.ring, spare);
+  st.issue(1, sm.ring + R::SLOT, spare);
+#pragma unroll
+  for (int i = 0; i < NP; i++)
+    if (lane + 64 * i < parts) join_stats(part[i].x, part[i].y, M, den);
+  for (int i = lane + 64 * NP; i < parts; i += 64) join_stats(src[i].x, src[i].y, M, den);
+  for (int d = p.rp; d < 64; d <<= 1) join_stats(__shfl_xor(M, d), __shfl_xor(den, d), M, den);
   const float inv = real && den != 0.f ? 1.0f / den : 0.f;
   if (!real) M = INFINITY;  // lanes of no head: probabilities of zero
   {
@@ -816,7 +847,7 @@ void track_values_kernel(TrackParams p) {
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         rel[r] = exp2_raw(cu.sc[i][r] - M);
-        x[r] = mul_lo_half(rel[r], nv[r]);
+        x[r] = by_half(rel[r], nv[r]);
       }
       // tiles with tokens that are not there, or with the newest one (uniform)
       const int first = (st.tile0 + t0 + mine) * kTile + 4 * q4;
@@ -928,23 +959,37 @@ void track_values_kernel(TrackParams p) {
       p.positions[((int64_t)pg * p.Hkv + kvh) * p.block_size + t % p.block_size] =
           p.ends[ps.b] - 1;
   }
-  float* const row =
-      p.po + (((int64_t)(ps.Pb + ps.j) * R::SUB + sub) * p.Hq + kvh * p.ratio + n) * PD;
-  const float osc = inv * p.osc;
+  if constexpr (QC) {  // hi and lo columns
 #pragma unroll
-  for (int r = 0; r < 4; r++) {
-    float y[NO];
+    for (int i = 0; i < NO; i++)
 #pragma unroll
-    for (int i = 0; i < NO; i++) {
-      y[i] = O[i][r];
-      if constexpr (QC) y[i] += ror8(y[i]);
-      y[i] *= osc;
-    }
-    if (n < p.ratio)
+      for (int r = 0; r < 4; r++) O[i][r] += ror8(O[i][r]);
+  }
+  // the waves of a head meet in LDS, halving their number each time
+#pragma unroll
+  for (int half = R::SUB / 2; half > 0; half /= 2) {
+    float4_t* const buf = reinterpret_cast<float4_t*>(&sm) + lane;
+    static_assert(kWaves / 2 * NO * 1024 <= sizeof(Lds), "half the waves' outputs fit");
+    barrier();
+    if (sub >= half && sub < 2 * half)
+#pragma unroll
+      for (int i = 0; i < NO; i++) buf[((w - half * G) * NO + i) * 64] = O[i];
+    lds_written();
+    barrier();
+    if (sub < half)
+#pragma unroll
+      for (int i = 0; i < NO; i++) O[i] += buf[(w * NO + i) * 64];
+    lds_written();
+  }
+  if (sub == 0 && n < p.ratio) {
+    float* const row = p.po + ((int64_t)(ps.Pb + ps.j) * p.Hq + kvh * p.ratio + n) * PD;
+    const float osc = inv * p.osc;
+#pragma unroll
+    for (int r = 0; r < 4; r++)
 #pragma unroll
       for (int i = 0; i < NO; i += 4)
         *reinterpret_cast<float4_t*>(row + (4 * q4 + r) * NO + i) =
-            float4_t{y[i], y[i + 1], y[i + 2], y[i + 3]};
+            float4_t{O[i][r], O[i + 1][r], O[i + 2][r], O[i + 3][r]} * osc;
   }
 }
 
@@ -954,9 +999,10 @@ template <int PD>
 __device__ __forceinline__ float split_row(const void* q, int64_t off, bool bf16, int hd,
                                            const float* signs, _Float16* hi, _Float16* lo) {
   constexpr int E = PD / 64;
-  float x[E];
+  float x[E], sg[E];
   load_row<E>(q, off, bf16, hd, x);
-  rotate_row<E>(signs, x);
+  load_signs<E>(signs, sg);
+  rotate_row<E>(signs != nullptr, sg, x);
   float mx = 0.f;
 #pragma unroll
   for (int k = 0; k < E; k++) mx = fmaxf(mx, fabsf(x[k]));
@@ -977,14 +1023,14 @@ __device__ __forceinline__ float split_row(const void* q, int64_t off, bool bf16
 template <int PD>
 __global__ __launch_bounds__(256) void track_join_kernel(const float* __restrict__ po,
                                                          const int32_t* __restrict__ split,
-                                                         int sub, int Hq, int hd, int bf16,
+                                                         int Hq, int hd, int bf16,
                                                          const float* __restrict__ signs,
                                                          void* __restrict__ o) {
   constexpr int E = PD / 64;
   __shared__ float part[3][PD];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int b = blockIdx.x / Hq, h = blockIdx.x % Hq;
-  const int r0 = split[b] * sub, r1 = split[b + 1] * sub;
+  const int r0 = split[b], r1 = split[b + 1];
   float x[E];
 #pragma unroll
   for (int k = 0; k < E; k++) x[k] = 0.f;
@@ -1253,8 +1299,8 @@ void window_kernel(WindowParams p) {
       for (int m = 0; m < MT; m++)
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-          acc[m][i] = mul_lo_half(acc[m][i], kn[m][i / 2]);
-          acc[m][i + 1] = mul_lo_half(acc[m][i + 1], kn[m][i / 2] >> 16);
+          acc[m][i] = by_half(acc[m][i], kn[m][i / 2]);
+          acc[m][i + 1] = by_half(acc[m][i + 1], kn[m][i / 2] >> 16);
         }
       if constexpr (SUM) {
         if (clear) {
@@ -1450,7 +1496,7 @@ int track_units(int batch, int pd, int g, int hg, bool qc) {
 struct TrackWs {
   size_t stats, split, s, po, total;
 };
-TrackWs track_ws(int batch, int64_t entries, int hq, int hkv, int pd, int bs, int units, int sub) {
+TrackWs track_ws(int batch, int64_t entries, int hq, int hkv, int pd, int bs, int units) {
   const int ratio = hq / hkv;
   int rp = 1;
   while (rp < ratio) rp <<= 1;
@@ -1461,11 +1507,11 @@ TrackWs track_ws(int batch, int64_t entries, int hq, int hkv, int pd, int bs, in
     at += up256(n);
     return r;
   };
-  w.stats = take((size_t)hkv * units * sub * rp * 8);
+  w.stats = take((size_t)hkv * units * rp * 8);
   w.split = take((size_t)(batch + 2) * 4);
   // (a tile at least: tiles outside the table read the first one)
   w.s = take((size_t)max(entries, (int64_t)1) * bs * hq * 4);
-  w.po = take((size_t)units * sub * hq * pd * 4);
+  w.po = take((size_t)units * hq * pd * 4);
   w.total = at;
   return w;
 }
@@ -1549,7 +1595,7 @@ extern "C" int64_t tq_decode_tracked_workspace_bytes(int32_t batch, int64_t num_
     return kEinval;
   }
   return (int64_t)track_ws(batch, num_indices, num_qo_heads, num_kv_heads, padded_dim, block_size,
-                           units, kWaves / g)
+                           units)
       .total;
 }
 
@@ -1575,7 +1621,7 @@ extern "C" int tq_decode_paged_tracked(
     return kEinval;
   }
   const int pd = padded_dim, ratio = num_qo_heads / num_kv_heads;
-  const int g = group_of(pd, num_kv_heads, ratio), sub = kWaves / g;
+  const int g = group_of(pd, num_kv_heads, ratio);
   const bool qc = ratio <= 8;
   const int units = track_units(batch, pd, g, num_kv_heads / g, qc);
   if (units <= 0) {
@@ -1583,7 +1629,7 @@ extern "C" int tq_decode_paged_tracked(
     return kEinval;
   }
   const TrackWs ws =
-      track_ws(batch, num_indices, num_qo_heads, num_kv_heads, pd, block_size, units, sub);
+      track_ws(batch, num_indices, num_qo_heads, num_kv_heads, pd, block_size, units);
   if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < (int64_t)ws.total) {
     set_error("%s: the workspace must be 16-byte aligned and hold %lld bytes, got %lld", who,
               (long long)ws.total, (long long)workspace_bytes);
@@ -1617,7 +1663,6 @@ extern "C" int tq_decode_paged_tracked(
   p.osc = isq / kValueScale;
   p.s = reinterpret_cast<float*>(base + ws.s);
   p.stats = reinterpret_cast<float2*>(base + ws.stats);
-  p.stat_rows = (int64_t)units * sub;
   p.split = reinterpret_cast<int32_t*>(base + ws.split);
   p.po = reinterpret_cast<float*>(base + ws.po);
   p.weights = weights;
@@ -1633,10 +1678,10 @@ extern "C" int tq_decode_paged_tracked(
               (int64_t)units * p.HG, kThreads, targs, stream);
   if (rc) return rc;
   {
-    int ob = o_dtype == TQ_BF16, sb = sub;
+    int ob = o_dtype == TQ_BF16;
     const float* po = p.po;
     const int32_t* split = p.split;
-    void* args[] = {&po, &split, &sb, &hq, &hd, &ob, &signs, &o};
+    void* args[] = {&po, &split, &hq, &hd, &ob, &signs, &o};
     const void* fn = pd == 64    ? reinterpret_cast<const void*>(&track_join_kernel<64>)
                      : pd == 128 ? reinterpret_cast<const void*>(&track_join_kernel<128>)
                                  : reinterpret_cast<const void*>(&track_join_kernel<256>);
