@@ -74,6 +74,8 @@ struct TrackParams {
   const int32_t* seq_lens;
   int64_t entries;  // of the page table
   int num_blocks, B, Hq, Hkv, ratio, rp, block_size, HG, units;
+  int pair;       // see share_of
+  int rows;       // parts of the plan at most: units, or twice as many
   const void* q;
   int64_t q_sb, q_sh;
   int q_bf16, hd;
@@ -81,24 +83,25 @@ struct TrackParams {
   float csc;  // score constant (log2 units)
   float osc;  // output constant
   float* s;   // scores, log2 units [table tile][Hkv][ratio][16]
-  float2* stats;  // (max, sum) [Hkv][units][rp]
+  float2* stats;  // (max, sum) [Hkv][rows][rp]
   int32_t* split;
-  float* po;  // partial outputs [unit][Hq][PD]
+  float* po;  // partial outputs [rows][Hq][PD]
   float* weights;
   int32_t* positions;
   const int32_t* ends;
 };
 
-// The unit that workgroup `u` serves (plan_slot of tq_plan.h); st: at least
-// 8 KB of LDS, free again afterwards.
+// The unit that workgroup `u` serves (plan_slot of tq_plan.h), `per` parts a
+// unit; st: at least 8 KB of LDS, free again afterwards.
 template <int A, typename Params>
-__device__ __forceinline__ PlanSlot unit_of(const Params& p, int* st, int u, bool writer) {
+__device__ __forceinline__ PlanSlot unit_of(const Params& p, int* st, int u, int per,
+                                            bool writer) {
   const int lane = threadIdx.x & 63;
   if (p.B <= 64) {
     const bool in = lane < p.B;
     const int len = in ? max(p.seq_lens[lane], 0) : 0;
     const int ip = in ? p.indptr[lane] : 0;
-    return plan_slot<A>([&](int) { return len; }, [&](int) { return ip; }, p.B, 1, p.units, u, 1,
+    return plan_slot<A>([&](int) { return len; }, [&](int) { return ip; }, p.B, 1, p.units, u, per,
                         p.split, writer);
   }
   for (int i = threadIdx.x; i < kPlanMost; i += blockDim.x) {
@@ -109,9 +112,41 @@ __device__ __forceinline__ PlanSlot unit_of(const Params& p, int* st, int u, boo
   const PlanSlot r =
       plan_slot<A>([&](int i) { return st[64 * i + lane]; },
                    [&](int i) { return st[kPlanMost + 64 * i + lane]; }, p.B, (p.B + 63) >> 6,
-                   p.units, u, 1, p.split, writer);
+                   p.units, u, per, p.split, writer);
   __syncthreads();
   return r;
+}
+
+// What a workgroup of the two streaming kernels serves: tokens [c0, c1) of the
+// unit's sequence, for head group hg, as part `row` of the plan's.
+//
+// pair > 0: the grid is two workgroups a CU, and blocks u and u + grid / 2, which
+// the dispatcher puts on one CU, share a unit: the one that came first gets
+// `pair` percent of its tokens (rounded up to a tile).  Its waves are older and
+// win the arbitration, so of two equal shares the second finished 10 of 42 us
+// later at 8 x 32768 tokens, alone on its CU.
+struct Share {
+  PlanSlot ps;
+  int c0, c1, hg, row;
+};
+__device__ __forceinline__ Share share_of(const TrackParams& p, int* st, bool writer) {
+  const int half = gridDim.x >> 1;
+  const int second = p.pair > 0 && (int)blockIdx.x >= half;
+  const int bid = blockIdx.x - second * half, per = p.pair > 0 ? 2 : 1;
+  Share s;
+  s.hg = bid % p.HG;
+  s.ps = unit_of<kPlanAlign>(p, st, bid / p.HG, per, writer);
+  s.c0 = s.ps.j * s.ps.U;
+  s.c1 = s.c0 + s.ps.U;
+  if (p.pair > 0) {
+    const int cut = s.c0 + min((s.ps.U * p.pair / 100 + 15) & ~15, s.ps.U);
+    s.c0 = second ? cut : s.c0;
+    s.c1 = second ? s.c1 : cut;
+  }
+  s.c0 = min(s.c0, s.ps.L);
+  s.c1 = min(s.c1, s.ps.L);
+  s.row = per * (s.ps.Pb + s.ps.j) + second;
+  return s;
 }
 
 // A unit's tiles: where each lies, and the copies of a step.  Lane i of a
@@ -439,15 +474,18 @@ void track_scores_kernel(TrackParams p) {
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int q4 = lane >> 4, n = lane & 15;
-  const int hg = blockIdx.x % p.HG;
-  const PlanSlot ps = unit_of<kPlanAlign>(p, reinterpret_cast<int*>(sm.lut), blockIdx.x / p.HG,
-                                          blockIdx.x == 0 && w == 0);
+  const Share sh = share_of(p, reinterpret_cast<int*>(sm.lut), blockIdx.x == 0 && w == 0);
+  const PlanSlot& ps = sh.ps;
   if (ps.b < 0) return;
-  const int c0 = ps.j * ps.U, c1 = min(c0 + ps.U, ps.L);
+  const int c0 = sh.c0, c1 = sh.c1, hg = sh.hg;
+  const int kvh = hg * G + w % G, sub = w / G;
+  if (c0 >= c1) {  // a short unit's second share (uniform)
+    if (sub == 0 && lane < p.rp)
+      p.stats[((int64_t)kvh * p.rows + sh.row) * p.rp + lane] = make_float2(kNone, 0.f);
+    return;
+  }
   Stream<PD, G> st(p, ps, c0, c1, w, hg);
   const int steps = (st.tiles + R::TPS - 1) / R::TPS;
-
-  const int kvh = hg * G + w % G, sub = w / G;
   const int head = QC ? n & 7 : n;
   // q' of the workgroup's heads: each wave rotates every eighth row into LDS
   // (where the table goes later), fp32 with the 16-byte pieces of a row in an
@@ -635,7 +673,7 @@ void track_scores_kernel(TrackParams p) {
       }
   }
   if (sub == 0 && lane < p.rp)
-    p.stats[((int64_t)kvh * p.units + ps.Pb + ps.j) * p.rp + lane] =
+    p.stats[((int64_t)kvh * p.rows + sh.row) * p.rp + lane] =
         lane < p.ratio ? make_float2(m, l) : make_float2(kNone, 0.f);
 }
 
@@ -731,14 +769,18 @@ void track_values_kernel(TrackParams p) {
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int q4 = lane >> 4, n = lane & 15;
-  const int hg = blockIdx.x % p.HG;
-  const PlanSlot ps =
-      unit_of<kPlanAlign>(p, reinterpret_cast<int*>(sm.lut), blockIdx.x / p.HG, false);
+  const Share sh = share_of(p, reinterpret_cast<int*>(sm.lut), false);
+  const PlanSlot& ps = sh.ps;
   if (ps.b < 0) return;
-  const int c0 = ps.j * ps.U, c1 = min(c0 + ps.U, ps.L);
+  const int c0 = sh.c0, c1 = sh.c1, hg = sh.hg;
+  const int kvh = hg * G + w % G, sub = w / G;
+  if (c0 >= c1) {  // (as above: a row of zeros)
+    float* const row = p.po + ((int64_t)sh.row * p.Hq + hg * G * p.ratio) * PD;
+    for (int i = threadIdx.x; i < G * p.ratio * PD; i += kThreads) row[i] = 0.f;
+    return;
+  }
   Stream<PD, G> st(p, ps, c0, c1, w, hg);
   const int steps = (st.tiles + R::TPS - 1) / R::TPS;
-  const int kvh = hg * G + w % G, sub = w / G;
   const int head = QC ? n & 7 : n;
   const bool real = head < p.ratio;
 
@@ -747,8 +789,9 @@ void track_values_kernel(TrackParams p) {
   // copies)
   constexpr int NP = 8;
   float M = kNone, den = 0.f;
-  const int parts = (ps.L + ps.U - 1) / ps.U * p.rp;
-  const float2* const src = p.stats + ((int64_t)kvh * p.units + ps.Pb) * p.rp;
+  const int per = p.pair > 0 ? 2 : 1;
+  const int parts = (ps.L + ps.U - 1) / ps.U * per * p.rp;
+  const float2* const src = p.stats + ((int64_t)kvh * p.rows + per * ps.Pb) * p.rp;
   float2 part[NP];
 #pragma unroll
   for (int i = 0; i < NP; i++) part[i] = src[min(lane + 64 * i, parts - 1)];
@@ -982,7 +1025,7 @@ void track_values_kernel(TrackParams p) {
     lds_written();
   }
   if (sub == 0 && n < p.ratio) {
-    float* const row = p.po + ((int64_t)(ps.Pb + ps.j) * p.Hq + kvh * p.ratio + n) * PD;
+    float* const row = p.po + ((int64_t)sh.row * p.Hq + kvh * p.ratio + n) * PD;
     const float osc = inv * p.osc;
 #pragma unroll
     for (int r = 0; r < 4; r++)
@@ -1181,7 +1224,7 @@ void window_kernel(WindowParams p) {
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kvh = blockIdx.x / p.units, u = blockIdx.x % p.units;
-  const PlanSlot ps = unit_of<TOK>(p, reinterpret_cast<int*>(sm.lut), u,
+  const PlanSlot ps = unit_of<TOK>(p, reinterpret_cast<int*>(sm.lut), u, 1,
                                    !SUM && blockIdx.x == 0 && w == 0);
   if (ps.b < 0) return;
   const int q_len = p.q_start[ps.b + 1] - p.q_start[ps.b];
@@ -1483,20 +1526,36 @@ TrackFn track_fn(int pd, int g, bool qc) {
 #undef TQ_ONE
 }
 
-// work units of a tracked decode: the workgroups that the scores kernel keeps
-// resident, at least one per sequence
-int track_units(int batch, int pd, int g, int hg, bool qc) {
+// Work units of a tracked decode: the workgroups that the scores kernel keeps
+// resident, at least one per sequence; in pairs where that is two a CU.
+struct TrackPlan {
+  int units, pair, rows;
+  int64_t blocks;
+};
+constexpr int kPairShare = 62;
+TrackPlan track_plan(int batch, int pd, int g, int hg, bool qc) {
   const Occupancy occ =
       occupancy(reinterpret_cast<const void*>(track_fn<false>(pd, g, qc)), kThreads);
-  if (occ.cus <= 0 || occ.per_cu <= 0) return 0;
-  return max(batch, occ.cus * occ.per_cu / hg);
+  TrackPlan t = {0, 0, 0, 0};
+  if (occ.cus <= 0 || occ.per_cu <= 0) return t;
+  t.units = max(batch, occ.cus * occ.per_cu / hg);
+  t.rows = t.units;
+  // (not at head size 64, where the shares finish together: 32.1 + 26.6 us
+  // unpaired, 32.6 + 27.6 paired, 48 ragged sequences)
+  if (pd > 64 && occ.per_cu == 2 && occ.cus % hg == 0 && occ.cus / hg >= batch) {
+    t.units = occ.cus / hg;
+    t.pair = kPairShare;
+    t.rows = 2 * t.units;
+  }
+  t.blocks = (int64_t)t.rows * hg;
+  return t;
 }
 
 // A tracked decode's workspace
 struct TrackWs {
   size_t stats, split, s, po, total;
 };
-TrackWs track_ws(int batch, int64_t entries, int hq, int hkv, int pd, int bs, int units) {
+TrackWs track_ws(int batch, int64_t entries, int hq, int hkv, int pd, int bs, int parts) {
   const int ratio = hq / hkv;
   int rp = 1;
   while (rp < ratio) rp <<= 1;
@@ -1507,11 +1566,11 @@ TrackWs track_ws(int batch, int64_t entries, int hq, int hkv, int pd, int bs, in
     at += up256(n);
     return r;
   };
-  w.stats = take((size_t)hkv * units * rp * 8);
+  w.stats = take((size_t)hkv * parts * rp * 8);
   w.split = take((size_t)(batch + 2) * 4);
   // (a tile at least: tiles outside the table read the first one)
   w.s = take((size_t)max(entries, (int64_t)1) * bs * hq * 4);
-  w.po = take((size_t)units * hq * pd * 4);
+  w.po = take((size_t)parts * hq * pd * 4);
   w.total = at;
   return w;
 }
@@ -1589,13 +1648,13 @@ extern "C" int64_t tq_decode_tracked_workspace_bytes(int32_t batch, int64_t num_
   if (rc) return rc;
   if (batch == 0) return 0;
   const int ratio = num_qo_heads / num_kv_heads, g = group_of(padded_dim, num_kv_heads, ratio);
-  const int units = track_units(batch, padded_dim, g, num_kv_heads / g, ratio <= 8);
-  if (units <= 0) {
+  const TrackPlan plan = track_plan(batch, padded_dim, g, num_kv_heads / g, ratio <= 8);
+  if (plan.units <= 0) {
     set_error("decode_tracked: occupancy query failed");
     return kEinval;
   }
   return (int64_t)track_ws(batch, num_indices, num_qo_heads, num_kv_heads, padded_dim, block_size,
-                           units)
+                           plan.rows)
       .total;
 }
 
@@ -1623,13 +1682,13 @@ extern "C" int tq_decode_paged_tracked(
   const int pd = padded_dim, ratio = num_qo_heads / num_kv_heads;
   const int g = group_of(pd, num_kv_heads, ratio);
   const bool qc = ratio <= 8;
-  const int units = track_units(batch, pd, g, num_kv_heads / g, qc);
-  if (units <= 0) {
+  const TrackPlan plan = track_plan(batch, pd, g, num_kv_heads / g, qc);
+  if (plan.units <= 0) {
     set_error("%s: occupancy query failed", who);
     return kEinval;
   }
   const TrackWs ws =
-      track_ws(batch, num_indices, num_qo_heads, num_kv_heads, pd, block_size, units);
+      track_ws(batch, num_indices, num_qo_heads, num_kv_heads, pd, block_size, plan.rows);
   if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < (int64_t)ws.total) {
     set_error("%s: the workspace must be 16-byte aligned and hold %lld bytes, got %lld", who,
               (long long)ws.total, (long long)workspace_bytes);
@@ -1651,7 +1710,9 @@ extern "C" int tq_decode_paged_tracked(
   while (p.rp < ratio) p.rp <<= 1;
   p.block_size = block_size;
   p.HG = num_kv_heads / g;
-  p.units = units;
+  p.units = plan.units;
+  p.pair = plan.pair;
+  p.rows = plan.rows;
   p.q = q;
   p.q_sb = q_stride_b;
   p.q_sh = q_stride_h;
@@ -1671,11 +1732,11 @@ extern "C" int tq_decode_paged_tracked(
   int hq = num_qo_heads, hd = head_dim;
   void* targs[] = {&p};
   rc = launch(who, reinterpret_cast<const void*>(track_fn<false>(pd, g, qc)),
-              (int64_t)units * p.HG, kThreads, targs, stream);
+              plan.blocks, kThreads, targs, stream);
   if (rc) return rc;
   p.slab = v_slab;
   rc = launch(who, reinterpret_cast<const void*>(track_fn<true>(pd, g, qc)),
-              (int64_t)units * p.HG, kThreads, targs, stream);
+              plan.blocks, kThreads, targs, stream);
   if (rc) return rc;
   {
     int ob = o_dtype == TQ_BF16;
