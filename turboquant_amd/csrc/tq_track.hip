@@ -1205,7 +1205,7 @@ __device__ __forceinline__ void read_operands(uint32_t at, half8_t* f) {
 // tiles together: a tile's operands (PD * 128 bytes) come into LDS one ahead
 // of their use, by direct-to-LDS copies that the four waves share.
 template <int PD, int MT, bool SUM>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PD == 256 ? 2 : 3)))
 void window_kernel(WindowParams p) {
   constexpr int KS = PD / 16;
   constexpr int EBS = Rows<PD, 1>::EBS;
@@ -1217,7 +1217,7 @@ void window_kernel(WindowParams p) {
       uint64_t lut[4096];
       uint8_t q[2][QT];
     };
-    float2 wave[SUM ? 1 : 4][32];    // a row tile's (max, sum) of each wave
+    float2 wave[SUM ? 1 : 2][SUM ? 1 : 4][32];  // a row tile's (max, sum) of each wave
     float2 rows[SUM ? 1 : 1024];     // running (max, sum) of the unit
   };
   __shared__ Lds sm;
@@ -1264,6 +1264,7 @@ void window_kernel(WindowParams p) {
     uint32_t kn[MT][8];
     uint32_t okm[MT];
     int64_t place[MT];  // index of this lane's token in weights, -1: none
+    float old[MT];      // and its weight
 #pragma unroll
     for (int m = 0; m < MT; m++) {
       const int t = t0 + 32 * m + col;
@@ -1279,6 +1280,7 @@ void window_kernel(WindowParams p) {
         }
       }
       okm[m] = (uint32_t)__ballot(place[m] >= 0);
+      if constexpr (SUM) old[m] = p.weights[max(place[m], (int64_t)0)];
       const uint32_t* src = reinterpret_cast<const uint32_t*>(p.slab + at + half * (PD / 4));
       const uint32_t norm = *reinterpret_cast<const uint32_t*>(p.slab + at + PD / 2) & 0xffffu;
       uint32_t c[KS];
@@ -1306,15 +1308,35 @@ void window_kernel(WindowParams p) {
 #pragma unroll
     for (int m = 0; m < MT; m++) all = all && okm[m] == 0xffffffffu;
     __syncthreads();  // the table is no longer read
+    // a row tile's scale and normaliser, one tile ahead and in front of the copies
+    float next_q = qs[col], next_l = SUM ? lse[col] : 0.f;
     issue(0);
+    // the waves' statistics of tile rt, joined by one of them; tile rt + 1 has
+    // buffers of its own, so the barrier of each tile is enough
+    auto join_tile = [&](int rt) {
+      if (w == (rt & 3) && half == 0) {
+        float2 a = sm.rows[rt * 32 + col];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const float2 b = sm.wave[rt & 1][k][col];
+          join_stats(b.x, b.y, a.x, a.y);
+        }
+        sm.rows[rt * 32 + col] = a;
+      }
+    };
 
     for (int rt = 0; rt < p.tiles; rt++) {
       __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
       barrier();  // tile rt is there, and nobody reads the other buffer
-      if (rt + 1 < p.tiles) issue(rt + 1);
       const int row = rt * 32 + col;
-      const float cq = qs[row] * p.csc;
-      const float ls = SUM ? lse[row] : 0.f;
+      const float cq = next_q * p.csc, ls = next_l;
+      if (rt + 1 < p.tiles) {
+        next_q = qs[row + 32];
+        if constexpr (SUM) next_l = lse[row + 32];
+        issue(rt + 1);
+      }
+      if constexpr (!SUM)
+        if (rt) join_tile(rt - 1);
       float16_t acc[MT];
 #pragma unroll
       for (int m = 0; m < MT; m++)
@@ -1326,18 +1348,26 @@ void window_kernel(WindowParams p) {
         half8_t f[4];
         read_operands(at + k * 2048, f);
 #pragma unroll
-        for (int y = 0; y < 2; y++)
+        for (int z = 0; z < 3; z++)  // hi hi, lo hi, hi lo
 #pragma unroll
-          for (int m = 0; m < MT; m++) {
-            acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[m][k + y], f[2 * y], acc[m], 0, 0, 0);
-            acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl[m][k + y], f[2 * y], acc[m], 0, 0, 0);
-            acc[m] =
-                __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[m][k + y], f[2 * y + 1], acc[m], 0, 0, 0);
-          }
+          for (int y = 0; y < 2; y++)
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+              acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                  z == 1 ? kl[m][k + y] : kh[m][k + y], f[2 * y + (z == 2)], acc[m], 0, 0, 0);
       }
-      // the last token that this row's query sees; the tile's first row sees least
-      const int see = ps.L - p.window + row / p.ratio;
+      // Tokens that this row's query sees: the tile's first row sees least.  Bit c of
+      // seen(m): the token of accumulator row c (+ 4 in the upper half) is there and
+      // seen; made anew for each tile, as masks kept over the loop spill.
       const bool clear = all && t0 + 32 * MT - 1 <= ps.L - p.window + rt * 32 / p.ratio;
+      auto seen = [&](int m) {
+        uint32_t ok = okm[m];
+#if defined(__HIP_DEVICE_COMPILE__)
+        asm volatile("" : "+s"(ok));
+#endif
+        const int last = ps.L - p.window + row / p.ratio - (t0 + 32 * m);
+        return (ok & (last < 0 ? 0u : 0xffffffffu >> (31 - min(last, 31)))) >> (4 * half);
+      };
 #pragma unroll
       for (int m = 0; m < MT; m++)
 #pragma unroll
@@ -1346,60 +1376,56 @@ void window_kernel(WindowParams p) {
           acc[m][i + 1] = by_half(acc[m][i + 1], kn[m][i / 2] >> 16);
         }
       if constexpr (SUM) {
-        if (clear) {
-#pragma unroll
-          for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) got[m][i] += exp2_raw(fmaf(acc[m][i], cq, -ls));
-        } else {
-#pragma unroll
-          for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-              const int t = t0 + 32 * m + 8 * (i / 4) + 4 * half + i % 4;
-              got[m][i] += t <= see ? exp2_raw(fmaf(acc[m][i], cq, -ls)) : 0.f;
-            }
-        }
-      } else {
-        float mx = kNone, l = 0.f;
         if (!clear) {
 #pragma unroll
-          for (int m = 0; m < MT; m++)
+          for (int m = 0; m < MT; m++) {
+            const uint32_t bits = seen(m);
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-              const int tr = 8 * (i / 4) + 4 * half + i % 4;
-              const bool ok = ((okm[m] >> tr) & 1) && t0 + 32 * m + tr <= see;
-              acc[m][i] = ok ? acc[m][i] * cq : -INFINITY;
-              mx = vmax(mx, acc[m][i]);
-            }
+            for (int i = 0; i < 16; i++)
+              acc[m][i] = bits & (1u << (8 * (i / 4) + i % 4)) ? fmaf(acc[m][i], cq, -ls)
+                                                              : -INFINITY;
+          }
         } else {
 #pragma unroll
           for (int m = 0; m < MT; m++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-              acc[m][i] *= cq;
-              mx = vmax(mx, acc[m][i]);
-            }
+            for (int i = 0; i < 16; i++) acc[m][i] = fmaf(acc[m][i], cq, -ls);
         }
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) got[m][i] += exp2_raw(acc[m][i]);
+      } else {
+        float mx = kNone, l = 0.f;
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) acc[m][i] *= cq;
+        if (!clear) {
+#pragma unroll
+          for (int m = 0; m < MT; m++) {
+            const uint32_t bits = seen(m);
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+              acc[m][i] = bits & (1u << (8 * (i / 4) + i % 4)) ? acc[m][i] : -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) mx = vmax3(mx, acc[m][i], acc[m][i + 1]);
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
           for (int i = 0; i < 16; i++) l += exp2_raw(acc[m][i] - mx);
         join_stats(__shfl_xor(mx, 32), __shfl_xor(l, 32), mx, l);
-        if (half == 0) sm.wave[w][col] = make_float2(mx, l);
+        if (half == 0) sm.wave[rt & 1][w][col] = make_float2(mx, l);
         lds_written();
-        barrier();
-        if (w == 0 && half == 0) {
-          float2 a = sm.rows[row];
-#pragma unroll
-          for (int k = 0; k < 4; k++) {
-            const float2 b = sm.wave[k][col];
-            join_stats(b.x, b.y, a.x, a.y);
-          }
-          sm.rows[row] = a;
-          lds_written();
-        }
       }
+    }
+    if constexpr (!SUM) {
+      barrier();
+      join_tile(p.tiles - 1);
     }
     if constexpr (SUM) {
 #pragma unroll
@@ -1421,7 +1447,7 @@ void window_kernel(WindowParams p) {
         if (half == 0 && place[m] >= 0) {
           const int t = t0 + 32 * m + col;
           if (t < ps.L - q_len) {
-            p.weights[place[m]] += mine;
+            p.weights[place[m]] = old[m] + mine;
           } else {
             p.weights[place[m]] = mine;
             if (p.positions) p.positions[place[m]] = p.ends[ps.b] - ps.L + t;
@@ -1757,12 +1783,12 @@ struct WindowWs {
   size_t qf, qs, stats, lse, split, total;
   int tiles, units;
 };
-// units of a window call: two workgroups a CU over the kv heads, at least one
+// units of a window call: three workgroups a CU over the kv heads, at least one
 // per sequence
 WindowWs window_ws(int batch, int window, int ratio, int hkv, int pd, int cus) {
   WindowWs w;
   w.tiles = (window * ratio + 31) / 32;
-  w.units = max(batch, 2 * cus / hkv);
+  w.units = max(batch, 3 * cus / hkv);
   size_t at = 0;
   auto take = [&](size_t n) {
     const size_t r = at;
@@ -1875,12 +1901,12 @@ extern "C" int tq_track_window(const void* q, int64_t num_rows, int64_t q_stride
   const void *fr, *f0, *f1;
   if (pd == 64) {
     fr = reinterpret_cast<const void*>(&rotate_window_kernel<64>);
-    f0 = reinterpret_cast<const void*>(&window_kernel<64, 2, false>);
-    f1 = reinterpret_cast<const void*>(&window_kernel<64, 2, true>);
+    f0 = reinterpret_cast<const void*>(&window_kernel<64, 1, false>);
+    f1 = reinterpret_cast<const void*>(&window_kernel<64, 1, true>);
   } else if (pd == 128) {
     fr = reinterpret_cast<const void*>(&rotate_window_kernel<128>);
-    f0 = reinterpret_cast<const void*>(&window_kernel<128, 2, false>);
-    f1 = reinterpret_cast<const void*>(&window_kernel<128, 2, true>);
+    f0 = reinterpret_cast<const void*>(&window_kernel<128, 1, false>);
+    f1 = reinterpret_cast<const void*>(&window_kernel<128, 1, true>);
   } else {
     fr = reinterpret_cast<const void*>(&rotate_window_kernel<256>);
     f0 = reinterpret_cast<const void*>(&window_kernel<256, 1, false>);
