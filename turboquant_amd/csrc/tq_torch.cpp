@@ -157,6 +157,120 @@ bool decode_balanced(const Tensor& q, const Tensor& kv_cache, const Tensor& indi
                                   o.data_ptr(), st) == 0;
 }
 
+// --------------------------------------------------------------- cache budget
+
+// weights fp32 and positions int32 (or none, and ends with them) beside the cache
+bool record_of(const Tensor& weights, const OptTensor& positions, const OptTensor& ends,
+               const Cache& c, int64_t batch, c10::Device dev) {
+  const auto beside = [&](const Tensor& t) {
+    return t.dim() == 3 && t.size(0) == c.num_blocks && t.size(1) == c.heads &&
+           t.size(2) == c.block_size;
+  };
+  if (!is_f32(weights, dev) || !beside(weights)) return false;
+  if (ends.has_value() && !on(*ends, dev)) return false;
+  if (!positions.has_value()) return true;
+  return is_i32(*positions, dev) && beside(*positions) && ends.has_value() &&
+         is_i32(*ends, dev) && ends->numel() >= batch;
+}
+int32_t* opt_i32(const OptTensor& t) { return t.has_value() ? t->data_ptr<int32_t>() : nullptr; }
+
+// ops.decode_paged_tracked
+bool decode_tracked(const Tensor& q, const Tensor& kv_cache, const Tensor& indices,
+                    const Tensor& indptr, const Tensor& seq_lens, int64_t num_kv_heads,
+                    int64_t head_dim, int64_t padded_dim, double sm_scale, const OptTensor& signs,
+                    const Tensor& o, const Tensor& weights, const OptTensor& positions,
+                    const OptTensor& ends) {
+  const c10::Device dev = q.device();
+  Cache c;
+  const float* sp = nullptr;
+  const int qt = dtype_code(q.scalar_type()), ot = dtype_code(o.scalar_type());
+  if (!on(q, dev) || q.dim() != 3 || q.size(2) != head_dim || q.stride(2) != 1 || !is_half(qt) ||
+      !on(o, dev) || !is_half(ot) || !o.is_contiguous() || o.sizes() != q.sizes() ||
+      !is_i32(indices, dev) || !is_i32(indptr, dev) || !is_i32(seq_lens, dev) ||
+      !cache_of(kv_cache, dev, c) || c.heads != num_kv_heads ||
+      !signs_of(signs, padded_dim, dev, sp))
+    return false;
+  const int64_t b = q.size(0), hq = q.size(1);
+  if (b == 0 || seq_lens.numel() < b || indptr.numel() < b ||
+      !record_of(weights, positions, ends, c, b, dev))
+    return false;
+  const c10::DeviceGuard guard(dev);
+  const int64_t bytes = tq_decode_tracked_workspace_bytes(b, indices.numel(), hq, num_kv_heads,
+                                                          padded_dim, c.block_size);
+  if (bytes <= 0) return false;
+  const Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  if (!on(ws, dev)) return false;
+  return tq_decode_paged_tracked(
+             q.const_data_ptr(), q.stride(0), q.stride(1), qt, c.k, c.v, cptr<int32_t>(indices),
+             indices.numel(), cptr<int32_t>(indptr), cptr<int32_t>(seq_lens), b, hq, num_kv_heads,
+             head_dim, padded_dim, c.block_size, c.ebs, c.num_blocks, (float)sm_scale, sp,
+             o.data_ptr(), ot, weights.data_ptr<float>(), opt_i32(positions), opt_i32(ends),
+             ws.data_ptr(), bytes, stream_of(dev)) == 0;
+}
+
+// ops.track_window
+bool track_window(const Tensor& q, const Tensor& starts, int64_t window, const Tensor& kv_cache,
+                  const Tensor& indices, const Tensor& indptr, const Tensor& seq_lens,
+                  int64_t num_kv_heads, int64_t head_dim, int64_t padded_dim, double sm_scale,
+                  const OptTensor& signs, const Tensor& weights, const OptTensor& positions,
+                  const OptTensor& ends) {
+  const c10::Device dev = q.device();
+  Cache c;
+  const float* sp = nullptr;
+  const int qt = dtype_code(q.scalar_type());
+  if (!on(q, dev) || q.dim() != 3 || q.size(2) != head_dim || q.stride(2) != 1 || !is_half(qt) ||
+      q.size(0) == 0 || !is_i32(starts, dev) || starts.numel() < 2 || !is_i32(indices, dev) ||
+      !is_i32(indptr, dev) || !is_i32(seq_lens, dev) || !cache_of(kv_cache, dev, c) ||
+      c.heads != num_kv_heads || window < 1 || window > 1024 ||
+      !signs_of(signs, padded_dim, dev, sp))
+    return false;
+  const int64_t b = starts.numel() - 1, hq = q.size(1);
+  if (seq_lens.numel() < b || indptr.numel() < b ||
+      !record_of(weights, positions, ends, c, b, dev))
+    return false;
+  const c10::DeviceGuard guard(dev);
+  const int64_t bytes = tq_track_window_workspace_bytes(b, window, hq, num_kv_heads, padded_dim);
+  if (bytes <= 0) return false;
+  const Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  if (!on(ws, dev)) return false;
+  return tq_track_window(q.const_data_ptr(), q.size(0), q.stride(0), q.stride(1), qt,
+                         cptr<int32_t>(starts), window, c.k, cptr<int32_t>(indices),
+                         indices.numel(), cptr<int32_t>(indptr), cptr<int32_t>(seq_lens), b, hq,
+                         num_kv_heads, head_dim, padded_dim, c.block_size, c.ebs, c.num_blocks,
+                         (float)sm_scale, sp, weights.data_ptr<float>(), opt_i32(positions),
+                         opt_i32(ends), ws.data_ptr(), bytes, stream_of(dev)) == 0;
+}
+
+// ops.evict_paged
+bool evict(const Tensor& kv_cache, const Tensor& weights, const OptTensor& positions,
+           const Tensor& indices, const Tensor& indptr, const Tensor& seq_lens,
+           const OptTensor& ends, int64_t budget, int64_t recent, int64_t sink,
+           const Tensor& new_lens) {
+  const c10::Device dev = kv_cache.device();
+  Cache c;
+  if (!cache_of(kv_cache, dev, c) || !is_i32(indices, dev) || !is_i32(indptr, dev) ||
+      !is_i32(seq_lens, dev) || !is_i32(new_lens, dev))
+    return false;
+  const int64_t b = seq_lens.numel();
+  const int64_t pd = c.ebs == 48 ? 64 : c.ebs == 80 ? 128 : c.ebs == 144 ? 256 : 0;
+  if (b == 0 || pd == 0 || indptr.numel() < b || new_lens.numel() < b || budget < 1 ||
+      budget > INT32_MAX || recent < 0 || recent > budget || sink < 0 || sink > budget ||
+      !record_of(weights, positions, ends, c, b, dev))
+    return false;
+  const c10::DeviceGuard guard(dev);
+  const int64_t bytes =
+      tq_evict_workspace_bytes(b, c.heads, indices.numel(), c.block_size, budget);
+  if (bytes <= 0) return false;
+  const Tensor ws = at::empty({bytes}, kv_cache.options().dtype(at::kByte));
+  if (!on(ws, dev)) return false;
+  return tq_evict_paged(const_cast<uint8_t*>(c.k), const_cast<uint8_t*>(c.v),
+                        weights.data_ptr<float>(), opt_i32(positions), cptr<int32_t>(indices),
+                        indices.numel(), cptr<int32_t>(indptr), cptr<int32_t>(seq_lens),
+                        opt_i32(ends), b, c.heads, pd, c.block_size, c.ebs, c.num_blocks, budget,
+                        recent, sink, new_lens.data_ptr<int32_t>(), ws.data_ptr(), bytes,
+                        stream_of(dev)) == 0;
+}
+
 // -------------------------------------------------------------------- prefill
 
 using Request = std::array<int32_t, 5>;
@@ -509,6 +623,9 @@ PYBIND11_MODULE(_tq_torch, m) {
   const auto unlocked = py::call_guard<py::gil_scoped_release>();
   m.def("write_cache", &write_cache, unlocked);
   m.def("decode_balanced", &decode_balanced, unlocked);
+  m.def("decode_tracked", &decode_tracked, unlocked);
+  m.def("track_window", &track_window, unlocked);
+  m.def("evict", &evict, unlocked);
   m.def("prefill_batch", &prefill_batch, unlocked);
   m.def("prefill_gather", &prefill_gather, unlocked);
   m.def("mse_quantize", &mse_quantize, unlocked);

@@ -945,6 +945,10 @@ def decode_paged_tracked(q: torch.Tensor, kv_cache: torch.Tensor, indices: torch
     [B] counts the tokens each sequence has seen, evicted ones included.
     Sequences must not share pages.  tq_decode_paged_tracked; equal inputs give
     equal bits."""
+    if (_nat or _native()).decode_tracked(q, kv_cache, indices, indptr, seq_lens, num_kv_heads,
+                                          head_dim, padded_dim, sm_scale, signs, o, weights,
+                                          positions, ends):
+        return o
     what = "decode_paged_tracked"
     _require_gpu(q, kv_cache, indices, indptr, seq_lens, o, weights,
                  *(t for t in (positions, ends) if t is not None))
@@ -987,6 +991,10 @@ def track_window(q: torch.Tensor, query_start_loc: torch.Tensor, window: int,
     are observed, each over the tokens up to its own.  Weights of tokens cached
     before the chunk are added to, the chunk's own are set, with their
     positions.  window * Hq / H <= 1024.  tq_track_window."""
+    if (_nat or _native()).track_window(q, query_start_loc, window, kv_cache, indices, indptr,
+                                        seq_lens, num_kv_heads, head_dim, padded_dim, sm_scale,
+                                        signs, weights, positions, ends):
+        return
     what = "track_window"
     _require_gpu(q, query_start_loc, kv_cache, indices, indptr, seq_lens, weights,
                  *(t for t in (positions, ends) if t is not None))
@@ -1027,6 +1035,9 @@ def evict_paged(kv_cache: torch.Tensor, weights: torch.Tensor, positions: torch.
     order; nothing else is written.  new_lens int32 [B] (may be seq_lens) =
     min(seq_lens, budget).  positions and ends may be None if recent = sink =
     0.  Sequences must not share pages.  tq_evict_paged."""
+    if (_nat or _native()).evict(kv_cache, weights, positions, indices, indptr, seq_lens, ends,
+                                 budget, recent, sink, new_lens):
+        return new_lens
     what = "evict_paged"
     _require_gpu(kv_cache, weights, indices, indptr, seq_lens, new_lens,
                  *(t for t in (positions, ends) if t is not None))
