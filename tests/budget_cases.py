@@ -158,21 +158,3 @@ def evict(c, budget, recent, sink):
             for slab in cache:
                 slab[pg[to], off[to], h] = slab[pg[of], off[of], h]
     return cache, acc, pos, np.minimum(c.lens, budget).astype(np.int32)
-
-
-def scores_error(c, q):
-    """Bound on a score's absolute error (natural units) from the kernel's
-    arithmetic: operands of 22 bits on both sides, fp32 sums of pd terms, and a
-    score in log2 units rounded to fp32 a few times.  Used with the largest
-    |q'| |K^| that the case can have (Cauchy-Schwarz)."""
-    qn = np.sqrt((q.astype(np.float64) ** 2).sum(-1)).max()
-    kn = 0.0
-    norm = c.cache[0, ..., c.pd // 2:c.pd // 2 + 2].copy().view(np.float16).astype(np.float64)
-    finite = np.isfinite(norm)
-    if finite.any():
-        kn = np.abs(norm[finite]).max() * 2.7326368
-    # each operand off by at most 2^-22 of its row's largest element (hi + lo),
-    # sums of up to 4 pd products in fp32 with errors of 2^-24 each against the
-    # partial sums, eight roundings of the scaled score, and exp2 / log2 of it
-    u = 2.0 ** -24
-    return qn * kn * c.scale * (8 * u + 4 * u * math.sqrt(c.pd) + 8 * u)

@@ -411,3 +411,308 @@ def test_evict_in_place_lengths_and_graph():
             assert torch.equal(t[k], want[k]), k
     cache, acc, pos, lens = C.evict(c, 120, 20, 4)
     assert np.array_equal(want["cache"].cpu().numpy(), cache)
+
+
+# ------------------------------------------------------------------ together
+
+@pytest.mark.parametrize("hq,hkv,hd,page,dtype", [(8, 2, 128, 16, "fp16"), (6, 3, 80, 32, "bf16"),
+                                                  (16, 2, 256, 16, "bf16"), (8, 8, 64, 48, "fp16")])
+def test_prompt_then_cut_then_decode(hq, hkv, hd, page, dtype):
+    """As a server uses them: prompts written and observed, cut to the budget,
+    then decode steps that write, attend and record, with a cut every few of
+    them; each call against its 64-bit form from the state that it found."""
+    from turboquant_amd.budget import CacheRecord
+    prompt, budget, steps, every = [150, 61, 1], 64, 13, 5
+    c = C.make(41, [p + steps for p in prompt], hq, hkv, hd, page=page, packed=False)
+    width = len(c.indices) // 3
+    table = dev(c.indices.reshape(3, width))
+    c.cache[:] = 0
+    cache = dev(c.cache)
+    signs = dev(c.signs)
+    rec = CacheRecord.beside(cache, budget, recent=9, sink=3, window=7)
+    rec.weights.fill_(float("nan"))  # whatever was there before
+    c.weights[:], c.positions[:] = np.nan, 0
+    pd, lens, seen = c.pd, np.array(prompt, np.int32), np.array(prompt, np.int32)
+    args = (hkv, hd, pd, c.scale, signs)
+
+    def rows(n):
+        return (torch.from_numpy(c.rng.standard_normal((n, hkv, hd))).to(TYPES[dtype]).to(DEV),
+                torch.from_numpy(c.rng.standard_normal((n, hkv, hd))).to(TYPES[dtype]).to(DEV))
+
+    def write(b, at, k, v):
+        pg = c.indices.reshape(3, width)[b][at // page]
+        ops.quantize_write_kv_cache(cache, k, v, signs, dev((pg * page + at % page)
+                                                            .astype(np.int32)), hd, pd)
+
+    def check(q, starts, window, o=None):
+        c.cache, c.lens, c.ends = cache.cpu().numpy(), lens.copy(), seen.copy()
+        ref_o, ref_w, ref_p = C.attend(c, q, starts, window, True, decode=o is not None)
+        got = rec.weights.cpu().numpy()
+        known = np.isfinite(ref_w)
+        assert np.array_equal(known, np.isfinite(got))
+        d = copy.copy(c)
+        d.weights = np.where(np.isfinite(c.weights), c.weights, 0).astype(np.float32)
+        check_weights(d, np.where(known, got, 0), np.where(known, ref_w, 0), q,
+                      window * hq // hkv)
+        assert np.array_equal(rec.positions.cpu().numpy(), ref_p)
+        if o is not None:
+            check_o(c, o, ref_o, q, dtype)
+        c.weights, c.positions = got, ref_p
+
+    def cut():
+        nonlocal lens
+        new = rec.evict(cache, table, dev(lens), dev(seen))
+        c.lens, c.ends = lens.copy(), seen.copy()
+        c.cache, c.weights, c.positions, lens = C.evict(c, budget, 9, 3)
+        assert np.array_equal(new.cpu().numpy(), lens)
+        assert np.array_equal(cache.cpu().numpy(), c.cache)
+        assert np.array_equal(rec.weights.cpu().numpy(), c.weights, equal_nan=True)
+        assert np.array_equal(rec.positions.cpu().numpy(), c.positions)
+
+    for b, p in enumerate(prompt):
+        write(b, np.arange(p), *rows(p))
+    starts = np.concatenate(([0], np.cumsum(prompt))).astype(np.int32)
+    q, qx = queries(c, int(starts[-1]), dtype)
+    rec.observe(q, dev(starts), cache, table, dev(lens), dev(seen), *args)
+    check(qx, starts, 7)
+    cut()
+    assert lens.tolist() == [64, 61, 1]
+    for step in range(steps):
+        k, v = rows(3)
+        for b in range(3):
+            write(b, lens[b:b + 1].copy(), k[b:b + 1], v[b:b + 1])
+        lens, seen = lens + 1, seen + 1
+        q, qx = queries(c, 3, dtype)
+        o = torch.empty((3, hq, hd), dtype=TYPES[dtype], device=DEV)
+        rec.decode(q, cache, table, dev(lens), dev(seen), *args, o)
+        check(qx, np.arange(4), 1, o)
+        if step % every == every - 1:
+            cut()
+    assert lens.max() <= budget + every
+
+
+def test_two_graphs_and_a_stream_share_nothing():
+    """Two captured decode calls and an eager one on a third stream, replayed
+    together over caches of their own: workspaces are not shared."""
+    cs = [C.make(50 + i, [400 + 30 * i, 77], 8, 2, 128) for i in range(3)]
+    ts = [tensors(c) for c in cs]
+    qs = [queries(c, 2, "fp16") for c in cs]
+    os_ = [torch.zeros((2, 8, 128), dtype=torch.float16, device=DEV) for _ in cs]
+    w0 = [t["weights"].clone() for t in ts]
+
+    def call(i):
+        c, t = cs[i], ts[i]
+        t["weights"].copy_(w0[i])
+        ops.decode_paged_tracked(qs[i][0], t["cache"], t["indices"], t["indptr"], t["seq"], 2, 128,
+                                 128, c.scale, t["signs"], os_[i], t["weights"], t["positions"],
+                                 t["ends"])
+    want = []
+    for i in range(3):
+        call(i)
+        want.append((os_[i].clone(), ts[i]["weights"].clone()))
+    torch.cuda.synchronize()
+    graphs = []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(i)
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(5):
+        for i in range(3):
+            os_[i].zero_()
+            ts[i]["weights"].zero_()
+        torch.cuda.synchronize()
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                graphs[i].replay() if i < 2 else call(i)
+        torch.cuda.synchronize()
+        for i in range(3):
+            assert torch.equal(os_[i], want[i][0]) and torch.equal(ts[i]["weights"], want[i][1])
+
+
+def test_native_and_python_forms_agree():
+    """The C++ form takes the ordinary call; a call that it leaves alone (an
+    op's tensor subclass, here signs that are not contiguous) gives the same."""
+    c = C.make(60, [300, 40], 8, 2, 128)
+    nat = ops._native()
+    signs2 = dev(np.stack((c.signs, c.signs), 1))[:, 0]
+    assert not signs2.is_contiguous()
+    got = []
+    for signs in (dev(c.signs), signs2):
+        t = tensors(c)
+        c.rng = np.random.default_rng(1)
+        q, _ = queries(c, 2, "fp16")
+        o = torch.empty((2, 8, 128), dtype=torch.float16, device=DEV)
+        args = (q, t["cache"], t["indices"], t["indptr"], t["seq"], 2, 128, 128, c.scale, signs, o,
+                t["weights"], t["positions"], t["ends"])
+        if signs is signs2:
+            assert not nat.decode_tracked(*args)
+        ops.decode_paged_tracked(*args)
+        starts = torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV)
+        ops.track_window(q, starts, 1, *args[1:10], *args[11:])
+        new = torch.empty(2, dtype=torch.int32, device=DEV)
+        ev = (t["cache"], t["weights"], t["positions"], t["indices"], t["indptr"], t["seq"],
+              t["ends"], 100, 5, 5, new)
+        assert nat.evict(*ev[:6], t["ends"].long(), *ev[7:]) is False
+        ops.evict_paged(*ev)
+        got.append((o, t["weights"], t["positions"], t["cache"], new))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
+def test_registered_ops_run():
+    ops.register_ops()
+    c = C.make(61, [90, 40], 8, 2, 64)
+    t = tensors(c)
+    q, qx = queries(c, 2, "fp16")
+    o = torch.empty((2, 8, 64), dtype=torch.float16, device=DEV)
+    v5 = torch.ops.turboquant_v5
+    assert v5.decode_paged_tracked(q, t["cache"], t["indices"], t["indptr"], t["seq"], 2, 64, 64,
+                                   c.scale, t["signs"], o, t["weights"], t["positions"],
+                                   t["ends"]) is None
+    ref_o, ref_w, _ = C.attend(c, qx, np.arange(3), 1, True, decode=True)
+    check_weights(c, t["weights"].cpu().numpy(), ref_w, qx, 4)
+    check_o(c, o, ref_o, qx, "fp16")
+    starts = torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV)
+    v5.track_window(q, starts, 4, t["cache"], t["indices"], t["indptr"], t["seq"], 2, 64, 64,
+                    c.scale, t["signs"], t["weights"], None, None)
+    new = torch.empty(2, dtype=torch.int32, device=DEV)
+    v5.evict_paged(t["cache"], t["weights"], None, t["indices"], t["indptr"], t["seq"], None, 50, 0,
+                   0, new)
+    assert new.tolist() == [50, 40]
+
+
+def test_refused_calls_raise_from_the_library():
+    c = C.make(62, [90], 8, 2, 64)
+    t = tensors(c)
+    new = torch.empty(1, dtype=torch.int32, device=DEV)
+    args = (t["cache"], t["weights"], t["positions"], t["indices"], t["indptr"], t["seq"],
+            t["ends"])
+    for budget, recent, sink in ((0, 0, 0), (8, 9, 0), (8, 4, 5), (8, -1, 0)):
+        with pytest.raises(RuntimeError, match="evict"):
+            ops.evict_paged(*args, budget, recent, sink, new)
+    with pytest.raises(RuntimeError, match="evict"):
+        ops.evict_paged(t["cache"], t["weights"], None, *args[3:], 8, 2, 0, new)
+    q = torch.zeros((1, 8, 64), dtype=torch.float16, device=DEV)
+    starts = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    for window in (0, 257):
+        with pytest.raises(RuntimeError, match="track_window"):
+            ops.track_window(q, starts, window, t["cache"], t["indices"], t["indptr"], t["seq"], 2,
+                             64, 64, c.scale, None, t["weights"])
+
+
+# ------------------------------------------------------------ backend and harness
+
+class _Meta:
+    def __init__(self, **kw):
+        self.__dict__.update(kw)
+
+
+@pytest.mark.parametrize("hd,dtype", [(128, "fp16"), (96, "bf16")])
+def test_backend_fills_its_record(hd, dtype):
+    """forward with a record: a prompt batch is observed after its attention, a
+    decode batch attends through the tracked op; a mixed batch too."""
+    from turboquant_amd.budget import CacheRecord
+    from turboquant_amd.vllm_backend_fused import TurboQuantBackend, TurboQuantFusedImpl
+    hq, hkv, page, lens = 8, 2, 16, [40, 23]
+    impl = TurboQuantFusedImpl(hq, hd, 1 / math.sqrt(hd), hkv, None, None, "fp8")
+    plain = TurboQuantFusedImpl(hq, hd, 1 / math.sqrt(hd), hkv, None, None, "fp8")
+    shape = TurboQuantBackend.get_kv_cache_shape(8, page, hkv, hd, "fp8")
+    cache = torch.zeros(shape, dtype=torch.uint8, device=DEV)
+    impl.record = CacheRecord.beside(cache, 64, window=5)
+    table = torch.arange(8, dtype=torch.int32, device=DEV).view(2, 4)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(3)
+
+    def step(chunks, seq):
+        n = sum(chunks)
+        k, v = (torch.randn((n, hkv, hd), generator=g, device=DEV).to(TYPES[dtype])
+                for _ in range(2))
+        q = torch.randn((n, hq * hd), generator=g, device=DEV).to(TYPES[dtype])
+        slots = torch.tensor([int(table[b, t // page]) * page + t % page
+                              for b, (ql, s) in enumerate(zip(chunks, seq))
+                              for t in range(s - ql, s)], dtype=torch.int32, device=DEV)
+        starts = torch.tensor([0, chunks[0], n], dtype=torch.int32, device=DEV)
+        meta = _Meta(max_query_len=max(chunks), num_actual_tokens=n, block_table=table,
+                     seq_lens=torch.tensor(seq, dtype=torch.int32, device=DEV),
+                     query_start_loc=starts, slot_mapping=slots)
+        impl.do_kv_cache_update(None, k, v, cache, slots)
+        a = (q, k.reshape(n, -1), v.reshape(n, -1), cache, meta)
+        before = impl.record.weights.cpu().numpy()
+        got, want = impl.forward(None, *a), plain.forward(None, *a)
+        # two kernels of the same attention: each within the decode tolerance
+        assert (got.float() - want.float()).abs().max() < 2 * (2e-3 + 1e-2 * want.abs().max())
+        c = C.make(1, seq, hq, hkv, hd, page=page)
+        c.cache, c.indices = cache.cpu().numpy(), table.cpu().numpy().reshape(-1)
+        c.indptr, c.nb = np.array([0, 4, 8], np.int32), 8
+        c.weights, c.positions = before, np.zeros_like(before, np.int32)
+        c.ends, c.signs = np.array(seq, np.int32), impl._signs.cpu().numpy()
+        qx = q.double().cpu().numpy().reshape(n, hq, hd)
+        _, ref, _ = C.attend(c, qx, starts.cpu().numpy(), 5 if max(chunks) > 1 else 1)
+        check_weights(c, impl.record.weights.cpu().numpy(), ref, qx, 5 * hq // hkv)
+    step([40, 23], lens)
+    step([1, 1], [41, 24])
+    step([1, 7], [42, 31])
+
+
+def test_harness_decodes_under_a_budget():
+    """The end-to-end loop with a budget: eager and captured steps give the same
+    tokens, caches stay inside it, and every layer and head keeps the first and
+    the newest positions, each once."""
+    from turboquant_amd import e2e
+    shape = e2e.ModelShape.tiny(2)
+    g = torch.Generator(device="cpu")
+    g.manual_seed(7)
+    prompts = torch.randint(0, shape.vocab, (3, 200), generator=g)
+    rule = dict(budget=96, recent=16, sink=4, window=8, cut_every=4)
+    tokens = []
+    for graph in (False, True):
+        r = e2e.Runner(shape, 3, 220, DEV, seed=5, **rule)
+        for b in range(3):
+            r.prefill(b, prompts[b, :200 - 60 * b].to(DEV))
+        assert r.lens.tolist() == [96, 96, 80]
+        if graph:
+            r.capture(14)
+            tokens.append(r.decode_graph(14).clone())
+        else:
+            tokens.append(r.decode_eager(14).clone())
+        torch.cuda.synchronize()
+        assert r.pos.tolist() == [214, 154, 94]
+        assert r.lens.tolist() == [98, 98, 94]
+        for impl in r.impls:
+            pos = impl.record.positions.cpu().numpy()
+            for b in range(3):
+                n, seen = int(r.lens[b]), int(r.pos[b])
+                t = np.arange(n)
+                pg = r.block_table[b].cpu().numpy()[t // 16]
+                for h in range(shape.kv_heads):
+                    kept = set(pos[pg, h, t % 16].tolist())
+                    assert len(kept) == n and kept <= set(range(seen))
+                    assert set(range(4)) | set(range(seen - 16, seen)) <= kept
+    assert torch.equal(tokens[0], tokens[1])
+
+
+def test_harness_budget_above_every_length_changes_nothing_kept():
+    """A budget that nothing exceeds: the tokens of the run without one, but for
+    the rounding between two kernels of the same attention."""
+    from turboquant_amd import e2e
+    shape = e2e.ModelShape.tiny(2)
+    g = torch.Generator(device="cpu")
+    g.manual_seed(9)
+    prompts = torch.randint(0, shape.vocab, (2, 100), generator=g)
+    outs = []
+    for rule in ({}, dict(budget=4096)):
+        r = e2e.Runner(shape, 2, 110, DEV, seed=6, **rule)
+        for b in range(2):
+            r.prefill(b, prompts[b].to(DEV))
+        r.probe = []
+        r.decode_eager(1)
+        outs.append([p[4].float() for p in r.probe])
+        if rule:
+            assert r.lens.tolist() == [101, 101]
+            total = torch.stack([impl.record.weights.sum() for impl in r.impls])
+            # 32 observed queries and one decode step, over two sequences, 32 heads
+            assert torch.allclose(total, torch.full_like(total, 2 * 33 * 32), rtol=1e-5)
+    a, b = outs[0][0], outs[1][0]  # the first layer sees the same inputs
+    assert (a - b).abs().max() < 2 * (2e-3 + 1e-2 * a.abs().max())

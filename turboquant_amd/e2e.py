@@ -22,6 +22,11 @@ chunk); the decode step of the whole batch (embedding, 36 layers, final norm,
 LM head, greedy argmax, position advance) is captured once in a HIP graph
 and replayed once per output token.
 
+Optionally (``budget``) every layer keeps its sequences inside a cache budget:
+the prompt's last queries and the decode steps record what each cached entry
+receives, prompts are cut to the budget right after their prefill, and decoded
+sequences whenever ``cut_every`` tokens have come on top (budget.CacheRecord).
+
 Optionally (``keep_fp16_kv``) the runner also keeps an fp16 copy of every
 layer's K/V and can decode the same model with plain fp16-KV SDPA attention,
 so the greedy tokens of the two runs can be compared.
@@ -38,6 +43,7 @@ import torch
 import torch.nn.functional as F
 
 from . import ops
+from .budget import CacheRecord
 from .vllm_backend_fused import TurboQuantBackend, TurboQuantFusedImpl
 
 BLOCK = 16
@@ -74,6 +80,7 @@ class Meta:
     seq_lens: torch.Tensor | None
     query_start_loc: torch.Tensor
     slot_mapping: torch.Tensor | None
+    tokens_seen: torch.Tensor | None = None  # where tokens have been evicted
 
 
 def build_weights(shape: ModelShape, seed: int, device) -> dict:
@@ -193,6 +200,11 @@ class Runner:
     device: torch.device
     seed: int = 0
     keep_fp16_kv: bool = False
+    budget: int = 0               # cached tokens per sequence, 0: no cuts
+    recent: int = 0
+    sink: int = 4
+    window: int = 32
+    cut_every: int = 64
     weights: dict = field(default=None, repr=False)
 
     def __post_init__(self):
@@ -220,10 +232,18 @@ class Runner:
             self.kv16 = [torch.zeros((2, self.batch, s.kv_heads, self.max_tokens, s.head_dim),
                                      dtype=torch.float16, device=dev)
                          for _ in range(s.layers)]
+        if self.budget:
+            for impl, cache in zip(self.impls, self.caches):
+                impl.record = CacheRecord.beside(cache, self.budget, recent=self.recent,
+                                                 sink=self.sink, window=self.window)
         # decode state (fixed buffers, updated inside the captured step)
         self.pos = torch.zeros(self.batch, dtype=torch.int64, device=dev)
         self.tok = torch.zeros(self.batch, dtype=torch.int64, device=dev)
         self.seq_lens = torch.zeros(self.batch, dtype=torch.int32, device=dev)
+        # cached tokens, and tokens seen (pos + 1 inside a step): with a budget only
+        self.lens = torch.zeros(self.batch, dtype=torch.int32, device=dev)
+        self.seen = torch.zeros(self.batch, dtype=torch.int32, device=dev)
+        self.since_cut = 0
         self.slots = torch.zeros(self.batch, dtype=torch.int32, device=dev)
         self.qsl = torch.arange(self.batch + 1, dtype=torch.int32, device=dev)
         self.out_buf = None
@@ -291,11 +311,23 @@ class Runner:
                                 self.caches[li], meta)
         x = self._layers(x, pos, attend)
         first = greedy(self._logits(x[-1:]))
+        if self.budget:
+            self.lens[b], self.seen[b] = L, L
+            self._cut(slice(b, b + 1))
         self.pos[b] = L
         self.tok[b] = first[0]
         self.first_pos = self.pos.clone()
         self.first_tok = self.tok.clone()
         return int(first[0])
+
+    # ------------------------------------------------------------ budget
+    def _cut(self, which=slice(None)):
+        """Cuts the sequences `which` to the budget, in every layer."""
+        lens, seen, table = self.lens[which], self.seen[which], self.block_table[which]
+        new = torch.empty_like(lens)
+        for impl, cache in zip(self.impls, self.caches):
+            impl.record.evict(cache, table, lens, seen, new)
+        lens.copy_(new)
 
     # ------------------------------------------------------------ decode
     def _decode_body(self):
@@ -303,10 +335,15 @@ class Runner:
         s = self.shape
         pos = self.pos
         bt = self.block_table
-        page = bt.gather(1, (pos // BLOCK)[:, None]).squeeze(1).to(torch.int64)
-        self.slots.copy_((page * BLOCK + pos % BLOCK).to(torch.int32))
-        self.seq_lens.copy_((pos + 1).to(torch.int32))
+        # the new token's place in the cache: its position, or behind what is kept
+        at = self.lens.to(torch.int64) if self.budget else pos
+        page = bt.gather(1, (at // BLOCK)[:, None]).squeeze(1).to(torch.int64)
+        self.slots.copy_((page * BLOCK + at % BLOCK).to(torch.int32))
+        self.seq_lens.copy_((at + 1).to(torch.int32))
         meta = Meta(1, self.batch, bt, self.seq_lens, self.qsl, self.slots)
+        if self.budget:
+            self.seen.copy_((pos + 1).to(torch.int32))
+            meta.tokens_seen = self.seen
         x = F.embedding(self.tok, self.weights["embed"])
 
         def attend(li, lw, q, k, v):
@@ -322,7 +359,17 @@ class Runner:
         self.tok.copy_(nxt)
         self.out_buf.index_copy_(0, self.step_idx, nxt[None, :])
         self.pos.add_(1)
+        if self.budget:
+            self.lens.add_(1)
         self.step_idx.add_(1)
+
+    def _step_done(self):
+        """After each decode step: the cut, every cut_every of them."""
+        if self.budget:
+            self.since_cut += 1
+            if self.since_cut >= self.cut_every:
+                self._cut()
+                self.since_cut = 0
 
     def _start_decode(self, steps: int):
         self.out_buf = torch.zeros((steps, self.batch), dtype=torch.int64, device=self.device)
@@ -333,6 +380,7 @@ class Runner:
         self._start_decode(steps)
         for _ in range(steps):
             self._decode_body()
+            self._step_done()
         return self.out_buf
 
     @torch.no_grad()
@@ -342,22 +390,29 @@ class Runner:
         workspace and loads the kernels); the state (pos, tok) is restored
         afterwards, so decoding continues from where the caller was.  The
         warm-up's cache writes land in the slots the first replay rewrites."""
-        saved = (self.pos.clone(), self.tok.clone())
+        saved = (self.pos.clone(), self.tok.clone(), self.lens.clone())
+        # (the warm-up's weights are taken back too; what it writes for the new
+        # token is written again)
+        kept = [impl.record.weights.clone() for impl in self.impls] if self.budget else []
+
+        def restore():
+            self.pos.copy_(saved[0])
+            self.tok.copy_(saved[1])
+            self.lens.copy_(saved[2])
+            for impl, w in zip(self.impls, kept):
+                impl.record.weights.copy_(w)
+            self.step_idx.zero_()
         self._start_decode(steps)
         self._decode_body()
         torch.cuda.synchronize()
-        self.pos.copy_(saved[0])
-        self.tok.copy_(saved[1])
-        self.step_idx.zero_()
+        restore()
         st = torch.cuda.Stream()
         st.wait_stream(torch.cuda.current_stream())
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g, stream=st):
             self._decode_body()
         torch.cuda.synchronize()
-        self.pos.copy_(saved[0])
-        self.tok.copy_(saved[1])
-        self.step_idx.zero_()
+        restore()
         self.graph = g
         self.graph_steps = steps
         return g
@@ -370,6 +425,7 @@ class Runner:
         self.step_idx.zero_()
         for _ in range(steps):
             self.graph.replay()
+            self._step_done()
         return self.out_buf[:steps]
 
     # ------------------------------------------------------- fp16 reference
@@ -493,7 +549,8 @@ def attention_vs_fp16(r: Runner) -> dict:
 
 
 def run(shape: ModelShape, batch: int = 8, prompt_len: int = 32768, new_tokens: int = 256,
-        seed: int = 0, compare_steps: int = 0, device: str = "cuda:0", log=None) -> dict:
+        seed: int = 0, compare_steps: int = 0, device: str = "cuda:0", log=None,
+        **rule) -> dict:
     """Prefill `batch` random prompts of `prompt_len` tokens one after another,
     then decode `new_tokens` - 1 more tokens for the whole batch with graph
     replays (the first output token comes from the prefill).  Returns the
@@ -507,11 +564,14 @@ def run(shape: ModelShape, batch: int = 8, prompt_len: int = 32768, new_tokens: 
     * with compare_steps > 0, the greedy-token agreement with the same model
       decoded over fp16 K/V for that many steps from the same prefill.
     Graph capture (a one-time setup, as a server does at start-up) is timed
-    separately and not counted."""
+    separately and not counted.  rule: budget, recent, sink, window, cut_every of
+    the Runner (cuts are part of the prefill and decode times)."""
+    if rule.get("budget") and compare_steps:
+        raise ValueError("the runs to compare with keep every token: no budget")
     dev = torch.device(device)
     say = log or (lambda *a: None)
     r = Runner(shape, batch, prompt_len + new_tokens, dev, seed,
-               keep_fp16_kv=compare_steps > 0)
+               keep_fp16_kv=compare_steps > 0, **rule)
     g = torch.Generator(device="cpu")
     g.manual_seed(seed + 2)
     prompts = torch.randint(0, shape.vocab, (batch, prompt_len), generator=g)
@@ -582,6 +642,9 @@ def run(shape: ModelShape, batch: int = 8, prompt_len: int = 32768, new_tokens: 
         "layers": shape.layers,
         "first_tokens": first.tolist(),
     })
+    if r.budget:
+        res.update({"budget": r.budget, "recent": r.recent, "sink": r.sink,
+                    "cut_every": r.cut_every, "cached_tokens": r.lens.tolist()})
     r.tokens = toks
     return res
 
@@ -596,10 +659,18 @@ def main(argv=None):
     ap.add_argument("--compare", type=int, default=0,
                     help="greedy-agreement steps against an fp16-KV run")
     ap.add_argument("--seed", type=int, default=0)
+    ap.add_argument("--budget", type=int, default=0,
+                    help="cached tokens per sequence (0: all are kept)")
+    ap.add_argument("--recent", type=int, default=0, help="newest tokens that are always kept")
+    ap.add_argument("--sink", type=int, default=4, help="first tokens that are always kept")
+    ap.add_argument("--window", type=int, default=32, help="observed queries of a prompt")
+    ap.add_argument("--cut-every", type=int, default=64, help="decode steps between cuts")
     a = ap.parse_args(argv)
+    rule = dict(budget=a.budget, recent=a.recent, sink=a.sink, window=a.window,
+                cut_every=a.cut_every) if a.budget else {}
     shape = ModelShape.tiny(a.layers) if a.tiny else ModelShape(layers=a.layers)
     res = run(shape, a.batch, a.prompt, a.new, a.seed, a.compare,
-              log=lambda m: print(m, flush=True))
+              log=lambda m: print(m, flush=True), **rule)
     print(json.dumps(res))
 
 

@@ -138,6 +138,9 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
             (split plan made on the GPU from seq_lens), or the reference's
             turboquant_v5::decode_v5_from_cache_paged_splitkv_ws with
             TQ_FORCE_KERNEL=gfx950_static.
+    With a budget.CacheRecord as `record`, decode goes through
+    turboquant_v5::decode_paged_tracked and every other batch is observed after
+    its attention (turboquant_v5::track_window).
     Prefill / mixed batches: _prefill_mixed (decode rows through the decode
     kernel, chunks with cached context over the dequantized context plus the
     fresh chunk, fresh prompts as in the reference, vllm_backend_fused.py:335-371).
@@ -162,6 +165,8 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
         self._decode_op_name = None
         self._write_op = None
         self._rows_op = None
+        # a budget.CacheRecord beside this layer's cache: forward fills it
+        self.record = None
 
     # ---------------------------------------------------------------- setup
     @staticmethod
@@ -451,6 +456,27 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
                               attn_metadata, output)
         return output
 
+    def _forward_recorded(self, q, kv_cache, attn_metadata, output, decode):
+        """With a record: the attention of a decode batch, which fills it, or
+        (decode False, after the batch's prefill) the record alone."""
+        sl = attn_metadata.seq_lens.to(torch.int32).contiguous()
+        seen = getattr(attn_metadata, "tokens_seen", None)
+        seen = sl if seen is None else seen.to(torch.int32).contiguous()
+        half = (torch.float16, torch.bfloat16)
+        if q.dtype not in half:
+            q = q.to(torch.float16)
+        geometry = (self.num_kv_heads, self.head_size, self._pd, self.scale, self._signs)
+        if not decode:
+            qsl = attn_metadata.query_start_loc.to(torch.int32).contiguous()
+            self.record.observe(q, qsl, kv_cache, attn_metadata.block_table, sl, seen, *geometry)
+            return output
+        o = output if output.dtype in half and output.is_contiguous() else \
+            torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        self.record.decode(q, kv_cache, attn_metadata.block_table, sl, seen, *geometry, o)
+        if o is not output:
+            output.copy_(o)
+        return output
+
     def _decode_rows(self, dec, qsl, query, kv_cache, bt, attn_metadata, output):
         """The decode rows `dec` (request indices, q_len 1) of a mixed batch
         through the balanced decode op; at most BALANCED_MAX_BATCH of them."""
@@ -507,6 +533,8 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
                     self._prefill_fresh(q, k, v, attn_metadata, out3)
                 else:
                     self._prefill_mixed(q, k, v, kv_cache, attn_metadata, out3)
+                    if self.record is not None:
+                        self._forward_recorded(q, kv_cache, attn_metadata, out3, False)
                 return output
             return super().forward(layer, query, key, value, kv_cache, attn_metadata,
                                    output, output_scale, **kwargs)
@@ -534,6 +562,9 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
             q3 = q.view(rows)
             out3 = (output if output.shape[0] == num_actual else output[:num_actual]).view(rows)
             batch_size = num_actual
+            if self.record is not None:
+                self._forward_recorded(q3, kv_cache, attn_metadata, out3, True)
+                return output
             # the balanced plan takes up to BALANCED_MAX_BATCH sequences; a
             # larger decode batch takes the reference's static-split op (same
             # kernels, host-planned splits)
