@@ -275,6 +275,15 @@ def test_window_lengths(lens, chunks):
     run_window(C.make(sum(lens) + 1, lens, 12, 4, 96), chunks, 8)
 
 
+@pytest.mark.parametrize("window", [5, 17, 24, 40, 70, 100])
+def test_window_of_many_sequences(window):
+    # 12 sequences of 8 kv heads: the second pass joins the statistics itself
+    # up to 16 row tiles, whose number does not divide the half waves here
+    lens = [3, 0, 260, 17, 129, 500, 64, 1, 90, 33, 1030, 128]
+    chunks = [3, 0, 100, 1, 129, 80, 0, 1, 9, 33, 70, 128]
+    run_window(C.make(900 + window, lens, 24, 8, 128), chunks, window)
+
+
 def test_window_without_rotation_or_positions_and_peaked():
     run_window(C.make(21, [129, 40], 8, 2, 64), [50, 40], 8, signs=False)
     run_window(C.make(22, [129, 40], 8, 2, 64), [50, 40], 8, record=False)

@@ -1130,7 +1130,7 @@ struct WindowParams {
   const float* qs;    // [B][Hkv][32 tiles]
   float csc;
   float2* stats;  // [Hkv][units][32 tiles]
-  float* lse;     // [B][Hkv][32 tiles], log2 units, +inf: adds nothing
+  float* lse;     // [B][Hkv][32 tiles] from window_lse_kernel; null: none ran
   int32_t* split;
   float* weights;
   int32_t* positions;
@@ -1142,13 +1142,12 @@ __global__ __launch_bounds__(256) void rotate_window_kernel(
     const void* __restrict__ q, int64_t q_rows, int64_t q_sb, int64_t q_sh, int bf16, int hd,
     WindowParams p, const float* __restrict__ signs, _Float16* __restrict__ qf, float* __restrict__ qs) {
   constexpr int E = PD / 64;
-  const int64_t rows = (int64_t)p.B * p.Hkv * p.tiles * 32;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
-  if (row >= rows) return;
-  const int rho = (int)(row % (p.tiles * 32));
-  const int64_t bh = row / (p.tiles * 32);
-  const int kvh = (int)(bh % p.Hkv), b = (int)(bh / p.Hkv);
+  const uint32_t bt = blockIdx.x / 8;  // eight workgroups a tile, a row per wave
+  const int tile = (int)(bt % (uint32_t)p.tiles), in = blockIdx.x % 8 * 4 + (threadIdx.x >> 6);
+  const uint32_t bh = bt / (uint32_t)p.tiles;
+  const int kvh = (int)(bh % (uint32_t)p.Hkv), b = (int)(bh / (uint32_t)p.Hkv);
+  const int rho = tile * 32 + in;
   const int i = rho / p.ratio, h = rho % p.ratio;
   const int q0 = p.q_start[b], q1 = p.q_start[b + 1];
   const int64_t at = (int64_t)q1 - p.window + i;
@@ -1157,17 +1156,26 @@ __global__ __launch_bounds__(256) void rotate_window_kernel(
   if (i < p.window && at >= max(q0, 0) && at < q_rows)
     inv = split_row<PD>(q, at * q_sb + (int64_t)(kvh * p.ratio + h) * q_sh, bf16, hd, signs, hi,
                         lo);
-  // dim d is element d % 8 of half (d / 8) % ... : lane half d / (PD/2), step
-  // (d % (PD/2)) / 8
-  _Float16* const tile = qf + (bh * p.tiles + rho / 32) * (int64_t)(PD / 16) * 2 * 512;
+  // dim d is element d % 8 of step (d % (PD / 2)) / 8 in lane half d / (PD / 2);
+  // two dims a store, at head size 64 from two lanes (one stores hi, one lo)
+  const int d = E == 1 ? lane & ~1 : lane * E;
+  _Float16* const to = qf + (int64_t)bt * (PD / 16) * 1024 + d % (PD / 2) / 8 * 1024 +
+                       (d / (PD / 2) * 32 + in) * 8 + d % 8;
+  if constexpr (E == 1) {
+    const uint32_t h16 = __builtin_bit_cast(uint16_t, hi[0]);
+    const uint32_t l16 = __builtin_bit_cast(uint16_t, lo[0]);
+    const bool odd = lane & 1;
+    const uint32_t mine = odd ? l16 : h16, other = __shfl_xor(odd ? h16 : l16, 1);
+    *reinterpret_cast<uint32_t*>(to + (odd ? 512 : 0)) = odd ? mine << 16 | other : other << 16 | mine;
+  } else {
+    typedef _Float16 row_t __attribute__((ext_vector_type(E)));
+    row_t a, c;
 #pragma unroll
-  for (int k = 0; k < E; k++) {
-    const int d = lane * E + k, half = d / (PD / 2), ks = d % (PD / 2) / 8;
-    _Float16* const to = tile + ks * 1024 + (half * 32 + rho % 32) * 8 + d % 8;
-    to[0] = hi[k];
-    to[512] = lo[k];
+    for (int k = 0; k < E; k++) a[k] = hi[k], c[k] = lo[k];
+    *reinterpret_cast<row_t*>(to) = a;
+    *reinterpret_cast<row_t*>(to + 512) = c;
   }
-  if (lane == 0) qs[row] = inv;
+  if (lane == 0) qs[(int64_t)bt * 32 + in] = inv;
 }
 
 // hi and lo operands of 8 codes, in registers of their own
@@ -1197,6 +1205,75 @@ __device__ __forceinline__ void read_operands(uint32_t at, half8_t* f) {
 #endif
 }
 
+// A row's normaliser in log2 units from its maximum and sum.  Rows past the
+// window or before the chunk's first query (scale 0) add nothing: +inf.
+__device__ __forceinline__ float lse_of(float2 x, float scale) {
+  return scale != 0.f && x.y != 0.f ? x.x + log2f(x.y) : INFINITY;
+}
+// (max, sum) of a row over units g, g + step, ... of n, `src` at the first one's
+__device__ __forceinline__ float2 join_units(const float2* src, int stride, int g, int n, int step) {
+  float2 a = make_float2(kNone, 0.f);
+#pragma unroll 8
+  for (int u = g; u < n; u += step) {
+    const float2 x = src[(int64_t)u * stride];
+    join_stats(x.x, x.y, a.x, a.y);
+  }
+  return a;
+}
+
+// The normalisers of a sequence's rows from its units' maxima and sums: a
+// workgroup takes 32 rows, thread (r, g) their units g, g + 8, ...
+__global__ __launch_bounds__(256) void window_lse_kernel(WindowParams p) {
+  __shared__ float2 part[8][32];
+  const int R = p.tiles * 32, r = threadIdx.x & 31, g = threadIdx.x >> 5;
+  const int tile = blockIdx.x % p.tiles;
+  const int64_t bh = blockIdx.x / p.tiles;
+  const int kvh = (int)(bh % p.Hkv), b = (int)(bh / p.Hkv);
+  const int row = tile * 32 + r;
+  const int u0 = p.split[b], u1 = p.split[b + 1];
+  float2 a = join_units(p.stats + ((int64_t)kvh * p.units + u0) * R + row, R, g, u1 - u0, 8);
+  part[g][r] = a;
+  __syncthreads();
+  if (g) return;
+#pragma unroll
+  for (int k = 1; k < 8; k++) join_stats(part[k][r].x, part[k][r].y, a.x, a.y);
+  const int64_t at = bh * R + row;
+  p.lse[at] = lse_of(a, p.qs[at]);
+}
+
+// All rows' normalisers into LDS (256 threads): window_lse_kernel's, or without
+// it from the sequence's n units at u0 here, where half a wave takes a tile and,
+// with fewer than 8 tiles, groups of them share its units.  (A barrier follows.)
+__device__ __forceinline__ void row_lse(const WindowParams& p, int kvh, int64_t bh, int u0, int n,
+                                        float2 (*part)[4][32], float* lse) {
+  const int R = p.tiles * 32, r = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const float* const qs = p.qs + bh * R;
+  if (p.lse) {
+    for (int i = threadIdx.x; i < R; i += 256) lse[i] = p.lse[bh * R + i];
+    return;
+  }
+  const float2* const src = p.stats + ((int64_t)kvh * p.units + u0) * R + r;
+  if (p.tiles >= 8) {
+    for (int t = w; t < p.tiles; t += 8) {
+      const int row = t * 32 + r;
+      lse[row] = lse_of(join_units(src + t * 32, R, 0, n, 1), qs[row]);
+    }
+    return;
+  }
+  const int groups = 8 / p.tiles, t = w % p.tiles, g = w / p.tiles;
+  float2 a = make_float2(kNone, 0.f);
+  if (g < groups) a = join_units(src + t * 32, R, g, n, groups);
+  part[w >> 2][w & 3][r] = a;
+  __syncthreads();
+  if (g) return;
+  for (int k = 1; k < groups; k++) {
+    const int v = t + k * p.tiles;
+    const float2 b = part[v >> 2][v & 3][r];
+    join_stats(b.x, b.y, a.x, a.y);
+  }
+  lse[t * 32 + r] = lse_of(a, qs[t * 32 + r]);
+}
+
 // One pass of the keys over the rows.  SUM false: each row's maximum and sum
 // over the unit's tokens; true: each token's sum of weights over the rows,
 // added to (or, for the chunk's own tokens, set as) its weight.
@@ -1217,8 +1294,9 @@ void window_kernel(WindowParams p) {
       uint64_t lut[4096];
       uint8_t q[2][QT];
     };
-    float2 wave[SUM ? 1 : 2][SUM ? 1 : 4][32];  // a row tile's (max, sum) of each wave
-    float2 rows[SUM ? 1 : 1024];     // running (max, sum) of the unit
+    float2 wave[2][4][32];        // a row tile's (max, sum) of each wave
+    float2 rows[SUM ? 1 : 1024];  // running (max, sum) of the unit
+    float lse[SUM ? 1024 : 1];    // the rows' normalisers
   };
   __shared__ Lds sm;
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
@@ -1234,7 +1312,7 @@ void window_kernel(WindowParams p) {
   const uint8_t* const qf =
       reinterpret_cast<const uint8_t*>(p.qf) + bh * p.tiles * (int64_t)QT;
   const float* const qs = p.qs + bh * p.tiles * 32;
-  const float* const lse = SUM ? p.lse + bh * p.tiles * 32 : nullptr;
+  if constexpr (SUM) row_lse(p, kvh, bh, u - ps.j, (ps.L + ps.U - 1) / ps.U, sm.wave, sm.lse);
   if constexpr (!SUM)
     for (int i = threadIdx.x; i < p.tiles * 32; i += 256) sm.rows[i] = make_float2(kNone, 0.f);
   const uint32_t lanec = 8 * (lane & 15);
@@ -1308,8 +1386,8 @@ void window_kernel(WindowParams p) {
 #pragma unroll
     for (int m = 0; m < MT; m++) all = all && okm[m] == 0xffffffffu;
     __syncthreads();  // the table is no longer read
-    // a row tile's scale and normaliser, one tile ahead and in front of the copies
-    float next_q = qs[col], next_l = SUM ? lse[col] : 0.f;
+    // a row tile's scale, one tile ahead and in front of the copies
+    float next_q = qs[col];
     issue(0);
     // the waves' statistics of tile rt, joined by one of them; tile rt + 1 has
     // buffers of its own, so the barrier of each tile is enough
@@ -1329,10 +1407,9 @@ void window_kernel(WindowParams p) {
       __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
       barrier();  // tile rt is there, and nobody reads the other buffer
       const int row = rt * 32 + col;
-      const float cq = next_q * p.csc, ls = next_l;
+      const float cq = next_q * p.csc, ls = SUM ? sm.lse[row] : 0.f;
       if (rt + 1 < p.tiles) {
         next_q = qs[row + 32];
-        if constexpr (SUM) next_l = lse[row + 32];
         issue(rt + 1);
       }
       if constexpr (!SUM)
@@ -1430,20 +1507,21 @@ void window_kernel(WindowParams p) {
     if constexpr (SUM) {
 #pragma unroll
       for (int m = 0; m < MT; m++) {
-        float mine = 0.f;  // the sum of this lane's token, in lanes 0 .. 31
+        // Each step adds over one bit of the column and halves the values that a
+        // lane holds: lane (col, half) ends with accumulator row col % 16's sum.
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          float g = got[m][i];
-          g += xor_lane(g, 1);
-          g += xor_lane(g, 2);
-          g += xor_lane(g, 4);
-          g += ror8(g);
-          g = xor16_sum(g);
-          const float other = __shfl_xor(g, 32);
-          const int r0 = 8 * (i / 4) + i % 4;  // half 0's row; half 1's is 4 further
-          if (col == r0) mine = half ? other : g;
-          if (col == r0 + 4) mine = half ? g : other;
+        for (int step = 0; step < 4; step++) {
+          const bool bit = col >> step & 1;
+#pragma unroll
+          for (int i = 0; i < 8 >> step; i++) {
+            const float keep = bit ? got[m][2 * i + 1] : got[m][2 * i];
+            const float give = bit ? got[m][2 * i] : got[m][2 * i + 1];
+            got[m][i] = keep + (step == 3 ? ror8(give) : xor_lane(give, 1 << step));
+          }
         }
+        // token col's row is 4 (col / 8) + col % 4 of half col / 4 % 2
+        const float mine =
+            __shfl(xor16_sum(got[m][0]), (col & 4) * 8 + (col >> 3) * 4 + (col & 3));
         if (half == 0 && place[m] >= 0) {
           const int t = t0 + 32 * m + col;
           if (t < ps.L - q_len) {
@@ -1461,33 +1539,6 @@ void window_kernel(WindowParams p) {
     float2* const out = p.stats + ((int64_t)kvh * p.units + u) * p.tiles * 32;
     for (int i = threadIdx.x; i < p.tiles * 32; i += 256) out[i] = sm.rows[i];
   }
-}
-
-// The normalisers of a sequence's rows from its units' maxima and sums: a
-// workgroup takes 32 rows, thread (r, g) their units g, g + 8, ...
-__global__ __launch_bounds__(256) void window_lse_kernel(WindowParams p) {
-  __shared__ float2 part[8][32];
-  const int R = p.tiles * 32, r = threadIdx.x & 31, g = threadIdx.x >> 5;
-  const int tile = blockIdx.x % p.tiles;
-  const int64_t bh = blockIdx.x / p.tiles;
-  const int kvh = (int)(bh % p.Hkv), b = (int)(bh / p.Hkv);
-  const int row = tile * 32 + r;
-  const int u0 = p.split[b], u1 = p.split[b + 1];
-  const float2* const src = p.stats + (int64_t)kvh * p.units * R + row;
-  float m = kNone, l = 0.f;
-#pragma unroll 4
-  for (int u = u0 + g; u < u1; u += 8) {
-    const float2 x = src[(int64_t)u * R];
-    join_stats(x.x, x.y, m, l);
-  }
-  part[g][r] = make_float2(m, l);
-  __syncthreads();
-  if (g) return;
-#pragma unroll
-  for (int k = 1; k < 8; k++) join_stats(part[k][r].x, part[k][r].y, m, l);
-  // rows past the window or before the chunk's first query add nothing
-  const int64_t at = bh * R + row;
-  p.lse[at] = p.qs[at] != 0.f && l != 0.f ? m + log2f(l) : INFINITY;
 }
 
 // ---- host ------------------------------------------------------------------
@@ -1804,6 +1855,15 @@ WindowWs window_ws(int batch, int window, int ratio, int hkv, int pd, int cus) {
   w.total = at;
   return w;
 }
+// Whether the second pass joins the units' statistics itself, in each workgroup
+// again: where a thread would read at most 16 of them (units of a sequence of
+// average length x row tiles, over 8 half waves).  A launch less, measured with
+// 12 reads (4 prompts of up to 1500 tokens, 128 rows) 33.2 -> 30.4 us and with 8
+// (head size 64, 32 rows) 39.4 -> 37.5; with 86 (32768 tokens, 256 rows) it
+// would be 154 -> 170.
+bool join_here(const WindowWs& w, int batch) {
+  return (int64_t)w.units * w.tiles <= (int64_t)128 * batch;
+}
 int check_window(int window, int ratio) {
   if (window < 1 || window * (int64_t)ratio > 1024) {
     set_error("track_window: window %d x %d q heads per kv head out of range (1 .. 1024 rows)",
@@ -1889,7 +1949,7 @@ extern "C" int tq_track_window(const void* q, int64_t num_rows, int64_t q_stride
   p.qs = reinterpret_cast<float*>(base + ws.qs);
   p.csc = sm_scale * 1.4426950408889634f / (sqrtf((float)pd) * kLevelScale);
   p.stats = reinterpret_cast<float2*>(base + ws.stats);
-  p.lse = reinterpret_cast<float*>(base + ws.lse);
+  p.lse = join_here(ws, batch) ? nullptr : reinterpret_cast<float*>(base + ws.lse);
   p.split = reinterpret_cast<int32_t*>(base + ws.split);
   p.weights = weights;
   p.positions = positions;
@@ -1913,13 +1973,15 @@ extern "C" int tq_track_window(const void* q, int64_t num_rows, int64_t q_stride
     f1 = reinterpret_cast<const void*>(&window_kernel<256, 1, true>);
   }
   void* rargs[] = {&q, &num_rows, &q_stride_tok, &q_stride_h, &bf, &hd, &p, &signs, &qf, &qs};
-  rc = launch(who, fr, (rows + 3) / 4, 256, rargs, stream);
+  rc = launch(who, fr, rows / 4, 256, rargs, stream);
   if (rc) return rc;
   void* args[] = {&p};
   rc = launch(who, f0, (int64_t)ws.units * num_kv_heads, 256, args, stream);
   if (rc) return rc;
-  rc = launch(who, reinterpret_cast<const void*>(&window_lse_kernel), rows / 32, 256, args,
-              stream);
-  if (rc) return rc;
+  if (p.lse) {
+    rc = launch(who, reinterpret_cast<const void*>(&window_lse_kernel), rows / 32, 256, args,
+                stream);
+    if (rc) return rc;
+  }
   return launch(who, f1, (int64_t)ws.units * num_kv_heads, 256, args, stream);
 }
