@@ -156,7 +156,13 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(EvictParams p) {
     const int q = j * kSelThreads + tid, s = tiles[q >> 2];
     return s < 0 ? -1 : s + 4 * (q & 3);
   };
+  // The keys, and the first pass over them while they come: their upper 12 bits
+  // counted.  Protected ones and zeros are many: counted in registers, not in one
+  // LDS counter each.
   if (tid < 3) many[tid] = 0;
+  for (int i = tid; i < kBins / 4; i += kSelThreads)
+    reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
+  uint32_t held = 0, zeros = 0;
 #pragma unroll 1
   for (int ch = 0; ch < chunks; ch++) {
     constexpr int H = 4;  // quads in flight
@@ -187,59 +193,56 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(EvictParams p) {
                        2 < left ? key_of(wt[j].z, ps[j].z, sink, span) : 0u,
                        3 < left ? key_of(wt[j].w, ps[j].w, sink, span) : 0u));
       }
+#pragma unroll 1
+      for (int j = j0; j < j0 + H && run(ch, j) < n; j++) {
+        const uint4 q = get(ch, j);
+        const uint32_t k[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          held += k[e] == kHeld;
+          zeros += k[e] == kZero;
+          if (k[e] != kHeld && k[e] != kZero) atomicAdd(&hist[k[e] >> 20], 1u);
+        }
+      }
     }
   }
+  held = wave_scan(held);
+  zeros = wave_scan(zeros);
+  if (lane == 63 && held + zeros) {
+    atomicAdd(&hist[kHeld >> 20], held);
+    atomicAdd(&hist[kZero >> 20], zeros);
+    atomicAdd(&many[0], held);
+    atomicAdd(&many[1], zeros);
+  }
 
-  // The budget-th largest key, 12 + 10 + 10 bits at a time.  Protected ones and
-  // zeros are many: counted in registers, not in one LDS counter each.
+  // The budget-th largest key, 12 + 10 + 10 bits at a time.
   uint32_t need = (uint32_t)p.budget, prefix = 0, equal = 0;
   uint32_t listed = 0;  // keys of the first pass's bin in `list`, 0: not listed
 #pragma unroll 1
   for (int pass = 0; pass < 3; pass++) {
     const int bits = pass == 0 ? 12 : 10, shift = 20 - 10 * pass;
     const int bins = 1 << bits;
-    for (int i = tid; i < bins / 4; i += kSelThreads)
-      reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    if (pass == 0) {
-      uint32_t held = 0, zeros = 0;
+    if (pass) {
+      for (int i = tid; i < bins / 4; i += kSelThreads)
+        reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
+      __syncthreads();
+      if (listed) {
+        for (uint32_t i = tid; i < listed; i += kSelThreads) {
+          const uint32_t k = list[i];
+          if (k >> (shift + 10) == prefix) atomicAdd(&hist[k >> shift & 1023], 1u);
+        }
+      } else {
 #pragma unroll 1
-      for (int ch = 0; ch < chunks; ch++)
+        for (int ch = 0; ch < chunks; ch++)
 #pragma unroll 1
-        for (int j = 0; j < kQuads && run(ch, j) < n; j++) {
-          const uint4 q = get(ch, j);
-          const uint32_t k[4] = {q.x, q.y, q.z, q.w};
+          for (int j = 0; j < kQuads && run(ch, j) < n; j++) {
+            const uint4 q = get(ch, j);
+            const uint32_t k[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            held += k[e] == kHeld;
-            zeros += k[e] == kZero;
-            if (k[e] != kHeld && k[e] != kZero) atomicAdd(&hist[k[e] >> 20], 1u);
+            for (int e = 0; e < 4; e++)
+              if (k[e] >> (shift + 10) == prefix) atomicAdd(&hist[k[e] >> shift & 1023], 1u);
           }
-        }
-      held = wave_scan(held);
-      zeros = wave_scan(zeros);
-      if (lane == 63 && held + zeros) {
-        atomicAdd(&hist[kHeld >> 20], held);
-        atomicAdd(&hist[kZero >> 20], zeros);
-        atomicAdd(&many[0], held);
-        atomicAdd(&many[1], zeros);
       }
-    } else if (listed) {
-      for (uint32_t i = tid; i < listed; i += kSelThreads) {
-        const uint32_t k = list[i];
-        if (k >> (shift + 10) == prefix) atomicAdd(&hist[k >> shift & 1023], 1u);
-      }
-    } else {
-#pragma unroll 1
-      for (int ch = 0; ch < chunks; ch++)
-#pragma unroll 1
-        for (int j = 0; j < kQuads && run(ch, j) < n; j++) {
-          const uint4 q = get(ch, j);
-          const uint32_t k[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-            if (k[e] >> (shift + 10) == prefix) atomicAdd(&hist[k[e] >> shift & 1023], 1u);
-        }
     }
     __syncthreads();
     // bins from the top, four a thread: the one where the count reaches need
