@@ -303,7 +303,7 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(EvictParams p) {
             at = __builtin_amdgcn_readlane(at, 63) + sum - m;
 #pragma unroll
             for (int e = 0; e < 4; e++)
-              if (k[e] >> 20 == prefix) list[at++] = k[e];
+              if (k[e] >> 20 == prefix && at < kList) list[at++] = k[e];
           }
         listed = equal;
       }
@@ -332,6 +332,7 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(EvictParams p) {
   static_assert(kQuads * kSelWaves == 128, "scan() takes two counts a lane");
   int32_t* const dst = p.dst + (int64_t)blockIdx.x * p.cap;
   int32_t* const src = p.src + (int64_t)blockIdx.x * p.cap;
+  const uint32_t cap = (uint32_t)p.cap;
   const bool ties = equal != need;
   const uint32_t from = ties && cut != kHeld ? cut + 1 : cut;  // kept: keys >= from
   uint32_t eq_base = 0, hole_base = 0, more_base = 0;
@@ -410,7 +411,7 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(EvictParams p) {
         }
 #pragma unroll
         for (int e = 0; e < 4; e++)
-          if (mark[e]) to[rank++] = slot < 0 ? -1 : slot + e;
+          if (mark[e] && rank < cap) to[rank++] = slot < 0 ? -1 : slot + e;
       }
     }
     hole_base = hole_next;
@@ -418,7 +419,9 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(EvictParams p) {
     __syncthreads();  // tot is read
   }
   // exactly budget entries are kept, so there are as many holes as sources
-  if (tid == 0) p.moves[blockIdx.x] = (int32_t)more_base;
+  // (the bounds by cap and kList hold by themselves; they are for page tables whose
+  // ranges overlap, where another sequence's keys may stand in the workspace)
+  if (tid == 0) p.moves[blockIdx.x] = (int32_t)min(more_base, cap);
 }
 
 // Entry moves: a move takes 2 EBS / 16 lanes for the codes and norms of K and V
