@@ -83,6 +83,18 @@ def test_refusals(monkeypatch, call, key, shape, dtype, match):
         call(_args(**{key: bad}))
 
 
+def test_integers_that_32_bits_would_wrap_are_refused(monkeypatch):
+    monkeypatch.setattr(ops, "_require_gpu", lambda *t: None)
+    a, wrap = _args(), 2 ** 32
+    for call in (lambda: _window(a, window=wrap + 4), lambda: _evict(a, budget=wrap + 8),
+                 lambda: _evict(a, recent=wrap), lambda: _evict(a, sink=-wrap),
+                 lambda: ops.decode_paged_tracked(
+                     a["q"], a["cache"], a["indices"], a["indptr"], a["seq"], 2, 128, wrap + 128,
+                     0.1, None, a["o"], a["weights"], a["positions"], a["ends"])):
+        with pytest.raises(RuntimeError, match="out of range"):
+            call()
+
+
 def test_positions_need_ends(monkeypatch):
     monkeypatch.setattr(ops, "_require_gpu", lambda *t: None)
     for call in (_decode, _window, _evict):

@@ -191,7 +191,7 @@ bool decode_tracked(const Tensor& q, const Tensor& kv_cache, const Tensor& indic
       !signs_of(signs, padded_dim, dev, sp))
     return false;
   const int64_t b = q.size(0), hq = q.size(1);
-  if (b == 0 || seq_lens.numel() < b || indptr.numel() < b ||
+  if (b == 0 || padded_dim > 256 || seq_lens.numel() < b || indptr.numel() < b ||
       !record_of(weights, positions, ends, c, b, dev))
     return false;
   const c10::DeviceGuard guard(dev);
@@ -221,7 +221,7 @@ bool track_window(const Tensor& q, const Tensor& starts, int64_t window, const T
   if (!on(q, dev) || q.dim() != 3 || q.size(2) != head_dim || q.stride(2) != 1 || !is_half(qt) ||
       q.size(0) == 0 || !is_i32(starts, dev) || starts.numel() < 2 || !is_i32(indices, dev) ||
       !is_i32(indptr, dev) || !is_i32(seq_lens, dev) || !cache_of(kv_cache, dev, c) ||
-      c.heads != num_kv_heads || window < 1 || window > 1024 ||
+      c.heads != num_kv_heads || padded_dim > 256 || window < 1 || window > 1024 ||
       !signs_of(signs, padded_dim, dev, sp))
     return false;
   const int64_t b = starts.numel() - 1, hq = q.size(1);

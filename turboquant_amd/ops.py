@@ -876,6 +876,13 @@ def _int32(t, n, name, what):
                            "entries")
 
 
+def _fit_int32(what, **values):
+    """Integers that the library takes in 32 bits, where they would wrap."""
+    for name, v in values.items():
+        if not -2 ** 31 <= int(v) < 2 ** 31:
+            raise RuntimeError(f"{what}: {name} {v} out of range")
+
+
 def _check_tables(batch, indices, indptr, seq_lens, what):
     _int32(indices, 0, "indices", what)
     _int32(indptr, batch, "indptr", what)
@@ -955,6 +962,7 @@ def decode_paged_tracked(q: torch.Tensor, kv_cache: torch.Tensor, indices: torch
     _check_q(q, head_dim, num_kv_heads, padded_dim, what)
     nb, bs, ebs = _cache_geometry(kv_cache, num_kv_heads, what)
     b, hq, _ = q.shape
+    _fit_int32(what, padded_dim=padded_dim)
     _check_tables(b, indices, indptr, seq_lens, what)
     _check_record(kv_cache, weights, positions, ends, b, what)
     if o.dtype not in (torch.float16, torch.bfloat16) or tuple(o.shape) != tuple(q.shape) \
@@ -1003,6 +1011,7 @@ def track_window(q: torch.Tensor, query_start_loc: torch.Tensor, window: int,
     b, hq = query_start_loc.numel() - 1, q.size(1)
     if b < 0:
         raise RuntimeError(f"{what}: query_start_loc must hold batch + 1 entries")
+    _fit_int32(what, window=window, padded_dim=padded_dim)
     _int32(query_start_loc, b + 1, "query_start_loc", what)
     _check_tables(b, indices, indptr, seq_lens, what)
     _check_record(kv_cache, weights, positions, ends, b, what)
@@ -1046,6 +1055,7 @@ def evict_paged(kv_cache: torch.Tensor, weights: torch.Tensor, positions: torch.
     _check_tables(b, indices, indptr, seq_lens, what)
     _check_record(kv_cache, weights, positions, ends, b, what)
     _int32(new_lens, b, "new_lens", what)
+    _fit_int32(what, budget=budget, recent=recent, sink=sink)
     pd = {48: 64, 80: 128, 144: 256}.get(ebs)
     if pd is None:
         raise RuntimeError(f"{what}: kv_cache entries of {ebs} bytes")
