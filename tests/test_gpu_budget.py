@@ -361,6 +361,15 @@ def test_evict_long(n, budget):
     run_evict(spread(C.make(n, [n, 900], 1, 1, 64)), budget, 100, 4)
 
 
+@pytest.mark.parametrize("batch,hkv,hd", [(64, 1, 64), (65, 1, 64), (70, 12, 64), (3, 20, 256)])
+def test_evict_many_rows_of_moves(batch, hkv, hd):
+    # one, two and three rows of 64 (sequence, head group)s, the last group of
+    # 4 heads; one long sequence whose rounds outnumber the others'
+    lens = [(37 * b) % 90 for b in range(batch)]
+    lens[batch // 2] = 3000
+    run_evict(spread(C.make(batch + hkv, lens, hkv, hkv, hd)), 40, 8, 2)
+
+
 def test_evict_ties_nan_and_infinities():
     c = spread(C.make(31, [400, 200], 2, 2, 128))
     w = c.weights

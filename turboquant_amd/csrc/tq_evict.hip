@@ -425,36 +425,77 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(EvictParams p) {
 }
 
 // Entry moves: a move takes 2 EBS / 16 lanes for the codes and norms of K and V
-// and one for weight and position.  A workgroup takes runs of move numbers for
-// up to eight heads of a sequence: the i-th holes of the heads lie close
-// together, and so do the pieces of cache lines that they share.
-constexpr int kMoveHeads = 8;
+// and one for weight and position.  A round is a run of move numbers for up to
+// eight heads of a sequence: the i-th holes of the heads lie close together, and
+// so do the pieces of cache lines that they share.  The rounds of up to 64
+// (sequence, head group)s are numbered through, so that a few long sequences
+// keep every workgroup busy, and rounds that follow one another go to one XCD
+// (workgroups x mod 8), whose L2 holds the lines they share.
+constexpr int kMoveHeads = 8, kMoveRows = 64, kXcds = 8;
 template <int EBS>
 __global__ __launch_bounds__(256) void move_kernel(EvictParams p) {
   constexpr int E = EBS / 16, C = 2 * E + 1, NI = 4, PAIRS = 256 * NI / C;
+  static_assert(PAIRS <= 256, "a move a thread");
   __shared__ int to_s[PAIRS], of_s[PAIRS];
+  const int lane = threadIdx.x & 63;
   const int groups = (p.Hkv + kMoveHeads - 1) / kMoveHeads;
-  const int b = blockIdx.y / groups, h0 = blockIdx.y % groups * kMoveHeads;
-  const int heads = min(kMoveHeads, p.Hkv - h0);
-  if (h0 == 0 && blockIdx.x == 0 && threadIdx.x == 0)
-    p.new_lens[b] = min(p.seq_lens[b], p.budget);
-  const int32_t* const moves = p.moves + b * p.Hkv + h0;
-  int most = 0;
+  // lane i of every wave: (sequence, head group) i of the grid row, its rounds
+  // and those before
+  const int row = blockIdx.y * kMoveRows + lane;
+  const int lb = row / groups, lh = row - lb * groups, lh0 = lh * kMoveHeads;
+  int lrounds = 0;
+  if (lb < p.B) {
+    const int heads = min(kMoveHeads, p.Hkv - lh0);
+    int most = 0;
 #pragma unroll
-  for (int i = 0; i < kMoveHeads; i++) most = max(most, moves[min(i, heads - 1)]);
-  const int per = PAIRS / heads, pairs = per * heads;  // move numbers a round
-  for (int64_t m0 = (int64_t)blockIdx.x * per; m0 < most; m0 += (int64_t)gridDim.x * per) {
+    for (int i = 0; i < kMoveHeads; i++)
+      most = max(most, p.moves[lb * p.Hkv + lh0 + min(i, heads - 1)]);
+    const int per = PAIRS / heads;
+    lrounds = (int)(((uint32_t)most + per - 1) / per);
+    if (lh == 0 && blockIdx.x == 0 && threadIdx.x < 64)
+      p.new_lens[lb] = min(p.seq_lens[lb], p.budget);
+  }
+  const uint32_t lend = wave_scan((uint32_t)lrounds);
+  const uint32_t rounds = __builtin_amdgcn_readlane(lend, 63);
+  // 2^run rounds of every 2^(run + 3) in a row are one XCD's
+  const uint32_t x = blockIdx.x;
+  int run = min(5, 31 - __builtin_clz(gridDim.x / kXcds));
+  while (run > 0 && (uint32_t)kXcds << run > rounds) run--;
+  const uint32_t in = x & ((kXcds << run) - 1);
+  uint32_t r = x - in + (in % kXcds << run) + in / kXcds;
+
+  // this thread's move of a round (pairs <= 256), loaded a round ahead
+  int to = -1, of = -1, nh = 1, nh0 = 0, npairs = 0;  // of the loaded round
+  const auto load = [&](uint32_t round) {
+    to = -1;
+    if (round >= rounds) return;
+    const int k = __popcll(__ballot(lend <= round));
+    const int b = __builtin_amdgcn_readlane(lb, k);
+    nh0 = __builtin_amdgcn_readlane(lh0, k);
+    nh = min(kMoveHeads, p.Hkv - nh0);
+    const int per = PAIRS / nh;
+    npairs = per * nh;
+    const int im = (int)threadIdx.x / nh, hm = (int)threadIdx.x - im * nh;
+    const int64_t m =
+        (int64_t)(round - (k ? __builtin_amdgcn_readlane(lend, max(k - 1, 0)) : 0)) * per + im;
+    const int bh = b * p.Hkv + nh0 + hm;
+    if ((int)threadIdx.x < npairs && m < p.cap) {
+      const int n = p.moves[bh];
+      const int d = p.dst[bh * p.cap + m], s = p.src[bh * p.cap + m];
+      to = m < n && s >= 0 ? d : -1;  // (-1: none, or on no page of the cache)
+      of = s;
+    }
+  };
+  load(r);
+  for (; r < rounds; r += gridDim.x) {
+    const int heads = nh, h0 = nh0, pairs = npairs;
     __syncthreads();
-    for (int i = threadIdx.x; i < pairs; i += 256) {
-      const int h = i % heads;
-      const int64_t m = m0 + i / heads;
-      const int64_t at = (int64_t)(b * p.Hkv + h0 + h) * p.cap + m;
-      const bool ok = m < moves[h];
-      const int to = ok ? p.dst[at] : -1, of = ok ? p.src[at] : -1;
-      to_s[i] = to >= 0 && of >= 0 ? to : -1;  // none, or on no page of the cache
-      of_s[i] = of;
+    if ((int)threadIdx.x < pairs) {
+      to_s[threadIdx.x] = to;
+      of_s[threadIdx.x] = of;
     }
     __syncthreads();
+    load(r + gridDim.x);
     uint4 v[NI];
     int64_t at[NI];
     int c[NI];
@@ -624,14 +665,13 @@ extern "C" int tq_evict_paged(uint8_t* k_slab, uint8_t* v_slab, float* weights, 
   hipLaunchKernelGGL(select_kernel, dim3((unsigned)bh), dim3(kSelThreads), 0, st, p);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess) {
-    // one round each, and no more workgroups than keep the GPU busy
+    // four workgroups a CU: with more at once fewer of the lines that rounds
+    // have in common are shared (a grid row needs some of its own)
     const int64_t y = (int64_t)batch * ((num_kv_heads + kMoveHeads - 1) / kMoveHeads);
-    const int per = 1024 / (2 * ebs / 16 + 1) /
-                    (num_kv_heads < kMoveHeads ? num_kv_heads : kMoveHeads);
-    int64_t gx = (ws.cap + per - 1) / per;
-    const int64_t most = 4096 / y > 1 ? 4096 / y : 1;
-    gx = gx < 1 ? 1 : (gx < most ? gx : most);
-    const dim3 grid((unsigned)gx, (unsigned)y);
+    const int64_t rows = (y + kMoveRows - 1) / kMoveRows;
+    int64_t gx = 1024;
+    while (gx > 64 && gx * rows > 1024) gx /= 2;
+    const dim3 grid((unsigned)gx, (unsigned)rows);
     if (ebs == 48)
       hipLaunchKernelGGL(move_kernel<48>, grid, dim3(256), 0, st, p);
     else if (ebs == 80)
