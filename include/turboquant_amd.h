@@ -192,14 +192,18 @@ int tq_decode_balanced_rows(int32_t batch, int32_t num_qo_heads, int32_t num_kv_
  *             that the entry received, summed over the q heads of its kv head;
  *             16-byte aligned
  *   positions int32 [num_blocks, num_kv_heads, block_size]: the position in
- *             its sequence that the entry came from
+ *             its sequence that the entry came from; 16-byte aligned for the
+ *             eviction
  * num_indices is the length of `indices`; table entries at or behind it, and
  * pages outside [0, num_blocks), count as empty: their tokens get no weight
- * and are not written.  No two sequences of a call share a page (they would
- * race for its weights and entries).  `ends` int32 [batch]: the number of
- * tokens that each sequence has seen, evicted ones included.  batch <= 1024,
- * num_kv_heads <= 4096, num_blocks * block_size < 2^31, the sum of seq_lens <
- * 2^30.  A workspace serves one call at a time and holds nothing between calls.
+ * and are not written.  A page stands once in the tables of a call (two
+ * sequences would race for its weights and entries).  `ends` int32 [batch]: the
+ * number of tokens that each sequence has seen, evicted ones included.  batch
+ * <= 1024 (eviction: batch * num_kv_heads <= 65535), num_kv_heads <= 4096,
+ * num_blocks * block_size < 2^31, the sum of seq_lens < 2^30.  A workspace
+ * serves one call at a time and holds nothing between calls; the tracked
+ * decode's holds a score for every token of the table and q head (num_indices *
+ * block_size * num_qo_heads * 4 bytes), the others' are small beside it.
  */
 
 /*

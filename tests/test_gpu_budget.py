@@ -627,6 +627,39 @@ class _Meta:
         self.__dict__.update(kw)
 
 
+def test_offsets_beyond_32_bits():
+    """Pages at the end of a cache of 8.8 GB (a slab is over 2^32 bytes) give the
+    bits that the same pages in a small cache give."""
+    c = spread(C.make(77, [300, 129, 40], 16, 8, 128))
+    q, _ = queries(c, 3, "fp16")
+    chunk, _ = queries(c, 60, "bf16")
+    starts = dev(np.array([0, 40, 50, 60], np.int32))
+    got = []
+    for blocks in (c.nb, 430_000):
+        t, at = tensors(c), blocks - c.nb
+        big = {k: torch.empty(n, dtype=t[k].dtype, device=DEV) for k, n in
+               (("cache", (2, blocks, 16, 8, 80)), ("weights", (blocks, 8, 16)),
+                ("positions", (blocks, 8, 16)))}
+        big["cache"][:, at:] = t["cache"]
+        for k in ("weights", "positions"):
+            big[k][at:] = t[k]
+        indices, o, new = t["indices"] + at, torch.empty_like(q), torch.empty_like(t["seq"])
+        tables = (indices, t["indptr"], t["seq"], 8, 128, 128, c.scale, t["signs"])
+        state = (big["weights"], big["positions"], t["ends"])
+        ops.track_window(chunk, starts, 7, big["cache"], *tables, *state)
+        ops.decode_paged_tracked(q, big["cache"], *tables, o, *state)
+        ops.evict_paged(big["cache"], big["weights"], big["positions"], indices, t["indptr"],
+                        t["seq"], t["ends"], 50, 10, 4, new)
+        torch.cuda.synchronize()
+        got.append((o, new, big["cache"][:, at:].clone(), big["weights"][at:].clone(),
+                    big["positions"][at:].clone()))
+        del big
+    torch.cuda.empty_cache()
+    assert not torch.equal(got[0][2], tensors(c)["cache"])
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+
+
 @pytest.mark.parametrize("hd,dtype", [(128, "fp16"), (96, "bf16")])
 def test_backend_fills_its_record(hd, dtype):
     """forward with a record: a prompt batch is observed after its attention, a

@@ -95,9 +95,12 @@ __device__ __forceinline__ uint32_t lanes_below(uint64_t mask, uint32_t base) {
                                    __builtin_amdgcn_mbcnt_lo((uint32_t)mask, base));
 }
 
-// (Loops over a chunk's quads stay loops: unrolled, with the keys in registers,
-// the kernel was 42 KB of code, and fetching it cost a small call more than its
-// work.)
+// Bound by the latencies of one workgroup's phases: 35 us at 32768 tokens (tile
+// slots 2, loads with the first counts 11, the bin's list 4, other passes 1,
+// ranks 3, source and destination lists 6.5) and 12 at 2050, on one CU a row.
+// Loops over a chunk's quads stay loops: unrolled, with the keys in registers, the
+// kernel was 42 KB of code, and fetching it cost a small call more than its work;
+// eight quads in flight instead of four cost 1.7 and 1.2 us.
 __global__ __launch_bounds__(kSelThreads) void select_kernel(EvictParams p) {
   __shared__ uint4 keys[kQuads * kSelThreads];
   __shared__ __attribute__((aligned(16))) uint32_t hist[kBins];
@@ -430,7 +433,8 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(EvictParams p) {
 // so do the pieces of cache lines that they share.  The rounds of up to 64
 // (sequence, head group)s are numbered through, so that a few long sequences
 // keep every workgroup busy, and rounds that follow one another go to one XCD
-// (workgroups x mod 8), whose L2 holds the lines they share.
+// (workgroups x mod 8), whose L2 holds the lines they share: 50.5 us for 8 x 32768
+// tokens cut to 8192, 63.2 with rounds dealt out one by one.
 constexpr int kMoveHeads = 8, kMoveRows = 64, kXcds = 8;
 template <int EBS>
 __global__ __launch_bounds__(256) void move_kernel(EvictParams p) {
@@ -618,7 +622,8 @@ extern "C" int tq_evict_paged(uint8_t* k_slab, uint8_t* v_slab, float* weights, 
     set_error("evict: %lld blocks of %d tokens out of range", (long long)num_blocks, block_size);
     return kEinval;
   }
-  if (!k_slab || !v_slab || !weights || (!indices && num_indices) || !indptr || !seq_lens || !new_lens ||
+  if (!k_slab || !v_slab || !weights || (!indices && num_indices) || !indptr || !seq_lens ||
+      !new_lens ||
       ((recent || sink) && !positions) || (positions && !ends)) {
     set_error("evict: null pointer");
     return kEinval;
@@ -665,8 +670,11 @@ extern "C" int tq_evict_paged(uint8_t* k_slab, uint8_t* v_slab, float* weights, 
   hipLaunchKernelGGL(select_kernel, dim3((unsigned)bh), dim3(kSelThreads), 0, st, p);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess) {
-    // four workgroups a CU: with more at once fewer of the lines that rounds
-    // have in common are shared (a grid row needs some of its own)
+    // Four workgroups a CU (64 at least for a grid row): with more at once fewer of
+    // the lines that rounds have in common are shared, and those without work cost
+    // their launch.  8 x 32768 tokens / 48 ragged sequences at head size 64 / 32
+    // barely over their budget: 50.5 / 21.2 / 6.4 us, with 512 in all 57.9 / 22.0 /
+    // 5.5, with 2048 56.7 / 22.2 / 7.3.
     const int64_t y = (int64_t)batch * ((num_kv_heads + kMoveHeads - 1) / kMoveHeads);
     const int64_t rows = (y + kMoveRows - 1) / kMoveRows;
     int64_t gx = 1024;

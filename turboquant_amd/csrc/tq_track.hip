@@ -458,6 +458,14 @@ __device__ __forceinline__ int row_exponent(float mx) {
 // add up all four terms in one accumulator.  PACK (then, where a wave has two
 // tiles a step): lanes n < 8 take on the scores of the first tile and n >= 8
 // those of the second, which halves the work per score.
+//
+// Bound by memory.  8 x 32768 tokens, 32 q / 8 kv heads of 128: 46.5 us for 161
+// MB read and 32 MB of scores written; while it streams 5.6-6.3 TB/s, and 6-8 us
+// are the prologue (plan, q', table) in front of the first step.  Measured and
+// not kept, for the sum of a call's three kernels (114 us in that run): the next
+// two or four steps touched in L2 during the prologue, no gain and 3% slower;
+// one workgroup of 16 waves a CU instead of two of 8, 2% slower there and 11 to
+// 27% on shorter calls.
 template <int PD, int G, bool QC>
 __global__ __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(PD == 256 && !QC ? 2 : 4)))
@@ -752,6 +760,10 @@ __device__ __forceinline__ void nibble_pairs(uint32_t a, uint32_t b, uint32_t& e
 // r, product i) is r * (PD/16) + i.  QC: columns 0-7 hold the hi parts of p *
 // norm, 8-15 the lo parts.  Probabilities are relative to the sequence's
 // maximum in the product and normalised at the end.
+//
+// Bound by memory: 49.2 us for 201 MB read (entries, scores, weights) and 16 MB
+// written, sizes as above.  One kernel for keys and values and a small one for
+// the weights would move the same bytes and save one prologue, at most 6%.
 template <int PD, int G, bool QC>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(PD == 256 ? 2 : 4)))
 void track_values_kernel(TrackParams p) {
@@ -1062,7 +1074,8 @@ __device__ __forceinline__ float split_row(const void* q, int64_t off, bool bf16
 }
 
 // o = s FWHT(sum of the partial rows)/sqrt(pd): one workgroup per (sequence,
-// q head), its four waves sharing the partial rows
+// q head), its four waves sharing the partial rows.  A launch and two dependent
+// loads: 2.9 us for one sequence, 4.9 for 8 of 64 rows each.
 template <int PD>
 __global__ __launch_bounds__(256) void track_join_kernel(const float* __restrict__ po,
                                                          const int32_t* __restrict__ split,
@@ -1137,10 +1150,13 @@ struct WindowParams {
   const int32_t* ends;
 };
 
+// The rotated rows: hi and lo parts in the MFMA's order, and their scales; a wave
+// a row (5 us for 2048 rows of 128: latency).
 template <int PD>
 __global__ __launch_bounds__(256) void rotate_window_kernel(
     const void* __restrict__ q, int64_t q_rows, int64_t q_sb, int64_t q_sh, int bf16, int hd,
-    WindowParams p, const float* __restrict__ signs, _Float16* __restrict__ qf, float* __restrict__ qs) {
+    WindowParams p, const float* __restrict__ signs, _Float16* __restrict__ qf,
+    float* __restrict__ qs) {
   constexpr int E = PD / 64;
   const int lane = threadIdx.x & 63;
   const uint32_t bt = blockIdx.x / 8;  // eight workgroups a tile, a row per wave
@@ -1166,7 +1182,8 @@ __global__ __launch_bounds__(256) void rotate_window_kernel(
     const uint32_t l16 = __builtin_bit_cast(uint16_t, lo[0]);
     const bool odd = lane & 1;
     const uint32_t mine = odd ? l16 : h16, other = __shfl_xor(odd ? h16 : l16, 1);
-    *reinterpret_cast<uint32_t*>(to + (odd ? 512 : 0)) = odd ? mine << 16 | other : other << 16 | mine;
+    *reinterpret_cast<uint32_t*>(to + (odd ? 512 : 0)) =
+        odd ? mine << 16 | other : other << 16 | mine;
   } else {
     typedef _Float16 row_t __attribute__((ext_vector_type(E)));
     row_t a, c;
@@ -1211,7 +1228,8 @@ __device__ __forceinline__ float lse_of(float2 x, float scale) {
   return scale != 0.f && x.y != 0.f ? x.x + log2f(x.y) : INFINITY;
 }
 // (max, sum) of a row over units g, g + step, ... of n, `src` at the first one's
-__device__ __forceinline__ float2 join_units(const float2* src, int stride, int g, int n, int step) {
+__device__ __forceinline__ float2 join_units(const float2* src, int stride, int g, int n,
+                                             int step) {
   float2 a = make_float2(kNone, 0.f);
 #pragma unroll 8
   for (int u = g; u < n; u += step) {
@@ -1281,6 +1299,14 @@ __device__ __forceinline__ void row_lse(const WindowParams& p, int kvh, int64_t 
 // A workgroup's four waves hold 32 MT keys each as operands and walk the row
 // tiles together: a tile's operands (PD * 128 bytes) come into LDS one ahead
 // of their use, by direct-to-LDS copies that the four waves share.
+//
+// Bound by the matrix products, three for one (hi hi, lo hi, hi lo).  A prompt of
+// 32768 tokens, 256 rows, 8 kv heads of 128: 74 us for the statistics and 68 for
+// the weights, 0.70 and 0.76 PFLOP/s of products issued (a large library product:
+// 1.16); of a workgroup's 128 tokens 1.3 us go into the table, 2.7 into the keys
+// and 10-13 into the eight row tiles.  Three waves a SIMD hide one's exp2 behind
+// the others' products: two row sets a wave at two waves a SIMD spill, and a
+// higher wave priority around the products changed nothing.
 template <int PD, int MT, bool SUM>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PD == 256 ? 2 : 3)))
 void window_kernel(WindowParams p) {
@@ -1702,7 +1728,8 @@ int check_state(const char* who, const uint8_t* k, const uint8_t* v, const int32
               bs, hkv);
     return kEinval;
   }
-  if (!k || !v || (!indices && entries) || !indptr || !seq_lens || !weights || (positions && !ends)) {
+  if (!k || !v || (!indices && entries) || !indptr || !seq_lens || !weights ||
+      (positions && !ends)) {
     set_error("%s: null pointer", who);
     return kEinval;
   }
@@ -1749,8 +1776,8 @@ extern "C" int tq_decode_paged_tracked(
   if (rc || batch == 0) return rc;
   rc = check_rows(who, q, q_stride_b, q_stride_h, q_dtype, head_dim, padded_dim);
   if (rc) return rc;
-  rc = check_state(who, k_slab, v_slab, indices, indptr, seq_lens, num_indices, ebs, padded_dim, num_blocks,
-                   block_size, num_kv_heads, weights, positions, ends);
+  rc = check_state(who, k_slab, v_slab, indices, indptr, seq_lens, num_indices, ebs, padded_dim,
+                   num_blocks, block_size, num_kv_heads, weights, positions, ends);
   if (rc) return rc;
   if (!o || (o_dtype != TQ_F16 && o_dtype != TQ_BF16)) {
     set_error("%s: o must be fp16 or bf16", who);
@@ -1894,15 +1921,14 @@ extern "C" int64_t tq_track_window_workspace_bytes(int32_t batch, int32_t window
       .total;
 }
 
-extern "C" int tq_track_window(const void* q, int64_t num_rows, int64_t q_stride_tok, int64_t q_stride_h,
-                               int32_t q_dtype, const int32_t* query_start_loc, int32_t window,
-                               const uint8_t* k_slab, const int32_t* indices, int64_t num_indices,
-                               const int32_t* indptr, const int32_t* seq_lens, int32_t batch,
-                               int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
-                               int32_t padded_dim, int32_t block_size, int32_t ebs,
-                               int64_t num_blocks, float sm_scale, const float* signs,
-                               float* weights, int32_t* positions, const int32_t* ends,
-                               void* workspace, int64_t workspace_bytes, tq_stream_t stream) {
+extern "C" int tq_track_window(
+    const void* q, int64_t num_rows, int64_t q_stride_tok, int64_t q_stride_h, int32_t q_dtype,
+    const int32_t* query_start_loc, int32_t window, const uint8_t* k_slab, const int32_t* indices,
+    int64_t num_indices, const int32_t* indptr, const int32_t* seq_lens, int32_t batch,
+    int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim, int32_t padded_dim,
+    int32_t block_size, int32_t ebs, int64_t num_blocks, float sm_scale, const float* signs,
+    float* weights, int32_t* positions, const int32_t* ends, void* workspace,
+    int64_t workspace_bytes, tq_stream_t stream) {
   using namespace tq;
   const char* who = "track_window";
   int rc = check_track(who, batch, num_indices, num_qo_heads, num_kv_heads, padded_dim, block_size);
@@ -1910,8 +1936,8 @@ extern "C" int tq_track_window(const void* q, int64_t num_rows, int64_t q_stride
   if (rc || batch == 0) return rc;
   rc = check_rows(who, q, q_stride_tok, q_stride_h, q_dtype, head_dim, padded_dim);
   if (rc) return rc;
-  rc = check_state(who, k_slab, k_slab, indices, indptr, seq_lens, num_indices, ebs, padded_dim, num_blocks,
-                   block_size, num_kv_heads, weights, positions, ends);
+  rc = check_state(who, k_slab, k_slab, indices, indptr, seq_lens, num_indices, ebs, padded_dim,
+                   num_blocks, block_size, num_kv_heads, weights, positions, ends);
   if (rc) return rc;
   if (!query_start_loc || num_rows < 0) {
     set_error("%s: null pointer or negative row count", who);
