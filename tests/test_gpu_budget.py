@@ -284,6 +284,16 @@ def test_window_of_many_sequences(window):
     run_window(C.make(900 + window, lens, 24, 8, 128), chunks, window)
 
 
+def test_window_of_a_long_table():
+    # a table of 8192 tokens over 32 kv heads: the first pass takes two key tiles
+    # a wave; units of more than one chunk, ends inside a tile, bad pages
+    c = C.make(55, [4003, 700], 32, 32, 128)
+    c.indices[20], c.indices[130] = -1, c.nb
+    c.indices = np.concatenate([c.indices, np.full(512 - len(c.indices), -1, np.int32)])
+    run_window(c, [500, 700], 400)
+    run_window(c, [33, 1], 300, signs=False)
+
+
 def test_window_without_rotation_or_positions_and_peaked():
     run_window(C.make(21, [129, 40], 8, 2, 64), [50, 40], 8, signs=False)
     run_window(C.make(22, [129, 40], 8, 2, 64), [50, 40], 8, record=False)

@@ -277,22 +277,24 @@ __device__ __forceinline__ float by_half(float x, uint32_t n) {
 
 // The key table: code byte -> fp16 hi parts of its two levels (high nibble
 // first, as the dims go) in the low dword, their lo parts in the high one,
-// times kLevelScale; 16 copies, lane l reads copy l mod 16.  Two entries are a
+// times kLevelScale; 2^LOG copies, lane l reads copy l mod 2^LOG.  Two entries are a
 // whole MFMA operand (hi, lo, hi, lo of two dims each) against q' with every
 // pair of dims twice: with hi and lo parts in operands of their own each entry
 // would cost two moves.
+template <int LOG>  // log2 of the copies
 __device__ __forceinline__ void init_key_table(uint64_t* lut) {
   // a byte's copies are shared by blockDim.x / 256 threads, two copies a store
-  const int per = 16 * 256 / blockDim.x, byte = threadIdx.x * 256 / blockDim.x;
+  const int per = (256 << LOG) / blockDim.x, byte = threadIdx.x * 256 / blockDim.x;
   const float a = level(byte >> 4) * kLevelScale, b = level(byte & 15) * kLevelScale;
   const float ah = (float)(_Float16)a, bh = (float)(_Float16)b;
   const uint32_t hi = pack_half(ah, bh), lo = pack_half(a - ah, b - bh);
   u32x4* const to = reinterpret_cast<u32x4*>(lut + threadIdx.x * per);
 #pragma unroll
-  for (int i = 0; i < 16; i += 2)
+  for (int i = 0; i < 1 << LOG; i += 2)
     if (i < per) to[i / 2] = u32x4{hi, lo, hi, lo};
 }
-// the two operands of 8 codes; lanec = 8 * (lane mod 16)
+// the two operands of 8 codes; lanec = 8 * (lane mod the copies)
+template <int LOG>
 __device__ __forceinline__ void key_operands(uint32_t c, const uint64_t* lut, uint32_t lanec,
                                              half8_t& k0, half8_t& k1) {
   uint64_t e[4];
@@ -300,8 +302,8 @@ __device__ __forceinline__ void key_operands(uint32_t c, const uint64_t* lut, ui
   for (int i = 0; i < 2; i++) {
     const uint32_t h = lut_spread(c, i);
     const uint8_t* const t = reinterpret_cast<const uint8_t*>(lut);
-    e[2 * i] = *reinterpret_cast<const uint64_t*>(t + lut_mad<7, 0>(h, lanec));
-    e[2 * i + 1] = *reinterpret_cast<const uint64_t*>(t + lut_mad<7, 1>(h, lanec));
+    e[2 * i] = *reinterpret_cast<const uint64_t*>(t + lut_mad<LOG + 3, 0>(h, lanec));
+    e[2 * i + 1] = *reinterpret_cast<const uint64_t*>(t + lut_mad<LOG + 3, 1>(h, lanec));
   }
   typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
   k0 = __builtin_bit_cast(half8_t, u64x2{e[0], e[1]});
@@ -572,7 +574,7 @@ void track_scores_kernel(TrackParams p) {
   }
   lds_written();
   barrier();  // every wave has its q'
-  init_key_table(sm.lut);
+  init_key_table<4>(sm.lut);
   lds_written();
 
   const int mine = PACK && n >= 8 ? R::SUB : 0;  // this lane's tile behind the wave's first
@@ -622,7 +624,7 @@ void track_scores_kernel(TrackParams p) {
 #pragma unroll
       for (int k = 0; k < KB; k++) {
         half8_t k0, k1;
-        key_operands(c[i][k], sm.lut, lanec, k0, k1);
+        key_operands<4>(c[i][k], sm.lut, lanec, k0, k1);
         acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qa[2 * k], acc[i], 0, 0, 0);
         acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qa[2 * k + 1], acc[i], 0, 0, 0);
         if constexpr (!QC) {
@@ -1142,7 +1144,7 @@ struct WindowParams {
   const half8_t* qf;  // [B][Hkv][tiles][PD/16][hi, lo][64 lanes]
   const float* qs;    // [B][Hkv][32 tiles]
   float csc;
-  float2* stats;  // [Hkv][units][32 tiles]
+  float2* stats;  // [Hkv][units of the first pass][32 tiles]
   float* lse;     // [B][Hkv][32 tiles] from window_lse_kernel; null: none ran
   int32_t* split;
   float* weights;
@@ -1196,30 +1198,14 @@ __global__ __launch_bounds__(256) void rotate_window_kernel(
 }
 
 // hi and lo operands of 8 codes, in registers of their own
+template <int LOG>
 __device__ __forceinline__ void key_parts(uint32_t c, const uint64_t* lut, uint32_t lanec,
                                           half8_t& hi, half8_t& lo) {
   half8_t k0, k1;
-  key_operands(c, lut, lanec, k0, k1);
+  key_operands<LOG>(c, lut, lanec, k0, k1);
   const u32x4 a = __builtin_bit_cast(u32x4, k0), b = __builtin_bit_cast(u32x4, k1);
   hi = __builtin_bit_cast(half8_t, u32x4{a[0], a[2], b[0], b[2]});
   lo = __builtin_bit_cast(half8_t, u32x4{a[1], a[3], b[1], b[3]});
-}
-
-// operands of two steps of a row tile, hi and lo, from LDS (1 KB each)
-__device__ __forceinline__ void read_operands(uint32_t at, half8_t* f) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  u32x4 a, b, c, d;
-  asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:1024\n\t"
-               "ds_read_b128 %2, %4 offset:2048\n\tds_read_b128 %3, %4 offset:3072\n\t"
-               "s_waitcnt lgkmcnt(0)"
-               : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d) : "v"(at) : "memory");
-  f[0] = __builtin_bit_cast(half8_t, a);
-  f[1] = __builtin_bit_cast(half8_t, b);
-  f[2] = __builtin_bit_cast(half8_t, c);
-  f[3] = __builtin_bit_cast(half8_t, d);
-#else
-  (void)at; (void)f;
-#endif
 }
 
 // A row's normaliser in log2 units from its maximum and sum.  Rows past the
@@ -1298,28 +1284,32 @@ __device__ __forceinline__ void row_lse(const WindowParams& p, int kvh, int64_t 
 //
 // A workgroup's four waves hold 32 MT keys each as operands and walk the row
 // tiles together: a tile's operands (PD * 128 bytes) come into LDS one ahead
-// of their use, by direct-to-LDS copies that the four waves share.
+// of their use, by direct-to-LDS copies that the four waves share.  The copies go
+// out behind the products: in front of them, the compiler would wait for the
+// copies before it reads the other buffer.
 //
-// Bound by the matrix products, three for one (hi hi, lo hi, hi lo).  A prompt of
-// 32768 tokens, 256 rows, 8 kv heads of 128: 74 us for the statistics and 68 for
-// the weights, 0.70 and 0.76 PFLOP/s of products issued (a large library product:
-// 1.16); of a workgroup's 128 tokens 1.3 us go into the table, 2.7 into the keys
-// and 10-13 into the eight row tiles.  Three waves a SIMD hide one's exp2 behind
-// the others' products: two row sets a wave at two waves a SIMD spill, and a
-// higher wave priority around the products changed nothing.
+// Bound by the matrix products, three for one (hi hi, lo hi, hi lo), and the LDS
+// reads that feed them.  A prompt of 32768 tokens, 256 rows, 8 kv heads of 128:
+// 58 us for the statistics and 60 for the weights, 0.89 and 0.86 PFLOP/s of
+// products issued (a large library product: 1.16).  A higher wave priority around
+// the products, reads one to three steps ahead by hand and pages looked up a
+// chunk ahead changed nothing.
 template <int PD, int MT, bool SUM>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PD == 256 ? 2 : 3)))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PD == 256 || MT == 2 ? 2 : 3)))
 void window_kernel(WindowParams p) {
   constexpr int KS = PD / 16;
   constexpr int EBS = Rows<PD, 1>::EBS;
   constexpr int QT = PD * 128;  // bytes of a row tile's operands
   constexpr int TOK = 4 * 32 * MT;
+  // (log2 of) the table's copies: what the LDS holds beside the rows' operands, so
+  // that the table stays for all chunks.  16 copies in the operands' place, made
+  // anew for each chunk: 150 us instead of 143 at 32768 tokens, 37.4 instead of
+  // 29.2 for 3 chunks over 4000-16000 tokens at head size 64.
+  constexpr int COPIES = PD == 64 ? 3 : (PD == 128 ? 2 : 1);
   typedef float float16_t __attribute__((ext_vector_type(16)));
   struct __attribute__((aligned(16))) Lds {
-    union {
-      uint64_t lut[4096];
-      uint8_t q[2][QT];
-    };
+    uint64_t lut[256 << COPIES];
+    uint8_t q[2][QT];
     float2 wave[2][4][32];        // a row tile's (max, sum) of each wave
     float2 rows[SUM ? 1 : 1024];  // running (max, sum) of the unit
     float lse[SUM ? 1024 : 1];    // the rows' normalisers
@@ -1328,7 +1318,7 @@ void window_kernel(WindowParams p) {
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kvh = blockIdx.x / p.units, u = blockIdx.x % p.units;
-  const PlanSlot ps = unit_of<TOK>(p, reinterpret_cast<int*>(sm.lut), u, 1,
+  const PlanSlot ps = unit_of<TOK>(p, reinterpret_cast<int*>(sm.q), u, 1,
                                    !SUM && blockIdx.x == 0 && w == 0);
   if (ps.b < 0) return;
   const int q_len = p.q_start[ps.b + 1] - p.q_start[ps.b];
@@ -1341,7 +1331,9 @@ void window_kernel(WindowParams p) {
   if constexpr (SUM) row_lse(p, kvh, bh, u - ps.j, (ps.L + ps.U - 1) / ps.U, sm.wave, sm.lse);
   if constexpr (!SUM)
     for (int i = threadIdx.x; i < p.tiles * 32; i += 256) sm.rows[i] = make_float2(kNone, 0.f);
-  const uint32_t lanec = 8 * (lane & 15);
+  const uint32_t lanec = 8 * (lane & ((1 << COPIES) - 1));
+  init_key_table<COPIES>(sm.lut);
+  __syncthreads();
 
   // copies of row tile rt into buffer rt & 1
   auto issue = [&](int rt) {
@@ -1359,9 +1351,6 @@ void window_kernel(WindowParams p) {
 
   for (int cb = c0; cb < c1; cb += TOK) {
     const int t0 = cb + w * 32 * MT;
-    __syncthreads();  // the last chunk's operands are no longer read
-    init_key_table(sm.lut);
-    __syncthreads();
     // the keys of tokens t0 + 32 m + col, as operands; their norms (fp16) by row
     // of the product's layout: row 8 * (i / 4) + 4 * half + i % 4
     half8_t kh[MT][KS], kl[MT][KS];
@@ -1394,7 +1383,7 @@ void window_kernel(WindowParams p) {
         c[k] = v[0]; c[k + 1] = v[1]; c[k + 2] = v[2]; c[k + 3] = v[3];
       }
 #pragma unroll
-      for (int k = 0; k < KS; k++) key_parts(c[k], sm.lut, lanec, kh[m][k], kl[m][k]);
+      for (int k = 0; k < KS; k++) key_parts<COPIES>(c[k], sm.lut, lanec, kh[m][k], kl[m][k]);
 #pragma unroll
       for (int i = 0; i < 8; i++) {
         const int r = 8 * (i / 2) + 4 * half + 2 * (i % 2);
@@ -1411,7 +1400,7 @@ void window_kernel(WindowParams p) {
     bool all = t0 + 32 * MT <= c1;  // every token of the wave is there
 #pragma unroll
     for (int m = 0; m < MT; m++) all = all && okm[m] == 0xffffffffu;
-    __syncthreads();  // the table is no longer read
+    __syncthreads();  // the last chunk's operands are no longer read
     // a row tile's scale, one tile ahead and in front of the copies
     float next_q = qs[col];
     issue(0);
@@ -1436,7 +1425,6 @@ void window_kernel(WindowParams p) {
       const float cq = next_q * p.csc, ls = SUM ? sm.lse[row] : 0.f;
       if (rt + 1 < p.tiles) {
         next_q = qs[row + 32];
-        issue(rt + 1);
       }
       if constexpr (!SUM)
         if (rt) join_tile(rt - 1);
@@ -1445,20 +1433,31 @@ void window_kernel(WindowParams p) {
       for (int m = 0; m < MT; m++)
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[m][i] = 0.f;
-      const uint32_t at = lds_addr(sm.q[rt & 1]) + lane * 16;
+      const half8_t* const f = reinterpret_cast<const half8_t*>(sm.q[rt & 1]) + lane;
 #pragma unroll
-      for (int k = 0; k < KS; k += 2) {
-        half8_t f[4];
-        read_operands(at + k * 2048, f);
+      for (int k = 0; k < KS; k++) {
+        const half8_t fh = f[k * 128], fl = f[k * 128 + 64];
 #pragma unroll
-        for (int z = 0; z < 3; z++)  // hi hi, lo hi, hi lo
-#pragma unroll
-          for (int y = 0; y < 2; y++)
-#pragma unroll
-            for (int m = 0; m < MT; m++)
-              acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                  z == 1 ? kl[m][k + y] : kh[m][k + y], f[2 * y + (z == 2)], acc[m], 0, 0, 0);
+        for (int m = 0; m < MT; m++) {
+          acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[m][k], fh, acc[m], 0, 0, 0);
+          acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl[m][k], fh, acc[m], 0, 0, 0);
+          acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[m][k], fl, acc[m], 0, 0, 0);
+        }
       }
+#if defined(__HIP_DEVICE_COMPILE__)
+      // reads ahead of the products (head size 256, two waves a SIMD: 78 us instead
+      // of 83 at 16384 tokens)
+      __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+      for (int k = 0; k < KS - 3; k++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 9, 0);
+#endif
+      if (rt + 1 < p.tiles) issue(rt + 1);
       // Tokens that this row's query sees: the tile's first row sees least.  Bit c of
       // seen(m): the token of accumulator row c (+ 4 in the upper half) is there and
       // seen; made anew for each tile, as masks kept over the loop spill.
@@ -1862,7 +1861,8 @@ struct WindowWs {
   int tiles, units;
 };
 // units of a window call: three workgroups a CU over the kv heads, at least one
-// per sequence
+// per sequence (with 4, 6, 8 a CU 32768 tokens took 161, 159, 157 us for 157, and
+// 4 prompts of up to 1500 45, 46, 47 for 35)
 WindowWs window_ws(int batch, int window, int ratio, int hkv, int pd, int cus) {
   WindowWs w;
   w.tiles = (window * ratio + 31) / 32;
@@ -2002,12 +2002,23 @@ extern "C" int tq_track_window(
   rc = launch(who, fr, rows / 4, 256, rargs, stream);
   if (rc) return rc;
   void* args[] = {&p};
-  rc = launch(who, f0, (int64_t)ws.units * num_kv_heads, 256, args, stream);
+  // The first pass with two key tiles a wave, two workgroups a CU: half the LDS
+  // reads a product.  At head size 128 and where the table has two chunks of 256
+  // tokens a unit: 57.8 us instead of 64.8 at 32768 tokens, but 16.0 instead of
+  // 11.7 for 4 prompts of up to 1500.  (The second pass spills with two; so do
+  // both at head size 64.)
+  const int wide = max(batch, 2 * cus / num_kv_heads);
+  if (pd == 128 && p.lse && num_indices * block_size >= (int64_t)512 * wide) {
+    p.units = wide;
+    f0 = reinterpret_cast<const void*>(&window_kernel<128, 2, false>);
+  }
+  rc = launch(who, f0, (int64_t)p.units * num_kv_heads, 256, args, stream);
   if (rc) return rc;
   if (p.lse) {
     rc = launch(who, reinterpret_cast<const void*>(&window_lse_kernel), rows / 32, 256, args,
                 stream);
     if (rc) return rc;
+    p.units = ws.units;
   }
   return launch(who, f1, (int64_t)ws.units * num_kv_heads, 256, args, stream);
 }
