@@ -1861,8 +1861,8 @@ struct WindowWs {
   int tiles, units;
 };
 // units of a window call: three workgroups a CU over the kv heads, at least one
-// per sequence (with 4, 6, 8 a CU 32768 tokens took 161, 159, 157 us for 157, and
-// 4 prompts of up to 1500 45, 46, 47 for 35)
+// per sequence (with 4 or 6 a CU 32768 tokens took 132.5 us as with 3, 4 prompts
+// of up to 1500 34.2 and 38.5 for 29.4)
 WindowWs window_ws(int batch, int window, int ratio, int hkv, int pd, int cus) {
   WindowWs w;
   w.tiles = (window * ratio + 31) / 32;
@@ -1885,9 +1885,9 @@ WindowWs window_ws(int batch, int window, int ratio, int hkv, int pd, int cus) {
 // Whether the second pass joins the units' statistics itself, in each workgroup
 // again: where a thread would read at most 16 of them (units of a sequence of
 // average length x row tiles, over 8 half waves).  A launch less, measured with
-// 12 reads (4 prompts of up to 1500 tokens, 128 rows) 33.2 -> 30.4 us and with 8
-// (head size 64, 32 rows) 39.4 -> 37.5; with 86 (32768 tokens, 256 rows) it
-// would be 154 -> 170.
+// 12 reads (4 prompts of up to 1500 tokens, 128 rows) 30.4 -> 28.4 us and with 8
+// (head size 64, 32 rows) 29.7 -> 28.8; with 86 (32768 tokens, 256 rows) it
+// would be 130 -> 153.
 bool join_here(const WindowWs& w, int batch) {
   return (int64_t)w.units * w.tiles <= (int64_t)128 * batch;
 }
