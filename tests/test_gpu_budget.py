@@ -637,6 +637,14 @@ class _Meta:
         self.__dict__.update(kw)
 
 
+@pytest.mark.parametrize("batch,hq,hkv", [(1024, 2, 1), (2, 4096, 4096)])
+def test_documented_limits(batch, hq, hkv):
+    lens = [(7 * b) % 41 for b in range(batch)] if batch > 2 else [37, 20]
+    run_decode(C.make(batch, lens, hq, hkv, 64))
+    run_window(C.make(batch + 1, lens, hq, hkv, 64), [min(n, b % 9) for b, n in enumerate(lens)], 3)
+    run_evict(spread(C.make(batch + 2, lens, hq, hkv, 64)), 12, 3, 1)
+
+
 def test_offsets_beyond_32_bits():
     """Pages at the end of a cache of 8.8 GB (a slab is over 2^32 bytes) give the
     bits that the same pages in a small cache give."""
