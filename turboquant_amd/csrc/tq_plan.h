@@ -46,6 +46,16 @@ __device__ __forceinline__ float vmax3(float a, float b, float c) {
   return fmaxf(fmaxf(a, b), c);
 #endif
 }
+// largest magnitude of three
+__device__ __forceinline__ float vmax3_abs(float a, float b, float c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  float r;
+  asm("v_max3_f32 %0, |%1|, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+#else
+  return fmaxf(fmaxf(fabsf(a), fabsf(b)), fabsf(c));
+#endif
+}
 // max(x, x of lane l ror 8 within its row): one DPP max (the s_nop covers
 // the wait states of a DPP read after a VALU write of its source)
 __device__ __forceinline__ float max_ror8(float x) {

@@ -740,7 +740,12 @@ __device__ __forceinline__ void read_values(uint32_t row0, uint32_t row1, uint32
 #endif
 }
 
-constexpr float kValueScale = 1.4809800386428833f;  // levels near fp16 grid points (8.7e-5)
+// The V levels are one fp16 each (a second one would double the table reads that
+// feed the products): times this they lie within 8.7e-5 of fp16 grid points.
+constexpr float kValueScale = 1.4809800386428833f;
+// A wave scales the products probability x norm so that the largest one it has met
+// stays below 2^kTop.
+constexpr int kTop = 15;
 
 // fp16 pair, towards zero (a hi part: the lo part takes up the rest)
 __device__ __forceinline__ uint32_t pack_rtz(float a, float b) {
@@ -760,14 +765,23 @@ __device__ __forceinline__ void nibble_pairs(uint32_t a, uint32_t b, uint32_t& e
 // the scores' tile (16x16x16), or of a pair of tiles (PACK: 16x16x32, whose 8
 // k-values of a lane are tokens 4 * (l/16) .. + 3 of either tile).  Dim of (row
 // r, product i) is r * (PD/16) + i.  QC: columns 0-7 hold the hi parts of p *
-// norm, 8-15 the lo parts.  Probabilities are relative to the sequence's
-// maximum in the product and normalised at the end.
+// norm, 8-15 the lo parts; else p * norm is one fp16 (2^-12 relative, to nearest:
+// a second operand would cost a product more for each).  Probabilities are
+// relative to the sequence's maximum in the product and normalised at the end.
+//
+// p * norm has the range of fp32: V norms go down to 6e-8, and the tail of a
+// long sequence holds most of its weight in small pieces.  So the norms are
+// scaled by a power of two, which follows the largest p * norm that the wave has
+// met: what hi and lo parts lose is below 2^-38 of that one.  Unscaled, rows of
+// norm 0.01 lost up to a thousandth of such a tail and rows of norm 0.001 some
+// percent.  The scale changes rarely (a uniform branch), the products so far
+// with it; the check costs 1.3 us of 46 at 8 x 32768 tokens.
 //
 // Bound by memory: 49.2 us for 201 MB read (entries, scores, weights) and 16 MB
 // written, sizes as above.  One kernel for keys and values and a small one for
 // the weights would move the same bytes and save one prologue, at most 6%.
 template <int PD, int G, bool QC>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(PD == 256 ? 2 : 4)))
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4)))
 void track_values_kernel(TrackParams p) {
   using R = Rows<PD, G>;
   constexpr int NO = PD / 16;           // products per tile
@@ -842,6 +856,7 @@ void track_values_kernel(TrackParams p) {
   float4_t O[NO];
 #pragma unroll
   for (int i = 0; i < NO; i++) O[i] = float4_t{0.f, 0.f, 0.f, 0.f};
+  float scale = 0x1p100f;  // (uniform)
 
   // scores and weights of step s, loaded one step ahead of their use; lanes
   // whose tile is outside the unit or the cache read the arrays' start and are
@@ -899,12 +914,12 @@ void track_values_kernel(TrackParams p) {
     for (int i = 0; i < NS; i++) {
       const int t0 = s * R::TPS + sub + R::SUB * i, tl = PACK ? t0 + R::SUB : t0;
       uint32_t nv[4];
-      spread_norms(nr[i], nv);
+      spread_norms(__float_as_uint(lo_half(nr[i]) * scale), nv);
       float rel[4], g[4], x[4];
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         rel[r] = exp2_raw(cu.sc[i][r] - M);
-        x[r] = by_half(rel[r], nv[r]);
+        x[r] = rel[r] * __uint_as_float(nv[r]);
       }
       // tiles with tokens that are not there, or with the newest one (uniform)
       const int first = (st.tile0 + t0 + mine) * kTile + 4 * q4;
@@ -939,6 +954,21 @@ void track_values_kernel(TrackParams p) {
           if (r < left) cu.wt[i][r] = r == last ? g[r] : cu.wt[i][r] + g[r];
       }
       // B operand
+      const float big = vmax3_abs(vmax3_abs(x[0], x[1], x[2]), x[3], 0.f);
+      if (__any(big > (float)(1 << kTop))) {
+        float mx = max_ror8(big);
+        mx = vmax(mx, xor_lane(mx, 1));
+        mx = vmax(mx, xor_lane(mx, 2));
+        mx = vmax(mx, xor_lane(mx, 4));
+        mx = xor32_max(xor16_max(mx));
+        // (an infinite norm's outputs are no numbers whatever the scale)
+        const float by = ldexpf(1.0f, kTop - __builtin_amdgcn_frexp_expf(mx));
+        scale = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(scale * by)));
+#pragma unroll
+        for (int r = 0; r < 4; r++) x[r] *= by;
+#pragma unroll
+        for (int k = 0; k < NO; k++) O[k] *= by;
+      }
       uint32_t pb[4];
       if constexpr (QC) {
         uint32_t hi[2], lo[2];
@@ -1016,12 +1046,15 @@ void track_values_kernel(TrackParams p) {
       p.positions[((int64_t)pg * p.Hkv + kvh) * p.block_size + t % p.block_size] =
           p.ends[ps.b] - 1;
   }
-  if constexpr (QC) {  // hi and lo columns
+  // each wave's own scale taken out, hi and lo columns together
+  const float down = 1.0f / scale;
 #pragma unroll
-    for (int i = 0; i < NO; i++)
+  for (int i = 0; i < NO; i++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) O[i][r] += ror8(O[i][r]);
-  }
+    for (int r = 0; r < 4; r++) {
+      O[i][r] *= down;
+      if constexpr (QC) O[i][r] += ror8(O[i][r]);
+    }
   // the waves of a head meet in LDS, halving their number each time
 #pragma unroll
   for (int half = R::SUB / 2; half > 0; half /= 2) {
