@@ -139,7 +139,9 @@ __device__ __forceinline__ Share share_of(const TrackParams& p, int* st, bool wr
   s.c0 = s.ps.j * s.ps.U;
   s.c1 = s.c0 + s.ps.U;
   if (p.pair > 0) {
-    const int cut = s.c0 + min((s.ps.U * p.pair / 100 + 15) & ~15, s.ps.U);
+    // (64 bits: a sequence may have up to 2^30 tokens)
+    const int first = (int)(((int64_t)s.ps.U * p.pair / 100 + 15) & ~(int64_t)15);
+    const int cut = s.c0 + min(first, s.ps.U);
     s.c0 = second ? cut : s.c0;
     s.c1 = second ? s.c1 : cut;
   }
