@@ -197,13 +197,11 @@ int tq_decode_balanced_rows(int32_t batch, int32_t num_qo_heads, int32_t num_kv_
  * num_indices is the length of `indices`; table entries at or behind it, and
  * pages outside [0, num_blocks), count as empty: their tokens get no weight
  * and are not written.  A page stands once in the tables of a call (two
- * sequences would race for its weights and entries).  `ends` int32 [batch]: the
+ * sequences would race for its scores, weights and entries).  `ends` int32 [batch]: the
  * number of tokens that each sequence has seen, evicted ones included.  batch
  * <= 1024 (eviction: batch * num_kv_heads <= 65535), num_kv_heads <= 4096,
  * num_blocks * block_size < 2^31, the sum of seq_lens < 2^30.  A workspace
- * serves one call at a time and holds nothing between calls; the tracked
- * decode's holds a score for every token of the table and q head (num_indices *
- * block_size * num_qo_heads * 4 bytes), the others' are small beside it.
+ * serves one call at a time and holds nothing between calls.
  */
 
 /*
@@ -215,8 +213,12 @@ int tq_decode_balanced_rows(int32_t batch, int32_t num_qo_heads, int32_t num_kv_
  * ends - 1.  positions (and then ends) may be NULL.  o [batch, num_qo_heads,
  * head_dim] contiguous; a sequence without tokens gets a row of zeros.
  * The weights are fp32 sums of fp32 probabilities; equal inputs give equal bits.
+ *
+ * The workspace holds a score for every token and q head of `pages` pages, the
+ * smaller one of num_indices and num_blocks (a page stands once in the tables):
+ * pages * block_size * num_qo_heads * 4 bytes.
  */
-int64_t tq_decode_tracked_workspace_bytes(int32_t batch, int64_t num_indices,
+int64_t tq_decode_tracked_workspace_bytes(int32_t batch, int64_t pages,
                                           int32_t num_qo_heads, int32_t num_kv_heads,
                                           int32_t padded_dim, int32_t block_size);
 int tq_decode_paged_tracked(const void* q, int64_t q_stride_b, int64_t q_stride_h,

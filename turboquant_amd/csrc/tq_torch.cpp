@@ -17,6 +17,7 @@
 #include <torch/csrc/utils/pybind.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <array>
 #include <cmath>
 #include <optional>
@@ -195,8 +196,9 @@ bool decode_tracked(const Tensor& q, const Tensor& kv_cache, const Tensor& indic
       !record_of(weights, positions, ends, c, b, dev))
     return false;
   const c10::DeviceGuard guard(dev);
-  const int64_t bytes = tq_decode_tracked_workspace_bytes(b, indices.numel(), hq, num_kv_heads,
-                                                          padded_dim, c.block_size);
+  const int64_t bytes =
+      tq_decode_tracked_workspace_bytes(b, std::min<int64_t>(indices.numel(), c.num_blocks), hq,
+                                        num_kv_heads, padded_dim, c.block_size);
   if (bytes <= 0) return false;
   const Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
   if (!on(ws, dev)) return false;

@@ -82,7 +82,8 @@ struct TrackParams {
   const float* signs;
   float csc;  // score constant (log2 units)
   float osc;  // output constant
-  float* s;   // scores, log2 units [table tile][Hkv][ratio][16]
+  float* s;   // scores, log2 units [tile of the table, or of the cache][Hkv][ratio][16]
+  int by_page;  // which: a cache of fewer pages than the table has entries
   float2* stats;  // (max, sum) [Hkv][rows][rp]
   int32_t* split;
   float* po;  // partial outputs [rows][Hq][PD]
@@ -163,6 +164,7 @@ struct Stream {
   const TrackParams& p;
   int tile0, tiles;  // first tile of the sequence, tiles of the unit
   int ip, tpp;       // first table entry of the sequence, tiles per page
+  int row0;          // the unit's first tile in the table
   int w;
   int base, at0, at1, wt0, wt1;  // windows base and base + 1
   uint32_t goff[R::NJ];  // source offsets of this lane's copies inside a tile
@@ -170,7 +172,7 @@ struct Stream {
   __device__ __forceinline__ Stream(const TrackParams& pp, const PlanSlot& ps, int c0, int c1,
                                     int wave, int hg)
       : p(pp), tile0(c0 / kTile), tiles((c1 - c0 + kTile - 1) / kTile), ip(ps.ip),
-        tpp(pp.block_size / kTile), w(wave), base(0) {
+        tpp(pp.block_size / kTile), row0((int)((uint32_t)ps.ip * (uint32_t)tpp) + tile0), w(wave), base(0) {
     const int lane = threadIdx.x & 63;
     const int stride = p.Hkv * R::EBS;
     window(0, at0, wt0);
@@ -212,6 +214,12 @@ struct Stream {
   // place of tile t in the cache (-1: none) and in the weights
   __device__ __forceinline__ int place(int t) const {
     return __builtin_amdgcn_readlane(t < 64 * (base + 1) ? at0 : at1, t & 63);
+  }
+  // place of its scores: pages stand once in the tables, so that the scores of a
+  // table that is wider than the cache (rows padded to the longest context) take no
+  // more room than the cache's tokens
+  __device__ __forceinline__ int score_place(int t, int place) const {
+    return place < 0 || p.by_page ? place : row0 + t;
   }
   __device__ __forceinline__ int64_t weight_at(int t, int kvh) const {
     const int x = __builtin_amdgcn_readlane(t < 64 * (base + 1) ? wt0 : wt1, t & 63);
@@ -585,20 +593,17 @@ void track_scores_kernel(TrackParams p) {
   const uint32_t o_nrm = (sub + mine) * R::TILEB + (4 * q4 + (lane & 3)) * R::ROWB +
                          w % G * R::EBS + PD / 2;
   const uint32_t lanec = 8 * n;
-  // where this lane's scores of step s go: s * TPS tiles further
+  // this lane's scores inside a tile's
   const int64_t tile_floats = (int64_t)p.Hq * kTile;
-  float* const s_at = p.s + ((int64_t)ps.ip * st.tpp + st.tile0 + sub + mine) * tile_floats +
-                      (kvh * p.ratio + head) * kTile + 4 * q4;
+  float* const s_at = p.s + (kvh * p.ratio + head) * kTile + 4 * q4;
   float m = kNone, l = 0.f;
   float4_t sc[NS];
-  bool keep[NS];
+  int to[NS];  // their tile, -1: none
 
-  auto store = [&](int s) {  // the scores of step s
+  auto store = [&] {  // the scores of a step
 #pragma unroll
     for (int i = 0; i < NS; i++)
-      if (keep[i])
-        *reinterpret_cast<float4_t*>(s_at + (int64_t)(s * R::TPS + R::SUB * i) * tile_floats) =
-            sc[i];
+      if (to[i] >= 0) *reinterpret_cast<float4_t*>(s_at + to[i] * tile_floats) = sc[i];
   };
   const bool store_lane = head < p.ratio && (PACK || n < p.ratio);
 
@@ -616,7 +621,7 @@ void track_scores_kernel(TrackParams p) {
         read_keys<PD>(at + o_row + R::SUB * R::TILEB * i, at + o_nrm + R::SUB * R::TILEB * i, c[i],
                       nr[i]);
     }
-    if (s) store(s - 1);
+    if (s) store();
     barrier();  // every wave has read the slot
     st.issue(s + 2, sm.ring + (s & 1) * R::SLOT, spare);
     float4_t acc[R::NTW];
@@ -652,11 +657,11 @@ void track_scores_kernel(TrackParams p) {
       // all tokens of the tiles are there (uniform); else masks
       const int tl = PACK ? t0 + R::SUB : t0;  // the last tile
       const int p0 = st.place(t0), p1 = PACK ? st.place(tl) : p0;
-      keep[i] = store_lane;
+      const int a0 = st.score_place(t0, p0), a1 = PACK ? st.score_place(tl, p1) : a0;
+      to[i] = store_lane ? (mine ? a1 : a0) : -1;
       if (p0 < 0 || p1 < 0 || (st.tile0 + tl + 1) * kTile > c1) {
         const bool there = (mine ? p1 : p0) >= 0;
         const int left = c1 - (st.tile0 + t0 + mine) * kTile - 4 * q4;
-        keep[i] = keep[i] && there;
 #pragma unroll
         for (int r = 0; r < 4; r++) x[r] = there && r < left ? x[r] : -INFINITY;
       }
@@ -664,7 +669,7 @@ void track_scores_kernel(TrackParams p) {
       add_scores(x, m, l);
     }
   }
-  store(steps - 1);
+  store();
   // no copy may land after the workgroup's LDS is given away
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
   // a head's lanes meet: its other tile's, then the token groups
@@ -852,9 +857,7 @@ void track_values_kernel(TrackParams p) {
                          w % G * R::EBS + PD / 2;
   const uint32_t lanec = 4 * (lane & 31);
   const int64_t tile_floats = (int64_t)p.Hq * kTile;
-  const float* const s_at = p.s +
-                            ((int64_t)ps.ip * st.tpp + st.tile0 + sub + mine) * tile_floats +
-                            (kvh * p.ratio + min(head, p.ratio - 1)) * kTile + 4 * q4;
+  const float* const s_at = p.s + (kvh * p.ratio + min(head, p.ratio - 1)) * kTile + 4 * q4;
   float4_t O[NO];
 #pragma unroll
   for (int i = 0; i < NO; i++) O[i] = float4_t{0.f, 0.f, 0.f, 0.f};
@@ -871,17 +874,18 @@ void track_values_kernel(TrackParams p) {
 #pragma unroll
     for (int i = 0; i < NS; i++) {
       const int t0 = s * R::TPS + sub + R::SUB * i;
-      const bool ok0 = st.place(t0) >= 0;
-      const int64_t w0 = ok0 ? st.weight_at(t0, kvh) : -1;
+      const int p0 = st.place(t0), a0 = st.score_place(t0, p0);
+      const int64_t w0 = p0 >= 0 ? st.weight_at(t0, kvh) : -1;
       int64_t at = w0;
+      int of = a0;
       if constexpr (PACK) {
-        const bool ok1 = st.place(t0 + R::SUB) >= 0;
-        const int64_t w1 = ok1 ? st.weight_at(t0 + R::SUB, kvh) : -1;
+        const int p1 = st.place(t0 + R::SUB), a1 = st.score_place(t0 + R::SUB, p1);
+        const int64_t w1 = p1 >= 0 ? st.weight_at(t0 + R::SUB, kvh) : -1;
         at = mine ? w1 : w0;
+        of = mine ? a1 : a0;
       }
       a.at[i] = at;
-      a.sc[i] = *reinterpret_cast<const float4_t*>(
-          at >= 0 ? s_at + (int64_t)(s * R::TPS + R::SUB * i) * tile_floats : p.s);
+      a.sc[i] = *reinterpret_cast<const float4_t*>(at >= 0 ? s_at + of * tile_floats : p.s);
       a.wt[i] = *reinterpret_cast<const float4_t*>(p.weights + (at >= 0 ? at : 0) + 4 * q4);
     }
   };
@@ -1688,11 +1692,11 @@ TrackPlan track_plan(int batch, int pd, int g, int hg, bool qc) {
   return t;
 }
 
-// A tracked decode's workspace
+// A tracked decode's workspace, for scores of `pages` pages
 struct TrackWs {
   size_t stats, split, s, po, total;
 };
-TrackWs track_ws(int batch, int64_t entries, int hq, int hkv, int pd, int bs, int parts) {
+TrackWs track_ws(int batch, int64_t pages, int hq, int hkv, int pd, int bs, int parts) {
   const int ratio = hq / hkv;
   int rp = 1;
   while (rp < ratio) rp <<= 1;
@@ -1706,7 +1710,7 @@ TrackWs track_ws(int batch, int64_t entries, int hq, int hkv, int pd, int bs, in
   w.stats = take((size_t)hkv * parts * rp * 8);
   w.split = take((size_t)(batch + 2) * 4);
   // (a tile at least: tiles outside the table read the first one)
-  w.s = take((size_t)max(entries, (int64_t)1) * bs * hq * 4);
+  w.s = take((size_t)max(pages, (int64_t)1) * bs * hq * 4);
   w.po = take((size_t)parts * hq * pd * 4);
   w.total = at;
   return w;
@@ -1777,11 +1781,11 @@ int check_state(const char* who, const uint8_t* k, const uint8_t* v, const int32
 }  // namespace
 }  // namespace tq
 
-extern "C" int64_t tq_decode_tracked_workspace_bytes(int32_t batch, int64_t num_indices,
+extern "C" int64_t tq_decode_tracked_workspace_bytes(int32_t batch, int64_t pages,
                                                      int32_t num_qo_heads, int32_t num_kv_heads,
                                                      int32_t padded_dim, int32_t block_size) {
   using namespace tq;
-  const int rc = check_track("decode_tracked", batch, num_indices, num_qo_heads, num_kv_heads,
+  const int rc = check_track("decode_tracked", batch, pages, num_qo_heads, num_kv_heads,
                              padded_dim, block_size);
   if (rc) return rc;
   if (batch == 0) return 0;
@@ -1791,7 +1795,7 @@ extern "C" int64_t tq_decode_tracked_workspace_bytes(int32_t batch, int64_t num_
     set_error("decode_tracked: occupancy query failed");
     return kEinval;
   }
-  return (int64_t)track_ws(batch, num_indices, num_qo_heads, num_kv_heads, padded_dim, block_size,
+  return (int64_t)track_ws(batch, pages, num_qo_heads, num_kv_heads, padded_dim, block_size,
                            plan.rows)
       .total;
 }
@@ -1826,7 +1830,8 @@ extern "C" int tq_decode_paged_tracked(
     return kEinval;
   }
   const TrackWs ws =
-      track_ws(batch, num_indices, num_qo_heads, num_kv_heads, pd, block_size, plan.rows);
+      track_ws(batch, min(num_indices, num_blocks), num_qo_heads, num_kv_heads, pd, block_size,
+               plan.rows);
   if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < (int64_t)ws.total) {
     set_error("%s: the workspace must be 16-byte aligned and hold %lld bytes, got %lld", who,
               (long long)ws.total, (long long)workspace_bytes);
@@ -1861,6 +1866,7 @@ extern "C" int tq_decode_paged_tracked(
   p.csc = sm_scale * 1.4426950408889634f * isq / kLevelScale;
   p.osc = isq / kValueScale;
   p.s = reinterpret_cast<float*>(base + ws.s);
+  p.by_page = num_indices > num_blocks;
   p.stats = reinterpret_cast<float2*>(base + ws.stats);
   p.split = reinterpret_cast<int32_t*>(base + ws.split);
   p.po = reinterpret_cast<float*>(base + ws.po);

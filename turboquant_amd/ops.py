@@ -975,7 +975,8 @@ def decode_paged_tracked(q: torch.Tensor, kv_cache: torch.Tensor, indices: torch
     base = kv_cache.data_ptr()
     with torch.cuda.device(q.device):
         ws = _workspace(lib.tq_decode_tracked_workspace_bytes(
-            b, indices.numel(), hq, int(num_kv_heads), int(padded_dim), bs), q.device, what)
+            b, min(indices.numel(), nb), hq, int(num_kv_heads), int(padded_dim), bs), q.device,
+            what)
         rc = lib.tq_decode_paged_tracked(
             q.data_ptr(), q.stride(0), q.stride(1), _DTYPES[q.dtype], base,
             base + kv_cache.stride(0) * kv_cache.element_size(), indices.data_ptr(),
