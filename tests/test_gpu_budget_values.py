@@ -115,3 +115,16 @@ def test_norms_over_eight_decades(ratio, hkv, hd, order):
     set_norms(c, 1, norms)
     q = torch.from_numpy(c.rng.standard_normal((1, c.hq, c.hd))).to(torch.float16)
     run(c, q.to(DEV), q.double().numpy())
+
+
+@pytest.mark.parametrize("top", [20.0, 34.0, 45.0, 75.0])
+@pytest.mark.parametrize("ratio,hkv,hd", [(2, 256, 128), (10, 192, 64), (1, 128, 256)])
+def test_tiles_of_next_to_no_weight_in_front_of_heavy_ones(ratio, hkv, hd, top):
+    """Most tiles hold weights of e^-top of the heavy tokens', some 97 tokens apart,
+    so that a wave meets them in any order: its scale has to change by as much."""
+    c, q, qx = tail_case(hkv + hd, [1500], ratio, hkv, hd, top)
+    pg, off, _ = C.places(c, 0)
+    norms = np.abs(c.rng.standard_normal((c.nb, c.page, hkv))) / 60
+    norms[pg[60::97], off[60::97]] = 1.0 - 0.01 * c.rng.random((len(pg[60::97]), hkv))
+    set_norms(c, 0, norms)
+    run(c, q, qx)

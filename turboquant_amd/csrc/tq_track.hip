@@ -82,8 +82,10 @@ struct TrackParams {
   const float* signs;
   float csc;  // score constant (log2 units)
   float osc;  // output constant
-  float* s;   // scores, log2 units [tile of the table, or of the cache][Hkv][ratio][16]
-  int by_page;  // which: a cache of fewer pages than the table has entries
+  // scores, log2 units: [tile of the table][Hkv][ratio][16], or by_page, where the
+  // cache has fewer pages than the table entries, [page][Hkv][tile][ratio][16]
+  float* s;
+  int by_page;
   float2* stats;  // (max, sum) [Hkv][rows][rp]
   int32_t* split;
   float* po;  // partial outputs [rows][Hq][PD]
@@ -155,7 +157,7 @@ __device__ __forceinline__ Share share_of(const TrackParams& p, int* st, bool wr
 // A unit's tiles: where each lies, and the copies of a step.  Lane i of a
 // window holds what concerns tile 64 k + i: `at` its place in the cache in
 // tiles (page * tiles per page + place in the page; -1 outside the unit, the
-// table or the cache) and `wt` its place in the weights of kv head 0.  Two
+// table or the cache) and `wt` its place in the weights of kv head 0 (or -1).  Two
 // windows cover any three steps in a row, and tiles are looked up by readlane:
 // a load here would make the compiler wait for the copies in flight.
 template <int PD, int G>
@@ -189,7 +191,7 @@ struct Stream {
   __device__ __forceinline__ void window(int k, int& at, int& wt) const {
     const int t = 64 * k + (threadIdx.x & 63), g = tile0 + t;
     at = -1;
-    wt = 0;
+    wt = -1;
     const int64_t e = (int64_t)ip + g / tpp;
     if (t < tiles && e >= 0 && e < p.entries) {
       const int pg = p.indices[e];
@@ -211,19 +213,22 @@ struct Stream {
     asm volatile("s_waitcnt vmcnt(0)" : "+v"(at1), "+v"(wt1));
 #endif
   }
-  // place of tile t in the cache (-1: none) and in the weights
+  // place of tile t in the cache, -1: none
   __device__ __forceinline__ int place(int t) const {
     return __builtin_amdgcn_readlane(t < 64 * (base + 1) ? at0 : at1, t & 63);
   }
-  // place of its scores: pages stand once in the tables, so that the scores of a
-  // table that is wider than the cache (rows padded to the longest context) take no
-  // more room than the cache's tokens
-  __device__ __forceinline__ int score_place(int t, int place) const {
-    return place < 0 || p.by_page ? place : row0 + t;
-  }
-  __device__ __forceinline__ int64_t weight_at(int t, int kvh) const {
+  // the tile's place in kv head kvh's weights, in tiles, -1: none
+  __device__ __forceinline__ int weight_tile(int t, int kvh) const {
     const int x = __builtin_amdgcn_readlane(t < 64 * (base + 1) ? wt0 : wt1, t & 63);
-    return ((int64_t)x + (int64_t)kvh * tpp) * kTile;
+    return x < 0 ? -1 : x + kvh * tpp;
+  }
+  // ... of its scores, of a tile at weight_tile() w (the first one's if there is
+  // none).  Pages stand once in the tables, so that the scores of a table that is
+  // wider than the cache (rows padded to the longest context) take no more room than
+  // the cache's tokens.
+  __device__ __forceinline__ uint32_t score_tile(int t, int w, int kvh) const {
+    const uint32_t row = ((uint32_t)row0 + t) * p.Hkv + kvh;
+    return w < 0 ? 0u : p.by_page ? (uint32_t)w : row;
   }
   // the copies of step s into the slot at `dst` (spare: where a wave's copy
   // beyond the step's goes); every wave issues NJ of them, whatever they read:
@@ -594,16 +599,17 @@ void track_scores_kernel(TrackParams p) {
                          w % G * R::EBS + PD / 2;
   const uint32_t lanec = 8 * n;
   // this lane's scores inside a tile's
-  const int64_t tile_floats = (int64_t)p.Hq * kTile;
-  float* const s_at = p.s + (kvh * p.ratio + head) * kTile + 4 * q4;
+  float* const s_at = p.s + head * kTile + 4 * q4;
+  const uint32_t tile_floats = p.ratio * kTile;
   float m = kNone, l = 0.f;
   float4_t sc[NS];
-  int to[NS];  // their tile, -1: none
+  float* to[NS];  // where they go
+  bool keep[NS];
 
   auto store = [&] {  // the scores of a step
 #pragma unroll
     for (int i = 0; i < NS; i++)
-      if (to[i] >= 0) *reinterpret_cast<float4_t*>(s_at + to[i] * tile_floats) = sc[i];
+      if (keep[i]) *reinterpret_cast<float4_t*>(to[i]) = sc[i];
   };
   const bool store_lane = head < p.ratio && (PACK || n < p.ratio);
 
@@ -656,11 +662,13 @@ void track_scores_kernel(TrackParams p) {
       for (int r = 0; r < 4; r++) x[r] = by_half(x[r], nv[r]) * csc;
       // all tokens of the tiles are there (uniform); else masks
       const int tl = PACK ? t0 + R::SUB : t0;  // the last tile
-      const int p0 = st.place(t0), p1 = PACK ? st.place(tl) : p0;
-      const int a0 = st.score_place(t0, p0), a1 = PACK ? st.score_place(tl, p1) : a0;
-      to[i] = store_lane ? (mine ? a1 : a0) : -1;
+      const int p0 = st.weight_tile(t0, kvh), p1 = PACK ? st.weight_tile(tl, kvh) : p0;
+      const uint32_t a0 = st.score_tile(t0, p0, kvh);
+      to[i] = s_at + (uint64_t)(mine ? st.score_tile(tl, p1, kvh) : a0) * tile_floats;
+      keep[i] = store_lane;
       if (p0 < 0 || p1 < 0 || (st.tile0 + tl + 1) * kTile > c1) {
         const bool there = (mine ? p1 : p0) >= 0;
+        keep[i] = keep[i] && there;
         const int left = c1 - (st.tile0 + t0 + mine) * kTile - 4 * q4;
 #pragma unroll
         for (int r = 0; r < 4; r++) x[r] = there && r < left ? x[r] : -INFINITY;
@@ -751,8 +759,11 @@ __device__ __forceinline__ void read_values(uint32_t row0, uint32_t row1, uint32
 // feed the products): times this they lie within 8.7e-5 of fp16 grid points.
 constexpr float kValueScale = 1.4809800386428833f;
 // A wave scales the products probability x norm so that the largest one it has met
-// stays below 2^kTop.
-constexpr int kTop = 15;
+// stays below 2^kTop; where one passes that, below 2^kFresh.
+constexpr int kTop = 15, kFresh = 11;
+// Before the first product; a wave without any keeps it, and sums of up to 2^35 of
+// others' products, taken to that scale, stay finite.
+constexpr float kUnscaled = 0x1p60f;
 
 // fp16 pair, towards zero (a hi part: the lo part takes up the rest)
 __device__ __forceinline__ uint32_t pack_rtz(float a, float b) {
@@ -779,10 +790,10 @@ __device__ __forceinline__ void nibble_pairs(uint32_t a, uint32_t b, uint32_t& e
 // p * norm has the range of fp32: V norms go down to 6e-8, and the tail of a
 // long sequence holds most of its weight in small pieces.  So the norms are
 // scaled by a power of two, which follows the largest p * norm that the wave has
-// met: what hi and lo parts lose is below 2^-38 of that one.  Unscaled, rows of
+// met: what hi and lo parts lose is below 2^-34 of that one.  Unscaled, rows of
 // norm 0.01 lost up to a thousandth of such a tail and rows of norm 0.001 some
 // percent.  The scale changes rarely (a uniform branch), the products so far
-// with it; the check costs 1.3 us of 46 at 8 x 32768 tokens.
+// with it; check and first change cost 0.5 to 1 us.
 //
 // Bound by memory: 49.2 us for 201 MB read (entries, scores, weights) and 16 MB
 // written, sizes as above.  One kernel for keys and values and a small one for
@@ -856,37 +867,42 @@ void track_values_kernel(TrackParams p) {
   const uint32_t o_nrm = (sub + mine) * R::TILEB + (4 * q4 + (lane & 3)) * R::ROWB +
                          w % G * R::EBS + PD / 2;
   const uint32_t lanec = 4 * (lane & 31);
-  const int64_t tile_floats = (int64_t)p.Hq * kTile;
-  const float* const s_at = p.s + (kvh * p.ratio + min(head, p.ratio - 1)) * kTile + 4 * q4;
+  const float* const s_at = p.s + min(head, p.ratio - 1) * kTile + 4 * q4;
+  float* const w_at = p.weights + 4 * q4;
+  const uint32_t tile_floats = p.ratio * kTile;
   float4_t O[NO];
 #pragma unroll
   for (int i = 0; i < NO; i++) O[i] = float4_t{0.f, 0.f, 0.f, 0.f};
-  float scale = 0x1p100f;  // (uniform)
+  float scale = kUnscaled;  // (uniform)
 
   // scores and weights of step s, loaded one step ahead of their use; lanes
   // whose tile is outside the unit or the cache read the arrays' start and are
   // masked
   struct Ahead {
     float4_t sc[NS], wt[NS];
-    int64_t at[NS];  // of the weights, -1: none
+    int at[NS];     // tiles of the weights, -1: none
+    bool there[NS];  // all of a set's tiles are (uniform)
   } nx, cu;
   auto load = [&](int s, Ahead& a) {
 #pragma unroll
     for (int i = 0; i < NS; i++) {
       const int t0 = s * R::TPS + sub + R::SUB * i;
-      const int p0 = st.place(t0), a0 = st.score_place(t0, p0);
-      const int64_t w0 = p0 >= 0 ? st.weight_at(t0, kvh) : -1;
-      int64_t at = w0;
-      int of = a0;
+      const int w0 = st.weight_tile(t0, kvh);
+      const uint32_t s0 = st.score_tile(t0, w0, kvh);
+      int at = w0;
+      uint32_t of = s0;
+      a.there[i] = w0 >= 0;
       if constexpr (PACK) {
-        const int p1 = st.place(t0 + R::SUB), a1 = st.score_place(t0 + R::SUB, p1);
-        const int64_t w1 = p1 >= 0 ? st.weight_at(t0 + R::SUB, kvh) : -1;
+        const int w1 = st.weight_tile(t0 + R::SUB, kvh);
+        const uint32_t s1 = st.score_tile(t0 + R::SUB, w1, kvh);
         at = mine ? w1 : w0;
-        of = mine ? a1 : a0;
+        of = mine ? s1 : s0;
+        a.there[i] = w0 >= 0 && w1 >= 0;
       }
       a.at[i] = at;
-      a.sc[i] = *reinterpret_cast<const float4_t*>(at >= 0 ? s_at + of * tile_floats : p.s);
-      a.wt[i] = *reinterpret_cast<const float4_t*>(p.weights + (at >= 0 ? at : 0) + 4 * q4);
+      a.sc[i] = *reinterpret_cast<const float4_t*>(s_at + (uint64_t)of * tile_floats);
+      a.wt[i] =
+          *reinterpret_cast<const float4_t*>(w_at + (uint64_t)(uint32_t)max(at, 0) * kTile);
     }
   };
   const bool store_lane = PACK ? (n & 7) == 0 : n == 0;
@@ -894,7 +910,7 @@ void track_values_kernel(TrackParams p) {
 #pragma unroll
     for (int i = 0; i < NS; i++)
       if (a.at[i] >= 0 && store_lane)
-        *reinterpret_cast<float4_t*>(p.weights + a.at[i] + 4 * q4) = a.wt[i];
+        *reinterpret_cast<float4_t*>(w_at + (uint64_t)(uint32_t)a.at[i] * kTile) = a.wt[i];
   };
   load(0, cu);
 
@@ -929,8 +945,7 @@ void track_values_kernel(TrackParams p) {
       }
       // tiles with tokens that are not there, or with the newest one (uniform)
       const int first = (st.tile0 + t0 + mine) * kTile + 4 * q4;
-      const bool whole = st.place(t0) >= 0 && st.place(tl) >= 0 &&
-                         (st.tile0 + tl + 1) * kTile < ps.L;
+      const bool whole = cu.there[i] && (st.tile0 + tl + 1) * kTile < ps.L;
       if (!whole) {
         const int left = cu.at[i] >= 0 ? c1 - first : 0;
 #pragma unroll
@@ -968,12 +983,13 @@ void track_values_kernel(TrackParams p) {
         mx = vmax(mx, xor_lane(mx, 4));
         mx = xor32_max(xor16_max(mx));
         // (an infinite norm's outputs are no numbers whatever the scale)
-        const float by = ldexpf(1.0f, kTop - __builtin_amdgcn_frexp_expf(mx));
-        scale = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(scale * by)));
+        const float by = ldexpf(1.0f, kFresh - __builtin_amdgcn_frexp_expf(mx));
 #pragma unroll
         for (int r = 0; r < 4; r++) x[r] *= by;
+        if (s || i)  // (else they are zero)
 #pragma unroll
-        for (int k = 0; k < NO; k++) O[k] *= by;
+          for (int k = 0; k < NO; k++) O[k] *= by;
+        scale = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(scale * by)));
       }
       uint32_t pb[4];
       if constexpr (QC) {
@@ -1052,34 +1068,38 @@ void track_values_kernel(TrackParams p) {
       p.positions[((int64_t)pg * p.Hkv + kvh) * p.block_size + t % p.block_size] =
           p.ends[ps.b] - 1;
   }
-  // each wave's own scale taken out, hi and lo columns together
-  const float down = 1.0f / scale;
+  if constexpr (QC) {  // hi and lo columns
 #pragma unroll
-  for (int i = 0; i < NO; i++)
+    for (int i = 0; i < NO; i++)
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-      O[i][r] *= down;
-      if constexpr (QC) O[i][r] += ror8(O[i][r]);
-    }
-  // the waves of a head meet in LDS, halving their number each time
+      for (int r = 0; r < 4; r++) O[i][r] += ror8(O[i][r]);
+  }
+  // the waves of a head meet in LDS, halving their number each time; a sum has the
+  // scale of the wave that goes on
 #pragma unroll
   for (int half = R::SUB / 2; half > 0; half /= 2) {
     float4_t* const buf = reinterpret_cast<float4_t*>(&sm) + lane;
-    static_assert(kWaves / 2 * NO * 1024 <= sizeof(Lds), "half the waves' outputs fit");
+    float* const scales = reinterpret_cast<float*>(&sm + 1) - kWaves;
+    static_assert(kWaves / 2 * NO * 1024 + kWaves * 4 <= sizeof(Lds),
+                  "half the waves' outputs and their scales fit");
     barrier();
-    if (sub >= half && sub < 2 * half)
+    if (sub >= half && sub < 2 * half) {
+      scales[w - half * G] = scale;
 #pragma unroll
       for (int i = 0; i < NO; i++) buf[((w - half * G) * NO + i) * 64] = O[i];
+    }
     lds_written();
     barrier();
-    if (sub < half)
+    if (sub < half) {
+      const float by = scale / scales[w];
 #pragma unroll
-      for (int i = 0; i < NO; i++) O[i] += buf[(w * NO + i) * 64];
+      for (int i = 0; i < NO; i++) O[i] += buf[(w * NO + i) * 64] * by;
+    }
     lds_written();
   }
   if (sub == 0 && n < p.ratio) {
     float* const row = p.po + ((int64_t)sh.row * p.Hq + kvh * p.ratio + n) * PD;
-    const float osc = inv * p.osc;
+    const float osc = inv * p.osc / scale;
 #pragma unroll
     for (int r = 0; r < 4; r++)
 #pragma unroll
