@@ -262,6 +262,11 @@ int tq_track_window(const void* q, int64_t num_rows, int64_t q_stride_tok, int64
  * seq_lens itself) = min(seq_lens[b], budget).  recent + sink <= budget;
  * positions and ends may be NULL if both are 0.  Attention does not depend on
  * the order of the entries, so decode goes on with the new lengths.
+ *
+ * The workspace holds the lists of moves, batch * num_kv_heads * min(budget, room)
+ * * 8 bytes with room = num_indices * block_size, or, where that is over 64 MiB
+ * and more than this, room * num_kv_heads * 4; and for a room beyond 32768 the
+ * entries' keys, room * num_kv_heads * 4.
  */
 int64_t tq_evict_workspace_bytes(int32_t batch, int32_t num_kv_heads, int64_t num_indices,
                                  int32_t block_size, int32_t budget);

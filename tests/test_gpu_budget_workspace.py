@@ -9,7 +9,8 @@ import pytest
 import torch
 
 import budget_cases as C
-from test_gpu_budget import DEV, check_o, check_weights, dev, queries, tensors
+from test_gpu_budget import (DEV, check_o, check_weights, dev, queries, run_evict, spread,
+                             tensors)
 from turboquant_amd import _lib, ops
 
 pytestmark = pytest.mark.gpu
@@ -96,3 +97,31 @@ def test_decode_refuses_a_workspace_that_is_too_small():
                 None, ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream)
             assert rc == want
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("page,packed", [(16, True), (48, False)])
+def test_evict_with_lists_by_table_place(page, packed):
+    """300 sequences under a budget of 20000: lists of their own for every row
+    would be over 64 MiB, so they stand where the sequences' tokens do.  One
+    sequence is cut by one entry, one to half, one beyond 32768 tokens."""
+    lens = [(7 * b) % 60 for b in range(300)]
+    lens[3], lens[100], lens[299] = 20001, 40000, 26017
+    if not packed:
+        lens[100] = 33000
+    c = spread(C.make(320 + page, lens, 2, 2, 64, page=page, packed=packed))
+    own = 300 * 2 * 20000 * 8
+    assert own > 64 << 20
+    got = _lib.load().tq_evict_workspace_bytes(300, 2, len(c.indices), page, 20000)
+    assert got < own or not packed
+    run_evict(c, 20000, 700, 4)
+
+
+def test_evict_lists_by_table_place_of_bad_tables():
+    """... with pages outside the cache and tokens behind the table."""
+    lens = [(7 * b) % 60 for b in range(300)]
+    lens[3], lens[299] = 20500, 45000
+    c = spread(C.make(331, lens, 2, 2, 64))
+    for at in (5, 700, 1290, len(c.indices) - 2, len(c.indices) - 900):
+        c.indices[at] = -1 if at % 2 else c.nb
+    c.lens[299] = 47000
+    run_evict(c, 20000, 300, 4)

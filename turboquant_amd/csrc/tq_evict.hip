@@ -39,10 +39,13 @@ struct EvictParams {
   int num_blocks, B, Hkv, block_size, shift;  // shift: log2 block_size or -1
   int budget, recent, sink;
   int64_t cap;  // moves per (sequence, head) at most
+  int64_t half;  // lists by table place: their length per head; 0: a row's own lists
   float* weights;
   int32_t* positions;
   uint32_t* keys;  // [Hkv][entries * block_size], for sequences longer than kChunk
-  int32_t* dst;    // [B * Hkv][cap] entry slots (page * block_size + place, -1: none)
+  // entry slots (page * block_size + place, -1: none), [B * Hkv][cap] or
+  // [Hkv][half], see lists_of
+  int32_t* dst;
   int32_t* src;
   int32_t* moves;  // [B * Hkv]
   uint8_t* ks;
@@ -62,6 +65,18 @@ __device__ __forceinline__ int slot_of(const EvictParams& p, int ip, int i) {
 __device__ __forceinline__ int64_t state_at(const EvictParams& p, int slot, int h) {
   const int pg = p.shift >= 0 ? slot >> p.shift : slot / p.block_size;
   return ((int64_t)pg * p.Hkv + h) * p.block_size + (slot - pg * p.block_size);
+}
+
+// Where a (sequence, head)'s lists start, and the moves that they have room for.
+// n tokens make at most n / 2 moves, so by table place the lists of a sequence
+// whose table starts at ip take half of what its tokens would.
+struct Lists {
+  int64_t at, room;
+};
+__device__ __forceinline__ Lists lists_of(const EvictParams& p, int bh, int h, int ip) {
+  if (!p.half) return {bh * p.cap, p.cap};
+  const int64_t first = (int64_t)ip * p.block_size / 2;
+  return {h * p.half + first, p.half - first};
 }
 
 // Larger key, kept sooner: 0 no entry (set elsewhere), 1 NaN, then the weights
@@ -333,9 +348,10 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(EvictParams p) {
     return part[0];
   };
   static_assert(kQuads * kSelWaves == 128, "scan() takes two counts a lane");
-  int32_t* const dst = p.dst + (int64_t)blockIdx.x * p.cap;
-  int32_t* const src = p.src + (int64_t)blockIdx.x * p.cap;
-  const uint32_t cap = (uint32_t)p.cap;
+  const Lists lists = lists_of(p, blockIdx.x, h, ip);
+  int32_t* const dst = p.dst + lists.at;
+  int32_t* const src = p.src + lists.at;
+  const uint32_t cap = (uint32_t)min(lists.room, (int64_t)(p.half ? n / 2 : p.budget));
   const bool ties = equal != need;
   const uint32_t from = ties && cut != kHeld ? cut + 1 : cut;  // kept: keys >= from
   uint32_t eq_base = 0, hole_base = 0, more_base = 0;
@@ -447,8 +463,9 @@ __global__ __launch_bounds__(256) void move_kernel(EvictParams p) {
   // and those before
   const int row = blockIdx.y * kMoveRows + lane;
   const int lb = row / groups, lh = row - lb * groups, lh0 = lh * kMoveHeads;
-  int lrounds = 0;
+  int lrounds = 0, lip = 0;
   if (lb < p.B) {
+    if (p.half) lip = p.indptr[lb];
     const int heads = min(kMoveHeads, p.Hkv - lh0);
     int most = 0;
 #pragma unroll
@@ -483,9 +500,10 @@ __global__ __launch_bounds__(256) void move_kernel(EvictParams p) {
     const int64_t m =
         (int64_t)(round - (k ? __builtin_amdgcn_readlane(lend, max(k - 1, 0)) : 0)) * per + im;
     const int bh = b * p.Hkv + nh0 + hm;
-    if ((int)threadIdx.x < npairs && m < p.cap) {
+    const Lists lists = lists_of(p, bh, nh0 + hm, __builtin_amdgcn_readlane(lip, k));
+    if ((int)threadIdx.x < npairs && m < lists.room) {
       const int n = p.moves[bh];
-      const int d = p.dst[bh * p.cap + m], s = p.src[bh * p.cap + m];
+      const int d = p.dst[lists.at + m], s = p.src[lists.at + m];
       to = m < n && s >= 0 ? d : -1;  // (-1: none, or on no page of the cache)
       of = s;
     }
@@ -539,9 +557,14 @@ __global__ __launch_bounds__(256) void move_kernel(EvictParams p) {
 
 size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
+// Lists of their own for every row, up to this many bytes of them; beyond, by
+// table place, where they take 4 bytes per token of the table and head and no batch
+// multiplies a budget that few sequences, or none, can exceed.
+constexpr int64_t kOwnLists = 64 << 20;
+
 struct EvictWs {
   size_t dst, src, moves, keys, total;
-  int64_t cap;
+  int64_t cap, half;
 };
 EvictWs evict_ws(int batch, int hkv, int64_t entries, int bs, int budget) {
   EvictWs w;
@@ -553,8 +576,10 @@ EvictWs evict_ws(int batch, int hkv, int64_t entries, int bs, int budget) {
     at += up256(n);
     return r;
   };
-  w.dst = take((size_t)batch * hkv * w.cap * 4);
-  w.src = take((size_t)batch * hkv * w.cap * 4);
+  const int64_t rows = batch * hkv * w.cap, tables = hkv * (room / 2);
+  w.half = rows * 8 > kOwnLists && tables < rows ? room / 2 : 0;
+  w.dst = take((size_t)(w.half ? tables : rows) * 4);
+  w.src = take((size_t)(w.half ? tables : rows) * 4);
   w.moves = take((size_t)batch * hkv * 4);
   w.keys = take(room > kChunk ? (size_t)room * hkv * 4 : 0);
   w.total = at;
@@ -655,6 +680,7 @@ extern "C" int tq_evict_paged(uint8_t* k_slab, uint8_t* v_slab, float* weights, 
   p.recent = recent;
   p.sink = sink;
   p.cap = ws.cap;
+  p.half = ws.half;
   p.weights = weights;
   p.positions = positions;
   p.keys = num_indices * block_size > kChunk ? reinterpret_cast<uint32_t*>(base + ws.keys)
