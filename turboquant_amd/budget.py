@@ -28,6 +28,8 @@ import torch
 from . import ops
 from .geometry import BALANCED_MAX_BATCH
 
+STARTS_KEPT = 64  # row widths whose starts a record keeps (4 KB each)
+
 
 class CacheRecord:
     """Weights and positions of one layer's cache, and the rule of its cuts."""
@@ -43,7 +45,8 @@ class CacheRecord:
         self.weights = torch.zeros(shape, dtype=torch.float32, device=device)
         self.positions = torch.zeros(shape, dtype=torch.int32, device=device)
         self.budget, self.recent, self.sink, self.window = budget, recent, sink, window
-        self._indptr: dict[tuple[int, int], torch.Tensor] = {}
+        self._starts: dict[int, torch.Tensor] = {}  # by row width
+        self._last = None  # ((rows, width), indptr) of the last call
 
     @classmethod
     def beside(cls, kv_cache: torch.Tensor, budget: int, **rule) -> "CacheRecord":
@@ -52,17 +55,31 @@ class CacheRecord:
         return cls(nb, bs, h, budget, device=kv_cache.device, **rule)
 
     def _tables(self, block_table: torch.Tensor):
-        """(indices, indptr) of a strided page table; the indptr of a shape is made
-        once, by a call that is not being captured (a graph's memory is its own)."""
+        """(indices, indptr) of a strided page table."""
         if block_table.dtype != torch.int32 or not block_table.is_contiguous():
             block_table = block_table.to(torch.int32).contiguous()
         b, width = key = tuple(block_table.shape)
-        indptr = self._indptr.get(key)
-        if indptr is None:
-            indptr = torch.arange(b + 1, dtype=torch.int32, device=block_table.device) * width
-            if not (indptr.is_cuda and torch.cuda.is_current_stream_capturing()):
-                self._indptr[key] = indptr
-        return block_table.reshape(-1), indptr
+        if self._last is None or self._last[0] != key:
+            starts = self._starts_of(width, b, block_table)
+            if starts is None:  # this call's own, on its stream
+                return block_table.reshape(-1), torch.arange(
+                    b + 1, dtype=torch.int32, device=block_table.device) * width
+            self._last = key, starts[:b + 1]
+        return block_table.reshape(-1), self._last[1]
+
+    def _starts_of(self, width: int, rows: int, block_table: torch.Tensor):
+        """Starts of up to BALANCED_MAX_BATCH rows of `width` pages, or None.  Made
+        on the host and copied before the call returns, so that any stream may use
+        them, but not inside a capture (a graph's memory is its own); kept for good,
+        as a graph may hold them, for at most STARTS_KEPT widths."""
+        if rows > BALANCED_MAX_BATCH:
+            return None
+        starts = self._starts.get(width)
+        if starts is None and len(self._starts) < STARTS_KEPT and not (
+                block_table.is_cuda and torch.cuda.is_current_stream_capturing()):
+            starts = torch.arange(BALANCED_MAX_BATCH + 1, dtype=torch.int32) * width
+            starts = self._starts[width] = starts.to(block_table.device)
+        return starts
 
     def decode(self, q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor,
                seq_lens: torch.Tensor, tokens_seen: torch.Tensor, num_kv_heads: int,

@@ -140,7 +140,8 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
             TQ_FORCE_KERNEL=gfx950_static.
     With a budget.CacheRecord as `record`, decode goes through
     turboquant_v5::decode_paged_tracked and every other batch is observed after
-    its attention (turboquant_v5::track_window).
+    its attention (turboquant_v5::track_window); a batch that cannot be recorded
+    (no cache, no lengths, a cache that is not packed) is refused.
     Prefill / mixed batches: _prefill_mixed (decode rows through the decode
     kernel, chunks with cached context over the dequantized context plus the
     fresh chunk, fresh prompts as in the reference, vllm_backend_fused.py:335-371).
@@ -518,6 +519,12 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
             if output is None:
                 output = torch.zeros_like(query)
             return output
+
+        if self.record is not None and not (self._is_fp8 and kv_cache is not None
+                                            and attn_metadata.seq_lens is not None):
+            # a later cut would go by weights and positions that miss these tokens
+            raise RuntimeError("a cache record needs a packed (fp8) kv_cache and seq_lens with "
+                               "every batch")
 
         is_decode = attn_metadata.max_query_len == 1
         if not is_decode:
