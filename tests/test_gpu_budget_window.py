@@ -1,0 +1,88 @@
+"""Windows over keys whose norms are no numbers or infinite, and rows without a
+query beside them."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import budget_cases as C
+from test_gpu_budget import check_weights, dev, queries, tensors
+from turboquant_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def set_key_norm(c, b, t, h, value):
+    pg, off, _ = C.places(c, b)
+    half, n = c.pd // 2, c.pd // 64
+    c.cache[0, pg[t], off[t], h, half:half + 2 * n] = np.full(n, value, np.float16).view(np.uint8)
+
+
+def observe(c, q, starts, window):
+    t = tensors(c)
+    ops.track_window(q, dev(np.asarray(starts, np.int32)), window, t["cache"], t["indices"],
+                     t["indptr"], t["seq"], c.hkv, c.hd, c.pd, c.scale, t["signs"], t["weights"],
+                     t["positions"], t["ends"])
+    torch.cuda.synchronize()
+    return t["weights"].cpu().numpy()
+
+
+@pytest.mark.parametrize("hd,window,chunk", [(128, 9, 20), (64, 40, 50), (256, 3, 2), (128, 70, 300)])
+def test_a_norm_that_is_no_number_stays_with_its_head(hd, window, chunk):
+    """The last query sees it, so every weight of that head and sequence that the
+    query adds to is no number; other heads and sequences are as without it."""
+    c = C.make(401 + hd, [400, 90], 8, 2, hd)
+    clean = C.make(401 + hd, [400, 90], 8, 2, hd)
+    set_key_norm(c, 0, 33, 1, np.nan)
+    q, qx = queries(c, chunk + 5, "fp16")
+    w = observe(c, q, [0, chunk, chunk + 5], window)
+    _, ref, _ = C.attend(clean, qx, np.array([0, chunk, chunk + 5]), window)
+    pg, off, _ = C.places(c, 0)
+    assert np.isnan(w[pg, 1, off]).all()
+    w[pg, 1, off], ref[pg, 1, off] = 0, 0
+    clean.weights[pg, 1, off] = 0
+    check_weights(clean, w, ref, qx, window * 4)
+
+
+@pytest.mark.parametrize("hd,hq", [(128, 2), (64, 2), (256, 2), (128, 8)])
+def test_a_window_of_one_is_the_decode_where_norms_are_infinite(hd, hq):
+    """An infinite norm's score is one of the infinities by the sign of its
+    product: weight 0, or no number for the whole row; 31 or 28 rows of the tile
+    have no query and add to neither."""
+    c = C.make(411 + hd, [100, 70], hq, 2, hd)
+    for t in (5, 60):
+        for h in range(2):
+            set_key_norm(c, 0, t, h, np.inf)
+    some = False
+    for seed in range(12):  # both signs come up
+        c.rng = np.random.default_rng(seed)
+        q, _ = queries(c, 2, "fp16")
+        w = observe(c, q, [0, 1, 2], 1)
+        t = tensors(c)
+        o = torch.empty_like(q)
+        ops.decode_paged_tracked(q, t["cache"], t["indices"], t["indptr"], t["seq"], 2, c.hd, c.pd,
+                                 c.scale, t["signs"], o, t["weights"], t["positions"], t["ends"])
+        d = t["weights"].cpu().numpy()
+        assert np.array_equal(np.isnan(w), np.isnan(d))
+        known = ~np.isnan(w)
+        assert np.allclose(w[known], d[known], rtol=1e-4, atol=0)
+        pg, off, _ = C.places(c, 0)
+        some = some or not np.isnan(w[pg, :, off]).any(0).all()  # (of one head)
+    assert some or hq > 2
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_missing_rows_add_nothing_to_keys_without_a_finite_norm(hd):
+    """Chunks whose rows are all behind the end of q: tokens from before keep their
+    weights and the chunk's get 0, whatever the norms."""
+    c = C.make(421 + hd, [50, 40], 4, 2, hd)
+    for t, value in ((10, np.nan), (20, np.inf), (48, np.nan)):
+        set_key_norm(c, 0, t, 0, value)
+    q, _ = queries(c, 4, "fp16")
+    w = observe(c, q, [6, 9, 11], 4)
+    want = c.weights.copy()
+    for b, n, chunk in ((0, 50, 3), (1, 40, 2)):
+        pg, off, _ = C.places(c, b)
+        want[pg[n - chunk:], :, off[n - chunk:]] = 0
+    assert np.array_equal(w, want)

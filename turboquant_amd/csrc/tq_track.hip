@@ -1517,16 +1517,21 @@ void window_kernel(WindowParams p) {
       __builtin_amdgcn_sched_group_barrier(0x008, 9, 0);
 #endif
       if (rt + 1 < p.tiles) issue(rt + 1);
-      // Tokens that this row's query sees: the tile's first row sees least.  Bit c of
+      // Tokens that this row's query sees: the tile's first row sees least, and a row
+      // that gives no weights nothing (its products may be no numbers, where a norm is
+      // not finite; the first pass need not know, its statistics of such rows are not
+      // used).  Bit c of
       // seen(m): the token of accumulator row c (+ 4 in the upper half) is there and
       // seen; made anew for each tile, as masks kept over the loop spill.
-      const bool clear = all && t0 + 32 * MT - 1 <= ps.L - p.window + rt * 32 / p.ratio;
+      const bool none = SUM && ls == INFINITY;
+      const bool clear =
+          all && t0 + 32 * MT - 1 <= ps.L - p.window + rt * 32 / p.ratio && !__any(none);
       auto seen = [&](int m) {
         uint32_t ok = okm[m];
 #if defined(__HIP_DEVICE_COMPILE__)
         asm volatile("" : "+s"(ok));
 #endif
-        const int last = ps.L - p.window + row / p.ratio - (t0 + 32 * m);
+        const int last = none ? -1 : ps.L - p.window + row / p.ratio - (t0 + 32 * m);
         return (ok & (last < 0 ? 0u : 0xffffffffu >> (31 - min(last, 31)))) >> (4 * half);
       };
 #pragma unroll
