@@ -86,3 +86,37 @@ def test_missing_rows_add_nothing_to_keys_without_a_finite_norm(hd):
         pg, off, _ = C.places(c, b)
         want[pg[n - chunk:], :, off[n - chunk:]] = 0
     assert np.array_equal(w, want)
+
+
+@pytest.mark.parametrize("scale", [1e5, 1e9, 1e20, 1e30, 3e35])
+@pytest.mark.parametrize("hq,hkv,hd", [(8, 2, 128), (16, 1, 64), (2, 2, 256)])
+def test_scores_of_any_size(hq, hkv, hd, scale):
+    """Scores far beyond what exp2 takes: a row's whole weight is on one key, also
+    where every score is hugely negative (a sequence of one token among them)."""
+    c = C.make(431 + hd, [100, 1, 47], hq, hkv, hd)
+    t = tensors(c)
+    q, qx = queries(c, 3 + 40, "bf16", scale)
+    assert torch.isfinite(q).all()
+    k0 = c.weights.copy()
+    for starts, window, rows in (([0, 1, 2, 3], 1, 3), ([0, 30, 31, 40], 6, 40)):
+        x, xx = q[:rows], qx[:rows]
+        ref_o, ref, _ = C.attend(c, xx, np.array(starts), window, True, decode=window == 1)
+        # one token a row and head: whole numbers are added (or, if new, set)
+        fresh = np.zeros(k0.shape, bool)
+        for b in range(3):
+            pg, off, _ = C.places(c, b)
+            n, chunk = int(c.lens[b]), starts[b + 1] - starts[b]
+            fresh[pg[n - chunk:], :, off[n - chunk:]] = True
+        added = np.rint(ref - np.where(fresh, 0, k0))
+        assert np.abs(ref - np.where(fresh, 0, k0) - added).max() < 1e-9
+        want = np.where(fresh, added, k0 + added).astype(np.float32)
+        assert np.array_equal(observe(c, x, starts, window), want)
+        if window == 1:
+            o = torch.empty_like(x)
+            ops.decode_paged_tracked(x, t["cache"], t["indices"], t["indptr"], t["seq"], hkv, hd,
+                                     c.pd, c.scale, t["signs"], o, t["weights"], t["positions"],
+                                     t["ends"])
+            assert np.array_equal(t["weights"].cpu().numpy(), want)
+            # one value row: its level's 8.7e-5, and the output's rounding
+            err = np.abs(o.double().cpu().numpy() - ref_o)
+            assert (err <= 2.0 ** -8 * np.abs(ref_o) + 2e-4 * 30).all() and np.isfinite(err).all()

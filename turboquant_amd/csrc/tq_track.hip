@@ -39,7 +39,7 @@ namespace {
 
 constexpr int kThreads = 512;  // 8 waves
 constexpr int kWaves = 8;
-constexpr float kNone = -1e30f;  // maximum of no scores (finite: no inf - inf)
+constexpr float kNone = -0x1.fffffep127f;  // maximum of no scores (finite: no inf - inf)
 constexpr float kLevelScale = 64.0f;
 
 // ---- cached rows in LDS ----------------------------------------------------
@@ -392,6 +392,7 @@ __device__ __forceinline__ void spread_norms(uint32_t n, uint32_t* v) {
 
 // running maximum and sum of exp2 over four more scores
 __device__ __forceinline__ void add_scores(const float4_t& x, float& m, float& l) {
+#pragma clang fp contract(off)  // (scores that are stored rounded)
   const float mx = vmax3(vmax3(m, x[0], x[1]), x[2], x[3]);
   float e = 0.f;
 #pragma unroll
@@ -465,7 +466,7 @@ __device__ __forceinline__ void rotate_row(bool rotate, const float* s, float* x
 // exponent: x * 2^e = hi + lo to 22 bits, the lo parts of the large elements
 // normal numbers.
 __device__ __forceinline__ int row_exponent(float mx) {
-  return mx > 0.f && mx < INFINITY ? max(-100, min(100, 7 - ilogbf(mx))) : 0;
+  return mx > 0.f && mx < INFINITY ? min(100, 7 - ilogbf(mx)) : 0;
 }
 
 // ---- the keys: scores, and the splits' maxima and sums ----------------------
@@ -1356,6 +1357,9 @@ __device__ __forceinline__ void row_lse(const WindowParams& p, int kvh, int64_t 
 template <int PD, int MT, bool SUM>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PD == 256 || MT == 2 ? 2 : 3)))
 void window_kernel(WindowParams p) {
+  // A score is a rounded product in both passes: one fused with what is subtracted
+  // from it could pass the row's maximum by more than exp2 takes.
+#pragma clang fp contract(off)
   constexpr int KS = PD / 16;
   constexpr int EBS = Rows<PD, 1>::EBS;
   constexpr int QT = PD * 128;  // bytes of a row tile's operands
@@ -1548,14 +1552,14 @@ void window_kernel(WindowParams p) {
             const uint32_t bits = seen(m);
 #pragma unroll
             for (int i = 0; i < 16; i++)
-              acc[m][i] = bits & (1u << (8 * (i / 4) + i % 4)) ? fmaf(acc[m][i], cq, -ls)
+              acc[m][i] = bits & (1u << (8 * (i / 4) + i % 4)) ? acc[m][i] * cq - ls
                                                               : -INFINITY;
           }
         } else {
 #pragma unroll
           for (int m = 0; m < MT; m++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) acc[m][i] = fmaf(acc[m][i], cq, -ls);
+            for (int i = 0; i < 16; i++) acc[m][i] = acc[m][i] * cq - ls;
         }
 #pragma unroll
         for (int m = 0; m < MT; m++)
