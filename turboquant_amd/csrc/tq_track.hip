@@ -464,7 +464,7 @@ __device__ __forceinline__ void rotate_row(bool rotate, const float* s, float* x
 }
 // The power of two that brings a row's largest magnitude into [128, 256), as an
 // exponent: x * 2^e = hi + lo to 22 bits, the lo parts of the large elements
-// normal numbers.
+// normal numbers (and not below 2^-100: what it is taken out by stays one too).
 __device__ __forceinline__ int row_exponent(float mx) {
   return mx > 0.f && mx < INFINITY ? min(100, 7 - ilogbf(mx)) : 0;
 }
