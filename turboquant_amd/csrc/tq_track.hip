@@ -123,11 +123,12 @@ __device__ __forceinline__ PlanSlot unit_of(const Params& p, int* st, int u, int
 // What a workgroup of the two streaming kernels serves: tokens [c0, c1) of the
 // unit's sequence, for head group hg, as part `row` of the plan's.
 //
-// pair > 0: the grid is two workgroups a CU, and blocks u and u + grid / 2, which
-// the dispatcher puts on one CU, share a unit: the one that came first gets
-// `pair` percent of its tokens (rounded up to a tile).  Its waves are older and
-// win the arbitration, so of two equal shares the second finished 10 of 42 us
-// later at 8 x 32768 tokens, alone on its CU.
+// pair > 0: the grid is two workgroups a CU, and blocks u and u + grid / 2 share a
+// unit: the one that came first gets `pair` percent of its tokens (rounded up to a
+// tile).  Alone on the card the two were seen on one CU; the older one's waves win
+// the arbitration there, so of two equal shares the second finished 10 of 42 us
+// later at 8 x 32768 tokens.  Nothing but the time rests on where they run: beside
+// other streams the shares are just uneven.
 struct Share {
   PlanSlot ps;
   int c0, c1, hg, row;
@@ -358,7 +359,7 @@ __device__ __forceinline__ void read_keys(uint32_t row, uint32_t nrm, uint32_t* 
   (void)row; (void)nrm; (void)c; n = 0;
 #endif
 }
-template <int PD>  // 64 or 128; STEP: bytes from the first tile to the second
+template <int PD>  // 64 or 128
 __device__ __forceinline__ void read_key_pair(uint32_t row0, uint32_t row1, uint32_t nrm,
                                               uint32_t (*c)[PD / 32], uint32_t& n) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -1710,8 +1711,13 @@ TrackPlan track_plan(int batch, int pd, int g, int hg, bool qc) {
   if (occ.cus <= 0 || occ.per_cu <= 0) return t;
   t.units = max(batch, occ.cus * occ.per_cu / hg);
   t.rows = t.units;
-  // (not at head size 64, where the shares finish together: 32.1 + 26.6 us
-  // unpaired, 32.6 + 27.6 paired, 48 ragged sequences)
+  // Calls with pairs / with as many single units: 8 x 32768 tokens 93.9 / 95.3 us,
+  // 32 x 8192 93.2 / 94.5, 32 x 16384 of 8 q / 1 kv heads 42.2 / 43.5, head size 256
+  // 24 ragged sequences 60.1 / 63.0 and 8 x 32768 60.5 / 63.3; where a call is short
+  // the uneven shares cost: 8 x 4096 36.4 / 34.9, 1 x 32768 51.3 / 49.9, at head size
+  // 256 59.9 / 58.4.  Pairs in halves: 95.7, 95.0, 43.5, 62.4, 62.9, 35.1, 50.1, 58.5.
+  // (Not at head size 64, where the shares finish together: 32.1 + 26.6 us
+  // unpaired, 32.6 + 27.6 paired, 48 ragged sequences.)
   if (pd > 64 && occ.per_cu == 2 && occ.cus % hg == 0 && occ.cus / hg >= batch) {
     t.units = occ.cus / hg;
     t.pair = kPairShare;
@@ -1953,11 +1959,14 @@ WindowWs window_ws(int batch, int window, int ratio, int hkv, int pd, int cus) {
   return w;
 }
 // Whether the second pass joins the units' statistics itself, in each workgroup
-// again: where a thread would read at most 16 of them (units of a sequence of
-// average length x row tiles, over 8 half waves).  A launch less, measured with
+// again: where a thread would read at most 16 of them for a sequence of average
+// length (its units x row tiles, over 8 half waves).  A launch less, measured with
 // 12 reads (4 prompts of up to 1500 tokens, 128 rows) 30.4 -> 28.4 us and with 8
 // (head size 64, 32 rows) 29.7 -> 28.8; with 86 (32768 tokens, 256 rows) it
-// would be 130 -> 153.
+// would be 130 -> 153.  Lengths are on the GPU, so a skewed batch is judged by its
+// average too, and the threads of a long sequence's workgroups read more (units x
+// row tiles / 8 at most): one prompt of 32768 tokens among 16, 64 queries, takes
+// 148.8 us like this and 147.0 with the launch, one of 8192 among 4 39.1 and 38.2.
 bool join_here(const WindowWs& w, int batch) {
   return (int64_t)w.units * w.tiles <= (int64_t)128 * batch;
 }
