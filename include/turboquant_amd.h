@@ -240,6 +240,11 @@ int tq_decode_paged_tracked(const void* q, int64_t q_stride_b, int64_t q_stride_
  * index); a sequence with an empty chunk keeps its weights.  q has num_rows
  * rows; observed rows outside them count as missing.  window *
  * num_qo_heads / num_kv_heads <= 1024.
+ *
+ * The workspace holds the observed rows of every sequence, batch * num_kv_heads *
+ * rows * (4 * padded_dim + 8) bytes with rows = window * num_qo_heads /
+ * num_kv_heads rounded up to 32, and 8 * rows bytes for each work unit, at most
+ * max(batch * num_kv_heads, 3 * compute units) of them.
  */
 int64_t tq_track_window_workspace_bytes(int32_t batch, int32_t window, int32_t num_qo_heads,
                                         int32_t num_kv_heads, int32_t padded_dim);

@@ -478,9 +478,11 @@ __device__ __forceinline__ int row_exponent(float mx) {
 // tiles a step): lanes n < 8 take on the scores of the first tile and n >= 8
 // those of the second, which halves the work per score.
 //
-// Bound by memory.  8 x 32768 tokens, 32 q / 8 kv heads of 128: 46.5 us for 161
-// MB read and 32 MB of scores written; while it streams 5.6-6.3 TB/s, and 6-8 us
-// are the prologue (plan, q', table) in front of the first step.  Measured and
+// Bound by memory.  8 x 32768 tokens, 32 q / 8 kv heads of 128: 44.4 us for 169
+// MB read and 34 MB of scores written; 5.4 TB/s while it streams, and 6-8 us are
+// the prologue (plan, q', table) in front of the first step.  At head sizes 64 and
+// 256 (28.4 and 29.7 us for 103 and 86 MB) the prologue is a quarter of it and VALU
+// instructions are issued in 58 and 64% of the busy cycles.  Measured and
 // not kept, for the sum of a call's three kernels (114 us in that run): the next
 // two or four steps touched in L2 during the prologue, no gain and 3% slower;
 // one workgroup of 16 waves a CU instead of two of 8, 2% slower there and 11 to
@@ -797,8 +799,10 @@ __device__ __forceinline__ void nibble_pairs(uint32_t a, uint32_t b, uint32_t& e
 // percent.  The scale changes rarely (a uniform branch), the products so far
 // with it; check and first change cost 0.5 to 1 us.
 //
-// Bound by memory: 49.2 us for 201 MB read (entries, scores, weights) and 16 MB
-// written, sizes as above.  One kernel for keys and values and a small one for
+// Bound by memory: 44.8 us for 211 MB read (entries, scores, weights) and 17 MB
+// written, sizes as above (32.5 and 29.5 us for 118 and 97 MB at head sizes 64 and
+// 256, VALU issue in 65% of the busy cycles).  One kernel for keys and values and a
+// small one for
 // the weights would move the same bytes and save one prologue, at most 6%.
 template <int PD, int G, bool QC>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4)))
@@ -1509,8 +1513,8 @@ void window_kernel(WindowParams p) {
         }
       }
 #if defined(__HIP_DEVICE_COMPILE__)
-      // reads ahead of the products (head size 256, two waves a SIMD: 78 us instead
-      // of 83 at 16384 tokens)
+      // reads ahead of the products (head size 256, two waves a SIMD: a call of 78 us
+      // instead of 83, 16384 tokens, 64 queries of 16 q / 2 kv heads)
       __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
 #pragma unroll
       for (int k = 0; k < KS - 3; k++) {
