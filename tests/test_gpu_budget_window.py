@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import budget_cases as C
-from test_gpu_budget import check_weights, dev, queries, tensors
+from test_gpu_budget import DEV, check_weights, dev, queries, tensors
 from turboquant_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -120,3 +120,55 @@ def test_scores_of_any_size(hq, hkv, hd, scale):
             # one value row: its level's 8.7e-5, and the output's rounding
             err = np.abs(o.double().cpu().numpy() - ref_o)
             assert (err <= 2.0 ** -8 * np.abs(ref_o) + 2e-4 * 30).all() and np.isfinite(err).all()
+
+
+def test_a_captured_window_with_other_lengths():
+    """Replays after new lengths, chunks and tables have been written, with eager work
+    between them: what an eager call gives."""
+    c = C.make(441, [700, 90, 1], 16, 4, 128, packed=False)
+    t = tensors(c)
+    q, _ = queries(c, 400, "bf16")
+    starts = torch.tensor([0, 300, 390, 391], dtype=torch.int32, device=DEV)
+    first = {k: t[k].clone() for k in ("weights", "positions")}
+
+    def call():
+        for k, v in first.items():
+            t[k].copy_(v)
+        ops.track_window(q, starts, 20, t["cache"], t["indices"], t["indptr"], t["seq"], 4, 128, 128,
+                         c.scale, t["signs"], t["weights"], t["positions"], t["ends"])
+    call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call()
+    for lens, chunks in (([700, 90, 1], [300, 90, 1]), ([700, 2, 0], [1, 2, 0]), ([16, 90, 1], [16, 0, 1]),
+                         ([650, 90, 1], [100, 90, 1])):
+        t["seq"].copy_(torch.tensor(lens, dtype=torch.int32))
+        starts.copy_(torch.tensor([0, *np.cumsum(chunks)], dtype=torch.int32))
+        t["ends"].copy_(t["seq"] + 5)
+        g.replay()
+        torch.cuda.synchronize()
+        got = [t[k].clone() for k in first]
+        call()
+        torch.cuda.synchronize()
+        for a, k in zip(got, first):
+            assert torch.equal(a, t[k])
+
+
+@pytest.mark.parametrize("hd,hq", [(64, 32), (256, 32), (96, 96)])
+def test_a_window_over_units_of_several_chunks(hd, hq):
+    """32 kv heads leave few units: each walks several chunks of 128 tokens, in both
+    passes; row tiles of one and of three, bad pages inside."""
+    c = C.make(451 + hd, [5003, 900], hq, 32, hd)
+    c.indices[20], c.indices[230] = -1, c.nb
+    t = tensors(c)
+    starts = np.array([0, 60, 70], np.int32)
+    for window in (3, 70):
+        q, qx = queries(c, 70, "fp16")
+        for k in ("weights", "positions"):
+            t[k].copy_(dev(getattr(c, k)))
+        ops.track_window(q, dev(starts), window, t["cache"], t["indices"], t["indptr"], t["seq"], 32,
+                         hd, c.pd, c.scale, t["signs"], t["weights"], t["positions"], t["ends"])
+        _, ref, pos = C.attend(c, qx, starts, window)
+        check_weights(c, t["weights"].cpu().numpy(), ref, qx, window * hq // 32)
+        assert np.array_equal(t["positions"].cpu().numpy(), pos)
