@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define TQ_ABI_VERSION 13 /* what tq_abi_version() returns */
+#define TQ_ABI_VERSION 14 /* what tq_abi_version() returns */
 
 typedef struct ihipStream_t* tq_stream_t; /* == hipStream_t */
 
@@ -182,6 +182,34 @@ int tq_decode_partials_balanced(const void* q, int64_t q_stride_b, int64_t q_str
  */
 int tq_decode_balanced_rows(int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
                             int32_t padded_dim);
+
+/*
+ * Decode attention over a sliding window with sinks (no counterpart in the
+ * reference, whose decode attends over every cached token): the newest token
+ * of a sequence, seq_len - 1, sees the tokens t >= seq_len - window and those
+ * with t < sink.  q, o and the cache as in tq_decode_paged_balanced_rows
+ * (head_dim a multiple of 8); any batch.  window >= 1, sink >= 0.
+ *
+ * Page-table entries of pages that hold no token in sight are not read and may
+ * hold anything; num_indices is the length of `indices`, and tokens whose
+ * entry lies outside [0, num_indices), or names a page outside [0,
+ * num_blocks), count as absent.  A sequence without a token in sight gets a row
+ * of zeros.  The tokens in sight of any 1024 consecutive sequences add up to
+ * less than 2^30.  The workspace (any device memory of the given size, 16-byte
+ * aligned) serves one call at a time and holds nothing between calls; equal
+ * inputs give equal bits.
+ */
+int64_t tq_decode_window_workspace_bytes(int32_t batch, int32_t num_qo_heads,
+                                         int32_t num_kv_heads, int32_t padded_dim);
+int tq_decode_paged_window(const void* q, int64_t q_stride_b, int64_t q_stride_h,
+                           int32_t q_dtype, const uint8_t* k_slab, const uint8_t* v_slab,
+                           const int32_t* indices, int64_t num_indices, const int32_t* indptr,
+                           const int32_t* seq_lens, int32_t batch, int32_t num_qo_heads,
+                           int32_t num_kv_heads, int32_t head_dim, int32_t padded_dim,
+                           int32_t block_size, int32_t ebs, int64_t num_blocks, float sm_scale,
+                           const float* signs, int32_t window, int32_t sink, void* o,
+                           int32_t o_dtype, void* workspace, int64_t workspace_bytes,
+                           tq_stream_t stream);
 
 /*
  * Cache budget: attention that records what each cached entry receives, and

@@ -95,10 +95,14 @@ SIGNATURES = {
     "tq_evict_workspace_bytes": (_I64, [_I32, _I32, _I64, _I32, _I32]),
     "tq_evict_paged": (_I32, [_P, _P, _P, _P, _P, _I64, _P, _P, _P, _I32, _I32, _I32, _I32, _I32,
                               _I64, _I32, _I32, _I32, _P, _P, _I64, _P]),
+    "tq_decode_window_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32]),
+    "tq_decode_paged_window": (_I32, [_P, _I64, _I64, _I32, _P, _P, _P, _I64, _P, _P, _I32, _I32,
+                                      _I32, _I32, _I32, _I32, _I32, _I64, _F32, _P, _I32, _I32, _P,
+                                      _I32, _P, _I64, _P]),
     "tq_last_error": (ctypes.c_char_p, []),
     "tq_abi_version": (_I32, []),
 }
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 _lib = None
 

@@ -125,6 +125,10 @@ struct DecodeParams {
   // split_out[b + 1]; block 0 stores that table and U (split_out[B + 1]).
   int units;
   int32_t* split_out;
+  // sliding window (WIN kernels): the newest token, L - 1, sees the tokens
+  // t >= L - window and t < sink; `entries`: length of `indices`
+  int window, sink;
+  int64_t entries;
   float qk_scale;     // sm_scale * log2(e) / (sqrt(pd) * kCbScale)
   float inv_sqrt_pd;  // 1/sqrt(pd)
   float pv_scale;     // 1/(sqrt(pd) * kCbScale)
@@ -132,6 +136,25 @@ struct DecodeParams {
 
 constexpr int kPlanMaxBatch = 1024;  // sequences a balanced plan takes
 static_assert(kPlanMaxBatch == kPlanMost, "the plan stages that many lengths");
+
+// The tiles of a sequence of L tokens that hold a token its newest one sees:
+// `sinks` tiles from the start, then all from tile `sinks + skip` on.  Left out
+// tiles closed up, they are the `len` tokens that the split plan and the kernel
+// walk (their own places `skip` tiles further from tile `sinks` on), all seen
+// but those in [h0, h1), fewer than two tiles at the two borders.
+struct WindowSpan {
+  int sinks, skip, len, h0, h1;
+};
+__device__ __forceinline__ WindowSpan window_span(int L, int window, int sink) {
+  const int lo = max(L - window, 0);  // first token of the window
+  WindowSpan r;
+  r.h0 = min(sink, lo);
+  r.sinks = r.h0 / kTile + (r.h0 % kTile ? 1 : 0);
+  r.skip = max(lo / kTile - r.sinks, 0);
+  r.len = L - r.skip * kTile;
+  r.h1 = lo - r.skip * kTile;
+  return r;
+}
 
 // Per-lane register geometry of the decode math for padded head size PD.
 template <int PD>
@@ -629,8 +652,12 @@ constexpr bool kPvLo = TQ_PV_LO != 0;
 // and slot reads only).
 // ROWS: q rows of p.hd elements, fp16 or bf16 (else fp16 rows of PD; as a
 // run-time choice this cost the fp16 path 0.1 .. 0.6 us a step).
+// WIN: attention over a sliding window and the sinks (PLAN only).  The tokens
+// below are those of window_span, so the plan, the page walk, the copies and
+// the steps are the same; only a tile's place in the page table and the masks
+// at the two borders differ, and hidden tiles are never looked up or read.
 template <int PD, int G, int PACK, bool QC, bool PLAN, int MATH = TQ_DECODE_MATH,
-          bool ROWS = false>
+          bool ROWS = false, bool WIN = false>
 __global__ __launch_bounds__(64 * G)
 __attribute__((amdgpu_waves_per_eu(PD == 256 ? 2 : (PACK == 1 ? 3 : 4))))
 void decode_partials_kernel(DecodeParams p) {
@@ -685,6 +712,11 @@ void decode_partials_kernel(DecodeParams p) {
   // partial row
   int b, L, ip, c0, c1;
   int64_t row;
+  [[maybe_unused]] WindowSpan ws = {};
+  auto tokens = [&](int len) -> int {  // of the plan
+    if constexpr (WIN) return window_span(len, p.window, p.sink).len;
+    return len;
+  };
   if constexpr (PLAN) {
     const int rowmul = p.pair_pct > 0 ? 2 : 1;
     const bool writer = blockIdx.x == 0 && w == 0;
@@ -695,20 +727,28 @@ void decode_partials_kernel(DecodeParams p) {
       const bool in = lane < p.B;
       const int len = in ? max(p.seq_lens[lane], 0) : 0;
       const int ipl = in ? p.indptr[lane] : 0;
-      ps = plan_slot([&](int) { return len; }, [&](int) { return ipl; }, p.B, 1, p.units, bid,
+      const int tok = tokens(len);
+      ps = plan_slot([&](int) { return tok; }, [&](int) { return ipl; }, p.B, 1, p.units, bid,
                      rowmul, p.split_out, writer);
+      if constexpr (WIN)
+        ws = window_span(__builtin_amdgcn_readlane(len, ps.b & 63), p.window, p.sink);
     } else {
       // staged in LDS where the dequant table goes (built later): lengths,
       // then page-table starts, kPlanMaxBatch of each
       int* const st = reinterpret_cast<int*>(sm.klut);
       for (int i = threadIdx.x; i < kPlanMaxBatch; i += 64 * G) {
-        st[i] = i < p.B ? max(p.seq_lens[i], 0) : 0;
+        const int len = i < p.B ? max(p.seq_lens[i], 0) : 0;
+        st[i] = tokens(len);
         st[kPlanMaxBatch + i] = i < p.B ? p.indptr[i] : 0;
+        if constexpr (WIN) st[2 * kPlanMaxBatch + i] = len;
       }
       __syncthreads();
       ps = plan_slot([&](int i) { return st[64 * i + lane]; },
                      [&](int i) { return st[kPlanMaxBatch + 64 * i + lane]; }, p.B,
                      (p.B + 63) >> 6, p.units, bid, rowmul, p.split_out, writer);
+      if constexpr (WIN)
+        ws = window_span(__builtin_amdgcn_readfirstlane(st[2 * kPlanMaxBatch + max(ps.b, 0)]),
+                         p.window, p.sink);
       __syncthreads();  // the staging area is free again
     }
     if (ps.b < 0) return;  // unit beyond the plan: no row (uniform over the workgroup)
@@ -718,7 +758,9 @@ void decode_partials_kernel(DecodeParams p) {
     c0 = ps.j * ps.U;
     c1 = c0 + ps.U;
     if (p.pair_pct > 0) {
-      const int first = min((ps.U * p.pair_pct / 100 + 15) & ~15, ps.U);
+      // (a unit of a long sequence among many can pass 2^31 / 100 tokens)
+      const int share = WIN ? (int)((int64_t)ps.U * p.pair_pct / 100) : ps.U * p.pair_pct / 100;
+      const int first = min((share + 15) & ~15, ps.U);
       c0 = mem ? c0 + first : c0;
       c1 = mem ? c1 : c0 + first;
       row = 2 * (int64_t)(ps.Pb + ps.j) + mem;
@@ -841,10 +883,20 @@ void decode_partials_kernel(DecodeParams p) {
     uint64_t tmask = 0;
     int wtile = 2 * step0;
     int npg = -1;
+    // tile t's place in the sequence
+    auto place = [&](int t) -> int {
+      if constexpr (WIN) return t < ws.sinks ? t : t + ws.skip;
+      return t;
+    };
     auto page_of = [&](int t) -> int {
+      if constexpr (WIN) {
+        const int64_t e = (int64_t)ip + place(t) / tpp;
+        return t <= tile_last && e >= 0 && e < p.entries ? p.indices[e] : -1;
+      }
       return t <= tile_last ? p.indices[ip + t / tpp] : -1;
     };
     auto set_tile = [&](int t, int pg, bool& ok, uint32_t& lo, uint32_t& hi) {
+      t = place(t);
       ok = pg >= 0 && pg < p.num_blocks;
       const int64_t off =
           ok ? ((int64_t)pg * p.block_size + (t % tpp) * kTile) * tokstride : 0;
@@ -1149,14 +1201,15 @@ void decode_partials_kernel(DecodeParams p) {
       const int t_first = 2 * k * kTile;  // first token of this step
       // (uniform; read back as a scalar so that it stays one)
       const bool full = __builtin_amdgcn_readfirstlane(
-                            (okT[0] && okT[1] && t_first >= c0 && t_first + 2 * kTile <= c1)
+                            (okT[0] && okT[1] && t_first >= c0 && t_first + 2 * kTile <= c1 &&
+                             (!WIN || t_first >= ws.h1 || t_first + 2 * kTile <= ws.h0))
                                 ? 1 : 0) != 0;
       if (!full) {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
           const int T = PACK == 2 ? ptile : i / 4;
           const int t = (2 * k + T) * kTile + 4 * q4 + (i & 3);
-          valid[i] = okT[T] && t >= c0 && t < c1;
+          valid[i] = okT[T] && t >= c0 && t < c1 && (!WIN || t >= ws.h1 || t < ws.h0);
         }
       }
       uint32_t pw[NV / 2], pl[NV / 2];
@@ -1241,8 +1294,9 @@ void decode_partials_kernel(DecodeParams p) {
   float* const stage = reinterpret_cast<float*>(&sm) + (size_t)w * ratio * PD;
   const int64_t orow0 = row * p.Hq + kvh * ratio;  // first row of this wave
   if (n < ratio) {
-    // o = pv_scale * O / lsum' (p' = p * pv_scale in both O and lsum')
-    const float inv = lt > 0.f ? p.pv_scale / lt : 0.0f;
+    // o = pv_scale * O / lsum' (p' = p * pv_scale in both O and lsum'; a NaN
+    // sum of a windowed row makes the row NaN)
+    const float inv = lt > 0.f || (WIN && lt != lt) ? p.pv_scale / lt : 0.0f;
     float* dst = stage + n * PD + q4 * (PD / 4);
 #pragma unroll
     for (int r = 0; r < 4; r++) {
@@ -1254,8 +1308,11 @@ void decode_partials_kernel(DecodeParams p) {
       }
     }
     // natural-log LSE: (m + log2(sum p)) * ln 2 = (mb + log2(lsum')) * ln 2
+    // (a NaN sum as an infinite one: its weight in the merge is NaN)
     if (q4 == 0)
-      p.plse[orow0 + n] = lt > 0.f ? (st.mb + __log2f(lt)) * 0.69314718055994531f : -INFINITY;
+      p.plse[orow0 + n] = lt > 0.f             ? (st.mb + __log2f(lt)) * 0.69314718055994531f
+                          : (WIN && lt != lt) ? INFINITY
+                                              : -INFINITY;
   }
   // LDS operations of a wave complete in order: the reads below see the
   // writes above
@@ -1470,12 +1527,12 @@ typedef void (*PartialsFn)(DecodeParams);
 // register set when ratio <= 8 (head size 256 keeps one tile per set: two
 // would exceed the register file); q hi/lo parts share one B operand when
 // the GQA ratio leaves 8 columns free.
-template <bool PLAN, bool ROWS>
+template <bool PLAN, bool ROWS, bool WIN = false>
 PartialsFn partials_kernel_t(int pd, int G, int ratio) {
   const bool pack2 = ratio <= 8 && pd <= 128;
   const bool qc = ratio <= 8;
 #define TQ_FN(PDV, GV, PK, QCV) \
-  &decode_partials_kernel<PDV, GV, PK, QCV, PLAN, TQ_DECODE_MATH, ROWS>
+  &decode_partials_kernel<PDV, GV, PK, QCV, PLAN, TQ_DECODE_MATH, ROWS, WIN>
 #define TQ_PICK_G(PDV, PK, QCV)                               \
   switch (G) {                                                \
     case 8: return TQ_FN(PDV, (PDV == 256 ? 4 : 8), PK, QCV); \
@@ -1498,6 +1555,11 @@ PartialsFn partials_kernel(int pd, int G, int ratio, bool plan, bool rows = fals
   return !plan  ? partials_kernel_t<false, false>(pd, G, ratio)
          : rows ? partials_kernel_t<true, true>(pd, G, ratio)
                 : partials_kernel_t<true, false>(pd, G, ratio);
+}
+
+PartialsFn window_kernel(int pd, int G, int ratio, bool rows) {
+  return rows ? partials_kernel_t<true, true, true>(pd, G, ratio)
+              : partials_kernel_t<true, false, true>(pd, G, ratio);
 }
 
 // Checks shared by the partials launchers and the parameter block they fill
@@ -2053,4 +2115,131 @@ extern "C" int tq_decode_balanced_rows(int32_t batch, int32_t num_qo_heads,
   }
   const int hg = num_kv_heads / G;
   return max(max(batch, occ.cus * occ.per_cu / hg), 2 * (occ.cus / hg));
+}
+
+namespace tq {
+namespace {
+
+// Workspace of a windowed decode of up to kPlanMaxBatch sequences: the row
+// table, the partial LSEs, the partial rows (fp16).
+struct WindowWs {
+  int rows;
+  int64_t lse, po, bytes;  // byte offsets, and the whole
+};
+int window_ws(int batch, int hq, int hkv, int pd, WindowWs& w) {
+  const int ratio = hkv > 0 && hq > 0 && hq % hkv == 0 ? hq / hkv : 0;
+  const bool ok = batch >= 0 && ratio >= 1 && ratio <= 16 && (pd == 64 || pd == 128 || pd == 256);
+  const int G = ok ? decode_group_size(pd, hkv, ratio) : 0;
+  if (G == 0) {
+    set_error("decode_window: unsupported geometry (%d q heads, %d kv heads, padded_dim %d)", hq,
+              hkv, pd);
+    return kEinval;
+  }
+  const int b = min(batch, kPlanMaxBatch), hg = hkv / G;
+  w.rows = b;
+  for (int rows = 0; rows < 2; rows++) {
+    const Occupancy occ =
+        occupancy(reinterpret_cast<const void*>(window_kernel(pd, G, ratio, rows != 0)), 64 * G);
+    if (occ.cus <= 0 || occ.per_cu <= 0) {
+      set_error("decode_window: occupancy query failed");
+      return kEinval;
+    }
+    w.rows = max(max(w.rows, occ.cus * occ.per_cu / hg), 2 * (occ.cus / hg));
+  }
+  w.lse = (int64_t)align256((size_t)(b + 2) * 4);
+  w.po = w.lse + (int64_t)align256((size_t)w.rows * hq * 4);
+  w.bytes = w.po + (int64_t)w.rows * hq * pd * 2;
+  return 0;
+}
+
+}  // namespace
+}  // namespace tq
+
+extern "C" int64_t tq_decode_window_workspace_bytes(int32_t batch, int32_t num_qo_heads,
+                                                    int32_t num_kv_heads, int32_t padded_dim) {
+  tq::WindowWs w;
+  const int rc = tq::window_ws(batch, num_qo_heads, num_kv_heads, padded_dim, w);
+  return rc ? rc : w.bytes;
+}
+
+extern "C" int tq_decode_paged_window(
+    const void* q, int64_t q_stride_b, int64_t q_stride_h, int32_t q_dtype, const uint8_t* k_slab,
+    const uint8_t* v_slab, const int32_t* indices, int64_t num_indices, const int32_t* indptr,
+    const int32_t* seq_lens, int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
+    int32_t head_dim, int32_t padded_dim, int32_t block_size, int32_t ebs, int64_t num_blocks,
+    float sm_scale, const float* signs, int32_t window, int32_t sink, void* o, int32_t o_dtype,
+    void* workspace, int64_t workspace_bytes, tq_stream_t stream) {
+  using namespace tq;
+  const char* who = "decode_window";
+  if (window < 1 || sink < 0) {
+    set_error("%s: window %d must be positive and sink %d not negative", who, window, sink);
+    return kEinval;
+  }
+  if (head_dim <= 0 || head_dim > padded_dim || head_dim % 8 != 0) {
+    set_error("%s: head_dim %d must be a multiple of 8 up to padded_dim %d", who, head_dim,
+              padded_dim);
+    return kEinval;
+  }
+  if ((q_dtype != TQ_F16 && q_dtype != TQ_BF16) || (o_dtype != TQ_F16 && o_dtype != TQ_BF16)) {
+    set_error("%s: q and o must be fp16 or bf16", who);
+    return kEinval;
+  }
+  if (num_indices < 0 || (batch > 0 && (!o || !workspace))) {
+    set_error("%s: null pointer or negative num_indices", who);
+    return kEinval;
+  }
+  if ((uintptr_t)o % 8 || (uintptr_t)workspace % 16) {
+    set_error("%s: o must be 8-byte aligned and the workspace 16-byte aligned", who);
+    return kEinval;
+  }
+  // the shared checks, in front of the first query of the device
+  DecodeParams p;
+  int rc = decode_setup(q, q_stride_b, q_stride_h, k_slab, v_slab, indices, indptr, seq_lens, batch,
+                        num_qo_heads, num_kv_heads, padded_dim, block_size, ebs, num_blocks,
+                        sm_scale, signs, static_cast<float*>(workspace),
+                        static_cast<float*>(workspace), p, head_dim, q_dtype == TQ_BF16);
+  if (rc || batch == 0) return rc;
+  WindowWs w;
+  rc = window_ws(batch, num_qo_heads, num_kv_heads, padded_dim, w);
+  if (rc) return rc;
+  if (workspace_bytes < w.bytes) {
+    set_error("%s: the workspace holds %lld bytes, fewer than tq_decode_window_workspace_bytes", who,
+              (long long)workspace_bytes);
+    return kEinval;
+  }
+  uint8_t* const ws = static_cast<uint8_t*>(workspace);
+  int32_t* const table = reinterpret_cast<int32_t*>(ws);
+  float* const lse = reinterpret_cast<float*>(ws + w.lse);
+  float* const po = reinterpret_cast<float*>(ws + w.po);
+  // a plan takes kPlanMaxBatch sequences; more go in slices, one after the
+  // other on the stream
+  for (int a = 0; a < batch; a += kPlanMaxBatch) {
+    const int n = min(batch - a, kPlanMaxBatch);
+    p.q = static_cast<const _Float16*>(q) + a * q_stride_b;
+    p.indptr = indptr + a;
+    p.seq_lens = seq_lens + a;
+    p.B = n;
+    p.po = po;
+    p.plse = lse;
+    p.window = window;
+    p.sink = sink;
+    p.entries = num_indices;
+    const PartialsFn fn =
+        window_kernel(padded_dim, p.G, p.ratio, head_dim != padded_dim || p.q_bf16 != 0);
+    BalancedGrid g;
+    rc = balanced_grid(fn, p, w.rows, g);
+    if (rc) return rc;
+    p.S = 1;
+    p.cs = 1;
+    p.units = g.units;
+    p.pair_pct = g.pair_pct;
+    p.split_out = table;
+    rc = launch_partials(fn, p, g.blocks, stream);
+    if (rc) return rc;
+    rc = combine_splits(po, lse, n, 1, table, g.rows, num_qo_heads, padded_dim, signs,
+                        static_cast<_Float16*>(o) + (int64_t)a * num_qo_heads * head_dim, stream,
+                        head_dim, o_dtype == TQ_BF16);
+    if (rc) return rc;
+  }
+  return 0;
 }

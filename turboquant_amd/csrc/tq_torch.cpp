@@ -273,6 +273,41 @@ bool evict(const Tensor& kv_cache, const Tensor& weights, const OptTensor& posit
                         stream_of(dev)) == 0;
 }
 
+// ------------------------------------------------------------ sliding windows
+
+bool window_ok(int64_t window, int64_t sink) {
+  return window >= 1 && window <= INT32_MAX && sink >= 0 && sink <= INT32_MAX;
+}
+
+// ops.decode_paged_window
+bool decode_window(const Tensor& q, const Tensor& kv_cache, const Tensor& indices,
+                   const Tensor& indptr, const Tensor& seq_lens, int64_t num_kv_heads,
+                   int64_t head_dim, int64_t padded_dim, double sm_scale, const OptTensor& signs,
+                   const Tensor& o, int64_t window, int64_t sink) {
+  const c10::Device dev = q.device();
+  Cache c;
+  const float* sp = nullptr;
+  const int qt = dtype_code(q.scalar_type()), ot = dtype_code(o.scalar_type());
+  if (!on(q, dev) || q.dim() != 3 || q.size(2) != head_dim || q.stride(2) != 1 || !is_half(qt) ||
+      !on(o, dev) || !is_half(ot) || !o.is_contiguous() || o.sizes() != q.sizes() ||
+      !is_i32(indices, dev) || !is_i32(indptr, dev) || !is_i32(seq_lens, dev) ||
+      !cache_of(kv_cache, dev, c) || c.heads != num_kv_heads || !window_ok(window, sink) ||
+      !signs_of(signs, padded_dim, dev, sp))
+    return false;
+  const int64_t b = q.size(0), hq = q.size(1);
+  if (b == 0 || padded_dim > 256 || seq_lens.numel() < b || indptr.numel() < b) return false;
+  const c10::DeviceGuard guard(dev);
+  const int64_t bytes = tq_decode_window_workspace_bytes(b, hq, num_kv_heads, padded_dim);
+  if (bytes <= 0) return false;
+  const Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  if (!on(ws, dev)) return false;
+  return tq_decode_paged_window(
+             q.const_data_ptr(), q.stride(0), q.stride(1), qt, c.k, c.v, cptr<int32_t>(indices),
+             indices.numel(), cptr<int32_t>(indptr), cptr<int32_t>(seq_lens), b, hq, num_kv_heads,
+             head_dim, padded_dim, c.block_size, c.ebs, c.num_blocks, (float)sm_scale, sp, window,
+             sink, o.data_ptr(), ot, ws.data_ptr(), bytes, stream_of(dev)) == 0;
+}
+
 // -------------------------------------------------------------------- prefill
 
 using Request = std::array<int32_t, 5>;
@@ -628,6 +663,7 @@ PYBIND11_MODULE(_tq_torch, m) {
   m.def("decode_tracked", &decode_tracked, unlocked);
   m.def("track_window", &track_window, unlocked);
   m.def("evict", &evict, unlocked);
+  m.def("decode_window", &decode_window, unlocked);
   m.def("prefill_batch", &prefill_batch, unlocked);
   m.def("prefill_gather", &prefill_gather, unlocked);
   m.def("mse_quantize", &mse_quantize, unlocked);

@@ -1079,6 +1079,65 @@ def evict_paged(kv_cache: torch.Tensor, weights: torch.Tensor, positions: torch.
 
 
 # --------------------------------------------------------------------------
+# sliding windows with sinks: a query at position P sees the keys j with
+# P - window < j <= P, and those with j < sink
+# --------------------------------------------------------------------------
+
+def _check_window(window, sink, what):
+    _fit_int32(what, window=window, sink=sink)
+    if window < 1 or sink < 0:
+        raise RuntimeError(f"{what}: window {window} must be positive and sink {sink} not negative")
+
+
+def decode_paged_window(q: torch.Tensor, kv_cache: torch.Tensor, indices: torch.Tensor,
+                        indptr: torch.Tensor, seq_lens: torch.Tensor, num_kv_heads: int,
+                        head_dim: int, padded_dim: int, sm_scale: float,
+                        signs: torch.Tensor | None, o: torch.Tensor, window: int,
+                        sink: int = 0) -> torch.Tensor:
+    """Decode attention over a sliding window: q [B, Hq, head_dim] (fp16 or
+    bf16, head_dim a multiple of 8), one new token per sequence whose K/V is in
+    the cache already, -> o [B, Hq, head_dim] (fp16 or bf16, contiguous).  The
+    newest token, seq_lens[b] - 1, sees the last `window` tokens and the first
+    `sink`.  The page table is read where it holds pages in sight only, so that
+    the others may have been given back (their entries may hold anything); a
+    sequence with nothing in sight gets zeros.  Any batch.
+    tq_decode_paged_window; equal inputs give equal bits."""
+    if (_nat or _native()).decode_window(q, kv_cache, indices, indptr, seq_lens, num_kv_heads,
+                                         head_dim, padded_dim, sm_scale, signs, o, window, sink):
+        return o
+    what = "decode_paged_window"
+    _require_gpu(q, kv_cache, indices, indptr, seq_lens, o)
+    _check_q(q, head_dim, num_kv_heads, padded_dim, what)
+    nb, bs, ebs = _cache_geometry(kv_cache, num_kv_heads, what)
+    b, hq, _ = q.shape
+    _fit_int32(what, padded_dim=padded_dim)
+    _check_window(window, sink, what)
+    _check_tables(b, indices, indptr, seq_lens, what)
+    if o.dtype not in (torch.float16, torch.bfloat16) or tuple(o.shape) != tuple(q.shape) \
+            or not o.is_contiguous():
+        raise RuntimeError(f"{what}: o must be contiguous fp16 or bf16 [B, Hq, head_dim]")
+    signs, sp = _signs_ptr(signs, padded_dim, q, what)
+    if b == 0:
+        return o
+    if q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8 or q.stride(1) < head_dim:
+        q = _aligned16(q)  # rows that the kernel's 16-byte loads cannot take
+    lib = _lib.load()
+    base = kv_cache.data_ptr()
+    with torch.cuda.device(q.device):
+        ws = _workspace(lib.tq_decode_window_workspace_bytes(b, hq, int(num_kv_heads),
+                                                             int(padded_dim)), q.device, what)
+        rc = lib.tq_decode_paged_window(
+            q.data_ptr(), q.stride(0), q.stride(1), _DTYPES[q.dtype], base,
+            base + kv_cache.stride(0) * kv_cache.element_size(), indices.data_ptr(),
+            indices.numel(), indptr.data_ptr(), seq_lens.data_ptr(), b, hq, int(num_kv_heads),
+            int(head_dim), int(padded_dim), bs, ebs, nb, float(sm_scale), sp, int(window),
+            int(sink), o.data_ptr(), _DTYPES[o.dtype], ws.data_ptr(), ws.numel(),
+            _stream_ptr(q.device))
+    _lib.check(rc, what)
+    return o
+
+
+# --------------------------------------------------------------------------
 # torch.library registration under the reference's namespaces and schemas
 # --------------------------------------------------------------------------
 _registered = False
@@ -1243,7 +1302,7 @@ def _register_fakes() -> None:
     def _budget_fake(*args):  # they write their arguments and return nothing
         return None
 
-    for name in ("decode_paged_tracked", "track_window", "evict_paged"):
+    for name in ("decode_paged_tracked", "track_window", "evict_paged", "decode_paged_window"):
         register_fake(f"turboquant_v5::{name}", _budget_fake, lib=_libs[1])
 
 
@@ -1318,6 +1377,10 @@ def register_ops() -> None:
              "Tensor indices, Tensor indptr, Tensor seq_lens, Tensor? ends, int budget, "
              "int recent, int sink, Tensor(d!) new_lens) -> ()")
     d.impl("evict_paged", nothing(evict_paged), "CUDA")
+    # the operators of windowed layers
+    d.define(f"decode_paged_window(Tensor q, Tensor kv_cache, {table}, {geometry}, Tensor(a!) o, "
+             "int window, int sink=0) -> ()")
+    d.impl("decode_paged_window", nothing(decode_paged_window), "CUDA")
     _native()  # binds the write and the two balanced ops
     _libs.extend([w, d])
     _register_fakes()
