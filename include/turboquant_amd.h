@@ -384,6 +384,25 @@ int tq_prefill_gather(const uint8_t* k_slab, const uint8_t* v_slab, const int32_
                       tq_stream_t stream);
 
 /*
+ * The same for layers under a sliding window (no counterpart in the reference):
+ * of request i's ctx_lens[i] cached tokens only the first min(sink, firsts[i])
+ * and those from firsts[i] on (0 <= firsts[i] <= ctx_lens[i]) are read back,
+ * one after the other without a gap, then come the fresh rows.  A chunk that
+ * starts behind ctx tokens needs firsts = max(0, ctx - window + 1).  Table
+ * entries of pages without a token to read are not looked up.  key and value
+ * may be null when every fresh_len is 0.
+ */
+int tq_prefill_gather_window(
+    const uint8_t* k_slab, const uint8_t* v_slab, const int32_t* block_table,
+    int64_t block_table_stride, int32_t num_kv_heads, int32_t head_dim, int32_t padded_dim,
+    int32_t block_size, int32_t ebs, int64_t num_blocks, const float* signs, const void* key,
+    const void* value, int32_t in_dtype, int64_t k_stride_tok, int64_t k_stride_head,
+    int64_t v_stride_tok, int64_t v_stride_head, const int32_t* table_rows, const int32_t* ctx_lens,
+    const int32_t* firsts, const int32_t* fresh_starts, const int32_t* fresh_lens,
+    const int32_t* out_starts, int32_t num_requests, int32_t sink, void* out_k, void* out_v,
+    tq_stream_t stream);
+
+/*
  * Causal GQA attention of a prefill chunk over fp16 K/V (head_dim 64, 128 or 256):
  * o[i, h] = softmax_j(q[i, h] . k[j, h / r] * sm_scale) v[j, h / r] over keys
  * j <= (kv_len - q_len) + i, r = num_qo_heads / num_kv_heads.  q, o: fp16
@@ -451,6 +470,30 @@ int tq_prefill_attention_batch(
     const int32_t* kv_lens, const int32_t* kv_sources, int32_t num_requests, int32_t num_qo_heads,
     int32_t num_kv_heads, int32_t head_dim, int32_t padded_dim, float sm_scale, void* workspace,
     int64_t workspace_bytes, tq_stream_t stream);
+
+/*
+ * The same attention under a sliding window with sinks (no counterpart in the
+ * reference): a query at place P of its request's keys sees the keys j with
+ * P - window < j <= P, and those with j < sink.  Keys are counted as they
+ * stand, so the rows that tq_prefill_gather_window closes up serve as they are:
+ * behind the sinks a key's distance from a query does not change.  Key tiles
+ * out of sight are not read, and a key that a query does not see does not
+ * touch its row, whatever its K and V hold (NaN and infinities too).  window
+ * >= 1, sink >= 0, sm_scale > 0; bf16 queries in fp16's range.  The workspace
+ * must hold tq_prefill_window_workspace_bytes.
+ */
+int64_t tq_prefill_window_workspace_bytes(const int32_t* q_lens, const int32_t* kv_lens,
+                                          int32_t num_requests, int32_t num_qo_heads,
+                                          int32_t padded_dim, int32_t window, int32_t sink);
+int tq_prefill_attention_window(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head, int32_t q_dtype, const void* k,
+    int64_t k_stride_tok, int64_t k_stride_head, const void* v, int64_t v_stride_tok,
+    int64_t v_stride_head, const void* k2, const void* v2, int64_t k2_stride_tok,
+    int64_t k2_stride_head, void* o, int64_t o_stride_tok, int64_t o_stride_head, int32_t o_dtype,
+    const int32_t* q_starts, const int32_t* q_lens, const int32_t* kv_starts,
+    const int32_t* kv_lens, const int32_t* kv_sources, int32_t num_requests, int32_t num_qo_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t padded_dim, float sm_scale, int32_t window,
+    int32_t sink, void* workspace, int64_t workspace_bytes, tq_stream_t stream);
 
 /*
  * The algorithm library's TurboQuantMSE quantizer (reference

@@ -134,3 +134,166 @@ def test_reference_decode():
                         128, c.scale, c.signs)
     assert np.abs(o[:1] - ref).max() < 1e-4
     assert W.sees(9, 12, 3, 2).tolist() == [True] * 2 + [False] * 5 + [True] * 3 + [False] * 2
+
+
+# ---------------------------------------------------- prefill and read-back
+
+def _prefill(monkeypatch=None, **bad):
+    a = dict(q=_meta((40, 8, 128), torch.float16), o=_meta((40, 8, 128), torch.float16),
+             reqs=[(0, 30, 0, 50, 0)], hkv=2, hd=128, pd=128, scale=0.1, window=4, sink=0,
+             k=_meta((60, 2, 128), torch.float16), v=_meta((60, 2, 128), torch.float16), k2=None,
+             v2=None)
+    a.update(bad)
+    return ops.prefill_attention_window(a["q"], a["o"], a["reqs"], a["hkv"], a["hd"], a["pd"],
+                                        a["scale"], a["window"], a["sink"], a["k"], a["v"], a["k2"],
+                                        a["v2"])
+
+
+@pytest.mark.parametrize("bad,match", [
+    (dict(window=0), "must be positive"), (dict(sink=-1), "not negative"),
+    (dict(window=2 ** 31), "out of range"), (dict(sink=2 ** 40), "out of range"),
+    (dict(scale=0.0), "sm_scale"), (dict(scale=-0.1), "sm_scale"),
+    (dict(scale=float("nan")), "sm_scale"), (dict(scale=float("inf")), "sm_scale"),
+    (dict(q=_meta((40, 8, 128), torch.float32)), "fp16 or bf16"),
+    (dict(o=_meta((41, 8, 128), torch.float16)), "q / o must be"),
+    (dict(k=_meta((60, 2, 128), torch.bfloat16)), "k / v must be"),
+    (dict(k=_meta((60, 4, 128), torch.float16)), "k / v must be"),
+    (dict(v=None), "go together"), (dict(v=_meta((61, 2, 128), torch.float16)), "go together"),
+    (dict(reqs=[(20, 30, 0, 50, 0)]), "out of range"),
+    (dict(reqs=[(0, 30, 20, 50, 0)]), "out of range"),
+    (dict(reqs=[(0, 30, 0, 29, 0)]), "out of range"),
+    (dict(reqs=[(0, 30, 0, 50, 1)]), "out of range"),
+    (dict(reqs=[(-1, 30, 0, 50, 0)]), "out of range"),
+])
+def test_prefill_refusals(monkeypatch, bad, match):
+    monkeypatch.setattr(ops, "_require_gpu", lambda *t: None)
+    with pytest.raises(RuntimeError, match=f"prefill_attention_window: .*{match}"):
+        _prefill(**bad)
+
+
+def _gather(**bad):
+    half = lambda *s: torch.zeros(s, dtype=torch.float16)
+    a = dict(cache=torch.zeros((2, 9, 16, 2, 80), dtype=torch.uint8),
+             table=torch.zeros((2, 3), dtype=torch.int32), key=half(20, 2, 128),
+             value=half(20, 2, 128), reqs=[(0, 40, 30, 0, 5, 0)], sink=4, hd=128, pd=128, signs=None,
+             k=half(19, 2, 128), v=half(19, 2, 128))
+    a.update(bad)
+    return ops.prefill_gather_window(a["cache"], a["table"], a["key"], a["value"], a["reqs"],
+                                     a["sink"], a["hd"], a["pd"], a["signs"], a["k"], a["v"])
+
+
+@pytest.mark.parametrize("bad,match", [
+    (dict(sink=-1), "negative"), (dict(sink=2 ** 31), "out of range"),
+    (dict(key=None), "go together"), (dict(key=None, value=None), "out of range"),
+    (dict(key=_meta((20, 2, 128), torch.float64)), "float dtype"),
+    (dict(key=_meta((20, 2, 96), torch.float16)), "key/value must be"),
+    (dict(k=_meta((19, 2, 64), torch.float16)), "out_k / out_v"),
+    (dict(k=_meta((19, 2, 128), torch.bfloat16)), "out_k / out_v"),
+    (dict(k=_meta((18, 2, 128), torch.float16)), "out of range"),
+    (dict(cache=_meta((2, 9, 16, 4, 80), torch.uint8)), "kv heads"),
+    (dict(cache=None), "needs the cache"), (dict(table=None), "needs the cache"),
+    (dict(table=_meta((2, 3), torch.int64)), "block_table"),
+    (dict(reqs=[(2, 40, 30, 0, 5, 0)]), "table row"),
+    (dict(reqs=[(0, 49, 39, 0, 5, 0)]), "pages do not cover"),
+    (dict(reqs=[(0, 40, 41, 0, 5, 0)]), "out of range"),
+    (dict(reqs=[(0, 40, -1, 0, 5, 0)]), "out of range"),
+    (dict(reqs=[(0, -1, -1, 0, 5, 0)]), "out of range"),
+    (dict(reqs=[(0, 40, 29, 0, 5, 0)]), "out of range"),
+    (dict(reqs=[(0, 40, 30, 16, 5, 0)]), "out of range"),
+    (dict(reqs=[(0, 40, 30, 0, 5, 1)]), "out of range"),
+    (dict(reqs=[(0, 40, 30, 0, 5, -1)]), "out of range"),
+    (dict(signs=_meta((64,), torch.float32)), "signs"),
+])
+def test_gather_refusals(monkeypatch, bad, match):
+    monkeypatch.setattr(ops, "_require_gpu", lambda *t: None)
+    with pytest.raises(RuntimeError, match=match):
+        _gather(**bad)
+
+
+def test_prefill_and_gather_refuse_cpu_tensors():
+    half = lambda *s: torch.zeros(s, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        _prefill(q=half(40, 8, 128), o=half(40, 8, 128), k=half(60, 2, 128), v=half(60, 2, 128))
+    with pytest.raises(RuntimeError, match="GPU only"):
+        _gather()
+
+
+def _ints(*x):
+    return (ctypes.c_int32 * max(1, len(x)))(*x)
+
+
+@pytest.mark.parametrize("bad,match", [
+    (dict(window=0), b"window"), (dict(sink=-1), b"sink"), (dict(scale=0.0), b"sm_scale"),
+    (dict(scale=float("nan")), b"sm_scale"), (dict(pd=96), b"padded_dim"),
+    (dict(hq=7), b"multiple"), (dict(hkv=0), b"multiple"), (dict(hd=100), b"multiple of 8"),
+    (dict(hd=136), b"multiple of 8"), (dict(qt=0), b"fp16 or bf16"), (dict(ql=(50,)), b"q_len"),
+    (dict(ql=(-1,)), b"q_len"), (dict(qs=(-1,)), b"bad request"), (dict(ks=(-1,)), b"bad request"),
+    (dict(q=None), b"null"), (dict(k=None), b"null"), (dict(src=(1,)), b"null"),
+    (dict(st=1001), b"strides"), (dict(kst=64), b"strides"), (dict(off=8), b"aligned"),
+    (dict(n=-1), b"bad sizes"),
+])
+def test_abi_refuses_bad_prefill_arguments(bad, match):
+    lib = _lib.load()
+    buf, p = _buffer()
+    a = dict(q=p, st=1024, qt=1, k=p, kst=256, qs=(0,), ql=(20,), ks=(0,), kl=(40,), src=(0,), n=1,
+             hq=8, hkv=2, hd=128, pd=128, scale=0.1, window=4, sink=0, off=0)
+    a.update(bad)
+    q = a["q"] and a["q"] + a["off"]
+    rc = lib.tq_prefill_attention_window(
+        q, a["st"], 128, a["qt"], a["k"], a["kst"], 128, a["k"], a["kst"], 128, None, None, 0, 0, p,
+        1024, 128, 1, _ints(*a["qs"]), _ints(*a["ql"]), _ints(*a["ks"]), _ints(*a["kl"]),
+        _ints(*a["src"]), a["n"], a["hq"], a["hkv"], a["hd"], a["pd"], a["scale"], a["window"],
+        a["sink"], p, 1 << 40, None)
+    assert rc == -22 and match in lib.tq_last_error(), lib.tq_last_error()
+
+
+def test_prefill_workspace_follows_the_window():
+    """(without a GPU the plan is that of 256 CUs)  A short chunk's keys are split
+    where its window is long, and need no workspace where it is short."""
+    lib = _lib.load()
+    size = lambda w, s=0: lib.tq_prefill_window_workspace_bytes(_ints(100), _ints(20000), 1, 4, 128,
+                                                                w, s)
+    assert size(0) == 0 and size(5, -1) == 0 and size(200) == 0
+    assert size(19000) > 0 and size(2 ** 31 - 1, 2 ** 31 - 1) == \
+        lib.tq_prefill_batch_workspace_bytes(_ints(100), _ints(20000), 1, 4, 128)
+
+
+@pytest.mark.parametrize("bad,match", [
+    (dict(sink=-1), b"negative"), (dict(first=None), b"null"), (dict(first=(41,)), b"bad request"),
+    (dict(first=(-1,)), b"bad request"), (dict(ctx=(-1,), first=(-1,)), b"bad request"),
+    (dict(fresh=(-1,)), b"bad request"), (dict(out=(-1,)), b"bad request"),
+    (dict(row=(-1,)), b"bad request"), (dict(key=None), b"null"), (dict(k=None), b"null"),
+    (dict(pd=96), b"padded_dim"), (dict(ebs=81), b"ebs"), (dict(dt=5), b"dtype"),
+    (dict(n=-1), b"bad sizes"), (dict(o=8), b"aligned"),
+])
+def test_abi_refuses_bad_gather_arguments(bad, match):
+    lib = _lib.load()
+    buf, p = _buffer()
+    a = dict(k=p, key=p, dt=1, row=(0,), ctx=(40,), first=(30,), fs=(0,), fresh=(5,), out=(0,), n=1,
+             sink=4, hd=128, pd=128, bs=16, ebs=80, o=0)
+    a.update(bad)
+    rc = lib.tq_prefill_gather_window(
+        a["k"], a["k"], p, 3, 2, a["hd"], a["pd"], a["bs"], a["ebs"], 9, None, a["key"], a["key"],
+        a["dt"], 256, 128, 256, 128, _ints(*a["row"]), _ints(*a["ctx"]),
+        None if a["first"] is None else _ints(*a["first"]), _ints(*a["fs"]), _ints(*a["fresh"]),
+        _ints(*a["out"]), a["n"], a["sink"], p + a["o"], p, None)
+    assert rc == -22 and match in lib.tq_last_error(), lib.tq_last_error()
+
+
+def test_reference_prefill():
+    """In 64 bits: a window over everything is causal attention; rows of a window
+    of one token and no sinks are their own value; values out of sight do not
+    count."""
+    g = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn((n, h, 8), generator=g, dtype=torch.float64)
+               for n, h in ((5, 4), (9, 2), (9, 2)))
+    o = W.prefill(q, k, v, [(0, 5, 0, 9, 0)], 2, 0.3, 9, 0)
+    for i in range(5):
+        for h in range(4):
+            p = (k[:5 + i, h // 2] @ q[i, h] * 0.3).softmax(0)
+            assert torch.allclose(o[i, h], p @ v[:5 + i, h // 2])
+    o = W.prefill(q, k, v, [(0, 5, 0, 9, 0)], 2, 0.3, 1, 0)
+    assert torch.allclose(o, v[4:].repeat_interleave(2, 1))
+    v[2], v[8] = torch.nan, torch.inf
+    o = W.prefill(q, k, v, [(0, 5, 0, 9, 0)], 2, 0.3, 3, 1)
+    assert torch.isnan(o[0]).all() and torch.isfinite(o[1:4]).all() and (o[4] == torch.inf).all()

@@ -60,3 +60,31 @@ def decode(c, q, window, sink, signs=True):
     if signs:
         o = (o @ C.hadamard(c.pd)) * c.signs
     return o[..., :c.hd]
+
+
+def prefill(q, k, v, requests, ratio, scale, window, sink):
+    """o [T, Hq, D] (0 in rows of no request) of q [T, Hq, D] over k, v [R, Hkv,
+    D], all in 64 bits; torch tensors, on their device."""
+    import torch
+    o = torch.zeros_like(q)
+    for qs, ql, ks, kl, _ in requests:
+        for at in range(0, ql, 2048):
+            n = min(2048, ql - at)
+            pos = torch.arange(kl - ql + at, kl - ql + at + n, device=q.device)[:, None]
+            j = torch.arange(kl, device=q.device)[None]
+            see = (j <= pos) & ((j > pos - window) | (j < sink))
+            used = torch.nonzero(see.any(0))[:, 0]
+            see = see[:, used]
+            for h in range(q.shape[1]):
+                kk, vv = k[ks + used, h // ratio], v[ks + used, h // ratio]
+                s = (q[qs + at:qs + at + n, h] @ kk.T) * scale
+                p = torch.where(see, s, -torch.inf).softmax(-1)
+                # a hidden key adds nothing, whatever its value; one in sight has
+                # a weight above zero
+                out = p @ torch.where(torch.isfinite(vv), vv, 0.0)
+                hit = lambda x: see.double() @ x.double() > 0
+                up, down = hit(vv == torch.inf), hit(vv == -torch.inf)
+                out = torch.where(up, torch.inf, torch.where(down, -torch.inf, out))
+                out = torch.where(hit(torch.isnan(vv)) | (up & down), torch.nan, out)
+                o[qs + at:qs + at + n, h] = out
+    return o

@@ -13,7 +13,8 @@
 // tq_dequant_paged reads back one sequence; tq_prefill_gather assembles the
 // keys and values of all requests of a prefill step in one launch: each
 // request's cached context read back, followed by its fresh rows converted to
-// fp16, both padded to pd elements.
+// fp16, both padded to pd elements.  tq_prefill_gather_window reads of that
+// context only what a sliding window with sinks leaves in sight, closed up.
 //
 // One pass over the entries, L = pd/32 lanes per vector (32 dims = 16 code
 // bytes per lane, one 16-byte load), four vectors per thread with every load
@@ -46,6 +47,7 @@ constexpr int kMaxReqs = 64;
 struct GatherReq {
   int ctx, fresh, dst_row, src_row, bt_row;
   int ctx_blk, fresh_blk;  // first workgroup of each part
+  int sinks, gap;          // a window: the ctx tokens from `sinks` on stand gap places further
 };
 
 struct ReadBackParams {
@@ -126,11 +128,13 @@ __device__ __forceinline__ int find_request(int n, int blk, First first) {
 }
 
 // Cached vectors [block's range) of tokens 0 .. num_tokens - 1 (`pages` their
-// page-table row) to out (token 0's row).  blk: workgroup within the range.
+// page-table row; those from `sinks` on stand `gap` places further in it) to out
+// (token 0's row).  blk: workgroup within the range.
 template <int PD>
 __device__ __forceinline__ void read_back(const ReadBackParams& p, const int32_t* pages,
                                           int num_tokens, int blk, _Float16* out,
-                                          const float* cb, _Float16* stage) {
+                                          const float* cb, _Float16* stage, uint32_t sinks = 0,
+                                          uint32_t gap = 0) {
   constexpr int L = PD / 32;  // lanes per vector, 32 dims (16 code bytes) each
   constexpr int VPB = 256 / L, NV = kVecsPerThread;
   const int lane = threadIdx.x % L;
@@ -152,6 +156,7 @@ __device__ __forceinline__ void read_back(const ReadBackParams& p, const int32_t
     const uint32_t dt = div_heads(p, r);
     tv[j] = tb + dt;
     hv[j] = r - dt * (uint32_t)p.H;
+    tv[j] += tv[j] >= sinks ? gap : 0u;
     const uint32_t page = p.block_shift >= 0 ? tv[j] >> p.block_shift
                                              : tv[j] / (uint32_t)p.block_size;
     pg[j] = live[j] ? pages[page] : -1;
@@ -343,13 +348,17 @@ __device__ __forceinline__ void copy_fresh(const ReadBackParams& p, const Gather
   }
 }
 
-template <int PD, bool GATHER>
+// what a launch reads: one sequence, a step's requests, or what a window leaves
+// of them (a kernel of its own: the other two do without the places' shift)
+enum Read { kPaged, kGather, kWindow };
+
+template <int PD, int READ>
 __global__ __launch_bounds__(256) void read_back_kernel(ReadBackParams p, int num_tokens) {
   __shared__ float cb[16];  // the codebook, indexed per lane
   __shared__ __attribute__((aligned(16))) _Float16 stage[4 * 64 * 32];
   if (threadIdx.x < 16) cb[threadIdx.x] = kCodebook[threadIdx.x];
   _Float16* out = blockIdx.y ? p.out_v : p.out_k;
-  if constexpr (!GATHER) {
+  if constexpr (READ == kPaged) {
     read_back<PD>(p, p.pages, num_tokens, blockIdx.x, out, cb, stage);
   } else {
     const int blk = (int)blockIdx.x - p.ctx_blocks;
@@ -358,7 +367,7 @@ __global__ __launch_bounds__(256) void read_back_kernel(ReadBackParams p, int nu
       const GatherReq& r = p.reqs[i];
       read_back<PD>(p, p.pages + (int64_t)r.bt_row * p.page_stride, r.ctx,
                     (int)blockIdx.x - r.ctx_blk, out + (int64_t)r.dst_row * p.out_stride_tok, cb,
-                    stage);
+                    stage, READ == kWindow ? r.sinks : 0, READ == kWindow ? r.gap : 0);
     } else {
       const int i = find_request(p.nreq, blk, [&](int r) { return p.reqs[r].fresh_blk; });
       copy_fresh<PD>(p, p.reqs[i], blk - p.reqs[i].fresh_blk);
@@ -405,14 +414,14 @@ void fill_geometry(ReadBackParams& p, const uint8_t* k_slab, const uint8_t* v_sl
   p.nreq = p.ctx_blocks = 0;
 }
 
-template <bool GATHER>
+template <int READ>
 hipError_t launch_read_back(int pd, dim3 grid, hipStream_t s, const ReadBackParams& p, int tokens) {
   if (pd == 64)
-    hipLaunchKernelGGL((read_back_kernel<64, GATHER>), grid, dim3(256), 0, s, p, tokens);
+    hipLaunchKernelGGL((read_back_kernel<64, READ>), grid, dim3(256), 0, s, p, tokens);
   else if (pd == 128)
-    hipLaunchKernelGGL((read_back_kernel<128, GATHER>), grid, dim3(256), 0, s, p, tokens);
+    hipLaunchKernelGGL((read_back_kernel<128, READ>), grid, dim3(256), 0, s, p, tokens);
   else
-    hipLaunchKernelGGL((read_back_kernel<256, GATHER>), grid, dim3(256), 0, s, p, tokens);
+    hipLaunchKernelGGL((read_back_kernel<256, READ>), grid, dim3(256), 0, s, p, tokens);
   return hipGetLastError();
 }
 
@@ -463,7 +472,7 @@ extern "C" int tq_dequant_paged(const uint8_t* k_slab, const uint8_t* v_slab,
   // full rows with 16-byte aligned dims: vector stores
   p.vec_store = head_dim == pd && out_stride_tok % 8 == 0 && (uintptr_t)out_k % 16 == 0 &&
                 (uintptr_t)out_v % 16 == 0;
-  const hipError_t e = launch_read_back<false>(pd, dim3((unsigned)blocks, 2),
+  const hipError_t e = launch_read_back<kPaged>(pd, dim3((unsigned)blocks, 2),
                                                reinterpret_cast<hipStream_t>(stream), p,
                                                (int)num_tokens);
   if (e != hipSuccess) {
@@ -473,16 +482,18 @@ extern "C" int tq_dequant_paged(const uint8_t* k_slab, const uint8_t* v_slab,
   return 0;
 }
 
-extern "C" int tq_prefill_gather(
-    const uint8_t* k_slab, const uint8_t* v_slab, const int32_t* block_table,
-    int64_t block_table_stride, int32_t num_kv_heads, int32_t head_dim, int32_t padded_dim,
-    int32_t block_size, int32_t ebs, int64_t num_blocks, const float* signs, const void* key,
-    const void* value, int32_t in_dtype, int64_t k_stride_tok, int64_t k_stride_head,
-    int64_t v_stride_tok, int64_t v_stride_head, const int32_t* table_rows, const int32_t* ctx_lens,
-    const int32_t* fresh_starts, const int32_t* fresh_lens, const int32_t* out_starts,
-    int32_t num_requests, void* out_k, void* out_v, tq_stream_t stream) {
-  using namespace tq;
-  const char* what = "prefill_gather";
+namespace tq {
+namespace {
+
+// tq_prefill_gather, and (firsts given) tq_prefill_gather_window
+int gather(const char* what, const int32_t* firsts, int32_t sink, const uint8_t* k_slab,
+           const uint8_t* v_slab, const int32_t* block_table, int64_t block_table_stride,
+           int32_t num_kv_heads, int32_t head_dim, int32_t padded_dim, int32_t block_size,
+           int32_t ebs, int64_t num_blocks, const float* signs, const void* key, const void* value,
+           int32_t in_dtype, int64_t k_stride_tok, int64_t k_stride_head, int64_t v_stride_tok,
+           int64_t v_stride_head, const int32_t* table_rows, const int32_t* ctx_lens,
+           const int32_t* fresh_starts, const int32_t* fresh_lens, const int32_t* out_starts,
+           int32_t num_requests, void* out_k, void* out_v, tq_stream_t stream) {
   const int pd = padded_dim;
   const int rc = check_geometry(what, pd, head_dim, num_kv_heads, block_size, num_blocks, ebs);
   if (rc) return rc;
@@ -495,7 +506,10 @@ extern "C" int tq_prefill_gather(
     return kEinval;
   }
   if (num_requests == 0) return 0;
-  if (!key || !value || !table_rows || !ctx_lens || !fresh_starts || !fresh_lens || !out_starts ||
+  bool fresh = !firsts;
+  if (firsts && fresh_lens)
+    for (int i = 0; i < num_requests; i++) fresh |= fresh_lens[i] != 0;
+  if ((fresh && (!key || !value)) || !table_rows || !ctx_lens || !fresh_starts || !fresh_lens || !out_starts ||
       !out_k || !out_v) {
     set_error("%s: null pointer", what);
     return kEinval;
@@ -506,7 +520,7 @@ extern "C" int tq_prefill_gather(
   }
   for (int i = 0; i < num_requests; i++) {
     if (ctx_lens[i] < 0 || fresh_lens[i] < 0 || fresh_starts[i] < 0 || out_starts[i] < 0 ||
-        table_rows[i] < 0) {
+        table_rows[i] < 0 || (firsts && (firsts[i] < 0 || firsts[i] > ctx_lens[i]))) {
       set_error("%s: bad request %d", what, i);
       return kEinval;
     }
@@ -540,6 +554,13 @@ extern "C" int tq_prefill_gather(
     for (int i = 0; i < p.nreq; i++) {
       GatherReq& r = p.reqs[i];
       r.ctx = ctx_lens[a + i];
+      r.sinks = r.gap = 0;
+      if (firsts) {
+        const int first = firsts[a + i];
+        r.sinks = sink < first ? sink : first;
+        r.gap = first - r.sinks;
+        r.ctx -= r.gap;
+      }
       r.fresh = fresh_lens[a + i];
       r.dst_row = out_starts[a + i];
       r.src_row = fresh_starts[a + i];
@@ -556,12 +577,53 @@ extern "C" int tq_prefill_gather(
     }
     if (cblk + fblk == 0) continue;
     p.ctx_blocks = (int)cblk;
-    const hipError_t e = launch_read_back<true>(pd, dim3((unsigned)(cblk + fblk), 2),
-                                                reinterpret_cast<hipStream_t>(stream), p, 0);
+    const dim3 grid((unsigned)(cblk + fblk), 2);
+    const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    const hipError_t e = firsts ? launch_read_back<kWindow>(pd, grid, st, p, 0)
+                                : launch_read_back<kGather>(pd, grid, st, p, 0);
     if (e != hipSuccess) {
       set_error("%s: launch failed: %s", what, hipGetErrorString(e));
       return (int)e;
     }
   }
   return 0;
+}
+
+}  // namespace
+}  // namespace tq
+
+extern "C" int tq_prefill_gather(
+    const uint8_t* k_slab, const uint8_t* v_slab, const int32_t* block_table,
+    int64_t block_table_stride, int32_t num_kv_heads, int32_t head_dim, int32_t padded_dim,
+    int32_t block_size, int32_t ebs, int64_t num_blocks, const float* signs, const void* key,
+    const void* value, int32_t in_dtype, int64_t k_stride_tok, int64_t k_stride_head,
+    int64_t v_stride_tok, int64_t v_stride_head, const int32_t* table_rows, const int32_t* ctx_lens,
+    const int32_t* fresh_starts, const int32_t* fresh_lens, const int32_t* out_starts,
+    int32_t num_requests, void* out_k, void* out_v, tq_stream_t stream) {
+  return tq::gather(
+      "prefill_gather", nullptr, 0, k_slab, v_slab, block_table, block_table_stride, num_kv_heads,
+      head_dim, padded_dim, block_size, ebs, num_blocks, signs, key, value, in_dtype, k_stride_tok, k_stride_head,
+      v_stride_tok, v_stride_head, table_rows, ctx_lens, fresh_starts, fresh_lens, out_starts,
+      num_requests, out_k, out_v, stream);
+}
+
+extern "C" int tq_prefill_gather_window(
+    const uint8_t* k_slab, const uint8_t* v_slab, const int32_t* block_table,
+    int64_t block_table_stride, int32_t num_kv_heads, int32_t head_dim, int32_t padded_dim,
+    int32_t block_size, int32_t ebs, int64_t num_blocks, const float* signs, const void* key,
+    const void* value, int32_t in_dtype, int64_t k_stride_tok, int64_t k_stride_head,
+    int64_t v_stride_tok, int64_t v_stride_head, const int32_t* table_rows, const int32_t* ctx_lens,
+    const int32_t* firsts, const int32_t* fresh_starts, const int32_t* fresh_lens,
+    const int32_t* out_starts, int32_t num_requests, int32_t sink, void* out_k, void* out_v, tq_stream_t stream) {
+  const char* what = "prefill_gather_window";
+  if (sink < 0 || (num_requests > 0 && !firsts)) {
+    tq::set_error("%s: sink %d is negative, or a null pointer", what, sink);
+    return tq::kEinval;
+  }
+  static const int32_t none = 0;
+  return tq::gather(
+      what, firsts ? firsts : &none, sink, k_slab, v_slab, block_table, block_table_stride,
+      num_kv_heads, head_dim, padded_dim, block_size, ebs, num_blocks, signs, key, value, in_dtype, k_stride_tok, k_stride_head,
+      v_stride_tok, v_stride_head, table_rows, ctx_lens, fresh_starts, fresh_lens, out_starts,
+      num_requests, out_k, out_v, stream);
 }

@@ -137,10 +137,26 @@ __device__ __forceinline__ PrefillRun find_run(const PrefillRun* runs, int n, in
   return runs[lo];
 }
 
-// key tiles that any row of query block qb sees
-template <int kBM, int kBN>
-__device__ __forceinline__ int block_tiles(const PrefillReq& rq, int qb) {
-  return (rq.lk - rq.lq + min((qb + 1) * kBM, rq.lq) + kBN - 1) / kBN;
+// The key tiles that a row of query block qb sees: `tiles` of them; with a
+// sliding window (window > 0: a row at position P sees the keys j with P -
+// window < j <= P, and j < sink) the first `sinks` tiles of the request and,
+// from tile `sinks` on, those `skip` further.
+struct TileSpan {
+  int tiles, sinks, skip;
+};
+__host__ __device__ inline TileSpan tile_span(int lq, int lk, int qb, int bm, int bn, int window,
+                                              int sink) {
+  const int off = lk - lq, first = off + qb * bm;
+  const int last = (qb + 1) * bm < lq ? (qb + 1) * bm : lq;
+  TileSpan r = {(off + last + bn - 1) / bn, 0, 0};
+  if (window > 0) {
+    const int lo = first - window + 1 > 0 ? first - window + 1 : 0;  // first key of the window
+    const int s = sink < lo ? sink : lo;
+    r.sinks = (s + bn - 1) / bn;
+    r.skip = lo / bn > r.sinks ? lo / bn - r.sinks : 0;
+    r.tiles -= r.skip;
+  }
+  return r;
 }
 struct PrefillBatch {
   const void* q;
@@ -156,6 +172,7 @@ struct PrefillBatch {
   float* ws_o;         // [row][Hq][kD]
   float* ws_ml;        // [row][Hq][2]
   int nruns, unit, y0;  // runs (0: items), their split_shares unit, this launch's first row
+  int window, sink;     // 0: every key up to the row's own
   PrefillReq reqs[kBatchReqs];
   union {
     PrefillItem items[kBatchItems];
@@ -167,6 +184,12 @@ static_assert(sizeof(PrefillBatch) <= 4096, "kernel argument");
 // hold neither the search nor the choice (five prompts of 229 .. 1326 tokens
 // 51.1 us; 51.8 with both in one kernel).
 struct PrefillRuns : PrefillBatch {};
+// The same two under a sliding window: the walk over the sinks' and the
+// window's tiles and the masks at the window's edge are in these kernels alone.
+struct PrefillWin : PrefillBatch {};
+struct PrefillWinRuns : PrefillBatch {};
+template <class PP>
+constexpr bool kWindowed = std::is_same_v<PP, PrefillWin> || std::is_same_v<PP, PrefillWinRuns>;
 
 // eight bf16 as eight fp16, round to nearest even (exact in fp16's range)
 __device__ __forceinline__ u32x4 bf16_to_f16(u32x4 x) {
@@ -200,6 +223,7 @@ __device__ __forceinline__ float sum32(float x) {
 // q_row0) over its key tiles [t0, t1)
 struct PrefillWork {
   int qb, q_row0, lq, lk, t0, t1, ws_row, hd;  // t1 < 0: nothing
+  int sinks, skip;                              // kWindowed: see TileSpan
   const _Float16* k;
   const _Float16* v;
   int64_t k_st, k_sh, v_st, v_sh;
@@ -246,8 +270,8 @@ __device__ __forceinline__ void request_of_work(const PrefillBatch& p, const Pre
   r.v = (rq.src ? p.v2 : p.v) + (int64_t)rq.k0 * r.v_st;
 }
 
-template <int kBM, int kBN, bool SPLIT>
-__device__ __forceinline__ PrefillWork prefill_work(const PrefillBatch& p) {
+template <int kBM, int kBN>
+__device__ __forceinline__ PrefillWork item_work(const PrefillBatch& p) {
   PrefillWork r;
   const PrefillItem it = p.items[blockIdx.y];
   r.qb = (int)(it.req_qb >> 6);
@@ -258,19 +282,172 @@ __device__ __forceinline__ PrefillWork prefill_work(const PrefillBatch& p) {
   return r;
 }
 
-template <int kBM, int kBN, bool SPLIT>
-__device__ __forceinline__ PrefillWork prefill_work(const PrefillRuns& p) {
+template <int kBM, int kBN>
+__device__ __forceinline__ PrefillWork run_work(const PrefillBatch& p, int window, int sink) {
   PrefillWork r;
   const int y = p.y0 + (int)blockIdx.y, z = (int)blockIdx.z;
   const PrefillRun run = find_run(p.runs, p.nruns, y);
   const PrefillReq rq = p.reqs[run.req];
   r.qb = (rq.lq + kBM - 1) / kBM - 1 - (y - run.first);
-  const int tiles = block_tiles<kBM, kBN>(rq, r.qb), ns = split_shares(tiles, p.unit);
+  const TileSpan sp = tile_span(rq.lq, rq.lk, r.qb, kBM, kBN, window, sink);
+  const int ns = split_shares(sp.tiles, p.unit);
   r.t0 = z * p.unit;
-  r.t1 = z >= ns ? -1 : ns > 1 ? min(tiles, r.t0 + p.unit) : tiles;
+  r.t1 = z >= ns ? -1 : ns > 1 ? min(sp.tiles, r.t0 + p.unit) : sp.tiles;
   r.ws_row = ns > 1 ? run.ws_row + z * rq.lq + r.qb * kBM : -1;
+  r.sinks = sp.sinks;
+  r.skip = sp.skip;
   request_of_work(p, rq, r);
   return r;
+}
+
+template <int kBM, int kBN, bool SPLIT>
+__device__ __forceinline__ PrefillWork prefill_work(const PrefillBatch& p) {
+  return item_work<kBM, kBN>(p);
+}
+template <int kBM, int kBN, bool SPLIT>
+__device__ __forceinline__ PrefillWork prefill_work(const PrefillRuns& p) {
+  return run_work<kBM, kBN>(p, 0, 0);
+}
+template <int kBM, int kBN, bool SPLIT>
+__device__ __forceinline__ PrefillWork prefill_work(const PrefillWin& p) {
+  PrefillWork r = item_work<kBM, kBN>(p);
+  const TileSpan sp = tile_span(r.lq, r.lk, r.qb, kBM, kBN, p.window, p.sink);
+  r.sinks = sp.sinks;
+  r.skip = sp.skip;
+  return r;
+}
+template <int kBM, int kBN, bool SPLIT>
+__device__ __forceinline__ PrefillWork prefill_work(const PrefillWinRuns& p) {
+  return run_work<kBM, kBN>(p, p.window, p.sink);
+}
+
+// a tile's place among the request's key tiles
+template <class PP>
+__device__ __forceinline__ int tile_place(const PrefillWork& wk, int kt) {
+  if constexpr (kWindowed<PP>) return kt < wk.sinks ? kt : kt + wk.skip;
+  return kt;
+}
+
+// Masks of a tile (keys kb ..) under a sliding window, scores laid out as below
+// (register j of block u: key 32 u + 8 (j / 4) + j % 4 from key kb + 4 hh on) for
+// the lane's row at position `pos` and a wave whose first row stands at `wpos`:
+// selects, so that a hidden key's score may be anything.
+template <int kBN>
+__device__ __forceinline__ void mask_window(f32x16* sacc, int kb, int hh, int pos, int wpos, int lk,
+                                            int window, int sink) {
+  constexpr int kNU = kBN / 32;
+  if (kb + kBN - 1 > wpos || kb + kBN > lk) {  // (uniform) beyond a row, or beyond the keys
+    const int lim = min(pos, lk - 1) - kb - 4 * hh;
+#pragma unroll
+    for (int u = 0; u < kNU; u++)
+#pragma unroll
+      for (int j = 0; j < 16; j++)
+        sacc[u][j] = 32 * u + 8 * (j >> 2) + (j & 3) > lim ? -INFINITY : sacc[u][j];
+  }
+  if (kb <= wpos + 31 - window && kb + kBN > sink) {  // (uniform) behind a row's window
+    const int low = max(pos - window, -1) - kb - 4 * hh;
+    const int first = max(sink - kb, 0) - 4 * hh;  // the tile's first key that is no sink
+#pragma unroll
+    for (int u = 0; u < kNU; u++)
+#pragma unroll
+      for (int j = 0; j < 16; j++) {
+        const int kk = 32 * u + 8 * (j >> 2) + (j & 3);
+        sacc[u][j] = kk <= low && kk >= first ? -INFINITY : sacc[u][j];
+      }
+  }
+}
+
+// whether a wave's rows from position `wpos` on see no key of the tile kb ..
+// because of their window
+template <int kBN>
+__device__ __forceinline__ bool behind_window(int kb, int wpos, int window, int sink) {
+  return kb >= sink && kb + kBN - 1 <= wpos - window;
+}
+
+// Rows of a windowed wave that came out NaN, computed again without the matrix
+// cores.  A tile's V rows enter the MFMAs for all of the wave's rows, those that
+// a row does not see with probability 0, and 0 times a NaN or an infinity is
+// NaN; here a row takes the keys in its sight alone (over this workgroup's
+// tiles).  So a row is NaN only if what it sees makes it so.  Such rows are rare:
+// the check costs a sum over the outputs.  rows: bit i: row row0 + i of the
+// request; store(row, dims V lane .. + V - 1 of O / sum, reference max in log2
+// units, sum).
+template <int kD, int kBN, class PP, class Store>
+__device__ __forceinline__ void recompute_rows(const PP& p, const PrefillWork& wk, int head, int g,
+                                               int row0, uint32_t rows, Store store) {
+  constexpr int V = kD / 64;  // dims per lane
+  const int lane = threadIdx.x & 63;
+  const _Float16* const kbase = wk.k + (int64_t)g * wk.k_sh;
+  const _Float16* const vbase = wk.v + (int64_t)g * wk.v_sh;
+  while (rows != 0) {  // uniform, as everything but the lanes' keys and dims
+    const int row = row0 + __builtin_ctz(rows);
+    rows &= rows - 1;
+    const int pos = wk.lk - wk.lq + row;
+    const _Float16* const qp = static_cast<const _Float16*>(p.q) +
+                               (int64_t)(wk.q_row0 + row) * p.q_st + (int64_t)head * p.q_sh;
+    float m = -INFINITY, l = 0.0f, acc[V];
+#pragma unroll
+    for (int e = 0; e < V; e++) acc[e] = 0.0f;
+    for (int kt = wk.t0; kt < wk.t1; kt++)
+      for (int j0 = 0; j0 < kBN; j0 += 64) {
+        const int key = tile_place<PP>(wk, kt) * kBN + j0 + lane;
+        const bool seen = key <= pos && (key > pos - p.window || key < p.sink);
+        float sc = 0.0f;
+        if (seen) {
+#pragma unroll 1
+          for (int d = 0; d < wk.hd; d += 8) {
+            u32x4 x = *reinterpret_cast<const u32x4*>(qp + d);
+            if (p.q_bf16) x = bf16_to_f16(x);
+            const half8_t a = __builtin_bit_cast(half8_t, x);
+            const half8_t b = *reinterpret_cast<const half8_t*>(kbase + (int64_t)key * wk.k_st + d);
+#pragma unroll
+            for (int e = 0; e < 8; e++) sc = __builtin_fmaf((float)a[e], (float)b[e], sc);
+          }
+        }
+        float top = seen ? sc : -INFINITY;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+        if (__builtin_amdgcn_ballot_w64(seen) == 0) continue;
+        const float mn = fmaxf(m, top);
+        const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * p.c);
+        const float pr = seen ? __builtin_amdgcn_exp2f((sc - mn) * p.c) : 0.0f;
+        float sum = pr;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+        l = l * alpha + sum;
+        m = mn;
+#pragma unroll
+        for (int e = 0; e < V; e++) acc[e] *= alpha;
+        for (uint64_t left = __builtin_amdgcn_ballot_w64(seen); left != 0; left &= left - 1) {
+          const int i = __builtin_ctzll(left);
+          const float w = __uint_as_float(
+              (uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(pr), i));
+          const _Float16* const vp = vbase + (int64_t)(key - lane + i) * wk.v_st + V * lane;
+#pragma unroll
+          for (int e = 0; e < V; e++) acc[e] = __builtin_fmaf(w, (float)vp[e], acc[e]);
+        }
+      }
+    // (a NaN sum stays NaN)
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int e = 0; e < V; e++) acc[e] *= inv;
+    store(row, acc, m == -INFINITY ? m : m * p.c, l);
+  }
+}
+
+// a row of o from recompute_rows
+template <int kD, class PP>
+__device__ __forceinline__ void store_row(const PP& p, const PrefillWork& wk, int head, int row,
+                                          const float* acc) {
+  constexpr int V = kD / 64;
+  const int lane = threadIdx.x & 63;
+  const int64_t at = (int64_t)(wk.q_row0 + row) * p.o_st + (int64_t)head * p.o_sh + V * lane;
+#pragma unroll
+  for (int e = 0; e < V; e++) {
+    if (V * lane + e >= wk.hd) continue;
+    if (p.o_bf16) static_cast<uint16_t*>(p.o)[at + e] = (uint16_t)pack_b2(acc[e], acc[e]);
+    else static_cast<_Float16*>(p.o)[at + e] = (_Float16)acc[e];
+  }
 }
 
 // The head of a workgroup.  Workgroups go to the 8 XCDs round robin, so with
@@ -315,7 +492,7 @@ void prefill_kernel(PP p) {
   const int hh = lane >> 5, n = lane & 31;
   const int head = head_of_block(), g = head / p.ratio;
   const PrefillWork wk = prefill_work<kBM, kBN, SPLIT>(p);
-  if (std::is_same_v<PP, PrefillRuns> && wk.t1 < 0) return;
+  if ((std::is_same_v<PP, PrefillRuns> || std::is_same_v<PP, PrefillWinRuns>) && wk.t1 < 0) return;
   const int q0 = wk.qb * kBM;
   const int off = wk.lk - wk.lq;
   const int qrow = q0 + 32 * w + n;  // this lane's query row (of its request)
@@ -411,6 +588,8 @@ void prefill_kernel(PP p) {
     // the wave's rows are q0 + 32w .. +31: nothing to do when all its keys
     // in this tile are beyond every row (uniform)
     if (kb > off + q0 + 32 * w + 31) return;
+    if constexpr (kWindowed<PP>)
+      if (behind_window<kBN>(kb, off + q0 + 32 * w, p.window, p.sink)) return;
     // S^T blocks: MFMA i = s * kNU + u adds k-step s of key block u.  The K
     // fragments are read kKP ahead of their MFMA and the schedule is pinned
     // (one MFMA, then one read): left to itself the compiler issued each
@@ -448,7 +627,9 @@ void prefill_kernel(PP p) {
     // score at tile key 4 hh + kk gets -inf (the sign bits of lim - kk spread
     // into 0xff800000) or +0 added; no compare masks, so no scalar registers
     // for them
-    if (kb + kBN - 1 > off + q0 + 32 * w || kb + kBN > wk.lk) {
+    if constexpr (kWindowed<PP>) {
+      mask_window<kBN>(sacc, kb, hh, qlim, off + q0 + 32 * w, wk.lk, p.window, p.sink);
+    } else if (kb + kBN - 1 > off + q0 + 32 * w || kb + kBN > wk.lk) {
       const int lim = min(qlim, wk.lk - 1) - kb - 4 * hh;
 #pragma unroll
       for (int u = 0; u < kNU; u++)
@@ -536,29 +717,41 @@ void prefill_kernel(PP p) {
 
   // this workgroup's tiles: all of them, or split z's share
   const int t0 = wk.t0, t1 = wk.t1;
-  if (t0 < t1) issue(t0, kbuf0, vbuf0);
+  auto at = [&](int kt) { return tile_place<PP>(wk, kt); };
+  if (t0 < t1) issue(at(t0), kbuf0, vbuf0);
   for (int kt = t0; kt < t1; kt += 2) {
     // tile kt: buffers 0
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's copies of tile kt
     __syncthreads();                     // everyone's copies of tile kt
-    if (kt + 1 < t1) issue(kt + 1, kbuf1, vbuf1);
-    tile(kt, kbuf0, vbuf0);
+    if (kt + 1 < t1) issue(at(kt + 1), kbuf1, vbuf1);
+    tile(at(kt), kbuf0, vbuf0);
     if (kt + 1 >= t1) break;
     // tile kt + 1: buffers 1
     __builtin_amdgcn_s_waitcnt(0x0f70);
     __syncthreads();
-    if (kt + 2 < t1) issue(kt + 2, kbuf0, vbuf0);
-    tile(kt + 1, kbuf1, vbuf1);
+    if (kt + 2 < t1) issue(at(kt + 2), kbuf0, vbuf0);
+    tile(at(kt + 1), kbuf1, vbuf1);
   }
 
   lsum = sum32(lsum);
   const float inv = lsum > 0.0f ? 1.0f / lsum : 0.0f;
+  [[maybe_unused]] uint32_t again = 0;  // (uniform) rows to be computed without the MFMAs
+  if constexpr (kWindowed<PP>) {
+    float z = 0.0f;
+#pragma unroll
+    for (int d = 0; d < kD / 32; d++)
+#pragma unroll
+      for (int j = 0; j < 16; j++) z = __builtin_fmaf(oacc[d][j], 0.0f, z);
+    const uint64_t bad = __builtin_amdgcn_ballot_w64(z != z && qrow < wk.lq);
+    again = (uint32_t)(bad | bad >> 32);
+  }
+  const bool mine = qrow < wk.lq && !(kWindowed<PP> && (again >> n & 1u));
   if (SPLIT || (kBatch && wk.ws_row >= 0)) {
     // this split's O / row sum and (mc, row sum); a split that held no visible
     // key for a row leaves mc = -inf, sum 0, O = 0.  One request: as fp16 (a
     // convex combination of V rows: safe).  Batch mode splits blocks that one
     // launch per request left whole, so what was a sum in fp32 stays one: fp32.
-    if (qrow < wk.lq) {
+    if (mine) {
       const int64_t r = (kBatch ? (int64_t)wk.ws_row + 32 * w + n
                                 : (int64_t)blockIdx.z * wk.lq + qrow) * gridDim.x + head;
       if constexpr (kBatch) {
@@ -583,11 +776,20 @@ void prefill_kernel(PP p) {
       }
       if (hh == 0) *reinterpret_cast<f32x2*>(p.ws_ml + 2 * r) = f32x2{mc, lsum};
     }
+    if constexpr (kWindowed<PP>)
+      if (again != 0)
+        recompute_rows<kD, kBN>(p, wk, head, g, q0 + 32 * w, again,
+                                [&](int row, const float* acc, float top, float sum) {
+          const int64_t r = ((int64_t)wk.ws_row + row - q0) * gridDim.x + head;
+#pragma unroll
+          for (int e = 0; e < kD / 64; e++) p.ws_o[r * kD + kD / 64 * lane + e] = acc[e];
+          if (lane == 0) *reinterpret_cast<f32x2*>(p.ws_ml + 2 * r) = f32x2{top, sum};
+        });
     return;
   }
 
   // o = O / sum, lane (hh, n) holds dims 32d + 8jq + 4hh + 0..3 of row qrow
-  if (qrow < wk.lq) {
+  if (mine) {
     _Float16* op = static_cast<_Float16*>(p.o) + (int64_t)(wk.q_row0 + qrow) * p.o_st +
                    (int64_t)head * p.o_sh + 4 * hh;
 #pragma unroll
@@ -603,6 +805,12 @@ void prefill_kernel(PP p) {
         *reinterpret_cast<u32x2*>(op + 32 * d + 8 * jq) = r;
       }
   }
+  if constexpr (kWindowed<PP>)
+    if (again != 0)
+      recompute_rows<kD, kBN>(p, wk, head, g, q0 + 32 * w, again,
+                              [&](int row, const float* acc, float, float) {
+        store_row<kD>(p, wk, head, row, acc);
+      });
 }
 
 // The same attention with RB row blocks of 32 query rows per wave: each K
@@ -715,6 +923,8 @@ void prefill_rb_kernel(PP p) {
   auto tile = [&](int kt, const uint8_t* kbuf, const uint8_t* vt) {
     const int kb = kt * kBN;
     if (kb > off + wrow0 + 32 * RB - 1) return;  // beyond every row of the wave
+    if constexpr (kWindowed<PP>)  // (the wave's first row sees furthest back)
+      if (behind_window<kBN>(kb, off + wrow0, p.window, p.sink)) return;
     constexpr int kKP = 4;
     constexpr int kNI = kNU * (kD / 16);
     f32x16 sacc[RB][kNU];
@@ -751,7 +961,9 @@ void prefill_rb_kernel(PP p) {
 #pragma unroll
     for (int rb = 0; rb < RB; rb++) {
       const int rfirst = wrow0 + 32 * rb;
-      if (kb + kBN - 1 > off + rfirst || kb + kBN > wk.lk) {
+      if constexpr (kWindowed<PP>) {
+        mask_window<kBN>(sacc[rb], kb, hh, off + rfirst + n, off + rfirst, wk.lk, p.window, p.sink);
+      } else if (kb + kBN - 1 > off + rfirst || kb + kBN > wk.lk) {
         const int lim = min(off + rfirst + n, wk.lk - 1) - kb - 4 * hh;
 #pragma unroll
         for (int u = 0; u < kNU; u++)
@@ -820,24 +1032,35 @@ void prefill_rb_kernel(PP p) {
     }
   };
 
-  if (ntiles > 0) issue(0, kbuf0, vbuf0);
+  auto at = [&](int kt) { return tile_place<PP>(wk, kt); };
+  if (ntiles > 0) issue(at(0), kbuf0, vbuf0);
   for (int kt = 0; kt < ntiles; kt += 2) {
     __builtin_amdgcn_s_waitcnt(0x0f70);
     __syncthreads();
-    if (kt + 1 < ntiles) issue(kt + 1, kbuf1, vbuf1);
-    tile(kt, kbuf0, vbuf0);
+    if (kt + 1 < ntiles) issue(at(kt + 1), kbuf1, vbuf1);
+    tile(at(kt), kbuf0, vbuf0);
     if (kt + 1 >= ntiles) break;
     __builtin_amdgcn_s_waitcnt(0x0f70);
     __syncthreads();
-    if (kt + 2 < ntiles) issue(kt + 2, kbuf0, vbuf0);
-    tile(kt + 1, kbuf1, vbuf1);
+    if (kt + 2 < ntiles) issue(at(kt + 2), kbuf0, vbuf0);
+    tile(at(kt + 1), kbuf1, vbuf1);
   }
 
 #pragma unroll
   for (int rb = 0; rb < RB; rb++) {
     const int qrow = wrow0 + 32 * rb + n;
     const float ls = sum32(lsum[rb]);
-    if (qrow < wk.lq) {
+    [[maybe_unused]] uint32_t again = 0;
+    if constexpr (kWindowed<PP>) {
+      float z = 0.0f;
+#pragma unroll
+      for (int d = 0; d < kD / 32; d++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) z = __builtin_fmaf(oacc[rb][d][j], 0.0f, z);
+      const uint64_t bad = __builtin_amdgcn_ballot_w64(z != z && qrow < wk.lq);
+      again = (uint32_t)(bad | bad >> 32);
+    }
+    if (qrow < wk.lq && !(kWindowed<PP> && (again >> n & 1u))) {
       const float inv = ls > 0.0f ? 1.0f / ls : 0.0f;
       _Float16* op = static_cast<_Float16*>(p.o) + (int64_t)(wk.q_row0 + qrow) * p.o_st +
                      (int64_t)head * p.o_sh + 4 * hh;
@@ -854,6 +1077,12 @@ void prefill_rb_kernel(PP p) {
           *reinterpret_cast<u32x2*>(op + 32 * d + 8 * jq) = r;
         }
     }
+    if constexpr (kWindowed<PP>)
+      if (again != 0)
+        recompute_rows<kD, kBN>(p, wk, head, g, wrow0 + 32 * rb, again,
+                                [&](int row, const float* acc, float, float) {
+          store_row<kD>(p, wk, head, row, acc);
+        });
   }
 }
 
@@ -900,7 +1129,7 @@ struct PrefillMerge {
   int hq, hd, o_bf16;
   const float* ws_o;
   const float* ws_ml;
-  int nruns, unit, y0;  // as in PrefillBatch
+  int nruns, unit, y0, window, sink;  // as in PrefillBatch
   union {
     PrefillGroup groups[kBatchItems];
     struct {
@@ -922,7 +1151,8 @@ __global__ __launch_bounds__(256) void prefill_batch_merge_kernel(PrefillMerge p
     const PrefillRun run = find_run(p.runs, p.nruns, y);
     const PrefillReq rq = p.reqs[run.req];
     const int qb = (rq.lq + kBM - 1) / kBM - 1 - (y - run.first);
-    g.nsplit = (uint16_t)split_shares(block_tiles<kBM, kBN>(rq, qb), p.unit);
+    g.nsplit = (uint16_t)split_shares(
+        tile_span(rq.lq, rq.lk, qb, kBM, kBN, p.window, p.sink).tiles, p.unit);
     if (g.nsplit < 2) return;
     g.q_row = rq.q0 + qb * kBM;
     g.ws_row = run.ws_row + qb * kBM;
@@ -1081,13 +1311,11 @@ double batch_time(size_t n, double groups, Tiles tiles) {
 }
 
 std::vector<QueryBlock> query_blocks(const int32_t* q_lens, const int32_t* kv_lens, int nreq,
-                                     int bm, int bn) {
+                                     int bm, int bn, int window, int sink) {
   std::vector<QueryBlock> blocks;
   for (int i = 0; i < nreq; i++)
-    for (int qb = 0; (int64_t)qb * bm < q_lens[i]; qb++) {
-      const int kend = kv_lens[i] - q_lens[i] + std::min((qb + 1) * bm, q_lens[i]);
-      blocks.push_back({i, qb, (kend + bn - 1) / bn});
-    }
+    for (int qb = 0; (int64_t)qb * bm < q_lens[i]; qb++)
+      blocks.push_back({i, qb, tile_span(q_lens[i], kv_lens[i], qb, bm, bn, window, sink).tiles});
   std::stable_sort(blocks.begin(), blocks.end(),
                    [](const QueryBlock& x, const QueryBlock& y) { return x.tiles > y.tiles; });
   return blocks;
@@ -1104,10 +1332,10 @@ std::vector<QueryBlock> query_blocks(const int32_t* q_lens, const int32_t* kv_le
 // blocks leave slots idle (256 tokens over 32k: 155 against 669 us) and costs
 // the merge, 4 .. 9 us.
 BatchPlan plan_batch(const int32_t* q_lens, const int32_t* kv_lens, int nreq, int heads,
-                     int head_dim) {
+                     int head_dim, int window, int sink) {
   BatchPlan bp;
   const double cus = device_cus() > 0 ? device_cus() : 256;
-  std::vector<QueryBlock> blocks = query_blocks(q_lens, kv_lens, nreq, 128, 64);
+  std::vector<QueryBlock> blocks = query_blocks(q_lens, kv_lens, nreq, 128, 64, window, sink);
   const double groups = (head_dim == 256 ? 1.0 : 2.0) * cus / heads;
   int64_t total = 0;
   for (const QueryBlock& b : blocks) total += b.tiles;
@@ -1169,7 +1397,7 @@ BatchPlan plan_batch(const int32_t* q_lens, const int32_t* kv_lens, int nreq, in
   }
   if (head_dim != 256) {
     const std::vector<QueryBlock> wide =
-        query_blocks(q_lens, kv_lens, nreq, 256, head_dim == 128 ? 128 : 64);
+        query_blocks(q_lens, kv_lens, nreq, 256, head_dim == 128 ? 128 : 64, window, sink);
     const double t = batch_time(wide.size(), (head_dim == 128 ? 1.0 : 2.0) * cus / heads,
                                 [&](size_t i) { return wide[i].tiles; });
     if (head_dim == 128 ? t * 3.84 <= best * 2.1 : t * 2.15 <= best * 1.15) {
@@ -1237,7 +1465,9 @@ hipError_t launch_batch(const BatchPlan& bp, int heads, hipStream_t st, PrefillB
   else std::copy(bp.items.begin(), bp.items.end(), p.items);
   for (p.y0 = 0; p.y0 < nrows; p.y0 += kGridRows) {
     const dim3 grid(heads, std::min(kGridRows, nrows - p.y0), bp.shares);
-    if (p.nruns) launch_batch_kernel<D>(bp.nw, grid, st, PrefillRuns{p});
+    if (p.window && p.nruns) launch_batch_kernel<D>(bp.nw, grid, st, PrefillWinRuns{p});
+    else if (p.window) launch_batch_kernel<D>(bp.nw, grid, st, PrefillWin{p});
+    else if (p.nruns) launch_batch_kernel<D>(bp.nw, grid, st, PrefillRuns{p});
     else launch_batch_kernel<D>(bp.nw, grid, st, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -1254,6 +1484,8 @@ hipError_t launch_batch(const BatchPlan& bp, int heads, hipStream_t st, PrefillB
   m.ws_ml = p.ws_ml;
   m.nruns = p.nruns;
   m.unit = p.unit;
+  m.window = p.window;
+  m.sink = p.sink;
   int ngroups = bp.rows, rows = 128;
   if (p.nruns) {
     std::copy(p.reqs, p.reqs + kBatchReqs, m.reqs);
@@ -1293,20 +1525,15 @@ bool batch_sizes_ok(const int32_t* q_lens, const int32_t* kv_lens, int32_t nreq,
   return true;
 }
 
-}  // namespace
-}  // namespace tq
-
-extern "C" int64_t tq_prefill_batch_workspace_bytes(const int32_t* q_lens, const int32_t* kv_lens,
-                                                    int32_t num_requests, int32_t num_qo_heads,
-                                                    int32_t padded_dim) {
-  using namespace tq;
+int64_t batch_workspace(const int32_t* q_lens, const int32_t* kv_lens, int32_t num_requests,
+                        int32_t num_qo_heads, int32_t padded_dim, int32_t window, int32_t sink) {
   if (!batch_sizes_ok(q_lens, kv_lens, num_requests, num_qo_heads, padded_dim)) return 0;
   int64_t most = 0;
   try {
     for (int a = 0; a < num_requests; a += kBatchReqs)
       most = std::max(most, batch_ws_bytes(plan_batch(q_lens + a, kv_lens + a,
                                                       std::min(kBatchReqs, num_requests - a),
-                                                      num_qo_heads, padded_dim),
+                                                      num_qo_heads, padded_dim, window, sink),
                                            num_qo_heads, padded_dim));
   } catch (...) {
     return 0;
@@ -1314,17 +1541,16 @@ extern "C" int64_t tq_prefill_batch_workspace_bytes(const int32_t* q_lens, const
   return most;
 }
 
-extern "C" int tq_prefill_attention_batch(
-    const void* q, int64_t q_stride_tok, int64_t q_stride_head, int32_t q_dtype, const void* k,
-    int64_t k_stride_tok, int64_t k_stride_head, const void* v, int64_t v_stride_tok,
-    int64_t v_stride_head, const void* k2, const void* v2, int64_t k2_stride_tok,
-    int64_t k2_stride_head, void* o, int64_t o_stride_tok, int64_t o_stride_head, int32_t o_dtype,
-    const int32_t* q_starts, const int32_t* q_lens, const int32_t* kv_starts,
-    const int32_t* kv_lens, const int32_t* kv_sources, int32_t num_requests, int32_t num_qo_heads,
-    int32_t num_kv_heads, int32_t head_dim, int32_t padded_dim, float sm_scale, void* workspace,
-    int64_t workspace_bytes, tq_stream_t stream) {
-  using namespace tq;
-  const char* what = "prefill_attention_batch";
+int attention_batch(
+    const char* what, int32_t window, int32_t sink, const void* q, int64_t q_stride_tok,
+    int64_t q_stride_head, int32_t q_dtype, const void* k, int64_t k_stride_tok,
+    int64_t k_stride_head, const void* v, int64_t v_stride_tok, int64_t v_stride_head,
+    const void* k2, const void* v2, int64_t k2_stride_tok, int64_t k2_stride_head, void* o,
+    int64_t o_stride_tok, int64_t o_stride_head, int32_t o_dtype, const int32_t* q_starts,
+    const int32_t* q_lens, const int32_t* kv_starts, const int32_t* kv_lens,
+    const int32_t* kv_sources, int32_t num_requests, int32_t num_qo_heads, int32_t num_kv_heads,
+    int32_t head_dim, int32_t padded_dim, float sm_scale, void* workspace, int64_t workspace_bytes,
+    tq_stream_t stream) {
   if (!batch_sizes_ok(q_lens, kv_lens, num_requests, num_qo_heads, padded_dim)) {
     set_error("%s: bad sizes (padded_dim 64, 128 or 256; 0 <= q_len <= kv_len)", what);
     return kEinval;
@@ -1408,11 +1634,14 @@ extern "C" int tq_prefill_attention_batch(
   p.q_bf16 = q_dtype == TQ_BF16;
   p.o_bf16 = o_dtype == TQ_BF16;
   p.c = sm_scale * 1.4426950408889634f;
+  p.window = window;
+  p.sink = sink;
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   try {
     for (int a = 0; a < num_requests; a += kBatchReqs) {
       const int n = std::min(kBatchReqs, num_requests - a);
-      const BatchPlan bp = plan_batch(q_lens + a, kv_lens + a, n, num_qo_heads, padded_dim);
+      const BatchPlan bp = plan_batch(q_lens + a, kv_lens + a, n, num_qo_heads, padded_dim,
+                                      window, sink);
       if (batch_ws_bytes(bp, num_qo_heads, padded_dim) > (workspace ? workspace_bytes : 0)) {
         set_error("%s: workspace smaller than tq_prefill_batch_workspace_bytes", what);
         return kEinval;
@@ -1436,6 +1665,67 @@ extern "C" int tq_prefill_attention_batch(
     return (int)hipErrorOutOfMemory;
   }
   return 0;
+}
+
+}  // namespace
+}  // namespace tq
+
+extern "C" int64_t tq_prefill_batch_workspace_bytes(const int32_t* q_lens, const int32_t* kv_lens,
+                                                    int32_t num_requests, int32_t num_qo_heads,
+                                                    int32_t padded_dim) {
+  return tq::batch_workspace(q_lens, kv_lens, num_requests, num_qo_heads, padded_dim, 0, 0);
+}
+
+extern "C" int tq_prefill_attention_batch(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head, int32_t q_dtype, const void* k,
+    int64_t k_stride_tok, int64_t k_stride_head, const void* v, int64_t v_stride_tok,
+    int64_t v_stride_head, const void* k2, const void* v2, int64_t k2_stride_tok,
+    int64_t k2_stride_head, void* o, int64_t o_stride_tok, int64_t o_stride_head, int32_t o_dtype,
+    const int32_t* q_starts, const int32_t* q_lens, const int32_t* kv_starts,
+    const int32_t* kv_lens, const int32_t* kv_sources, int32_t num_requests, int32_t num_qo_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t padded_dim, float sm_scale, void* workspace,
+    int64_t workspace_bytes, tq_stream_t stream) {
+  return tq::attention_batch(
+      "prefill_attention_batch", 0, 0, q, q_stride_tok, q_stride_head, q_dtype, k, k_stride_tok,
+      k_stride_head, v, v_stride_tok, v_stride_head, k2, v2, k2_stride_tok, k2_stride_head, o, o_stride_tok,
+      o_stride_head, o_dtype, q_starts, q_lens, kv_starts, kv_lens, kv_sources, num_requests,
+      num_qo_heads, num_kv_heads, head_dim, padded_dim, sm_scale, workspace, workspace_bytes,
+      stream);
+}
+
+extern "C" int64_t tq_prefill_window_workspace_bytes(const int32_t* q_lens, const int32_t* kv_lens,
+                                                     int32_t num_requests, int32_t num_qo_heads,
+                                                     int32_t padded_dim, int32_t window,
+                                                     int32_t sink) {
+  if (window < 1 || sink < 0) return 0;
+  return tq::batch_workspace(q_lens, kv_lens, num_requests, num_qo_heads, padded_dim, window, sink);
+}
+
+extern "C" int tq_prefill_attention_window(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head, int32_t q_dtype, const void* k,
+    int64_t k_stride_tok, int64_t k_stride_head, const void* v, int64_t v_stride_tok,
+    int64_t v_stride_head, const void* k2, const void* v2, int64_t k2_stride_tok,
+    int64_t k2_stride_head, void* o, int64_t o_stride_tok, int64_t o_stride_head, int32_t o_dtype,
+    const int32_t* q_starts, const int32_t* q_lens, const int32_t* kv_starts,
+    const int32_t* kv_lens, const int32_t* kv_sources, int32_t num_requests, int32_t num_qo_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t padded_dim, float sm_scale, int32_t window,
+    int32_t sink, void* workspace, int64_t workspace_bytes, tq_stream_t stream) {
+  const char* what = "prefill_attention_window";
+  if (window < 1 || sink < 0) {
+    tq::set_error("%s: window %d must be positive and sink %d not negative", what, window, sink);
+    return tq::kEinval;
+  }
+  // (a hidden key's score is -inf: times 0 it would be NaN)
+  if (!(sm_scale > 0.0f) || std::isinf(sm_scale)) {
+    tq::set_error("%s: sm_scale must be positive", what);
+    return tq::kEinval;
+  }
+  return tq::attention_batch(
+      what, window, sink, q, q_stride_tok, q_stride_head, q_dtype, k, k_stride_tok, k_stride_head,
+      v, v_stride_tok, v_stride_head, k2, v2, k2_stride_tok, k2_stride_head, o, o_stride_tok,
+      o_stride_head, o_dtype, q_starts, q_lens, kv_starts, kv_lens, kv_sources, num_requests,
+      num_qo_heads, num_kv_heads, head_dim, padded_dim, sm_scale, workspace, workspace_bytes,
+      stream);
 }
 
 extern "C" int64_t tq_prefill_workspace_bytes(int32_t q_len, int32_t kv_len, int32_t num_qo_heads,

@@ -311,20 +311,22 @@ bool decode_window(const Tensor& q, const Tensor& kv_cache, const Tensor& indice
 // -------------------------------------------------------------------- prefill
 
 using Request = std::array<int32_t, 5>;
+using WindowRequest = std::array<int32_t, 6>;
 
-std::array<std::vector<int32_t>, 5> columns(const std::vector<Request>& reqs) {
-  std::array<std::vector<int32_t>, 5> c;
+template <size_t N>
+std::array<std::vector<int32_t>, N> columns(const std::vector<std::array<int32_t, N>>& reqs) {
+  std::array<std::vector<int32_t>, N> c;
   for (auto& v : c) v.reserve(reqs.size());
-  for (const Request& r : reqs)
-    for (int i = 0; i < 5; i++) c[i].push_back(r[i]);
+  for (const auto& r : reqs)
+    for (size_t i = 0; i < N; i++) c[i].push_back(r[i]);
   return c;
 }
 
-// ops.prefill_attention_batch
-bool prefill_batch(const Tensor& q, const Tensor& o, const std::vector<Request>& reqs,
-                   int64_t num_kv_heads, int64_t head_dim, int64_t padded_dim, double sm_scale,
-                   const OptTensor& k, const OptTensor& v, const OptTensor& k2,
-                   const OptTensor& v2) {
+// ops.prefill_attention_batch, or (window > 0) ops.prefill_attention_window
+bool attention(const Tensor& q, const Tensor& o, const std::vector<Request>& reqs,
+               int64_t num_kv_heads, int64_t head_dim, int64_t padded_dim, double sm_scale,
+               int32_t window, int32_t sink, const OptTensor& k, const OptTensor& v,
+               const OptTensor& k2, const OptTensor& v2) {
   const c10::Device dev = q.device();
   const int qt = dtype_code(q.scalar_type()), ot = dtype_code(o.scalar_type());
   if (!on(q, dev) || !on(o, dev) || q.dim() != 3 || o.sizes() != q.sizes() ||
@@ -350,7 +352,10 @@ bool prefill_batch(const Tensor& q, const Tensor& o, const std::vector<Request>&
   const int32_t n = (int32_t)reqs.size(), hq = (int32_t)q.size(1);
   const c10::DeviceGuard guard(dev);
   const int64_t bytes =
-      tq_prefill_batch_workspace_bytes(c[1].data(), c[3].data(), n, hq, (int32_t)padded_dim);
+      window > 0 ? tq_prefill_window_workspace_bytes(c[1].data(), c[3].data(), n, hq,
+                                                     (int32_t)padded_dim, window, sink)
+                 : tq_prefill_batch_workspace_bytes(c[1].data(), c[3].data(), n, hq,
+                                                    (int32_t)padded_dim);
   Tensor ws;
   if (bytes > 0) {
     ws = at::empty({bytes}, q.options().dtype(at::kByte));
@@ -360,12 +365,88 @@ bool prefill_batch(const Tensor& q, const Tensor& o, const std::vector<Request>&
     return t.has_value() ? t->const_data_ptr() : nullptr;
   };
   const auto st = [](const OptTensor& t, int i) { return t.has_value() ? t->stride(i) : 0; };
+  if (window > 0)
+    return tq_prefill_attention_window(
+               q.const_data_ptr(), q.stride(0), q.stride(1), qt, ptr(k), st(k, 0), st(k, 1), ptr(v),
+               st(v, 0), st(v, 1), ptr(k2), ptr(v2), st(k2, 0), st(k2, 1), o.data_ptr(),
+               o.stride(0), o.stride(1), ot, c[0].data(), c[1].data(), c[2].data(), c[3].data(),
+               c[4].data(), n, hq, num_kv_heads, head_dim, padded_dim, (float)sm_scale, window,
+               sink, bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream_of(dev)) == 0;
   return tq_prefill_attention_batch(
              q.const_data_ptr(), q.stride(0), q.stride(1), qt, ptr(k), st(k, 0), st(k, 1), ptr(v),
              st(v, 0), st(v, 1), ptr(k2), ptr(v2), st(k2, 0), st(k2, 1), o.data_ptr(), o.stride(0),
              o.stride(1), ot, c[0].data(), c[1].data(), c[2].data(), c[3].data(), c[4].data(), n,
              hq, num_kv_heads, head_dim, padded_dim, (float)sm_scale,
              bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream_of(dev)) == 0;
+}
+
+bool prefill_batch(const Tensor& q, const Tensor& o, const std::vector<Request>& reqs,
+                   int64_t num_kv_heads, int64_t head_dim, int64_t padded_dim, double sm_scale,
+                   const OptTensor& k, const OptTensor& v, const OptTensor& k2,
+                   const OptTensor& v2) {
+  return attention(q, o, reqs, num_kv_heads, head_dim, padded_dim, sm_scale, 0, 0, k, v, k2, v2);
+}
+
+bool prefill_window(const Tensor& q, const Tensor& o, const std::vector<Request>& reqs,
+                    int64_t num_kv_heads, int64_t head_dim, int64_t padded_dim, double sm_scale,
+                    int64_t window, int64_t sink, const OptTensor& k, const OptTensor& v,
+                    const OptTensor& k2, const OptTensor& v2) {
+  return window_ok(window, sink) &&
+         attention(q, o, reqs, num_kv_heads, head_dim, padded_dim, sm_scale, (int32_t)window,
+                   (int32_t)sink, k, v, k2, v2);
+}
+
+// ops.prefill_gather_window
+bool gather_window(const OptTensor& kv_cache, const OptTensor& table, const OptTensor& key,
+                   const OptTensor& value, const std::vector<WindowRequest>& reqs, int64_t sink,
+                   int64_t head_dim, int64_t padded_dim, const OptTensor& signs,
+                   const Tensor& out_k, const Tensor& out_v) {
+  const c10::Device dev = out_k.device();
+  const float* sp = nullptr;
+  if (!window_ok(1, sink) || key.has_value() != value.has_value() ||
+      !signs_of(signs, padded_dim, dev, sp) || reqs.empty())
+    return false;
+  for (const Tensor* t : {&out_k, &out_v})
+    if (!on(*t, dev) || t->scalar_type() != at::kHalf || t->dim() != 3 ||
+        t->size(1) != out_k.size(1) || t->size(2) != padded_dim || !t->is_contiguous())
+      return false;
+  const int64_t h = out_k.size(1);
+  int kt = TQ_F16;
+  if (key.has_value()) {
+    kt = dtype_code(key->scalar_type());
+    if (!on(*key, dev) || !on(*value, dev) || kt < 0 ||
+        value->scalar_type() != key->scalar_type() || key->dim() != 3 ||
+        value->sizes() != key->sizes() || key->size(1) != h || key->size(2) != head_dim ||
+        key->stride(2) != 1 || value->stride(2) != 1)
+      return false;
+  }
+  // context needs the cache and its table; a step without any leaves both to ops.py
+  Cache c;
+  if (!kv_cache.has_value() || !table.has_value() || !cache_of(*kv_cache, dev, c) ||
+      c.heads != h || !on(*table, dev) || table->scalar_type() != at::kInt || table->dim() != 2 ||
+      table->stride(1) != 1)
+    return false;
+  const int64_t rows = std::min(out_k.size(0), out_v.size(0));
+  const int64_t fresh = key.has_value() ? key->size(0) : 0;
+  for (const WindowRequest& r : reqs) {  // table_row, ctx, first, fresh_start, fresh_len, out_start
+    if (r[2] < 0 || r[2] > r[1] || r[3] < 0 || r[4] < 0 || r[5] < 0 || r[0] < 0) return false;
+    const int64_t kept = std::min<int64_t>(sink, r[2]) + r[1] - r[2];
+    if (r[5] + kept + r[4] > rows || (int64_t)r[3] + r[4] > fresh ||
+        (kept > 0 && (r[0] >= table->size(0) || r[1] > table->size(1) * c.block_size)))
+      return false;
+  }
+  const auto cols = columns(reqs);
+  const c10::DeviceGuard guard(dev);
+  const auto ptr = [](const OptTensor& t) -> const void* {
+    return t.has_value() ? t->const_data_ptr() : nullptr;
+  };
+  const auto st = [](const OptTensor& t, int i) { return t.has_value() ? t->stride(i) : 0; };
+  return tq_prefill_gather_window(
+             c.k, c.v, cptr<int32_t>(*table), table->stride(0), h, head_dim, padded_dim,
+             c.block_size, c.ebs, c.num_blocks, sp, ptr(key), ptr(value), kt, st(key, 0),
+             st(key, 1), st(value, 0), st(value, 1), cols[0].data(), cols[1].data(),
+             cols[2].data(), cols[3].data(), cols[4].data(), cols[5].data(), (int32_t)reqs.size(),
+             sink, out_k.data_ptr(), out_v.data_ptr(), stream_of(dev)) == 0;
 }
 
 // ops.prefill_gather
@@ -665,7 +746,9 @@ PYBIND11_MODULE(_tq_torch, m) {
   m.def("evict", &evict, unlocked);
   m.def("decode_window", &decode_window, unlocked);
   m.def("prefill_batch", &prefill_batch, unlocked);
+  m.def("prefill_window", &prefill_window, unlocked);
   m.def("prefill_gather", &prefill_gather, unlocked);
+  m.def("gather_window", &gather_window, unlocked);
   m.def("mse_quantize", &mse_quantize, unlocked);
   m.def("mse_dequantize", &mse_dequantize, unlocked);
   m.def("qjl_halves", &qjl_halves, unlocked);

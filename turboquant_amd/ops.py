@@ -341,30 +341,37 @@ def prefill_attention_batch(q: torch.Tensor, o: torch.Tensor, requests, num_kv_h
     if (_nat or _native()).prefill_batch(q, o, requests, num_kv_heads, head_dim, padded_dim,
                                          sm_scale, k, v, k2, v2):
         return o
+    return _prefill_batch("prefill_attention_batch", q, o, requests, num_kv_heads, head_dim,
+                          padded_dim, sm_scale, k, v, k2, v2, None)
+
+
+def _prefill_batch(what, q, o, requests, num_kv_heads, head_dim, padded_dim, sm_scale, k, v, k2,
+                   v2, window):
+    """prefill_attention_batch, or under `window` = (window, sink)"""
     kvs = [t for t in (k, v, k2, v2) if t is not None]
     _require_gpu(q, o, *kvs)
     hq = q.size(1)
     if q.dim() != 3 or tuple(o.shape) != tuple(q.shape) or q.size(2) != head_dim:
-        raise RuntimeError("prefill_attention_batch: q / o must be [tokens, heads, head_dim]")
+        raise RuntimeError(f"{what}: q / o must be [tokens, heads, head_dim]")
     if q.dtype not in (torch.float16, torch.bfloat16) or \
             o.dtype not in (torch.float16, torch.bfloat16) or q.stride(2) != 1 or o.stride(2) != 1:
-        raise RuntimeError("prefill_attention_batch: q / o must be fp16 or bf16 with contiguous "
+        raise RuntimeError(f"{what}: q / o must be fp16 or bf16 with contiguous "
                            "dims")
     for t in kvs:
         if t.dtype != torch.float16 or t.dim() != 3 or t.stride(2) != 1 or \
                 tuple(t.shape[1:]) != (num_kv_heads, padded_dim):
-            raise RuntimeError("prefill_attention_batch: k / v must be fp16 [tokens, Hkv, "
+            raise RuntimeError(f"{what}: k / v must be fp16 [tokens, Hkv, "
                                "padded_dim] with contiguous dims")
     for a, b in ((k, v), (k2, v2)):
         if (a is None) != (b is None) or (a is not None and a.size(0) != b.size(0)):
-            raise RuntimeError("prefill_attention_batch: k and v must go together")
+            raise RuntimeError(f"{what}: k and v must go together")
     if k2 is not None and k2.stride() != v2.stride():
-        raise RuntimeError("prefill_attention_batch: k2 and v2 must share their strides")
+        raise RuntimeError(f"{what}: k2 and v2 must share their strides")
     for qs, ql, ks, kl, src in requests:
         kv = k2 if src else k
         if qs < 0 or ql < 0 or qs + ql > q.size(0) or kv is None or ks < 0 or kl < ql \
                 or ks + kl > kv.size(0):
-            raise RuntimeError("prefill_attention_batch: a request is out of range")
+            raise RuntimeError(f"{what}: a request is out of range")
     n = len(requests)
     cols = [(ctypes.c_int32 * max(1, n))(*c) for c in
             (zip(*requests) if n else ((),) * 5)]
@@ -372,15 +379,18 @@ def prefill_attention_batch(q: torch.Tensor, o: torch.Tensor, requests, num_kv_h
     st = lambda t: (0, 0) if t is None else (t.stride(0), t.stride(1))
     ptr = lambda t: None if t is None else t.data_ptr()
     with torch.cuda.device(q.device):
-        nbytes = int(lib.tq_prefill_batch_workspace_bytes(cols[1], cols[3], n, hq,
-                                                          int(padded_dim)))
+        call, size, more = lib.tq_prefill_attention_batch, lib.tq_prefill_batch_workspace_bytes, ()
+        if window is not None:
+            call, size = lib.tq_prefill_attention_window, lib.tq_prefill_window_workspace_bytes
+            more = (int(window[0]), int(window[1]))
+        nbytes = int(size(cols[1], cols[3], n, hq, int(padded_dim), *more))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
-        rc = lib.tq_prefill_attention_batch(
+        rc = call(
             q.data_ptr(), *st(q), _DTYPES[q.dtype], ptr(k), *st(k), ptr(v), *st(v), ptr(k2),
             ptr(v2), *st(k2), o.data_ptr(), *st(o), _DTYPES[o.dtype], *cols, n, hq,
-            int(num_kv_heads), int(head_dim), int(padded_dim), float(sm_scale), ptr(ws), nbytes,
-            _stream_ptr(q.device))
-    _lib.check(rc, "prefill_attention_batch")
+            int(num_kv_heads), int(head_dim), int(padded_dim), float(sm_scale), *more, ptr(ws),
+            nbytes, _stream_ptr(q.device))
+    _lib.check(rc, what)
     return o
 
 
@@ -442,18 +452,27 @@ def prefill_gather(kv_cache: torch.Tensor | None, block_table: torch.Tensor | No
     if (_nat or _native()).prefill_gather(kv_cache, block_table, key, value, requests, head_dim,
                                           padded_dim, signs, out_k, out_v):
         return
+    _gather("prefill_gather", kv_cache, block_table, key, value,
+            [(row, ctx, 0, fs, fl, dst) for row, ctx, fs, fl, dst in requests], head_dim,
+            padded_dim, signs, out_k, out_v, None)
+
+
+def _gather(what, kv_cache, block_table, key, value, requests, head_dim, padded_dim, signs, out_k,
+            out_v, sink):
+    """prefill_gather of requests (table_row, ctx, first, fresh_start, fresh_len,
+    out_start), every first 0, or (sink given) prefill_gather_window"""
     _require_gpu(key, value, out_k, out_v)
     if key.dtype not in _DTYPES or value.dtype != key.dtype:
         raise RuntimeError(f"key/value must share a float dtype, got {key.dtype}/{value.dtype}")
     if key.dim() != 3 or value.shape != key.shape or key.size(2) != head_dim \
             or key.stride(2) != 1 or value.stride(2) != 1:
-        raise RuntimeError("prefill_gather: key/value must be [tokens, heads, head_dim] with "
+        raise RuntimeError(f"{what}: key/value must be [tokens, heads, head_dim] with "
                            "contiguous dims")
     h = key.size(1)
     for t in (out_k, out_v):
         if t.dtype != torch.float16 or t.dim() != 3 or tuple(t.shape[1:]) != (h, padded_dim) \
                 or not t.is_contiguous():
-            raise RuntimeError("prefill_gather: out_k / out_v must be contiguous fp16 "
+            raise RuntimeError(f"{what}: out_k / out_v must be contiguous fp16 "
                                "[rows, H_kv, padded_dim]")
     rows = min(out_k.size(0), out_v.size(0))
     bs, nb, ebs, base, slab, bt, bt_rows = 16, 0, entry_bytes(head_dim)[2], 0, 0, 0, 0
@@ -470,13 +489,14 @@ def prefill_gather(kv_cache: torch.Tensor | None, block_table: torch.Tensor | No
         ebs = kv_cache.size(-1) * kv_cache.element_size()
         base, slab, bt, bt_rows = kv_cache.data_ptr(), nb * bs * h * ebs, block_table.data_ptr(), \
             block_table.size(0)
-    for row, ctx, fs, fl, dst in requests:
-        if ctx < 0 or fs < 0 or fl < 0 or dst < 0 or dst + ctx + fl > rows \
-                or fs + fl > key.size(0):
-            raise RuntimeError("prefill_gather: a request is out of range")
-        if ctx > 0 and (not bt or not 0 <= row < bt_rows):
-            raise RuntimeError("prefill_gather: cached context needs the cache and a table row")
-        if ctx > 0 and ctx > block_table.size(1) * bs:
+    for row, ctx, first, fs, fl, dst in requests:
+        kept = ctx if sink is None else min(sink, first) + ctx - first
+        if ctx < 0 or not 0 <= first <= ctx or fs < 0 or fl < 0 or dst < 0 \
+                or dst + kept + fl > rows or fs + fl > key.size(0):
+            raise RuntimeError(f"{what}: a request is out of range")
+        if kept > 0 and (not bt or not 0 <= row < bt_rows):
+            raise RuntimeError(f"{what}: cached context needs the cache and a table row")
+        if kept > 0 and ctx > block_table.size(1) * bs:
             raise RuntimeError("pages do not cover num_tokens")
     sp = 0
     if signs is not None and signs.numel() > 0:
@@ -491,12 +511,16 @@ def prefill_gather(kv_cache: torch.Tensor | None, block_table: torch.Tensor | No
     cols = [(ctypes.c_int32 * n)(*c) for c in zip(*requests)]
     lib = _lib.load()
     with torch.cuda.device(key.device):
-        rc = lib.tq_prefill_gather(
-            base, base + slab, bt, block_table.stride(0) if bt else 0, h, int(head_dim),
-            int(padded_dim), bs, ebs, nb, sp, key.data_ptr(), value.data_ptr(),
-            _DTYPES[key.dtype], key.stride(0), key.stride(1), value.stride(0), value.stride(1),
-            *cols, n, out_k.data_ptr(), out_v.data_ptr(), _stream_ptr(key.device))
-    _lib.check(rc, "prefill_gather")
+        source = (base, base + slab, bt, block_table.stride(0) if bt else 0, h, int(head_dim),
+                  int(padded_dim), bs, ebs, nb, sp, key.data_ptr(), value.data_ptr(),
+                  _DTYPES[key.dtype], key.stride(0), key.stride(1), value.stride(0),
+                  value.stride(1))
+        into = (out_k.data_ptr(), out_v.data_ptr(), _stream_ptr(key.device))
+        if sink is None:
+            rc = lib.tq_prefill_gather(*source, cols[0], cols[1], *cols[3:], n, *into)
+        else:
+            rc = lib.tq_prefill_gather_window(*source, *cols, n, int(sink), *into)
+    _lib.check(rc, what)
 
 
 def _floats(values) -> list | tuple:
@@ -1135,6 +1159,56 @@ def decode_paged_window(q: torch.Tensor, kv_cache: torch.Tensor, indices: torch.
             _stream_ptr(q.device))
     _lib.check(rc, what)
     return o
+
+
+def prefill_attention_window(q: torch.Tensor, o: torch.Tensor, requests, num_kv_heads: int,
+                             head_dim: int, padded_dim: int, sm_scale: float, window: int,
+                             sink: int = 0, k: torch.Tensor | None = None,
+                             v: torch.Tensor | None = None, k2: torch.Tensor | None = None,
+                             v2: torch.Tensor | None = None) -> torch.Tensor:
+    """prefill_attention_batch under a sliding window: a query at place P of its
+    request's keys sees the keys j with P - window < j <= P, and j < sink.  The
+    keys may be closed up as prefill_gather_window leaves them.  What K and V
+    hold for a key that a query does not see (NaN too) does not reach it.
+    sm_scale > 0.  tq_prefill_attention_window."""
+    if (_nat or _native()).prefill_window(q, o, requests, num_kv_heads, head_dim, padded_dim,
+                                          sm_scale, window, sink, k, v, k2, v2):
+        return o
+    what = "prefill_attention_window"
+    _check_window(window, sink, what)
+    if not 0 < float(sm_scale) < float("inf"):
+        raise RuntimeError(f"{what}: sm_scale {sm_scale} must be positive")
+    return _prefill_batch(what, q, o, requests, num_kv_heads, head_dim, padded_dim, sm_scale, k, v,
+                          k2, v2, (window, sink))
+
+
+def prefill_gather_window(kv_cache: torch.Tensor | None, block_table: torch.Tensor | None,
+                          key: torch.Tensor | None, value: torch.Tensor | None, requests, sink: int,
+                          head_dim: int, padded_dim: int, signs: torch.Tensor | None,
+                          out_k: torch.Tensor, out_v: torch.Tensor) -> None:
+    """prefill_gather of what a sliding window leaves in sight: `requests` are
+    (table_row, ctx, first, fresh_start, fresh_len, out_start) host integers; of
+    the ctx cached tokens the first min(sink, first) and those from `first` on
+    are read back, closed up, in front of the fresh rows.  A chunk behind ctx
+    tokens needs first = max(0, ctx - window + 1).  Table entries of pages without
+    a token to read may hold anything.  key and value may be None if no request
+    has fresh rows.  tq_prefill_gather_window."""
+    if (_nat or _native()).gather_window(kv_cache, block_table, key, value, requests, sink,
+                                         head_dim, padded_dim, signs, out_k, out_v):
+        return
+    what = "prefill_gather_window"
+    _fit_int32(what, sink=sink)
+    if sink < 0:
+        raise RuntimeError(f"{what}: sink {sink} is negative")
+    if (key is None) != (value is None):
+        raise RuntimeError(f"{what}: key and value must go together")
+    if key is None:  # no fresh rows: any of them is out of range
+        if out_k.dim() != 3:
+            raise RuntimeError(f"{what}: out_k / out_v must be contiguous fp16 "
+                               "[rows, H_kv, padded_dim]")
+        key = value = out_k.new_empty((0, out_k.size(1), head_dim))
+    _gather(what, kv_cache, block_table, key, value, requests, head_dim, padded_dim, signs, out_k,
+            out_v, sink)
 
 
 # --------------------------------------------------------------------------
