@@ -160,6 +160,43 @@ int tq_decode_paged_balanced_noalloc(const void* q, int64_t q_stride_b, int64_t 
                                      tq_stream_t stream);
 
 /*
+ * A layer's fused projection to what its attention takes, in one launch (no
+ * counterpart in the reference, whose models norm and rotate on their own and
+ * then write): row t of qkv (dtype TQ_F16 or TQ_BF16, qkv_row_stride elements
+ * apart) holds num_qo_heads q heads, then num_kv_heads k heads, then as many v
+ * heads of head_dim elements.  q and k heads are divided by sqrt(mean(x^2) +
+ * eps) and multiplied by their weight [head_dim] of the rows' type (both null:
+ * neither), then dims (i, i + rotated / 2), i < rotated / 2, turned by the
+ * angle of pair i, all in fp32, and rounded once to the rows' type: q_out
+ * [num_tokens, num_qo_heads, head_dim] and (if not null) k_out [num_tokens,
+ * num_kv_heads, head_dim].  K (as rounded) and V of tokens with 0 <=
+ * slot_mapping[t] < num_blocks * block_size go to that slot of the cache, the
+ * bytes of tq_quantize_write_kv_cache over those rows (which of several NaN
+ * elements gives a NaN norm its sign is left open); such slots must differ from
+ * token to token.
+ *
+ * cos_table, sin_table fp32 [table_rows, rotated / 2]; pair i takes the row
+ * positions[a * position_stride + t] (position_bytes 4 or 8: int32 or int64) of
+ * its axis a: the first sections[0] pairs belong to axis 0, the next
+ * sections[1] to axis 1, and so on, axes <= 4 of them (a HOST array, read
+ * before the call returns; they add up to rotated / 2).  A token with a
+ * position outside the tables gets NaN rows, and entries as the write of such
+ * rows leaves them.  eps is at least 2^-126; rotated is a multiple of 16,
+ * head_dim of 8; tensors are 16-byte aligned, and q_out, k_out and qkv do not
+ * overlap.
+ */
+int tq_norm_rope_write(const void* qkv, int64_t qkv_row_stride, int32_t dtype,
+                       const void* q_weight, const void* k_weight, float eps,
+                       const float* cos_table, const float* sin_table, int64_t table_rows,
+                       int32_t rotated, const void* positions, int32_t position_bytes,
+                       int64_t position_stride, const int32_t* sections, int32_t axes,
+                       void* k_slab, void* v_slab, const float* signs,
+                       const int32_t* slot_mapping, int64_t num_tokens, int32_t num_qo_heads,
+                       int32_t num_kv_heads, int32_t head_dim, int32_t padded_dim,
+                       int32_t block_size, int32_t ebs, int64_t num_blocks, void* q_out,
+                       void* k_out, tq_stream_t stream);
+
+/*
  * The first kernel of tq_decode_paged_balanced alone: the plan, the partial
  * rows (fp16 in partition_o) and partition_lse, and the row table in
  * split_rows; tq_combine_splits does not read a plan's rows, so this serves

@@ -107,9 +107,11 @@ def test_abi_refuses_bad_decode_arguments(bad, match):
 
 def test_schemas_declare_the_writes():
     ops.register_ops()
-    written = {"decode_paged_window": {"o"}}
+    written = {"turboquant_v5.decode_paged_window": {"o"},
+               "turboquant_write.norm_rope_write": {"kv_cache", "q", "k"}}
     for name, want in written.items():
-        schema = getattr(torch.ops.turboquant_v5, name).default._schema
+        space, name = name.split(".")
+        schema = getattr(getattr(torch.ops, space), name).default._schema
         got = {a.name for a in schema.arguments if a.alias_info and a.alias_info.is_write}
         assert got == want and not schema.returns
 
@@ -297,3 +299,113 @@ def test_reference_prefill():
     v[2], v[8] = torch.nan, torch.inf
     o = W.prefill(q, k, v, [(0, 5, 0, 9, 0)], 2, 0.3, 3, 1)
     assert torch.isnan(o[0]).all() and torch.isfinite(o[1:4]).all() and (o[4] == torch.inf).all()
+
+
+# ---------------------------------------------------- norm, rotation and write
+
+def _norm_write(**bad):
+    t = lambda s, d: torch.zeros(s, dtype=d)
+    half = torch.float16
+    a = dict(qkv=t((5, 12 * 128), half), qw=t((128,), half), kw=t((128,), half),
+             cos=t((30, 64), torch.float32), sin=t((30, 64), torch.float32),
+             pos=t((5,), torch.int64), cache=t((2, 4, 16, 2, 80), torch.uint8),
+             signs=t((128,), torch.float32), slots=t((5,), torch.int32), hq=8, hd=128, pd=128,
+             q=t((5, 8, 128), half), k=t((5, 2, 128), half), eps=1e-6, sections=None)
+    a.update(bad)
+    ops.norm_rope_write(a["qkv"], a["qw"], a["kw"], a["cos"], a["sin"], a["pos"], a["cache"],
+                        a["signs"], a["slots"], a["hq"], a["hd"], a["pd"], a["q"], a["k"], a["eps"],
+                        a["sections"])
+
+
+@pytest.mark.parametrize("bad,match", [
+    (dict(qkv=_meta((5, 12 * 128), torch.float32)), "qkv must be"),
+    (dict(qkv=_meta((5, 11 * 128), torch.float16)), "qkv must be"),
+    (dict(hq=9), "qkv must be"), (dict(hq=0), "q heads"), (dict(hq=2 ** 33), "out of range"),
+    (dict(qw=None), "both weights"), (dict(qw=_meta((128,), torch.bfloat16)), "q_weight"),
+    (dict(kw=_meta((64,), torch.float16)), "k_weight"),
+    (dict(cos=_meta((30, 64), torch.float16)), "cos and sin"),
+    (dict(sin=_meta((30, 32), torch.float32)), "cos and sin"),
+    (dict(pos=_meta((4,), torch.int64)), "positions"),
+    (dict(pos=_meta((5,), torch.int16)), "positions"),
+    (dict(pos=_meta((3, 5), torch.int64)), "sections"),
+    (dict(pos=_meta((3, 5), torch.int64), sections=(32, 32)), "sections"),
+    (dict(pos=_meta((3, 5), torch.int64), sections=(32, 32, 1)), "sections"),
+    (dict(pos=_meta((3, 5), torch.int64), sections=(65, -2, 1)), "sections"),
+    (dict(pos=_meta((5, 5), torch.int64), sections=(60, 1, 1, 1, 1)), "sections"),
+    (dict(slots=_meta((5,), torch.int64)), "slot_mapping"),
+    (dict(slots=_meta((4,), torch.int32)), "slot_mapping"),
+    (dict(q=_meta((5, 8, 128), torch.bfloat16)), "q must be"),
+    (dict(q=_meta((4, 8, 128), torch.float16)), "q must be"),
+    (dict(k=_meta((5, 8, 128), torch.float16)), "k must be"),
+    (dict(cache=_meta((1, 4, 16, 2, 80), torch.uint8)), "kv_cache"),
+    (dict(cache=_meta((4, 16, 2, 80), torch.uint8)), "kv_cache"),
+    (dict(signs=_meta((64,), torch.float32)), "signs"),
+])
+def test_norm_write_refusals(monkeypatch, bad, match):
+    monkeypatch.setattr(ops, "_require_gpu", lambda *t: None)
+    with pytest.raises(RuntimeError, match=f"norm_rope_write: .*{match}"):
+        _norm_write(**bad)
+
+
+def test_norm_write_refuses_cpu_tensors():
+    with pytest.raises(RuntimeError, match="GPU only"):
+        _norm_write()
+
+
+@pytest.mark.parametrize("bad,match", [
+    (dict(pd=96), b"padded_dim"), (dict(hd=100), b"head_dim"), (dict(hd=64), b"head_dim"),
+    (dict(hd=0), b"head_dim"), (dict(rot=0), b"rotated"), (dict(rot=24), b"rotated"),
+    (dict(rot=144), b"rotated"), (dict(dt=0), b"fp16 or bf16"), (dict(ebs=82), b"ebs"),
+    (dict(hq=0), b"bad sizes"), (dict(hkv=5000), b"bad sizes"), (dict(bs=0), b"bad sizes"),
+    (dict(n=-1), b"bad sizes"), (dict(rows=-1), b"bad sizes"), (dict(pb=2), b"positions"),
+    (dict(axes=0), b"positions"), (dict(axes=5), b"positions"), (dict(sec=(63,)), b"sections"),
+    (dict(sec=(65, -1), axes=2), b"sections"), (dict(kw=None), b"both weights"),
+    (dict(eps=0.0), b"eps"), (dict(eps=-1.0), b"eps"), (dict(eps=float("nan")), b"eps"),
+    (dict(eps=float("inf")), b"eps"), (dict(qkv=None), b"null"), (dict(cos=None), b"null"),
+    (dict(slots=None), b"null"), (dict(cache=None), b"null"), (dict(q=None), b"null"),
+    (dict(signs=None), b"null"), (dict(rows=0), b"empty"), (dict(st=1528), b"stride"),
+    (dict(st=1540), b"stride"), (dict(off=8), b"aligned"), (dict(q=0x1000), b"overlap"),
+    (dict(k=0x1000), b"overlap"),
+])
+def test_abi_refuses_bad_norm_write_arguments(bad, match):
+    lib = _lib.load()
+    at = lambda i: 0x1000 + (i << 24)  # addresses that are never read
+    a = dict(qkv=at(0), st=1536, dt=1, qw=at(1), kw=at(1), eps=1e-6, cos=at(2), rows=30, rot=128,
+             pos=at(3), pb=8, sec=(64,), axes=1, cache=at(4), signs=at(5), slots=at(6), n=5, hq=8,
+             hkv=2, hd=128, pd=128, bs=16, ebs=80, q=at(7), k=at(8), off=0)
+    a.update(bad)
+    qkv = a["qkv"] and a["qkv"] + a["off"]
+
+    def call():
+        return lib.tq_norm_rope_write(
+            qkv, a["st"], a["dt"], a["qw"], a["kw"], a["eps"], a["cos"], a["cos"], a["rows"],
+            a["rot"], a["pos"], a["pb"], 5, _ints(*a["sec"]), a["axes"], a["cache"], a["cache"],
+            a["signs"], a["slots"], a["n"], a["hq"], a["hkv"], a["hd"], a["pd"], a["bs"], a["ebs"],
+            9, a["q"], a["k"], None)
+    assert call() == -22 and match in lib.tq_last_error(), lib.tq_last_error()
+
+
+def test_norm_write_of_no_tokens_does_nothing():
+    lib = _lib.load()
+    assert lib.tq_norm_rope_write(None, 0, 1, None, None, 1e-6, None, None, 0, 128, None, 8, 0,
+                                  _ints(64), 1, None, None, None, None, 0, 8, 2, 128, 128, 16, 80, 9,
+                                  None, None, None) == 0
+
+
+def test_reference_norm_and_rotation():
+    """A rotation keeps a pair's length and turns it by its position's angle; the
+    norm makes the mean square 1."""
+    g = torch.Generator().manual_seed(2)
+    qkv = torch.randn((4, 3 * 8), generator=g, dtype=torch.float64)
+    ones = torch.ones(8)
+    angle = torch.arange(10)[:, None] * torch.tensor([[1.0, 0.1, 0.01]])
+    pos = torch.tensor([[0, 3, 9, 10], [5, 3, 2, 1]])
+    q, k, before = W.norm_rope(qkv, ones, ones, angle.cos(), angle.sin(), pos, (2, 1), 1, 1, 8,
+                               1e-12)
+    assert torch.allclose((before ** 2).mean(-1), torch.ones((4, 2), dtype=torch.float64))
+    assert torch.isnan(q[3]).all() and torch.isnan(k[3]).all()
+    z0 = torch.complex(before[:, 0, :3], before[:, 0, 3:6])[:3]
+    z1 = torch.complex(q[:, 0, :3], q[:, 0, 3:6])[:3]
+    turn = torch.stack((angle[pos[0, :3], 0], angle[pos[0, :3], 1], angle[pos[1, :3], 2]), 1)
+    assert torch.allclose(z1, z0 * torch.polar(torch.ones(3, 3), turn).to(z0.dtype), atol=1e-6)
+    assert torch.equal(q[:3, 0, 6:], before[:3, 0, 6:])

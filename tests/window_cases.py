@@ -88,3 +88,27 @@ def prefill(q, k, v, requests, ratio, scale, window, sink):
                 out = torch.where(hit(torch.isnan(vv)) | (up & down), torch.nan, out)
                 o[qs + at:qs + at + n, h] = out
     return o
+
+
+def norm_rope(qkv, qw, kw, cos, sin, positions, sections, hq, hkv, hd, eps):
+    """(q, k, their normed values in front of the rotation) [T, H, hd] in 64 bits
+    of qkv [T, (Hq + 2 Hkv) hd]; a position outside the tables gives NaN rows."""
+    import torch
+    n, half = len(qkv), cos.shape[1]
+    x = qkv.double().view(n, -1, hd)
+    pos = positions.view(-1, n).long()
+    inside = ((pos >= 0) & (pos < len(cos))).all(0)
+    at, c, s = 0, [], []
+    for p, m in zip(pos.clamp(0, len(cos) - 1), sections):
+        c.append(cos.double()[p, at:at + m])
+        s.append(sin.double()[p, at:at + m])
+        at += m
+    c, s = (torch.where(inside[:, None], torch.cat(t, 1), torch.nan)[:, None] for t in (c, s))
+    out = []
+    for y, w in ((x[:, :hq], qw), (x[:, hq:hq + hkv], kw)):
+        if w is not None:
+            y = y / torch.sqrt((y * y).mean(-1, keepdim=True) + eps) * w.double()
+        a, b = y[..., :half], y[..., half:2 * half]
+        z = torch.cat((a * c - b * s, b * c + a * s, y[..., 2 * half:]), -1)
+        out.append((torch.where(inside[:, None, None], z, torch.nan), y))
+    return out[0][0], out[1][0], torch.cat((out[0][1], out[1][1]), 1)

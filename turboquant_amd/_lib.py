@@ -107,6 +107,9 @@ SIGNATURES = {
     "tq_decode_paged_window": (_I32, [_P, _I64, _I64, _I32, _P, _P, _P, _I64, _P, _P, _I32, _I32,
                                       _I32, _I32, _I32, _I32, _I32, _I64, _F32, _P, _I32, _I32, _P,
                                       _I32, _P, _I64, _P]),
+    "tq_norm_rope_write": (_I32, [_P, _I64, _I32, _P, _P, _F32, _P, _P, _I64, _I32, _P, _I32, _I64,
+                                  _P, _I32, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32,
+                                  _I32, _I64, _P, _P, _P]),
     "tq_last_error": (ctypes.c_char_p, []),
     "tq_abi_version": (_I32, []),
 }

@@ -1,0 +1,417 @@
+// tq_norm_write.hip -- the rows of a layer's fused projection to what its
+// attention takes, in one pass: q and k heads normed and rotated, K and V
+// quantised into the packed cache.
+//
+// A row of qkv holds Hq q heads, H k heads and H v heads of hd elements.  Per q
+// and k head x (fp32 throughout):
+//   n = x / sqrt(mean(x^2) + eps) * w          (no weights: n = x)
+//   y_i        = n_i        c_i - n_{i+half} s_i
+//   y_{i+half} = n_{i+half} c_i + n_i        s_i      0 <= i < half
+//   y_d        = n_d                                  d >= 2 half
+// with (c_i, s_i) = (cos, sin)[pos[axis(i)], i]: positions of several axes (time,
+// height, width) share the pairs out in sections, one after the other.  y is
+// rounded once, to the row's type; q and k rows leave as they are rounded, and
+// the cache takes the rounded k and the v as they come, so its bytes are those
+// of tq_quantize_write_kv_cache over these rows (tq_quant.h, the same code).
+//
+// A workgroup takes 64 vectors (32 at pd 256) of one kind, K first (their work is
+// longest), then V, then q: the kind is uniform, and q workgroups leave before
+// the bucketize.  32 dims per lane, chunks of 8 as the
+// write has them: where half a rotation is a whole number of chunk rows (the
+// whole head at every padded size, half of it at 128 and 256) a pair stands in
+// one lane, else the partner chunk is read again (from L1).
+#include <algorithm>
+
+#include "tq_quant.h"
+
+namespace tq {
+namespace {
+
+constexpr int kMaxAxes = 4;
+
+struct NormWriteParams {
+  const uint16_t* qkv;
+  int64_t row;  // elements from row to row
+  const uint16_t* qw;
+  const uint16_t* kw;
+  float eps, inv_hd;
+  const float* cos_t;
+  const float* sin_t;
+  int64_t trows;
+  int half, axes;
+  int ends[kMaxAxes];  // the first pair behind each axis' section
+  const void* pos;
+  int pos64;
+  int64_t pos_st;  // entries from axis to axis
+  uint8_t* ks;
+  uint8_t* vs;
+  const float* signs;
+  const int32_t* slots;
+  uint32_t tokens, mq, mk;  // mq, mk: ceil(2^32 / heads)
+  int hq, hkv, hd, ebs;
+  int64_t nslots;
+  float scale;
+  uint16_t* q;
+  uint16_t* k;
+  uint32_t kblocks;
+};
+
+template <int DT>
+__device__ __forceinline__ float elem(const u32x4& v, int c) {
+  if constexpr (DT == TQ_BF16)
+    return __uint_as_float(c & 1 ? v[c / 2] & 0xffff0000u : v[c / 2] << 16);
+  return c & 1 ? hi_half_f(v[c / 2]) : lo_half_f(v[c / 2]);
+}
+
+// eight floats rounded to DT (to nearest even)
+template <int DT>
+__device__ __forceinline__ u32x4 round8(const float* y) {
+  typedef float f8 __attribute__((ext_vector_type(8)));
+  const f8 v = {y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]};
+  if constexpr (DT == TQ_BF16) {
+    typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+    return __builtin_bit_cast(u32x4, __builtin_convertvector(v, b8));
+  } else {
+    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+    return __builtin_bit_cast(u32x4, __builtin_convertvector(v, h8));
+  }
+}
+
+__device__ __forceinline__ void load8(const float* src, float* x) {
+  const float4 a = *reinterpret_cast<const float4*>(src);
+  const float4 b = *reinterpret_cast<const float4*>(src + 4);
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+
+// (cos, sin) of pairs i .. i + 7 of token t; inside: cleared where a position
+// has no table row (its reads go to row 0)
+__device__ __forceinline__ void angles(const NormWriteParams& p, uint32_t t, int i, float* c,
+                                       float* s, bool& inside) {
+  auto row_of = [&](int axis) -> int64_t {
+    const int64_t at = (int64_t)axis * p.pos_st + t;
+    const int64_t r = p.pos64 ? static_cast<const int64_t*>(p.pos)[at]
+                              : static_cast<const int32_t*>(p.pos)[at];
+    const bool ok = r >= 0 && r < p.trows;
+    inside = inside && ok;
+    return ok ? r : 0;
+  };
+  auto axis_of = [&](int pair) -> int {
+    int a = 0;
+    for (int x = 0; x + 1 < p.axes; x++) a += pair >= p.ends[x] ? 1 : 0;
+    return a;
+  };
+  const int first = axis_of(i);
+  if (p.axes == 1 || first == axis_of(i + 7)) {
+    const int64_t at = row_of(first) * p.half + i;
+    load8(p.cos_t + at, c);
+    load8(p.sin_t + at, s);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; e++) {  // a section ends inside the chunk
+    const int64_t at = row_of(axis_of(i + e)) * p.half + i + e;
+    c[e] = p.cos_t[at];
+    s[e] = p.sin_t[at];
+  }
+}
+
+// M: chunk rows from a pair's first half to its second (the pair in one lane), 0:
+// any rotation of whole 16 dims
+template <int PD, int DT, int M>
+__global__ __launch_bounds__(256) void norm_write_kernel(NormWriteParams p) {
+  using FG = FastGeom<PD>;
+  constexpr int P = FG::P, CPL = FG::CPL;
+  __shared__ __attribute__((aligned(512))) uint32_t tbl[128];
+  const int lane = threadIdx.x & 63;
+  const int pl = lane % P;
+  uint32_t blk = blockIdx.x;
+  const bool isq = blk >= 2 * p.kblocks, isv = !isq && blk >= p.kblocks;  // uniform
+  blk -= isq ? 2 * p.kblocks : isv ? p.kblocks : 0u;
+  const uint32_t H = (uint32_t)(isq ? p.hq : p.hkv);
+  uint32_t g = blk * (uint32_t)FG::VPB + (threadIdx.x >> 6) * FG::VPW + lane / P;
+  const bool live = g < p.tokens * H;
+  g = live ? g : 0u;  // lanes past the end work on the first vector and store nothing
+  const uint32_t t = H == 1 ? g : __umulhi(g, isq ? p.mq : p.mk);
+  const uint32_t h = g - t * H;
+  const uint16_t* const src =
+      p.qkv + (int64_t)t * p.row + (int64_t)(isq ? h : p.hq + (isv ? p.hkv : 0) + h) * p.hd;
+  u32x4 raw[CPL];
+#pragma unroll
+  for (int i = 0; i < CPL; i++) {
+    raw[i] = u32x4{0u, 0u, 0u, 0u};
+    if (8 * (pl + P * i) < p.hd) raw[i] = *reinterpret_cast<const u32x4*>(src + 8 * (pl + P * i));
+  }
+  if (!isv) {
+    const uint16_t* const wt = isq ? p.qw : p.kw;
+    bool inside = true;
+    float cs[CPL][8], sn[CPL][8];  // (M > 0: of the chunks of the first halves)
+#pragma unroll
+    for (int i = 0; i < CPL; i++) {
+      const int d = 8 * (pl + P * i);
+      if constexpr (M > 0) {
+        if (i < M) angles(p, t, d, cs[i], sn[i], inside);
+      } else {
+        if (d < 2 * p.half) angles(p, t, d < p.half ? d : d - p.half, cs[i], sn[i], inside);
+      }
+    }
+    float r = 1.0f;
+    if (wt) {  // uniform
+      auto sum_squares = [&](float f) -> float {
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < CPL; i++)
+#pragma unroll
+          for (int c = 0; c < 8; c++) {
+            const float x = elem<DT>(raw[i], c) * f;
+            ss = __builtin_fmaf(x, x, ss);
+          }
+        ss += xor_lane<1>(ss);
+        ss += xor_lane<2>(ss);
+        if constexpr (P == 8) ss += xor_lane<4>(ss);
+        return ss;
+      };
+      const float ss = sum_squares(1.0f);
+      r = rsqrtf(__builtin_fmaf(ss, p.inv_hd, p.eps));
+      if (DT == TQ_BF16 && __builtin_amdgcn_ballot_w64(ss == INFINITY) != 0) {
+        // squares beyond fp32 of values within it: those of the row times 2^-70
+        // (eps is nothing beside them)
+        const float down = 0x1p-70f, s2 = sum_squares(down);
+        if (ss == INFINITY) r = rsqrtf(s2 * p.inv_hd) * down;
+      }
+    }
+    // a lane sees the positions of its own pairs only: a vector is NaN if any of
+    // its lanes lacks a table row
+    float miss = inside ? 0.0f : 1.0f;
+    miss += xor_lane<1>(miss);
+    miss += xor_lane<2>(miss);
+    if constexpr (P == 8) miss += xor_lane<4>(miss);
+    if (miss != 0.0f) r = __builtin_nanf("");
+    auto normed = [&](const u32x4& x, int d, float* n) {
+      u32x4 w = {};
+      if (wt) w = *reinterpret_cast<const u32x4*>(wt + d);
+#pragma unroll
+      for (int c = 0; c < 8; c++) {
+        n[c] = elem<DT>(x, c) * r;
+        if (wt) n[c] *= elem<DT>(w, c);
+      }
+    };
+    float y[CPL][8];
+#pragma unroll
+    for (int i = 0; i < CPL; i++)
+      if (8 * (pl + P * i) < p.hd) normed(raw[i], 8 * (pl + P * i), y[i]);
+    if constexpr (M > 0) {
+#pragma unroll
+      for (int i = 0; i < M; i++)
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+          const float a = y[i][c], b = y[i + M][c];
+          y[i][c] = __builtin_fmaf(a, cs[i][c], -(b * sn[i][c]));
+          y[i + M][c] = __builtin_fmaf(b, cs[i][c], a * sn[i][c]);
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < CPL; i++) {
+        const int d = 8 * (pl + P * i);
+        if (d >= 2 * p.half) continue;
+        const bool low = d < p.half;
+        const int o = low ? d + p.half : d - p.half;
+        float b[8];
+        normed(*reinterpret_cast<const u32x4*>(src + o), o, b);
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+          const float turn = b[c] * sn[i][c];
+          y[i][c] = __builtin_fmaf(y[i][c], cs[i][c], low ? -turn : turn);
+        }
+      }
+    }
+    uint16_t* const out = isq ? p.q : p.k;
+#pragma unroll
+    for (int i = 0; i < CPL; i++) {
+      const int d = 8 * (pl + P * i);
+      if (d >= p.hd) continue;
+      raw[i] = round8<DT>(y[i]);
+      if (live && out) *reinterpret_cast<u32x4*>(out + ((int64_t)t * H + h) * p.hd + d) = raw[i];
+    }
+    if (isq) return;
+  }
+  const int32_t slot = live ? p.slots[t] : -1;
+  uint32_t lo2, hi2, packed[CPL];
+  bin_table(tbl, p.scale, lo2, hi2);
+  const float l2 = quantize_vector<PD, DT>(
+      raw, p.signs, p.scale, p.hd, tbl, lo2, hi2,
+      [&](int i, int c) -> float { return elem<DT>(raw[i], c); }, packed);
+  if (slot >= 0 && (int64_t)slot < p.nslots)
+    store_entry<PD>((isv ? p.vs : p.ks) + ((int64_t)slot * p.hkv + h) * (int64_t)p.ebs, pl, packed,
+                    l2);
+}
+
+template <int PD, int DT>
+hipError_t launch_norm_write(const NormWriteParams& p, dim3 grid, hipStream_t st) {
+  constexpr int P = FastGeom<PD>::P, CPL = FastGeom<PD>::CPL;
+  // chunk rows of half a rotation, where whole and (both halves) inside the lane
+  const int m = p.half % (8 * P) == 0 ? p.half / (8 * P) : 0;
+  if (m == 1)
+    hipLaunchKernelGGL((norm_write_kernel<PD, DT, 1>), grid, dim3(256), 0, st, p);
+  else if (CPL == 4 && m == 2)
+    hipLaunchKernelGGL((norm_write_kernel<PD, DT, CPL / 2>), grid, dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL((norm_write_kernel<PD, DT, 0>), grid, dim3(256), 0, st, p);
+  return hipGetLastError();
+}
+
+// whether [a, a + n) and [b, b + m) share a byte
+bool overlap(const void* a, int64_t n, const void* b, int64_t m) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return a && b && x < y + (uintptr_t)m && y < x + (uintptr_t)n;
+}
+
+}  // namespace
+}  // namespace tq
+
+extern "C" int tq_norm_rope_write(
+    const void* qkv, int64_t qkv_row_stride, int32_t dtype, const void* q_weight,
+    const void* k_weight, float eps, const float* cos_table, const float* sin_table,
+    int64_t table_rows, int32_t rotated, const void* positions, int32_t position_bytes,
+    int64_t position_stride, const int32_t* sections, int32_t axes, void* k_slab, void* v_slab,
+    const float* signs, const int32_t* slot_mapping, int64_t num_tokens, int32_t num_qo_heads,
+    int32_t num_kv_heads, int32_t head_dim, int32_t padded_dim, int32_t block_size, int32_t ebs,
+    int64_t num_blocks, void* q_out, void* k_out, tq_stream_t stream) {
+  using namespace tq;
+  const char* who = "norm_rope_write";
+  const int pd = padded_dim;
+  if (pd != 64 && pd != 128 && pd != 256) {
+    set_error("%s: padded_dim must be 64, 128 or 256, got %d", who, pd);
+    return kEinval;
+  }
+  if (head_dim <= 0 || head_dim > pd || (pd > 64 && 2 * head_dim <= pd) || head_dim % 8 != 0) {
+    set_error("%s: head_dim %d must be a multiple of 8 that pads to %d", who, head_dim, pd);
+    return kEinval;
+  }
+  if (rotated <= 0 || rotated > head_dim || rotated % 16 != 0) {
+    set_error("%s: %d rotated dims must be a multiple of 16 up to head_dim", who, rotated);
+    return kEinval;
+  }
+  if (dtype != TQ_F16 && dtype != TQ_BF16) {
+    set_error("%s: rows must be fp16 or bf16", who);
+    return kEinval;
+  }
+  if (ebs % 16 != 0 || ebs < pd / 2 + 2 * (pd / 64)) {
+    set_error("%s: ebs %d must be a multiple of 16 and >= %d", who, ebs, pd / 2 + 2 * (pd / 64));
+    return kEinval;
+  }
+  if (num_qo_heads <= 0 || num_kv_heads <= 0 || num_qo_heads > 4096 || num_kv_heads > 4096 ||
+      block_size <= 0 || num_tokens < 0 || num_blocks < 0 || table_rows < 0) {
+    set_error("%s: bad sizes", who);
+    return kEinval;
+  }
+  if ((position_bytes != 4 && position_bytes != 8) || axes < 1 || axes > kMaxAxes || !sections ||
+      position_stride < 0) {
+    set_error("%s: positions must be 32 or 64 bits wide, of 1 to %d axes with a section each", who,
+              kMaxAxes);
+    return kEinval;
+  }
+  int64_t pairs = 0;
+  for (int a = 0; a < axes; a++) {
+    if (sections[a] < 0) pairs = -1;
+    if (pairs >= 0) pairs += sections[a];
+  }
+  if (pairs != rotated / 2) {
+    set_error("%s: the sections must add up to the %d rotated pairs", who, rotated / 2);
+    return kEinval;
+  }
+  if ((q_weight == nullptr) != (k_weight == nullptr)) {
+    set_error("%s: both weights must be given, or none", who);
+    return kEinval;
+  }
+  // (below, the squares of small bf16 rows would be lost beside it)
+  if (q_weight && !(eps >= 0x1p-126f && eps < INFINITY)) {
+    set_error("%s: eps must be a positive, normal fp32 number", who);
+    return kEinval;
+  }
+  if (num_tokens == 0) return 0;
+  if (table_rows == 0 || !qkv || !cos_table || !sin_table || !positions || !k_slab || !v_slab ||
+      !signs || !slot_mapping || !q_out) {
+    set_error("%s: null pointer or empty tables", who);
+    return kEinval;
+  }
+  const int64_t width = (int64_t)(num_qo_heads + 2 * num_kv_heads) * head_dim;
+  if (qkv_row_stride < width || qkv_row_stride % 8 != 0) {
+    set_error("%s: the row stride %lld must be a multiple of 8 of at least %lld elements", who,
+              (long long)qkv_row_stride, (long long)width);
+    return kEinval;
+  }
+  const uintptr_t al = (uintptr_t)qkv | (uintptr_t)q_weight | (uintptr_t)k_weight |
+                       (uintptr_t)cos_table | (uintptr_t)sin_table | (uintptr_t)signs |
+                       (uintptr_t)q_out | (uintptr_t)k_out | (uintptr_t)k_slab |
+                       (uintptr_t)v_slab;
+  if ((al & 15) != 0 || (uintptr_t)positions % position_bytes != 0) {
+    set_error("%s: tensors must be 16-byte aligned", who);
+    return kEinval;
+  }
+  const int64_t in_bytes = 2 * ((num_tokens - 1) * qkv_row_stride + width);
+  const int64_t q_bytes = 2 * num_tokens * num_qo_heads * head_dim;
+  const int64_t k_bytes = 2 * num_tokens * num_kv_heads * head_dim;
+  if (overlap(qkv, in_bytes, q_out, q_bytes) || overlap(qkv, in_bytes, k_out, k_bytes) ||
+      overlap(q_out, q_bytes, k_out, k_bytes)) {
+    set_error("%s: q, k and the projection's rows must not overlap", who);
+    return kEinval;
+  }
+  NormWriteParams p = {};
+  p.row = qkv_row_stride;
+  p.qw = static_cast<const uint16_t*>(q_weight);
+  p.kw = static_cast<const uint16_t*>(k_weight);
+  p.eps = eps;
+  p.inv_hd = 1.0f / (float)head_dim;
+  p.cos_t = cos_table;
+  p.sin_t = sin_table;
+  p.trows = table_rows;
+  p.half = rotated / 2;
+  p.axes = axes;
+  for (int a = 0, end = 0; a < axes; a++) p.ends[a] = end += sections[a];
+  p.pos64 = position_bytes == 8;
+  p.pos_st = position_stride;
+  p.ks = static_cast<uint8_t*>(k_slab);
+  p.vs = static_cast<uint8_t*>(v_slab);
+  p.signs = signs;
+  p.hq = num_qo_heads;
+  p.hkv = num_kv_heads;
+  auto recip = [](int h) -> uint32_t {
+    return h == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + h - 1) / h);
+  };
+  p.mq = recip(num_qo_heads);
+  p.mk = recip(num_kv_heads);
+  p.hd = head_dim;
+  p.ebs = ebs;
+  p.nslots = num_blocks * (int64_t)block_size;
+  p.scale = 1.0f / sqrtf((float)pd);
+  const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const int vpb = pd == 64 ? FastGeom<64>::VPB : pd == 128 ? FastGeom<128>::VPB
+                                                           : FastGeom<256>::VPB;
+  // vector / heads by multiply-high is exact below 2^32 / heads: so many tokens
+  // a launch
+  const int64_t heads = std::max(num_qo_heads, num_kv_heads);
+  const int64_t most = std::min<int64_t>(((int64_t)1 << 31) / (heads * heads), (int64_t)1 << 24);
+  for (int64_t a = 0; a < num_tokens; a += most) {
+    p.tokens = (uint32_t)std::min(most, num_tokens - a);
+    p.qkv = static_cast<const uint16_t*>(qkv) + a * qkv_row_stride;
+    p.pos = static_cast<const uint8_t*>(positions) + a * position_bytes;
+    p.slots = slot_mapping + a;
+    p.q = static_cast<uint16_t*>(q_out) + a * num_qo_heads * head_dim;
+    p.k = k_out ? static_cast<uint16_t*>(k_out) + a * num_kv_heads * head_dim : nullptr;
+    p.kblocks = (uint32_t)(((int64_t)p.tokens * num_kv_heads + vpb - 1) / vpb);
+    const int64_t qblocks = ((int64_t)p.tokens * num_qo_heads + vpb - 1) / vpb;
+    const dim3 grid((unsigned)(2 * (int64_t)p.kblocks + qblocks));
+    hipError_t e;
+#define TQ_NW(PD)                                                       \
+  (dtype == TQ_F16 ? launch_norm_write<PD, TQ_F16>(p, grid, st)         \
+                   : launch_norm_write<PD, TQ_BF16>(p, grid, st))
+    e = pd == 64 ? TQ_NW(64) : pd == 128 ? TQ_NW(128) : TQ_NW(256);
+#undef TQ_NW
+    if (e != hipSuccess) {
+      set_error("%s: launch failed: %s", who, hipGetErrorString(e));
+      return (int)e;
+    }
+  }
+  return 0;
+}

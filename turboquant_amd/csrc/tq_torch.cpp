@@ -308,6 +308,65 @@ bool decode_window(const Tensor& q, const Tensor& kv_cache, const Tensor& indice
              sink, o.data_ptr(), ot, ws.data_ptr(), bytes, stream_of(dev)) == 0;
 }
 
+// ops.norm_rope_write
+bool norm_rope_write(const Tensor& qkv, const OptTensor& q_weight, const OptTensor& k_weight,
+                     const Tensor& cos, const Tensor& sin, const Tensor& positions,
+                     const Tensor& kv_cache, const Tensor& signs, const Tensor& slots,
+                     int64_t num_qo_heads, int64_t head_dim, int64_t padded_dim, const Tensor& q,
+                     const OptTensor& k, double eps,
+                     const std::optional<std::vector<int64_t>>& sections) {
+  const c10::Device dev = qkv.device();
+  Cache c;
+  const float* sp = nullptr;
+  const int dt = dtype_code(qkv.scalar_type());
+  if (!on(qkv, dev) || !is_half(dt) || qkv.dim() != 2 || qkv.stride(1) != 1 ||
+      !cache_of(kv_cache, dev, c) || num_qo_heads < 1 || num_qo_heads > 4096 || c.heads > 4096 ||
+      head_dim < 1 || head_dim > 256 || padded_dim > 256 ||
+      qkv.size(1) != (num_qo_heads + 2 * c.heads) * head_dim || !signs_of(signs, padded_dim, dev, sp) ||
+      !sp || !is_f32(cos, dev) || !is_f32(sin, dev) || cos.dim() != 2 ||
+      sin.sizes() != cos.sizes() || cos.size(1) > 128 || !is_i32(slots, dev))
+    return false;
+  const int64_t n = qkv.size(0);
+  const auto rows = [&](const Tensor& t, int64_t heads) {
+    return on(t, dev) && t.scalar_type() == qkv.scalar_type() && t.dim() == 3 && t.size(0) == n &&
+           t.size(1) == heads && t.size(2) == head_dim && t.is_contiguous();
+  };
+  const auto weight = [&](const Tensor& t) {
+    return on(t, dev) && t.scalar_type() == qkv.scalar_type() && t.dim() == 1 &&
+           t.size(0) == head_dim && t.is_contiguous();
+  };
+  const int64_t axes = positions.dim() == 2 ? positions.size(0) : 1;
+  const auto pt = positions.scalar_type();
+  if (n == 0 || !on(positions, dev) || (pt != at::kInt && pt != at::kLong) ||
+      (positions.dim() != 1 && positions.dim() != 2) || positions.size(-1) != n ||
+      !positions.is_contiguous() || axes < 1 || axes > 4 || slots.dim() != 1 ||
+      slots.size(0) != n || !rows(q, num_qo_heads) || (k.has_value() && !rows(*k, c.heads)) ||
+      q_weight.has_value() != k_weight.has_value() ||
+      (q_weight.has_value() && (!weight(*q_weight) || !weight(*k_weight))))
+    return false;
+  int32_t share[4] = {(int32_t)cos.size(1), 0, 0, 0};
+  if (sections.has_value()) {
+    if ((int64_t)sections->size() != axes) return false;
+    for (int64_t a = 0; a < axes; a++) {
+      if ((*sections)[a] < 0 || (*sections)[a] > 128) return false;
+      share[a] = (int32_t)(*sections)[a];
+    }
+  } else if (axes != 1) {
+    return false;
+  }
+  const c10::DeviceGuard guard(dev);
+  const auto ptr = [](const OptTensor& t) -> const void* {
+    return t.has_value() ? t->const_data_ptr() : nullptr;
+  };
+  return tq_norm_rope_write(
+             qkv.const_data_ptr(), qkv.stride(0), dt, ptr(q_weight), ptr(k_weight), (float)eps,
+             cptr<float>(cos), cptr<float>(sin), cos.size(0), 2 * cos.size(1),
+             positions.const_data_ptr(), pt == at::kLong ? 8 : 4, n, share, axes,
+             const_cast<uint8_t*>(c.k), const_cast<uint8_t*>(c.v), sp, cptr<int32_t>(slots), n,
+             num_qo_heads, c.heads, head_dim, padded_dim, c.block_size, c.ebs, c.num_blocks,
+             q.data_ptr(), k.has_value() ? k->data_ptr() : nullptr, stream_of(dev)) == 0;
+}
+
 // -------------------------------------------------------------------- prefill
 
 using Request = std::array<int32_t, 5>;
@@ -745,6 +804,7 @@ PYBIND11_MODULE(_tq_torch, m) {
   m.def("track_window", &track_window, unlocked);
   m.def("evict", &evict, unlocked);
   m.def("decode_window", &decode_window, unlocked);
+  m.def("norm_rope_write", &norm_rope_write, unlocked);
   m.def("prefill_batch", &prefill_batch, unlocked);
   m.def("prefill_window", &prefill_window, unlocked);
   m.def("prefill_gather", &prefill_gather, unlocked);

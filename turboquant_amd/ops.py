@@ -1211,6 +1211,91 @@ def prefill_gather_window(kv_cache: torch.Tensor | None, block_table: torch.Tens
             out_v, sink)
 
 
+def norm_rope_write(qkv: torch.Tensor, q_weight: torch.Tensor | None,
+                    k_weight: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor,
+                    positions: torch.Tensor, kv_cache: torch.Tensor, signs: torch.Tensor,
+                    slot_mapping: torch.Tensor, num_qo_heads: int, head_dim: int, padded_dim: int,
+                    q: torch.Tensor, k: torch.Tensor | None = None, eps: float = 1e-6,
+                    sections=None) -> None:
+    """A layer's fused projection to what its attention takes: the q, k and v
+    heads of qkv [tokens, (Hq + 2 H) * head_dim] (fp16 or bf16), q and k RMS-normed
+    per head with their weights [head_dim] (both None: not normed) and rotated,
+    into q [tokens, Hq, head_dim] and (if given) k [tokens, H, head_dim], and K and
+    V quantised into the slots of kv_cache that slot_mapping int32 [tokens] names
+    (negative: none; the others must differ), the bytes that
+    quantize_write_kv_cache writes for those rows.  cos and sin fp32 [rows,
+    rotated / 2] turn dims (i, i + rotated / 2) by the row of the token's position:
+    positions int32 or int64 [tokens], or [axes, tokens] with `sections`, the
+    number of pairs that follow each axis, in order.  A position outside the
+    tables gives NaN rows.  rotated must be a multiple of 16, head_dim of 8.
+    tq_norm_rope_write."""
+    if (_nat or _native()).norm_rope_write(qkv, q_weight, k_weight, cos, sin, positions, kv_cache,
+                                           signs, slot_mapping, num_qo_heads, head_dim, padded_dim,
+                                           q, k, eps, sections):
+        return
+    what = "norm_rope_write"
+    tensors = [t for t in (q_weight, k_weight, k) if t is not None]
+    _require_gpu(qkv, cos, sin, positions, kv_cache, signs, slot_mapping, q, *tensors)
+    half = (torch.float16, torch.bfloat16)
+    if kv_cache.dim() != 5:
+        raise RuntimeError(f"{what}: kv_cache must be contiguous [2, num_blocks, block_size, H, "
+                           "ebs]")
+    h = kv_cache.size(3)
+    nb, bs, ebs = _cache_geometry(kv_cache, h, what)
+    _fit_int32(what, num_qo_heads=num_qo_heads, head_dim=head_dim, padded_dim=padded_dim)
+    if num_qo_heads < 1 or head_dim < 1:
+        raise RuntimeError(f"{what}: {num_qo_heads} q heads of {head_dim} elements")
+    if qkv.dtype not in half or qkv.dim() != 2 or qkv.stride(1) != 1 \
+            or qkv.size(1) != (num_qo_heads + 2 * h) * head_dim:
+        raise RuntimeError(f"{what}: qkv must be fp16 or bf16 [tokens, (Hq + 2 H) * head_dim] with "
+                           "contiguous rows")
+    n = qkv.size(0)
+    if (q_weight is None) != (k_weight is None):
+        raise RuntimeError(f"{what}: both weights must be given, or none")
+    for t, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if t is not None and (t.dtype != qkv.dtype or tuple(t.shape) != (head_dim,)):
+            raise RuntimeError(f"{what}: {name} must be [head_dim] of the rows' type")
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 \
+            or sin.shape != cos.shape:
+        raise RuntimeError(f"{what}: cos and sin must be fp32 [rows, rotated / 2]")
+    if positions.dtype not in (torch.int32, torch.int64) or positions.dim() not in (1, 2) \
+            or positions.size(-1) != n:
+        raise RuntimeError(f"{what}: positions must be int32 or int64 [tokens] or [axes, tokens]")
+    axes = positions.size(0) if positions.dim() == 2 else 1
+    sections = [cos.size(1)] if sections is None and axes == 1 else list(sections or ())
+    if not 1 <= axes <= 4 or len(sections) != axes or sum(sections) != cos.size(1) \
+            or min(sections) < 0:
+        raise RuntimeError(f"{what}: sections {sections} must give each of the {axes} axes (at "
+                           f"most 4) its share of the {cos.size(1)} pairs")
+    if slot_mapping.dtype != torch.int32 or tuple(slot_mapping.shape) != (n,):
+        raise RuntimeError(f"{what}: slot_mapping must be int32 [tokens]")
+    for t, name, heads in ((q, "q", num_qo_heads), (k, "k", h)):
+        if t is not None and (t.dtype != qkv.dtype or tuple(t.shape) != (n, heads, head_dim)
+                              or not t.is_contiguous()):
+            raise RuntimeError(f"{what}: {name} must be contiguous [tokens, heads, head_dim] of the "
+                               "rows' type")
+    if signs.dtype != torch.float32 or signs.numel() < padded_dim:
+        raise RuntimeError(f"{what}: signs must be fp32 [padded_dim]")
+    if n == 0:
+        return
+    if qkv.data_ptr() % 16 or qkv.stride(0) % 8 or qkv.stride(0) < qkv.size(1):
+        qkv = _aligned16(qkv)
+    qw, kw = (None if t is None else _aligned16(t) for t in (q_weight, k_weight))
+    cos, sin, signs, slots = (_aligned16(t) for t in (cos, sin, signs, slot_mapping))
+    positions = positions.contiguous()
+    lib = _lib.load()
+    base = kv_cache.data_ptr()
+    with torch.cuda.device(qkv.device):
+        rc = lib.tq_norm_rope_write(
+            qkv.data_ptr(), qkv.stride(0), _DTYPES[qkv.dtype], _opt_ptr(qw), _opt_ptr(kw),
+            float(eps), cos.data_ptr(), sin.data_ptr(), cos.size(0), 2 * cos.size(1),
+            positions.data_ptr(), positions.element_size(), n, (ctypes.c_int32 * axes)(*sections),
+            axes, base, base + kv_cache.stride(0) * kv_cache.element_size(), signs.data_ptr(),
+            slots.data_ptr(), n, int(num_qo_heads), h, int(head_dim), int(padded_dim), bs, ebs, nb,
+            q.data_ptr(), _opt_ptr(k), _stream_ptr(qkv.device))
+    _lib.check(rc, what)
+
+
 # --------------------------------------------------------------------------
 # torch.library registration under the reference's namespaces and schemas
 # --------------------------------------------------------------------------
@@ -1376,6 +1461,8 @@ def _register_fakes() -> None:
     def _budget_fake(*args):  # they write their arguments and return nothing
         return None
 
+    register_fake("turboquant_write::norm_rope_write", _budget_fake, lib=_libs[0])
+
     for name in ("decode_paged_tracked", "track_window", "evict_paged", "decode_paged_window"):
         register_fake(f"turboquant_v5::{name}", _budget_fake, lib=_libs[1])
 
@@ -1455,6 +1542,11 @@ def register_ops() -> None:
     d.define(f"decode_paged_window(Tensor q, Tensor kv_cache, {table}, {geometry}, Tensor(a!) o, "
              "int window, int sink=0) -> ()")
     d.impl("decode_paged_window", nothing(decode_paged_window), "CUDA")
+    w.define("norm_rope_write(Tensor qkv, Tensor? q_weight, Tensor? k_weight, Tensor cos, "
+             "Tensor sin, Tensor positions, Tensor(a!) kv_cache, Tensor signs, "
+             "Tensor slot_mapping, int num_qo_heads, int head_dim, int padded_dim, Tensor(b!) q, "
+             "Tensor(c!)? k=None, float eps=1e-6, int[]? sections=None) -> ()")
+    w.impl("norm_rope_write", nothing(norm_rope_write), "CUDA")
     _native()  # binds the write and the two balanced ops
     _libs.extend([w, d])
     _register_fakes()
