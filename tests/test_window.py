@@ -409,3 +409,39 @@ def test_reference_norm_and_rotation():
     turn = torch.stack((angle[pos[0, :3], 0], angle[pos[0, :3], 1], angle[pos[1, :3], 2]), 1)
     assert torch.allclose(z1, z0 * torch.polar(torch.ones(3, 3), turn).to(z0.dtype), atol=1e-6)
     assert torch.equal(q[:3, 0, 6:], before[:3, 0, 6:])
+
+
+# ---------------------------------------------------- backend and end-to-end loop
+
+def test_backend_windows():
+    from turboquant_amd.vllm_backend_fused import TurboQuantFusedImpl
+    make = lambda w: TurboQuantFusedImpl(4, 64, 0.125, 2, None, w, "fp8")
+    assert make(None).window == 0 and make(128).window == 128 and make(128).sink == 0
+    for bad in (0, -1):
+        with pytest.raises(ValueError, match="sliding_window"):
+            make(bad)
+
+
+def test_a_record_does_not_go_with_a_window():
+    from turboquant_amd import e2e
+    from turboquant_amd.budget import CacheRecord
+    from turboquant_amd.vllm_backend_fused import TurboQuantFusedImpl
+    impl = TurboQuantFusedImpl(4, 64, 0.125, 2, None, 8, "fp8")
+    cache = torch.zeros((2, 5, 16, 2, 48), dtype=torch.uint8)
+    impl.record = CacheRecord.beside(cache, 8)
+    meta = e2e.Meta(1, 1, torch.zeros((1, 2), dtype=torch.int32),
+                    torch.ones(1, dtype=torch.int32), torch.tensor([0, 1]), None)
+    with pytest.raises(RuntimeError, match="sliding window"):
+        impl.forward(None, torch.zeros((1, 256)), None, None, cache, meta)
+    with pytest.raises(RuntimeError, match="packed"):
+        TurboQuantFusedImpl(4, 64, 0.125, 2, None, 8, "auto").project_and_update(
+            None, None, None, None, None, None, None, None)
+
+
+def test_e2e_refuses_a_window_beside_a_budget():
+    from turboquant_amd import e2e
+    for kw in (dict(budget=64), dict(keep_fp16_kv=True)):
+        with pytest.raises(ValueError, match="attention window"):
+            e2e.Runner(e2e.ModelShape.tiny(1), 1, 32, torch.device("cpu"), attention_window=8, **kw)
+    with pytest.raises(ValueError, match="attention window"):
+        e2e.run(e2e.ModelShape.tiny(1), 1, 16, 4, compare_steps=2, device="cpu", attention_window=8)

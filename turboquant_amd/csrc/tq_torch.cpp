@@ -786,13 +786,40 @@ void balanced_op(const Tensor& q, const Tensor& kv_cache, const Tensor& indices,
               partition_o_ws, partition_lse_ws, split_indptr);
 }
 
+void window_op(const Tensor& q, const Tensor& kv_cache, const Tensor& indices,
+               const Tensor& indptr, const Tensor& seq_lens, int64_t num_kv_heads,
+               int64_t head_dim, int64_t padded_dim, double sm_scale, const OptTensor& signs,
+               const Tensor& o, int64_t window, int64_t sink) {
+  if (!decode_window(q, kv_cache, indices, indptr, seq_lens, num_kv_heads, head_dim, padded_dim,
+                     sm_scale, signs, o, window, sink))
+    in_python("decode_paged_window", q, kv_cache, indices, indptr, seq_lens, num_kv_heads,
+              head_dim, padded_dim, sm_scale, signs, o, window, sink);
+}
+
+void norm_write_op(const Tensor& qkv, const OptTensor& q_weight, const OptTensor& k_weight,
+                   const Tensor& cos, const Tensor& sin, const Tensor& positions,
+                   const Tensor& kv_cache, const Tensor& signs, const Tensor& slot_mapping,
+                   int64_t num_qo_heads, int64_t head_dim, int64_t padded_dim, const Tensor& q,
+                   const OptTensor& k, double eps, at::OptionalIntArrayRef sections) {
+  std::optional<std::vector<int64_t>> share;
+  if (sections.has_value()) share = sections->vec();
+  if (!norm_rope_write(qkv, q_weight, k_weight, cos, sin, positions, kv_cache, signs, slot_mapping,
+                       num_qo_heads, head_dim, padded_dim, q, k, eps, share))
+    in_python("norm_rope_write", qkv, q_weight, k_weight, cos, sin, positions, kv_cache, signs,
+              slot_mapping, num_qo_heads, head_dim, padded_dim, q, k, eps, share);
+}
+
 }  // namespace
 
-TORCH_LIBRARY_IMPL(turboquant_write, CUDA, m) { m.impl("quantize_write_kv_cache", write_op); }
+TORCH_LIBRARY_IMPL(turboquant_write, CUDA, m) {
+  m.impl("quantize_write_kv_cache", write_op);
+  m.impl("norm_rope_write", norm_write_op);
+}
 
 TORCH_LIBRARY_IMPL(turboquant_v5, CUDA, m) {
   m.impl("decode_paged_balanced_ws", balanced_op<false>);
   m.impl("decode_paged_balanced_rows_ws", balanced_op<true>);
+  m.impl("decode_paged_window", window_op);
 }
 
 PYBIND11_MODULE(_tq_torch, m) {

@@ -27,6 +27,11 @@ the prompt's last queries and the decode steps record what each cached entry
 receives, prompts are cut to the budget right after their prefill, and decoded
 sequences whenever ``cut_every`` tokens have come on top (budget.CacheRecord).
 
+Optionally (``attention_window``) the layers attend over a sliding window with
+``attention_sink`` first tokens, all but every ``full_every``-th of them, as
+models that mix the two kinds of layer do; q and k are then normed and rotated
+and K and V written in one launch (``project_and_update``).
+
 Optionally (``keep_fp16_kv``) the runner also keeps an fp16 copy of every
 layer's K/V and can decode the same model with plain fp16-KV SDPA attention,
 so the greedy tokens of the two runs can be compared.
@@ -175,6 +180,14 @@ def rope_tables(n: int, d: int, theta: float, device) -> tuple[torch.Tensor, tor
     return cos, sin
 
 
+def rope_angles(n: int, d: int, theta: float, device) -> tuple[torch.Tensor, torch.Tensor]:
+    """fp32 cos and sin [n, d / 2] of each pair's angle at each position (angles
+    in 64 bits: at far positions fp32 would lose what the tables hold)."""
+    inv = theta ** (-torch.arange(0, d, 2, device=device, dtype=torch.float64) / d)
+    ang = torch.arange(n, device=device, dtype=torch.float64)[:, None] * inv[None, :]
+    return ang.cos().float(), ang.sin().float()
+
+
 def rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
     """Rotate-half RoPE of x [T, H, D] with the table rows of its positions."""
     return torch.addcmul(x * cos[:, None, :], torch.roll(x, x.shape[-1] // 2, dims=-1),
@@ -205,11 +218,17 @@ class Runner:
     sink: int = 4
     window: int = 32
     cut_every: int = 64
+    attention_window: int = 0     # tokens a query sees, 0: all
+    attention_sink: int = 0       # first tokens that stay visible
+    full_every: int = 0           # every so many-th layer sees all, 0: none
     weights: dict = field(default=None, repr=False)
 
     def __post_init__(self):
         s = self.shape
         dev = self.device
+        if self.attention_window and (self.budget or self.keep_fp16_kv):
+            raise ValueError("an attention window goes neither with a budget nor with the fp16 "
+                             "K/V of the runs to compare with")
         if self.weights is None:
             self.weights = build_weights(s, self.seed, dev)
         self.pages_per_seq = math.ceil(self.max_tokens / BLOCK)
@@ -223,10 +242,18 @@ class Runner:
                                                       "fp8")
         self.caches = [torch.zeros(shape5, dtype=torch.uint8, device=dev)
                        for _ in range(s.layers)]
+        def sees_all(i):
+            return not self.attention_window or \
+                (self.full_every > 0 and (i + 1) % self.full_every == 0)
         self.impls = [TurboQuantFusedImpl(s.heads, s.head_dim, 1.0 / math.sqrt(s.head_dim),
-                                          s.kv_heads, None, None, "fp8")
-                      for _ in range(s.layers)]
+                                          s.kv_heads, None,
+                                          None if sees_all(i) else self.attention_window, "fp8")
+                      for i in range(s.layers)]
+        for impl in self.impls:
+            impl.sink = self.attention_sink
         self.cos, self.sin = rope_tables(self.max_tokens, s.head_dim, s.rope_theta, dev)
+        if self.attention_window:  # what project_and_update takes: fp32, one column a pair
+            self.cos, self.sin = rope_angles(self.max_tokens, s.head_dim, s.rope_theta, dev)
         self.kv16 = None
         if self.keep_fp16_kv:
             self.kv16 = [torch.zeros((2, self.batch, s.kv_heads, self.max_tokens, s.head_dim),
@@ -253,25 +280,34 @@ class Runner:
         self.probe = None
 
     # ------------------------------------------------------------ layers
-    def _qkv(self, lw, h, pos):
-        """q, k (normed, rotated), v of the normed tokens h at positions pos."""
+    def _qkv(self, li, lw, h, pos, slots):
+        """q, k (normed, rotated), v of the normed tokens h at positions pos; under a
+        window K and V are written to `slots` of the layer's cache as well."""
         s = self.shape
         t = h.shape[0]
         qkv = F.linear(h, lw["qkv"])
+        if self.attention_window:
+            return self.impls[li].project_and_update(qkv, lw["q_norm"], lw["k_norm"], self.cos,
+                                                     self.sin, pos, self.caches[li], slots, s.eps)
         q, k = qk_norm_rope(qkv, s, lw["q_norm"], lw["k_norm"], self.cos, self.sin, pos)
         v = qkv[:, (s.heads + s.kv_heads) * s.head_dim:].view(t, s.kv_heads, s.head_dim)
         return q, k, v
 
-    def _layers(self, x, pos, attend):
+    def _update(self, li, k, v, slots):
+        if not self.attention_window:  # (else _qkv has written them)
+            self.impls[li].do_kv_cache_update(None, k, v, self.caches[li], slots)
+
+    def _layers(self, x, pos, attend, slots=None):
         """Every layer over the residual stream x [T, hidden] (fp16,
         contiguous, updated in place): x += o_proj(attend(li, lw, q, k, v));
-        x += MLP(x).  attend returns the attention output [T, Hq * D]."""
+        x += MLP(x).  attend returns the attention output [T, Hq * D].  slots:
+        where the new tokens' K and V go (under a window)."""
         s = self.shape
         layers = self.weights["layers"]
         h = torch.empty_like(x)
         add_rms_norm(x, None, layers[0]["ln1"], h, s.eps)
         for li, lw in enumerate(layers):
-            q, k, v = self._qkv(lw, h, pos)
+            q, k, v = self._qkv(li, lw, h, pos, slots)
             o = attend(li, lw, q, k, v)
             add_rms_norm(x, F.linear(o, lw["o"]), lw["ln2"], h, s.eps)
             y = F.linear(silu_mul(F.linear(h, lw["gate_up"])), lw["down"])
@@ -303,13 +339,13 @@ class Runner:
 
         def attend(li, lw, q, k, v):
             impl = self.impls[li]
-            impl.do_kv_cache_update(None, k, v, self.caches[li], slots)
+            self._update(li, k, v, slots)
             if self.kv16 is not None:
                 self.kv16[li][0, b, :, :L] = k.transpose(0, 1)
                 self.kv16[li][1, b, :, :L] = v.transpose(0, 1)
             return impl.forward(None, q.reshape(L, -1), k.reshape(L, -1), v.reshape(L, -1),
                                 self.caches[li], meta)
-        x = self._layers(x, pos, attend)
+        x = self._layers(x, pos, attend, slots)
         first = greedy(self._logits(x[-1:]))
         if self.budget:
             self.lens[b], self.seen[b] = L, L
@@ -348,13 +384,13 @@ class Runner:
 
         def attend(li, lw, q, k, v):
             impl = self.impls[li]
-            impl.do_kv_cache_update(None, k, v, self.caches[li], self.slots)
+            self._update(li, k, v, self.slots)
             o = impl.forward(None, q.reshape(self.batch, -1), k.reshape(self.batch, -1),
                              v.reshape(self.batch, -1), self.caches[li], meta)
             if self.probe is not None:
                 self.probe.append((li, q.clone(), k.clone(), v.clone(), o.clone()))
             return o
-        x = self._layers(x, pos, attend)
+        x = self._layers(x, pos, attend, self.slots)
         nxt = greedy(self._logits(x))
         self.tok.copy_(nxt)
         self.out_buf.index_copy_(0, self.step_idx, nxt[None, :])
@@ -467,7 +503,7 @@ class Runner:
         forced [steps, B] (another run's tokens): teacher forcing, each step
         fed the forced history; returns (top-1 tokens, rank of the forced
         token among this run's logits), both [steps, B]."""
-        assert kv in ("fp16", "dequant")
+        assert kv in ("fp16", "dequant") and not self.attention_window
         assert kv == "dequant" or self.kv16 is not None
         s = self.shape
         out = torch.zeros((steps, self.batch), dtype=torch.int64, device=self.device)
@@ -565,9 +601,11 @@ def run(shape: ModelShape, batch: int = 8, prompt_len: int = 32768, new_tokens: 
       decoded over fp16 K/V for that many steps from the same prefill.
     Graph capture (a one-time setup, as a server does at start-up) is timed
     separately and not counted.  rule: budget, recent, sink, window, cut_every of
-    the Runner (cuts are part of the prefill and decode times)."""
-    if rule.get("budget") and compare_steps:
-        raise ValueError("the runs to compare with keep every token: no budget")
+    the Runner (cuts are part of the prefill and decode times), or
+    attention_window, attention_sink, full_every."""
+    if (rule.get("budget") or rule.get("attention_window")) and compare_steps:
+        raise ValueError("the runs to compare with keep and see every token: no budget and no "
+                         "attention window")
     dev = torch.device(device)
     say = log or (lambda *a: None)
     r = Runner(shape, batch, prompt_len + new_tokens, dev, seed,
@@ -577,7 +615,9 @@ def run(shape: ModelShape, batch: int = 8, prompt_len: int = 32768, new_tokens: 
     prompts = torch.randint(0, shape.vocab, (batch, prompt_len), generator=g)
     # one short throwaway prefill so that library initialisation (GEMM
     # heuristics, kernel loading) is not charged to the first request
-    warm = Runner(shape, 1, 64, dev, seed, weights=r.weights)
+    seen = {k: v for k, v in rule.items() if k in ("attention_window", "attention_sink",
+                                                   "full_every")}
+    warm = Runner(shape, 1, 64, dev, seed, weights=r.weights, **seen)
     warm.prefill(0, prompts[0, :48].to(dev))
     del warm
     torch.cuda.synchronize()
@@ -645,6 +685,9 @@ def run(shape: ModelShape, batch: int = 8, prompt_len: int = 32768, new_tokens: 
     if r.budget:
         res.update({"budget": r.budget, "recent": r.recent, "sink": r.sink,
                     "cut_every": r.cut_every, "cached_tokens": r.lens.tolist()})
+    if r.attention_window:
+        res.update({"attention_window": r.attention_window, "attention_sink": r.attention_sink,
+                    "full_every": r.full_every})
     r.tokens = toks
     return res
 
@@ -665,9 +708,18 @@ def main(argv=None):
     ap.add_argument("--sink", type=int, default=4, help="first tokens that are always kept")
     ap.add_argument("--window", type=int, default=32, help="observed queries of a prompt")
     ap.add_argument("--cut-every", type=int, default=64, help="decode steps between cuts")
+    ap.add_argument("--attention-window", type=int, default=0,
+                    help="tokens that a query of a windowed layer sees (0: all)")
+    ap.add_argument("--attention-sink", type=int, default=0,
+                    help="first tokens that stay visible under the window")
+    ap.add_argument("--full-every", type=int, default=0,
+                    help="every so many-th layer sees all tokens (0: none)")
     a = ap.parse_args(argv)
     rule = dict(budget=a.budget, recent=a.recent, sink=a.sink, window=a.window,
                 cut_every=a.cut_every) if a.budget else {}
+    if a.attention_window:
+        rule.update(attention_window=a.attention_window, attention_sink=a.attention_sink,
+                    full_every=a.full_every)
     shape = ModelShape.tiny(a.layers) if a.tiny else ModelShape(layers=a.layers)
     res = run(shape, a.batch, a.prompt, a.new, a.seed, a.compare,
               log=lambda m: print(m, flush=True), **rule)

@@ -1470,7 +1470,8 @@ def _register_fakes() -> None:
 def register_ops() -> None:
     """Define turboquant_write::* and turboquant_v5::* with the reference
     schemas and bind the HIP implementations to the CUDA dispatch key (the
-    write and the balanced decodes in C++, tq_torch.cpp; the others here)."""
+    writes, the balanced decodes and the windowed one in C++, tq_torch.cpp; the
+    others here)."""
     global _registered
     if _registered:
         return
@@ -1541,13 +1542,11 @@ def register_ops() -> None:
     # the operators of windowed layers
     d.define(f"decode_paged_window(Tensor q, Tensor kv_cache, {table}, {geometry}, Tensor(a!) o, "
              "int window, int sink=0) -> ()")
-    d.impl("decode_paged_window", nothing(decode_paged_window), "CUDA")
     w.define("norm_rope_write(Tensor qkv, Tensor? q_weight, Tensor? k_weight, Tensor cos, "
              "Tensor sin, Tensor positions, Tensor(a!) kv_cache, Tensor signs, "
              "Tensor slot_mapping, int num_qo_heads, int head_dim, int padded_dim, Tensor(b!) q, "
              "Tensor(c!)? k=None, float eps=1e-6, int[]? sections=None) -> ()")
-    w.impl("norm_rope_write", nothing(norm_rope_write), "CUDA")
-    _native()  # binds the write and the two balanced ops
+    _native()  # binds these, the write and the two balanced ops
     _libs.extend([w, d])
     _register_fakes()
     _registered = True

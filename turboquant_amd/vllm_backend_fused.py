@@ -142,6 +142,11 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
     turboquant_v5::decode_paged_tracked and every other batch is observed after
     its attention (turboquant_v5::track_window); a batch that cannot be recorded
     (no cache, no lengths, a cache that is not packed) is refused.
+    With a sliding_window (tokens that a query sees, its own among them) decode
+    goes through turboquant_v5::decode_paged_window and chunks through
+    ops.prefill_gather_window and ops.prefill_attention_window; `sink` (set on
+    the impl, 0) first tokens stay visible.  Pages that no later query sees may
+    be given back.  A record beside a window is refused.
     Prefill / mixed batches: _prefill_mixed (decode rows through the decode
     kernel, chunks with cached context over the dequantized context plus the
     fresh chunk, fresh prompts as in the reference, vllm_backend_fused.py:335-371).
@@ -168,6 +173,12 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
         self._rows_op = None
         # a budget.CacheRecord beside this layer's cache: forward fills it
         self.record = None
+        # tokens a query sees (0: all), and first tokens that stay visible
+        self.window = 0 if sliding_window is None else int(sliding_window)
+        if sliding_window is not None and self.window < 1:
+            raise ValueError(f"sliding_window {sliding_window} must be positive")
+        self.sink = 0
+        self._norm_write_op = self._window_op = None
 
     # ---------------------------------------------------------------- setup
     @staticmethod
@@ -260,6 +271,8 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
             ops.register_ops()
             self._write_op = torch.ops.turboquant_write.quantize_write_kv_cache
             self._rows_op = torch.ops.turboquant_v5.decode_paged_balanced_rows_ws
+            self._window_op = torch.ops.turboquant_v5.decode_paged_window
+            self._norm_write_op = torch.ops.turboquant_write.norm_rope_write
             self._decode_op, self._decode_op_name = pick_decode_op()
 
     # ---------------------------------------------------------------- write
@@ -285,6 +298,27 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
             reshape_and_cache_flash(key[:num_tokens], value[:num_tokens], key_cache,
                                     value_cache, slot_mapping, self.kv_cache_dtype,
                                     layer._k_scale, layer._v_scale)
+
+    @torch.no_grad()
+    def project_and_update(self, qkv, q_weight, k_weight, cos, sin, positions, kv_cache,
+                           slot_mapping, eps=1e-6, sections=None):
+        """(q, k, v) [tokens, heads, head_size] of a layer's fused projection qkv
+        [tokens, (Hq + 2 H) * head_size]: q and k normed per head and rotated, with
+        K and V written to the packed cache in the same launch, in the place of a
+        norm, a rotation and do_kv_cache_update (turboquant_write::norm_rope_write;
+        cos and sin fp32 [rows, rotated / 2], positions [tokens] or [axes, tokens]
+        with their sections).  v is a view of qkv."""
+        if not self._is_fp8:
+            raise RuntimeError("project_and_update needs a packed (fp8) kv_cache")
+        self._ensure(qkv.device)
+        self._ensure_kernels_loaded()
+        n, d, h = qkv.shape[0], self.head_size, self.num_kv_heads
+        q = torch.empty((n, self.num_heads, d), dtype=qkv.dtype, device=qkv.device)
+        k = torch.empty((n, h, d), dtype=qkv.dtype, device=qkv.device)
+        sm = slot_mapping if slot_mapping.dtype == torch.int32 else slot_mapping.to(torch.int32)
+        self._norm_write_op(qkv, q_weight, k_weight, cos, sin, positions, kv_cache, self._signs, sm,
+                            self.num_heads, d, self._pd, q, k, eps, sections)
+        return q, k, qkv[:, (self.num_heads + h) * d:].view(n, h, d)
 
     # -------------------------------------------------------------- forward
     @staticmethod
@@ -312,7 +346,8 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
         context read fp16 K/V where it is, everything else (cached context,
         bf16 or fp32 rows, a head size below its padded size) comes from one
         launch of the gather (tq_prefill_gather).  The reference runs
-        flash-attn per request here (vllm_backend_fused.py:335-371)."""
+        flash-attn per request here (vllm_backend_fused.py:335-371).  Under a
+        window the same with the cached tokens that the chunk still sees."""
         from . import ops
         d, pd, hkv = self.head_size, self._pd, self.num_kv_heads
         if pd > 256:
@@ -344,6 +379,7 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
             and min(key.stride(0), value.stride(0)) >= pd
         kv = (key, value) if in_place else (None, None)
         most = GATHER_BYTES // (4 * hkv * pd)  # rows of K and V
+        window, sink = self.window, self.sink
         at = 0
         while at < len(chunks):
             # the requests of a pass: gathered K and V up to GATHER_BYTES, one
@@ -352,11 +388,15 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
             while at < len(chunks):
                 i, a, ql, ctx = chunks[at]
                 if ctx > 0 or not in_place:
-                    if gathers and rows + ctx + ql > most:
+                    # the first token of the window of the chunk's first query
+                    first = max(0, ctx - window + 1) if window else 0
+                    kept = ctx - first + min(sink, first)
+                    if gathers and rows + kept + ql > most:
                         break
-                    gathers.append((i, ctx, a, ql, rows))
-                    reqs.append((a, ql, rows, ctx + ql, 1))
-                    rows += ctx + ql
+                    gathers.append((i, ctx, first, a, ql, rows) if window
+                                   else (i, ctx, a, ql, rows))
+                    reqs.append((a, ql, rows, kept + ql, 1))
+                    rows += kept + ql
                 else:
                     reqs.append((a, ql, a, ql, 0))
                 at += 1
@@ -365,8 +405,16 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
                 gk = torch.empty((rows, hkv, pd), dtype=torch.float16, device=query.device)
                 gv = torch.empty_like(gk)
                 k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (key, value))
-                ops.prefill_gather(kv_cache, bt, k, v, gathers, d, pd, self._signs, gk, gv)
-            ops.prefill_attention_batch(q, o, reqs, hkv, qd, pd, self.scale, *kv, gk, gv)
+                if window:
+                    ops.prefill_gather_window(kv_cache, bt, k, v, gathers, sink, d, pd,
+                                              self._signs, gk, gv)
+                else:
+                    ops.prefill_gather(kv_cache, bt, k, v, gathers, d, pd, self._signs, gk, gv)
+            if window:
+                ops.prefill_attention_window(q, o, reqs, hkv, qd, pd, self.scale, window, sink,
+                                             *kv, gk, gv)
+            else:
+                ops.prefill_attention_batch(q, o, reqs, hkv, qd, pd, self.scale, *kv, gk, gv)
         if o is not output:
             for _, a, ql, _ in chunks:
                 output[a:a + ql].copy_(o[a:a + ql, :, :d])
@@ -390,6 +438,28 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
                 and q.stride(2) == 1 and q.stride(0) % 8 == 0 and q.stride(1) % 8 == 0
                 and q.stride(1) >= self.head_size and q.data_ptr() % 16 == 0
                 and o.is_contiguous() and o.data_ptr() % 8 == 0)
+
+    def _decode_window(self, q, kv_cache, table, seq_lens, out):
+        """Windowed decode of one new token per row, q and out [n, Hq, head_size]."""
+        n, pages = q.shape[0], table.shape[1]
+        key = ("window", n, pages)
+        ws = self._v5_ws_cache.get(key)
+        if ws is None:
+            ws = self._v5_ws_cache[key] = {
+                "indptr": torch.arange(n + 1, dtype=torch.int32, device=q.device) * pages}
+        half, d = (torch.float16, torch.bfloat16), self.head_size
+        o = out
+        if q.dtype not in half:
+            q = q.to(torch.float16)
+        if d % 8:  # rows that the op does not take
+            q, d = F.pad(q, (0, self._pd - d)), self._pd
+        if o.dtype not in half or not o.is_contiguous() or d != self.head_size:
+            o = torch.empty((n, self.num_heads, d), dtype=q.dtype, device=q.device)
+        self._window_op(q, kv_cache, table.to(torch.int32).reshape(-1), ws["indptr"],
+                        seq_lens.to(torch.int32).contiguous(), self.num_kv_heads, d, self._pd,
+                        self.scale, self._signs, o, self.window, self.sink)
+        if o is not out:
+            out.copy_(o[:, :, :self.head_size])
 
     def _decode_ws(self, n, pages, device):
         """Balanced-decode workspace for n decode rows of a mixed batch."""
@@ -494,6 +564,14 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
                 idx = torch.tensor(dec, dtype=torch.long, device=dev)
                 q = query.index_select(0, rows)
                 sub_bt, sl = bt.index_select(0, idx), attn_metadata.seq_lens.index_select(0, idx)
+            if self.window:
+                if run:
+                    self._decode_window(q, kv_cache, sub_bt, sl, output[rows])
+                else:
+                    o = torch.empty_like(q)
+                    self._decode_window(q, kv_cache, sub_bt, sl, o)
+                    output.index_copy_(0, rows, o.to(output.dtype))
+                return output
             sub_bt, sl = sub_bt.to(torch.int32).contiguous(), sl.to(torch.int32).contiguous()
             ws = self._decode_ws(n, sub_bt.shape[1], dev)
             args = (kv_cache, sub_bt.reshape(-1), ws["indptr"], sl, self.num_kv_heads,
@@ -525,6 +603,10 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
             # a later cut would go by weights and positions that miss these tokens
             raise RuntimeError("a cache record needs a packed (fp8) kv_cache and seq_lens with "
                                "every batch")
+
+        if self.record is not None and self.window:
+            # its weights would be those of attention over every token
+            raise RuntimeError("a cache record does not go with a sliding window")
 
         is_decode = attn_metadata.max_query_len == 1
         if not is_decode:
@@ -569,6 +651,9 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
             q3 = q.view(rows)
             out3 = (output if output.shape[0] == num_actual else output[:num_actual]).view(rows)
             batch_size = num_actual
+            if self.window:
+                self._decode_window(q3, kv_cache, block_table, seq_lens, out3)
+                return output
             if self.record is not None:
                 self._forward_recorded(q3, kv_cache, attn_metadata, out3, True)
                 return output
