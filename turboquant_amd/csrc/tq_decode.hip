@@ -630,6 +630,91 @@ __device__ __forceinline__ uint32_t ror8u(uint32_t v) {
 #endif
 constexpr bool kPvLo = TQ_PV_LO != 0;
 
+// The math of one step (two tiles, read into d): scores, softmax, PV.  whole():
+// whether every token of the step counts (uniform); counts(T, i): whether token i
+// of tile T does.
+template <int PD, int PACK, bool QC, int SH, bool PLO, class Whole, class Counts>
+__device__ __forceinline__ void attend_step(const StepData<PD>& d, const half8_t* qb,
+                                            const half8_t* ql, uint32_t lanec, const uint32_t* lut,
+                                            Whole whole, Counts counts, int n, int q4, int ptile,
+                                            uint64_t hmask, float lpv, SoftmaxState<PD>& st) {
+  // scores of both tiles (scheduling barriers keep the two tiles'
+  // dequant temporaries from being live at the same time)
+  float4_t acc[2];
+  constexpr bool PM = PACK == 2;  // packed merge of the two tiles' unmerged sums
+  static_assert(PACK == 1 || QC, "two tiles per score set need the hi / lo columns");
+  acc[0] = tile_scores<PD, QC, SH, !PM>(d.k[0], qb, ql, lanec, lut);
+  __builtin_amdgcn_sched_barrier(0);
+  acc[1] = tile_scores<PD, QC, SH, !PM>(d.k[1], qb, ql, lanec, lut);
+  __builtin_amdgcn_sched_barrier(0);
+  if constexpr (PM) acc[0] = pack_merge(acc[0], acc[1]);
+  constexpr int NV = 4 * (2 / PACK);  // score values per lane
+  float sc[NV];
+  uint32_t nvr[NV];
+  bool valid[NV];
+#pragma unroll
+  for (int g = 0; g < 2 / PACK; g++) {
+    const uint32_t nkv = d.nkv[g];
+    const uint32_t nr[4] = {quad_bcast<0>(nkv), quad_bcast<1>(nkv), quad_bcast<2>(nkv),
+                            quad_bcast<3>(nkv)};
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      // tile 0's scores in lanes 0..7 of each row and tile 1's in 8..15
+      // (PACK 2), times the K norm straight from its fp16 half
+      const float a = PACK == 2 ? acc[0][r] : acc[g][r];
+      sc[4 * g + r] = mul_lo_half(a, nr[r]);
+      nvr[4 * g + r] = nr[r];
+    }
+  }
+  // (uniform; read back as a scalar so that it stays one)
+  const bool full = __builtin_amdgcn_readfirstlane(whole() ? 1 : 0) != 0;
+  if (!full) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int T = PACK == 2 ? ptile : i / 4;
+      valid[i] = counts(T, 4 * q4 + (i & 3));
+    }
+  }
+  uint32_t pw[NV / 2], pl[NV / 2];
+  softmax_step<PD, NV, PLO>(sc, nvr, full, valid, PACK == 2, hmask, lpv, st, pw, pl);
+  half8_t p8;
+  if constexpr (PACK == 2 && PLO) {
+    // lanes n < 8: hi parts of tile 0 (own) and tile 1 (lane n + 8);
+    // lanes n >= 8: lo parts of tile 0 (lane n - 8) and tile 1 (own)
+    const bool up = n >= 8;
+    const uint32_t r0 = ror8u(up ? pw[0] : pl[0]), r1 = ror8u(up ? pw[1] : pl[1]);
+    p8 = up ? as_half8(r0, r1, pl[0], pl[1]) : as_half8(pw[0], pw[1], r0, r1);
+  } else if constexpr (PACK == 2) {
+    p8 = as_half8(pw[0], pw[1], shl8(pw[0]), shl8(pw[1]));
+  } else if constexpr (PLO) {
+    // lanes n >= 8 hold the same scores as lane n - 8: their lo parts
+    p8 = n >= 8 ? as_half8(pl[0], pl[1], pl[2], pl[3]) : as_half8(pw[0], pw[1], pw[2], pw[3]);
+  } else {
+    p8 = as_half8(pw[0], pw[1], pw[2], pw[3]);
+  }
+  step_pv<PD, SH>(d.v[0], d.v[1], p8, st, lanec, lut);
+}
+
+// The dequant table: byte e -> fp16 values of its high nibble (low half) and its
+// low nibble (high half), built with the same table arithmetic as dq8, in LC
+// copies, four at a time (as inline assembly: copies in flight into LDS do not
+// touch it, which the compiler cannot tell).
+template <int LC>
+__device__ __forceinline__ void build_table(uint32_t* klut, int threads) {
+  for (int i = threadIdx.x; i < 64 * LC; i += threads) {
+    const int e = i / (LC / 4);
+    uint32_t x[4];
+    dq8((uint32_t)e * 0x01010101u, x);
+    [[maybe_unused]] const uint32_t val = (x[2] & 0xffffu) | (x[0] << 16);
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("ds_write_b128 %0, %1" : : "v"(lds_addr(&klut[4 * i])), "v"(u32x4{val, val, val, val}) : "memory");
+#endif
+  }
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#endif
+}
+
 #ifndef TQ_DECODE_MATH
 #define TQ_DECODE_MATH 2
 #endif
@@ -677,25 +762,7 @@ void decode_partials_kernel(DecodeParams p) {
   };
   __shared__ Lds sm;
 
-  // dequant table: byte e -> fp16 values of its high nibble (low half) and
-  // its low nibble (high half), built with the same table arithmetic as dq8,
-  // in RG::LC copies (written four at a time, as inline assembly: the
-  // copies in flight into the ring do not touch it, which the compiler
-  // cannot tell)
-  auto init_table = [&]() {
-    for (int i = threadIdx.x; i < 64 * RG::LC; i += 64 * G) {
-      const int e = i / (RG::LC / 4);
-      uint32_t x[4];
-      dq8((uint32_t)e * 0x01010101u, x);
-      [[maybe_unused]] const uint32_t val = (x[2] & 0xffffu) | (x[0] << 16);
-#if defined(__HIP_DEVICE_COMPILE__)
-      asm volatile("ds_write_b128 %0, %1" : : "v"(lds_addr(&sm.klut[4 * i])), "v"(u32x4{val, val, val, val}) : "memory");
-#endif
-    }
-#if defined(__HIP_DEVICE_COMPILE__)
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#endif
-  };
+  auto init_table = [&]() { build_table<RG::LC>(sm.klut, 64 * G); };
 
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // wave-uniform

@@ -118,11 +118,19 @@ __device__ __forceinline__ void angles(const NormWriteParams& p, uint32_t t, int
 
 // M: chunk rows from a pair's first half to its second (the pair in one lane), 0:
 // any rotation of whole 16 dims
-template <int PD, int DT, int M>
-__global__ __launch_bounds__(256) void norm_write_kernel(NormWriteParams p) {
+template <int M>
+struct NormRows {
+  NormWriteParams p;
+  template <int PD, int DT>
+  __device__ __forceinline__ bool rows(u32x4* raw, bool& live, int& kv, uint32_t& t, int& h) const;
+};
+
+template <int M>
+template <int PD, int DT>
+__device__ __forceinline__ bool NormRows<M>::rows(u32x4* raw, bool& live, int& kv, uint32_t& t,
+                                                  int& head) const {
   using FG = FastGeom<PD>;
   constexpr int P = FG::P, CPL = FG::CPL;
-  __shared__ __attribute__((aligned(512))) uint32_t tbl[128];
   const int lane = threadIdx.x & 63;
   const int pl = lane % P;
   uint32_t blk = blockIdx.x;
@@ -130,13 +138,14 @@ __global__ __launch_bounds__(256) void norm_write_kernel(NormWriteParams p) {
   blk -= isq ? 2 * p.kblocks : isv ? p.kblocks : 0u;
   const uint32_t H = (uint32_t)(isq ? p.hq : p.hkv);
   uint32_t g = blk * (uint32_t)FG::VPB + (threadIdx.x >> 6) * FG::VPW + lane / P;
-  const bool live = g < p.tokens * H;
+  live = g < p.tokens * H;
   g = live ? g : 0u;  // lanes past the end work on the first vector and store nothing
-  const uint32_t t = H == 1 ? g : __umulhi(g, isq ? p.mq : p.mk);
+  t = H == 1 ? g : __umulhi(g, isq ? p.mq : p.mk);
   const uint32_t h = g - t * H;
   const uint16_t* const src =
       p.qkv + (int64_t)t * p.row + (int64_t)(isq ? h : p.hq + (isv ? p.hkv : 0) + h) * p.hd;
-  u32x4 raw[CPL];
+  kv = isv ? 1 : 0;
+  head = (int)h;
 #pragma unroll
   for (int i = 0; i < CPL; i++) {
     raw[i] = u32x4{0u, 0u, 0u, 0u};
@@ -233,17 +242,9 @@ __global__ __launch_bounds__(256) void norm_write_kernel(NormWriteParams p) {
       raw[i] = round8<DT>(y[i]);
       if (live && out) *reinterpret_cast<u32x4*>(out + ((int64_t)t * H + h) * p.hd + d) = raw[i];
     }
-    if (isq) return;
+    if (isq) return false;
   }
-  const int32_t slot = live ? p.slots[t] : -1;
-  uint32_t lo2, hi2, packed[CPL];
-  bin_table(tbl, p.scale, lo2, hi2);
-  const float l2 = quantize_vector<PD, DT>(
-      raw, p.signs, p.scale, p.hd, tbl, lo2, hi2,
-      [&](int i, int c) -> float { return elem<DT>(raw[i], c); }, packed);
-  if (slot >= 0 && (int64_t)slot < p.nslots)
-    store_entry<PD>((isv ? p.vs : p.ks) + ((int64_t)slot * p.hkv + h) * (int64_t)p.ebs, pl, packed,
-                    l2);
+  return true;
 }
 
 template <int PD, int DT>
@@ -251,12 +252,14 @@ hipError_t launch_norm_write(const NormWriteParams& p, dim3 grid, hipStream_t st
   constexpr int P = FastGeom<PD>::P, CPL = FastGeom<PD>::CPL;
   // chunk rows of half a rotation, where whole and (both halves) inside the lane
   const int m = p.half % (8 * P) == 0 ? p.half / (8 * P) : 0;
-  if (m == 1)
-    hipLaunchKernelGGL((norm_write_kernel<PD, DT, 1>), grid, dim3(256), 0, st, p);
-  else if (CPL == 4 && m == 2)
-    hipLaunchKernelGGL((norm_write_kernel<PD, DT, CPL / 2>), grid, dim3(256), 0, st, p);
-  else
-    hipLaunchKernelGGL((norm_write_kernel<PD, DT, 0>), grid, dim3(256), 0, st, p);
+#define TQ_NW(M)                                                                               \
+  hipLaunchKernelGGL((write_fast_kernel<PD, DT, NormRows<M>>), grid, dim3(256), 0, st, p.ks, p.vs, \
+                     nullptr, nullptr, 0, 0, 0, 0, p.signs, p.slots, 0u, p.hkv, 0u, p.hd, p.ebs,   \
+                     p.nslots, p.scale, NormRows<M>{p})
+  if (m == 1) TQ_NW(1);
+  else if (CPL == 4 && m == 2) TQ_NW(CPL / 2);
+  else TQ_NW(0);
+#undef TQ_NW
   return hipGetLastError();
 }
 

@@ -1,5 +1,5 @@
-// tq_quant.h -- a vector of a K or V row to its packed cache entry, 32 dims per
-// lane: what the kernels that write whole aligned rows share.
+// tq_quant.h -- the fast kernel of the write, for rows as they come (tq_write.hip)
+// and rows that are computed on the way (tq_norm_write.hip).
 #pragma once
 
 #include <type_traits>
@@ -45,6 +45,57 @@ __device__ __forceinline__ float xor_lane(float x) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// Fast path: 32 dims per lane, P = PD/32 lanes per vector, rows in whole
+// 16-byte aligned pieces (fp16, bf16 or fp32; head_dim a multiple of 8, the
+// chunks past it zero).
+//
+// Lane p of a vector holds the 16-byte chunks j = p + P*i (i = 0..3), i.e.
+// dims d = 8j + c (c = 0..7): bits 0-2 of d are in-lane, the next log2(P)
+// bits pick the lane, the top two bits are in-lane again.  The reference's
+// lane t holds dims [t*VEC, (t+1)*VEC) with VEC = PD/32, so this lane holds
+// the reference lanes t = 8i + E*p + e (E = 8/VEC, e < E).  Both orders the
+// reference fixes come out unchanged:
+//  * sum-of-squares tree (shfl_down 16, 8, 4, 2, 1): levels 16 and 8 pair i
+//    and i + 2, i and i + 1 (in-lane); levels 4, 2, 1 pair the low three
+//    bits of t, which are lane bits (xor across lanes) from E up and in-lane
+//    below, in the reference's level order;
+//  * FWHT stages h = 1, 2, 4 (in-lane), h = 8 .. 4P (lane xor h/8), h = 8P
+//    and 16P (in-lane), ascending.
+// Every butterfly and every tree node is the same fp32 operation on the same
+// two operands as in the reference (fp32 addition is commutative, negation
+// is exact), so the bits are the same; only the lane that computes it and
+// the sign it is held with differ.
+//
+// Instruction savings over the generic kernel:
+//  * the sign flip is an XOR of the sign bits before conversion:
+//    (x*s)*inv == (x*inv)*s for s = +-1 (but for the sign of a zero, and both
+//    zeros give code 8);
+//  * a cross-lane butterfly is one fma with a DPP operand: lane l keeps
+//    z_l + sg_l * z_partner (sg = -1 on the upper lane), which is the
+//    reference's value times tau_l = +-1.  Negation commutes with the later
+//    in-lane butterflies, so every lane ends with tau_l = (-1)^popcount(lane
+//    bits) times the reference's values and folds tau_l into the 1/sqrt(pd)
+//    scale, an fma with a +0 addend that also turns -0 into +0 (both give
+//    code 8, as the reference's `val >= 0` does);
+//  * bucketize is one LDS lookup: |v| (as ordered integer bits, minus one
+//    for negative v so that `>=` becomes the reference's `>` on that side)
+//    is clamped to the four binades that hold the seven positive
+//    boundaries, and its exponent's low three bits plus its top three
+//    mantissa bits index a 64-entry table of (boundary inside this
+//    1/8-binade bin or none, 8 + boundaries below the bin).  Each bin holds
+//    at most one boundary (the tests check this for every head size), so
+//    code = (8 + below + (|v| >= boundary)) for v >= 0 and its 4-bit
+//    complement for v < 0.
+//  * a vector with an inf or NaN input is NaN everywhere after the FWHT
+//    (every output adds every input; inf * inv is inf * 0), i.e. code 0, as in
+//    the reference: one coordinate stands for all.  (A sum of squares that
+//    overflows on finite bf16 or fp32 inputs gives inv = 0, all codes 8.)
+//
+// VALU-bound (about 20 instructions per coordinate): 8192 tokens x 8 heads x
+// 128, K and V, 13.4 us for fp16 (3.2 TB/s), 12.9 for bf16 and 16.6 for fp32
+// rows; in the general kernel, whose bf16 and fp32 loads were single elements,
+// 23.3, 24.2 and 22.2 us (with that kernel's vector loads 23.0, 21.1 and 21.6).
 template <int PD>
 struct FastGeom {
   // 16-byte chunks (8 dims) per lane: 4, and 2 at pd 64, where 4 would leave
@@ -131,18 +182,77 @@ __device__ __forceinline__ float add_qxor(float r) {
   return r;
 }
 
-// The bin table of the fast bucketize in LDS (64 x (2 * boundary, 8 + below)) and
-// the clamp of its index, for boundaries b_k * scale.
-__device__ __forceinline__ void bin_table(uint32_t* tbl, float scale, uint32_t& lo2,
-                                          uint32_t& hi2) {
+// the rows of key and value as they come
+struct PlainRows {};
+
+template <int PD, int DT, class Src = PlainRows>
+__global__ __launch_bounds__(256) void write_fast_kernel(
+    uint8_t* __restrict__ k_slab, uint8_t* __restrict__ v_slab,
+    const void* __restrict__ key, const void* __restrict__ value,
+    int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
+    const float* __restrict__ signs, const int32_t* __restrict__ slots,
+    uint32_t per_kv, int H, uint32_t hmul, int head_dim, int ebs, int64_t nslots, float scale,
+    Src src) {
+#pragma clang fp contract(off)
+  using FG = FastGeom<PD>;
+  constexpr int P = FG::P, E = FG::E, VEC = FG::VEC, CPL = FG::CPL, PE = FG::PE;
+  constexpr int ND = 8 * CPL;  // dims per lane
+  constexpr int W = DT == TQ_F32 ? 2 : 1;       // 16-byte pieces per chunk
+  constexpr int ESZ = DT == TQ_F32 ? 4 : 2;
+  __shared__ __attribute__((aligned(512))) uint32_t tbl[128];  // 64 x (2 * boundary, 8 + below)
+
+  const int lane = threadIdx.x & 63;
+  const int p = lane % P;
+  u32x4 raw[CPL * W];
+  bool live = true;
+  int kv = 0, h = 0;
+  uint32_t t = 0;
+  [[maybe_unused]] const uint8_t* row = nullptr;
+  if constexpr (std::is_same_v<Src, PlainRows>) {
+    const uint32_t g = blockIdx.x * (uint32_t)FG::VPB + (threadIdx.x >> 6) * FG::VPW + lane / P;
+    live = g < 2 * per_kv;
+
+    // this vector's row: CPL chunks j = p + P*i, issued first
+    kv = g >= per_kv ? 1 : 0;
+    const uint32_t rem = g - (kv ? per_kv : 0u);
+    t = H == 1 ? rem : __umulhi(rem, hmul);  // rem / H, exact (hmul = ceil(2^32/H))
+    h = (int)(rem - t * (uint32_t)H);
+    // lanes past the end read row 0 of K (no branch, no zero fill); they
+    // store nothing (slot -1)
+    row =
+        !live ? static_cast<const uint8_t*>(key)
+        : kv  ? static_cast<const uint8_t*>(value) + ((int64_t)t * v_st + (int64_t)h * v_sh) * ESZ
+              : static_cast<const uint8_t*>(key) + ((int64_t)t * k_st + (int64_t)h * k_sh) * ESZ;
+    if (head_dim == PD) {  // uniform
+#pragma unroll
+      for (int i = 0; i < CPL; i++)
+#pragma unroll
+        for (int k = 0; k < W; k++)
+          raw[W * i + k] = *reinterpret_cast<const u32x4*>(row + 8 * ESZ * (p + P * i) + 16 * k);
+    } else {  // chunks past head_dim are zero (head_dim % 8 == 0)
+#pragma unroll
+      for (int i = 0; i < CPL; i++)
+#pragma unroll
+        for (int k = 0; k < W; k++) {
+          raw[W * i + k] = u32x4{0u, 0u, 0u, 0u};
+          if (8 * (p + P * i) < head_dim)
+            raw[W * i + k] = *reinterpret_cast<const u32x4*>(row + 8 * ESZ * (p + P * i) + 16 * k);
+        }
+    }
+  } else {
+    // rows that the source computes (false: the workgroup has nothing to write)
+    if (!src.template rows<PD, DT>(raw, live, kv, t, h)) return;
+  }
+  const int32_t slot = live ? slots[t] : -1;
+
   // boundaries b_k * scale (k = 1..7) as integer bits (positive floats order
   // as their bits); bin table over the four binades from the smallest one
   int32_t T[7];
 #pragma unroll
   for (int k = 0; k < 7; k++) T[k] = (int32_t)__float_as_uint(boundary_pos(k + 1) * scale);
   const int32_t e0 = T[0] >> 23;
-  lo2 = (uint32_t)e0 << 24;                // 2 * 2^e0 as bits
-  hi2 = ((uint32_t)(e0 + 4) << 24) - 1u;   // just below 2 * 2^(e0 + 4)
+  const uint32_t lo2 = (uint32_t)e0 << 24;                // 2 * 2^e0 as bits
+  const uint32_t hi2 = ((uint32_t)(e0 + 4) << 24) - 1u;   // just below 2 * 2^(e0 + 4)
   if (threadIdx.x < 64) {
     const int idx = threadIdx.x;
     const int e = e0 + (((idx >> 3) - e0) & 7);  // the exponent with these low bits
@@ -158,24 +268,7 @@ __device__ __forceinline__ void bin_table(uint32_t* tbl, float scale, uint32_t& 
     tbl[2 * idx] = thr2;
     tbl[2 * idx + 1] = below;
   }
-}
 
-// The codes of a vector from its CPL chunks of 8 elements (raw: 16-byte pieces,
-// element type DT, zero past head_dim), packed 8 to a dword per chunk; returns
-// the 2-norm.  as_it_came(i, c): element c of chunk row i as fp32, asked for
-// where the sum of squares is NaN.  Every thread of the workgroup takes part
-// (it waits for the bin table).
-template <int PD, int DT, class Came>
-__device__ __forceinline__ float quantize_vector(const u32x4* raw, const float* signs, float scale,
-                                                 int head_dim, const uint32_t* tbl, uint32_t lo2,
-                                                 uint32_t hi2, Came as_it_came, uint32_t* packed) {
-#pragma clang fp contract(off)
-  using FG = FastGeom<PD>;
-  constexpr int P = FG::P, E = FG::E, VEC = FG::VEC, CPL = FG::CPL, PE = FG::PE;
-  constexpr int ND = 8 * CPL;              // dims per lane
-  constexpr int W = DT == TQ_F32 ? 2 : 1;  // 16-byte pieces per chunk
-  const int lane = threadIdx.x & 63;
-  const int p = lane % P;
   // signed inputs: the sign bits of this lane's signs (+-1) flipped in (16-bit
   // types: the top bytes of two floats go to bytes 1 and 3, then the sign bits
   // are kept)
@@ -269,7 +362,20 @@ __device__ __forceinline__ float quantize_vector(const u32x4* raw, const float* 
     // a NaN input keeps its own sign in the stored norm, as the general kernel
     // leaves it: the squares of the values as they came (the same bits for
     // every other vector)
-    ss = sum_squares(as_it_came);
+    ss = sum_squares([&](int i, int c) -> float {
+      if (8 * (p + P * i) >= head_dim) return 0.0f;
+      if constexpr (!std::is_same_v<Src, PlainRows>) {
+        if constexpr (DT == TQ_F32) return __uint_as_float(raw[W * i + c / 4][c % 4]);
+        else if constexpr (DT == TQ_BF16)
+          return __uint_as_float(c & 1 ? raw[i][c / 2] & 0xffff0000u : raw[i][c / 2] << 16);
+        else return c & 1 ? hi_half_f(raw[i][c / 2]) : lo_half_f(raw[i][c / 2]);
+      }
+      const uint8_t* e = row + ESZ * (8 * (p + P * i) + c);
+      if constexpr (DT == TQ_F32) return *reinterpret_cast<const float*>(e);
+      else if constexpr (DT == TQ_BF16)
+        return __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(e) << 16);
+      else return (float)*reinterpret_cast<const _Float16*>(e);
+    });
   }
   // 3. IEEE sqrt and reciprocal; normalise (exact products of the fp16 inputs)
   const float l2 = __builtin_sqrtf(ss);
@@ -322,6 +428,7 @@ __device__ __forceinline__ float quantize_vector(const u32x4* raw, const float* 
   // 5. scale (with tau), bucketize through the bin table, pack
   const float ts = (__builtin_popcount(lane & (P - 1)) & 1) ? -scale : scale;
   __syncthreads();  // bin table ready
+  uint32_t packed[CPL];
 #pragma unroll
   for (int i = 0; i < CPL; i++) {
     uint32_t wd = 0;
@@ -341,30 +448,24 @@ __device__ __forceinline__ float quantize_vector(const u32x4* raw, const float* 
     }
     packed[i] = finite ? wd : 0u;
   }
-  return l2;
-}
-
-// A vector's packed codes and its norm, as fp16 repeated pd / 64 times, into its
-// cache entry (p: lane of the vector).
-template <int PD>
-__device__ __forceinline__ void store_entry(uint8_t* entry, int p, const uint32_t* packed,
-                                            float l2) {
-  constexpr int P = FastGeom<PD>::P, CPL = FastGeom<PD>::CPL;
+  if (live && slot >= 0 && (int64_t)slot < nslots) {
+    uint8_t* entry = (kv == 0 ? k_slab : v_slab) + ((int64_t)slot * H + h) * (int64_t)ebs;
 #pragma unroll
-  for (int i = 0; i < CPL; i++)
-    *reinterpret_cast<uint32_t*>(entry + 4 * (p + P * i)) = packed[i];
-  if (p == 0) {
-    const uint32_t nb = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)l2);
-    uint8_t* np = entry + PD / 2;
-    if constexpr (PD == 64) {
-      *reinterpret_cast<uint16_t*>(np) = (uint16_t)nb;
-    } else if constexpr (PD == 128) {
-      *reinterpret_cast<uint32_t*>(np) = nb | (nb << 16);
-    } else {
-      uint2 wq;
-      wq.x = nb | (nb << 16);
-      wq.y = wq.x;
-      *reinterpret_cast<uint2*>(np) = wq;
+    for (int i = 0; i < CPL; i++)
+      *reinterpret_cast<uint32_t*>(entry + 4 * (p + P * i)) = packed[i];
+    if (p == 0) {
+      const uint32_t nb = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)l2);
+      uint8_t* np = entry + PD / 2;
+      if constexpr (PD == 64) {
+        *reinterpret_cast<uint16_t*>(np) = (uint16_t)nb;
+      } else if constexpr (PD == 128) {
+        *reinterpret_cast<uint32_t*>(np) = nb | (nb << 16);
+      } else {
+        uint2 wq;
+        wq.x = nb | (nb << 16);
+        wq.y = wq.x;
+        *reinterpret_cast<uint2*>(np) = wq;
+      }
     }
   }
 }

@@ -260,126 +260,6 @@ __global__ __launch_bounds__(256) void write_kernel(
   }
 }
 
-// ---------------------------------------------------------------------------
-// Fast path: 32 dims per lane, P = PD/32 lanes per vector, rows in whole
-// 16-byte aligned pieces (fp16, bf16 or fp32; head_dim a multiple of 8, the
-// chunks past it zero).
-//
-// Lane p of a vector holds the 16-byte chunks j = p + P*i (i = 0..3), i.e.
-// dims d = 8j + c (c = 0..7): bits 0-2 of d are in-lane, the next log2(P)
-// bits pick the lane, the top two bits are in-lane again.  The reference's
-// lane t holds dims [t*VEC, (t+1)*VEC) with VEC = PD/32, so this lane holds
-// the reference lanes t = 8i + E*p + e (E = 8/VEC, e < E).  Both orders the
-// reference fixes come out unchanged:
-//  * sum-of-squares tree (shfl_down 16, 8, 4, 2, 1): levels 16 and 8 pair i
-//    and i + 2, i and i + 1 (in-lane); levels 4, 2, 1 pair the low three
-//    bits of t, which are lane bits (xor across lanes) from E up and in-lane
-//    below, in the reference's level order;
-//  * FWHT stages h = 1, 2, 4 (in-lane), h = 8 .. 4P (lane xor h/8), h = 8P
-//    and 16P (in-lane), ascending.
-// Every butterfly and every tree node is the same fp32 operation on the same
-// two operands as in the reference (fp32 addition is commutative, negation
-// is exact), so the bits are the same; only the lane that computes it and
-// the sign it is held with differ.
-//
-// Instruction savings over the generic kernel:
-//  * the sign flip is an XOR of the sign bits before conversion:
-//    (x*s)*inv == (x*inv)*s for s = +-1 (but for the sign of a zero, and both
-//    zeros give code 8);
-//  * a cross-lane butterfly is one fma with a DPP operand: lane l keeps
-//    z_l + sg_l * z_partner (sg = -1 on the upper lane), which is the
-//    reference's value times tau_l = +-1.  Negation commutes with the later
-//    in-lane butterflies, so every lane ends with tau_l = (-1)^popcount(lane
-//    bits) times the reference's values and folds tau_l into the 1/sqrt(pd)
-//    scale, an fma with a +0 addend that also turns -0 into +0 (both give
-//    code 8, as the reference's `val >= 0` does);
-//  * bucketize is one LDS lookup: |v| (as ordered integer bits, minus one
-//    for negative v so that `>=` becomes the reference's `>` on that side)
-//    is clamped to the four binades that hold the seven positive
-//    boundaries, and its exponent's low three bits plus its top three
-//    mantissa bits index a 64-entry table of (boundary inside this
-//    1/8-binade bin or none, 8 + boundaries below the bin).  Each bin holds
-//    at most one boundary (the tests check this for every head size), so
-//    code = (8 + below + (|v| >= boundary)) for v >= 0 and its 4-bit
-//    complement for v < 0.
-//  * a vector with an inf or NaN input is NaN everywhere after the FWHT
-//    (every output adds every input; inf * inv is inf * 0), i.e. code 0, as in
-//    the reference: one coordinate stands for all.  (A sum of squares that
-//    overflows on finite bf16 or fp32 inputs gives inv = 0, all codes 8.)
-//
-// VALU-bound (about 20 instructions per coordinate): 8192 tokens x 8 heads x
-// 128, K and V, 13.4 us for fp16 (3.2 TB/s), 12.9 for bf16 and 16.6 for fp32
-// rows; in the general kernel, whose bf16 and fp32 loads were single elements,
-// 23.3, 24.2 and 22.2 us (with that kernel's vector loads 23.0, 21.1 and 21.6).
-template <int PD, int DT>
-__global__ __launch_bounds__(256) void write_fast_kernel(
-    uint8_t* __restrict__ k_slab, uint8_t* __restrict__ v_slab,
-    const void* __restrict__ key, const void* __restrict__ value,
-    int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
-    const float* __restrict__ signs, const int32_t* __restrict__ slots,
-    uint32_t per_kv, int H, uint32_t hmul, int head_dim, int ebs, int64_t nslots, float scale) {
-#pragma clang fp contract(off)
-  using FG = FastGeom<PD>;
-  constexpr int P = FG::P, CPL = FG::CPL;
-  constexpr int W = DT == TQ_F32 ? 2 : 1;       // 16-byte pieces per chunk
-  constexpr int ESZ = DT == TQ_F32 ? 4 : 2;
-  __shared__ __attribute__((aligned(512))) uint32_t tbl[128];  // 64 x (2 * boundary, 8 + below)
-
-  const int lane = threadIdx.x & 63;
-  const int p = lane % P;
-  const uint32_t g = blockIdx.x * (uint32_t)FG::VPB + (threadIdx.x >> 6) * FG::VPW + lane / P;
-  const bool live = g < 2 * per_kv;
-
-  // this vector's row: CPL chunks j = p + P*i, issued first
-  const int kv = g >= per_kv ? 1 : 0;
-  const uint32_t rem = g - (kv ? per_kv : 0u);
-  const uint32_t t = H == 1 ? rem : __umulhi(rem, hmul);  // rem / H, exact (hmul = ceil(2^32/H))
-  const int h = (int)(rem - t * (uint32_t)H);
-  // lanes past the end read row 0 of K (no branch, no zero fill); they
-  // store nothing (slot -1)
-  u32x4 raw[CPL * W];
-  const uint8_t* row =
-      !live ? static_cast<const uint8_t*>(key)
-      : kv  ? static_cast<const uint8_t*>(value) + ((int64_t)t * v_st + (int64_t)h * v_sh) * ESZ
-            : static_cast<const uint8_t*>(key) + ((int64_t)t * k_st + (int64_t)h * k_sh) * ESZ;
-  if (head_dim == PD) {  // uniform
-#pragma unroll
-    for (int i = 0; i < CPL; i++)
-#pragma unroll
-      for (int k = 0; k < W; k++)
-        raw[W * i + k] = *reinterpret_cast<const u32x4*>(row + 8 * ESZ * (p + P * i) + 16 * k);
-  } else {  // chunks past head_dim are zero (head_dim % 8 == 0)
-#pragma unroll
-    for (int i = 0; i < CPL; i++)
-#pragma unroll
-      for (int k = 0; k < W; k++) {
-        raw[W * i + k] = u32x4{0u, 0u, 0u, 0u};
-        if (8 * (p + P * i) < head_dim)
-          raw[W * i + k] = *reinterpret_cast<const u32x4*>(row + 8 * ESZ * (p + P * i) + 16 * k);
-      }
-  }
-  const int32_t slot = live ? slots[t] : -1;
-
-  uint32_t lo2, hi2;
-  bin_table(tbl, scale, lo2, hi2);
-  uint32_t packed[CPL];
-  const float l2 = quantize_vector<PD, DT>(
-      raw, signs, scale, head_dim, tbl, lo2, hi2,
-      // the squares of the values as they came
-      [&](int i, int c) -> float {
-        if (8 * (p + P * i) >= head_dim) return 0.0f;
-        const uint8_t* e = row + ESZ * (8 * (p + P * i) + c);
-        if constexpr (DT == TQ_F32) return *reinterpret_cast<const float*>(e);
-        else if constexpr (DT == TQ_BF16)
-          return __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(e) << 16);
-        else return (float)*reinterpret_cast<const _Float16*>(e);
-      },
-      packed);
-  if (live && slot >= 0 && (int64_t)slot < nslots)
-    store_entry<PD>((kv == 0 ? k_slab : v_slab) + ((int64_t)slot * H + h) * (int64_t)ebs, p, packed,
-                    l2);
-}
-
 template <int PD>
 hipError_t launch_write(bool vec_ok, dim3 grid, hipStream_t stream, uint8_t* ks, uint8_t* vs,
                         const void* key, const void* value, int dtype, int64_t k_st,
@@ -407,7 +287,8 @@ hipError_t launch_write_fast(hipStream_t stream, uint8_t* ks, uint8_t* vs, const
   const dim3 grid((unsigned)blocks);
 #define TQ_FAST(DT)                                                                              \
   hipLaunchKernelGGL((write_fast_kernel<PD, DT>), grid, dim3(256), 0, stream, ks, vs, key, value, \
-                     k_st, k_sh, v_st, v_sh, signs, slots, per_kv, H, hmul, hd, ebs, nslots, scale)
+                     k_st, k_sh, v_st, v_sh, signs, slots, per_kv, H, hmul, hd, ebs, nslots, scale,   \
+                     PlainRows{})
   if (dtype == TQ_F16) TQ_FAST(TQ_F16);
   else if (dtype == TQ_BF16) TQ_FAST(TQ_BF16);
   else TQ_FAST(TQ_F32);
