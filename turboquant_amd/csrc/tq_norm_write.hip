@@ -12,14 +12,23 @@
 // height, width) share the pairs out in sections, one after the other.  y is
 // rounded once, to the row's type; q and k rows leave as they are rounded, and
 // the cache takes the rounded k and the v as they come, so its bytes are those
-// of tq_quantize_write_kv_cache over these rows (tq_quant.h, the same code).
+// of tq_quantize_write_kv_cache over these rows (tq_quant.h, the same kernel).
 //
-// A workgroup takes 64 vectors (32 at pd 256) of one kind, K first (their work is
-// longest), then V, then q: the kind is uniform, and q workgroups leave before
-// the bucketize.  32 dims per lane, chunks of 8 as the
-// write has them: where half a rotation is a whole number of chunk rows (the
+// A workgroup takes vectors of one kind.  K and V: 64 vectors (32 at pd 256), 32 dims per lane, chunks of 8 as
+// the write has them; where half a rotation is a whole number of chunk rows (the
 // whole head at every padded size, half of it at 128 and 256) a pair stands in
 // one lane, else the partner chunk is read again (from L1).
+// q: a wave takes heads of one token, one chunk of 8 dims per lane, so that every
+// load and store is 1 KB of consecutive bytes and the token's angles and the
+// weight are loaded once for 4 x (64 / lanes of a head) heads; the pair's partner
+// comes from lane ^ (half / 8) by DPP where half / 8 is a power of two.
+//
+// Bound by memory at large counts: 8192 tokens, 32 / 8 heads of 128 (193 MB) 51 us,
+// 3.8 TB/s against 5.1 of a large copy: q alone runs at 4.2, and K and V, whose
+// VALU work the plain write does in 13 us, take 20.  In front of the present form:
+// q heads in the write's layout and K and V first 54; two loads a q wave for four 54;
+// angles of all of a lane's pairs at once (105 registers) 52.  One decode step of 8
+// tokens 6.5 us, a chain of position, angles, norm and bucketize.
 #include <algorithm>
 
 #include "tq_quant.h"
@@ -47,13 +56,14 @@ struct NormWriteParams {
   uint8_t* vs;
   const float* signs;
   const int32_t* slots;
-  uint32_t tokens, mq, mk;  // mq, mk: ceil(2^32 / heads)
+  uint32_t tokens, mk, mg;  // ceil(2^32 / kv heads), ceil(2^32 / q groups)
+  int qgroups;              // waves that share a token's q heads
   int hq, hkv, hd, ebs;
   int64_t nslots;
   float scale;
   uint16_t* q;
   uint16_t* k;
-  uint32_t kblocks;
+  uint32_t kblocks, share;  // K workgroups; ceil(2^32 * groups of K and V / all)
 };
 
 template <int DT>
@@ -116,34 +126,139 @@ __device__ __forceinline__ void angles(const NormWriteParams& p, uint32_t t, int
   }
 }
 
-// M: chunk rows from a pair's first half to its second (the pair in one lane), 0:
-// any rotation of whole 16 dims
-template <int M>
+// 1 / sqrt(mean of squares + eps) of a vector, sum_squares(f) the sum of its
+// squares times f^2 on every lane of it
+template <int DT, class Sum>
+__device__ __forceinline__ float norm_scale(const NormWriteParams& p, Sum sum_squares) {
+  const float ss = sum_squares(1.0f);
+  float r = rsqrtf(__builtin_fmaf(ss, p.inv_hd, p.eps));
+  if (DT == TQ_BF16 && __builtin_amdgcn_ballot_w64(ss == INFINITY) != 0) {
+    // squares beyond fp32 of values within it: those of the row times 2^-70
+    // (eps is nothing beside them)
+    const float down = 0x1p-70f, s2 = sum_squares(down);
+    if (ss == INFINITY) r = rsqrtf(s2 * p.inv_hd) * down;
+  }
+  return r;
+}
+
+constexpr int kQRounds = 4;  // heads of a q wave: so many loads of 64 lanes
+
+// q heads of one token.  X: half a rotation in chunks where that is a power of
+// two, 0: any.
+template <int PD, int DT, int X>
+__device__ __forceinline__ void q_rows(const NormWriteParams& p, uint32_t blk) {
+  constexpr int L = PD / 8, R = 64 / L;  // lanes per head, heads per load
+  const int lane = threadIdx.x & 63;
+  const uint32_t wid = blk * 4u + (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (wid >= p.tokens * (uint32_t)p.qgroups) return;
+  const uint32_t t = p.qgroups == 1 ? wid : __umulhi(wid, p.mg);
+  const int c = lane % L, d = 8 * c;
+  const int first = (int)(wid - t * (uint32_t)p.qgroups) * (R * kQRounds);  // (uniform)
+  const int h0 = first + lane / L;
+  u32x4 raw[kQRounds];
+#pragma unroll
+  for (int i = 0; i < kQRounds; i++) {
+    raw[i] = u32x4{0u, 0u, 0u, 0u};
+    if (d < p.hd && h0 + i * R < p.hq)
+      raw[i] = *reinterpret_cast<const u32x4*>(p.qkv + (int64_t)t * p.row +
+                                               (int64_t)(h0 + i * R) * p.hd + d);
+  }
+  u32x4 w = {};
+  if (p.qw && d < p.hd) w = *reinterpret_cast<const u32x4*>(p.qw + d);
+  const int hb = X ? X : p.half / 8;  // chunks of half a rotation
+  const bool low = c < hb, turned = c < 2 * hb;
+  float cs[8], sn[8];
+  bool inside = true;
+  if (turned) angles(p, t, low ? d : d - p.half, cs, sn, inside);
+  // (NaN rows where any lane's pairs lack a table row)
+  const bool all_in = __builtin_amdgcn_ballot_w64(!inside) == 0;
+#pragma unroll
+  for (int i = 0; i < kQRounds; i++) {
+    if (first + i * R >= p.hq) return;
+    float r = 1.0f;
+    if (p.qw) {  // uniform
+      auto sum_squares = [&](float f) -> float {
+        float ss = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float x = elem<DT>(raw[i], e) * f;
+          ss = __builtin_fmaf(x, x, ss);
+        }
+        ss += xor_lane<1>(ss);
+        ss += xor_lane<2>(ss);
+        ss += xor_lane<4>(ss);
+        if constexpr (L >= 16) ss += xor_lane<8>(ss);
+        if constexpr (L >= 32) ss += xor_lane<16>(ss);
+        return ss;
+      };
+      r = norm_scale<DT>(p, sum_squares);
+    }
+    if (!all_in) r = __builtin_nanf("");
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      y[e] = elem<DT>(raw[i], e) * r;
+      if (p.qw) y[e] *= elem<DT>(w, e);
+    }
+    float b[8];
+    if constexpr (X > 0) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) b[e] = xor_lane<X>(y[e]);
+    } else {
+      const int from = turned ? (low ? lane + hb : lane - hb) : lane;
+#pragma unroll
+      for (int e = 0; e < 8; e++) b[e] = __shfl(y[e], from);
+    }
+    if (turned) {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        y[e] = __builtin_fmaf(y[e], cs[e], low ? -(b[e] * sn[e]) : b[e] * sn[e]);
+    }
+    if (d < p.hd && h0 + i * R < p.hq)
+      *reinterpret_cast<u32x4*>(p.q + ((int64_t)t * p.hq + h0 + i * R) * p.hd + d) =
+          round8<DT>(y);
+  }
+}
+
+// X: half a rotation in chunks of 8 dims where that is a power of two, 0: any
+template <int X>
 struct NormRows {
   NormWriteParams p;
   template <int PD, int DT>
   __device__ __forceinline__ bool rows(u32x4* raw, bool& live, int& kv, uint32_t& t, int& h) const;
 };
 
-template <int M>
+template <int X>
 template <int PD, int DT>
-__device__ __forceinline__ bool NormRows<M>::rows(u32x4* raw, bool& live, int& kv, uint32_t& t,
+__device__ __forceinline__ bool NormRows<X>::rows(u32x4* raw, bool& live, int& kv, uint32_t& t,
                                                   int& head) const {
   using FG = FastGeom<PD>;
   constexpr int P = FG::P, CPL = FG::CPL;
+  // chunk rows from a pair's first half to its second where the pair stands in
+  // one lane (0: it does not)
+  constexpr int M = X % P == 0 && X / P <= CPL / 2 ? X / P : 0;
   const int lane = threadIdx.x & 63;
   const int pl = lane % P;
-  uint32_t blk = blockIdx.x;
-  const bool isq = blk >= 2 * p.kblocks, isv = !isq && blk >= p.kblocks;  // uniform
-  blk -= isq ? 2 * p.kblocks : isv ? p.kblocks : 0u;
-  const uint32_t H = (uint32_t)(isq ? p.hq : p.hkv);
+  // Groups of eight workgroups (one per XCD) of K and V, whose time is VALU work,
+  // stand evenly among those of q, whose time is memory: group g is the next of
+  // them where g * share / 2^32 passes a whole number (uniform).
+  const uint32_t grp = blockIdx.x >> 3, ahead = __umulhi(grp, p.share);
+  if ((uint32_t)(((uint64_t)(grp + 1) * p.share) >> 32) == ahead) {
+    q_rows<PD, DT, X>(p, 8 * (grp - ahead) + (blockIdx.x & 7));
+    return false;
+  }
+  uint32_t blk = 8 * ahead + (blockIdx.x & 7);
+  if (blk >= 2 * p.kblocks) return false;
+  const bool isv = blk >= p.kblocks;
+  blk -= isv ? p.kblocks : 0u;
+  const uint32_t H = (uint32_t)p.hkv;
   uint32_t g = blk * (uint32_t)FG::VPB + (threadIdx.x >> 6) * FG::VPW + lane / P;
   live = g < p.tokens * H;
   g = live ? g : 0u;  // lanes past the end work on the first vector and store nothing
-  t = H == 1 ? g : __umulhi(g, isq ? p.mq : p.mk);
+  t = H == 1 ? g : __umulhi(g, p.mk);
   const uint32_t h = g - t * H;
   const uint16_t* const src =
-      p.qkv + (int64_t)t * p.row + (int64_t)(isq ? h : p.hq + (isv ? p.hkv : 0) + h) * p.hd;
+      p.qkv + (int64_t)t * p.row + (int64_t)(p.hq + (isv ? p.hkv : 0) + h) * p.hd;
   kv = isv ? 1 : 0;
   head = (int)h;
 #pragma unroll
@@ -152,18 +267,12 @@ __device__ __forceinline__ bool NormRows<M>::rows(u32x4* raw, bool& live, int& k
     if (8 * (pl + P * i) < p.hd) raw[i] = *reinterpret_cast<const u32x4*>(src + 8 * (pl + P * i));
   }
   if (!isv) {
-    const uint16_t* const wt = isq ? p.qw : p.kw;
+    const uint16_t* const wt = p.kw;
     bool inside = true;
-    float cs[CPL][8], sn[CPL][8];  // (M > 0: of the chunks of the first halves)
-#pragma unroll
-    for (int i = 0; i < CPL; i++) {
-      const int d = 8 * (pl + P * i);
-      if constexpr (M > 0) {
-        if (i < M) angles(p, t, d, cs[i], sn[i], inside);
-      } else {
-        if (d < 2 * p.half) angles(p, t, d < p.half ? d : d - p.half, cs[i], sn[i], inside);
-      }
-    }
+    // the angles of the first pairs ahead of the norm
+    float cs[8], sn[8];
+    if (M > 0 || 8 * pl < 2 * p.half)
+      angles(p, t, M > 0 || 8 * pl < p.half ? 8 * pl : 8 * pl - p.half, cs, sn, inside);
     float r = 1.0f;
     if (wt) {  // uniform
       auto sum_squares = [&](float f) -> float {
@@ -180,22 +289,8 @@ __device__ __forceinline__ bool NormRows<M>::rows(u32x4* raw, bool& live, int& k
         if constexpr (P == 8) ss += xor_lane<4>(ss);
         return ss;
       };
-      const float ss = sum_squares(1.0f);
-      r = rsqrtf(__builtin_fmaf(ss, p.inv_hd, p.eps));
-      if (DT == TQ_BF16 && __builtin_amdgcn_ballot_w64(ss == INFINITY) != 0) {
-        // squares beyond fp32 of values within it: those of the row times 2^-70
-        // (eps is nothing beside them)
-        const float down = 0x1p-70f, s2 = sum_squares(down);
-        if (ss == INFINITY) r = rsqrtf(s2 * p.inv_hd) * down;
-      }
+      r = norm_scale<DT>(p, sum_squares);
     }
-    // a lane sees the positions of its own pairs only: a vector is NaN if any of
-    // its lanes lacks a table row
-    float miss = inside ? 0.0f : 1.0f;
-    miss += xor_lane<1>(miss);
-    miss += xor_lane<2>(miss);
-    if constexpr (P == 8) miss += xor_lane<4>(miss);
-    if (miss != 0.0f) r = __builtin_nanf("");
     auto normed = [&](const u32x4& x, int d, float* n) {
       u32x4 w = {};
       if (wt) w = *reinterpret_cast<const u32x4*>(wt + d);
@@ -205,59 +300,88 @@ __device__ __forceinline__ bool NormRows<M>::rows(u32x4* raw, bool& live, int& k
         if (wt) n[c] *= elem<DT>(w, c);
       }
     };
-    float y[CPL][8];
-#pragma unroll
-    for (int i = 0; i < CPL; i++)
-      if (8 * (pl + P * i) < p.hd) normed(raw[i], 8 * (pl + P * i), y[i]);
+    // Chunk rows (pairs of them) one after the other, each rounded back into raw
+    // before the next one's loads: the registers of all angles at once would halve
+    // the waves that fit a SIMD.
     if constexpr (M > 0) {
 #pragma unroll
-      for (int i = 0; i < M; i++)
-#pragma unroll
-        for (int c = 0; c < 8; c++) {
-          const float a = y[i][c], b = y[i + M][c];
-          y[i][c] = __builtin_fmaf(a, cs[i][c], -(b * sn[i][c]));
-          y[i + M][c] = __builtin_fmaf(b, cs[i][c], a * sn[i][c]);
+      for (int i = 0; i < CPL; i++) {
+        if (i >= M && i < 2 * M) continue;
+        const int d = 8 * (pl + P * i);
+        if (d >= p.hd) continue;  // (never of a pair)
+        if (i > 0) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (i < M) angles(p, t, d, cs, sn, inside);
         }
+        float a[8];
+        normed(raw[i], d, a);
+        if (i < M) {
+          float b[8], y[8];
+          normed(raw[i + M], d + p.half, b);
+#pragma unroll
+          for (int c = 0; c < 8; c++) {
+            y[c] = __builtin_fmaf(a[c], cs[c], -(b[c] * sn[c]));
+            b[c] = __builtin_fmaf(b[c], cs[c], a[c] * sn[c]);
+          }
+          raw[i] = round8<DT>(y);
+          raw[i + M] = round8<DT>(b);
+        } else {
+          raw[i] = round8<DT>(a);
+        }
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < CPL; i++) {
         const int d = 8 * (pl + P * i);
-        if (d >= 2 * p.half) continue;
+        if (i > 0) __builtin_amdgcn_sched_barrier(0);
+        if (d >= p.hd) continue;
         const bool low = d < p.half;
-        const int o = low ? d + p.half : d - p.half;
-        float b[8];
-        normed(*reinterpret_cast<const u32x4*>(src + o), o, b);
+        if (i > 0 && d < 2 * p.half) angles(p, t, low ? d : d - p.half, cs, sn, inside);
+        float a[8];
+        normed(raw[i], d, a);
+        if (d < 2 * p.half) {
+          const int o = low ? d + p.half : d - p.half;
+          float b[8];
+          normed(*reinterpret_cast<const u32x4*>(src + o), o, b);
 #pragma unroll
-        for (int c = 0; c < 8; c++) {
-          const float turn = b[c] * sn[i][c];
-          y[i][c] = __builtin_fmaf(y[i][c], cs[i][c], low ? -turn : turn);
+          for (int c = 0; c < 8; c++) {
+            const float turn = b[c] * sn[c];
+            a[c] = __builtin_fmaf(a[c], cs[c], low ? -turn : turn);
+          }
         }
+        raw[i] = round8<DT>(a);
       }
     }
-    uint16_t* const out = isq ? p.q : p.k;
+    // a lane sees the positions of its own pairs only: a vector is NaN if any of
+    // its lanes lacks a table row
+    float miss = inside ? 0.0f : 1.0f;
+    miss += xor_lane<1>(miss);
+    miss += xor_lane<2>(miss);
+    if constexpr (P == 8) miss += xor_lane<4>(miss);
+    uint16_t* const out = p.k;
 #pragma unroll
     for (int i = 0; i < CPL; i++) {
       const int d = 8 * (pl + P * i);
       if (d >= p.hd) continue;
-      raw[i] = round8<DT>(y[i]);
+      if (miss != 0.0f) raw[i] = u32x4{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
       if (live && out) *reinterpret_cast<u32x4*>(out + ((int64_t)t * H + h) * p.hd + d) = raw[i];
     }
-    if (isq) return false;
   }
   return true;
 }
 
 template <int PD, int DT>
 hipError_t launch_norm_write(const NormWriteParams& p, dim3 grid, hipStream_t st) {
-  constexpr int P = FastGeom<PD>::P, CPL = FastGeom<PD>::CPL;
-  // chunk rows of half a rotation, where whole and (both halves) inside the lane
-  const int m = p.half % (8 * P) == 0 ? p.half / (8 * P) : 0;
-#define TQ_NW(M)                                                                               \
-  hipLaunchKernelGGL((write_fast_kernel<PD, DT, NormRows<M>>), grid, dim3(256), 0, st, p.ks, p.vs, \
+#define TQ_NW(X)                                                                               \
+  hipLaunchKernelGGL((write_fast_kernel<PD, DT, NormRows<X>>), grid, dim3(256), 0, st, p.ks, p.vs, \
                      nullptr, nullptr, 0, 0, 0, 0, p.signs, p.slots, 0u, p.hkv, 0u, p.hd, p.ebs,   \
-                     p.nslots, p.scale, NormRows<M>{p})
-  if (m == 1) TQ_NW(1);
-  else if (CPL == 4 && m == 2) TQ_NW(CPL / 2);
+                     p.nslots, p.scale, NormRows<X>{p})
+  const int x = p.half / 8;  // (at most PD / 16)
+  if (x == 1) TQ_NW(1);
+  else if (x == 2) TQ_NW(2);
+  else if (x == 4) TQ_NW(4);
+  else if (PD >= 128 && x == 8) TQ_NW((PD >= 128 ? 8 : 0));
+  else if (PD >= 256 && x == 16) TQ_NW((PD >= 256 ? 16 : 0));
   else TQ_NW(0);
 #undef TQ_NW
   return hipGetLastError();
@@ -382,7 +506,9 @@ extern "C" int tq_norm_rope_write(
   auto recip = [](int h) -> uint32_t {
     return h == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + h - 1) / h);
   };
-  p.mq = recip(num_qo_heads);
+  const int wave_heads = kQRounds * 64 / (pd / 8);  // of a q wave
+  p.qgroups = (num_qo_heads + wave_heads - 1) / wave_heads;
+  p.mg = recip(p.qgroups);
   p.mk = recip(num_kv_heads);
   p.hd = head_dim;
   p.ebs = ebs;
@@ -403,8 +529,10 @@ extern "C" int tq_norm_rope_write(
     p.q = static_cast<uint16_t*>(q_out) + a * num_qo_heads * head_dim;
     p.k = k_out ? static_cast<uint16_t*>(k_out) + a * num_kv_heads * head_dim : nullptr;
     p.kblocks = (uint32_t)(((int64_t)p.tokens * num_kv_heads + vpb - 1) / vpb);
-    const int64_t qblocks = ((int64_t)p.tokens * num_qo_heads + vpb - 1) / vpb;
-    const dim3 grid((unsigned)(2 * (int64_t)p.kblocks + qblocks));
+    const int64_t qblocks = ((int64_t)p.tokens * p.qgroups + 3) / 4;
+    const int64_t kgroups = (2 * (int64_t)p.kblocks + 7) / 8, groups = kgroups + (qblocks + 7) / 8;
+    p.share = (uint32_t)((((uint64_t)kgroups << 32) + groups - 1) / groups);
+    const dim3 grid((unsigned)(8 * groups));
     hipError_t e;
 #define TQ_NW(PD)                                                       \
   (dtype == TQ_F16 ? launch_norm_write<PD, TQ_F16>(p, grid, st)         \
