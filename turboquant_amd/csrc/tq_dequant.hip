@@ -130,13 +130,13 @@ __device__ __forceinline__ int find_request(int n, int blk, First first) {
 // Cached vectors [block's range) of tokens 0 .. num_tokens - 1 (`pages` their
 // page-table row; those from `sinks` on stand `gap` places further in it) to out
 // (token 0's row).  blk: workgroup within the range.
-template <int PD>
+template <int PD, int NV = kVecsPerThread>
 __device__ __forceinline__ void read_back(const ReadBackParams& p, const int32_t* pages,
                                           int num_tokens, int blk, _Float16* out,
                                           const float* cb, _Float16* stage, uint32_t sinks = 0,
                                           uint32_t gap = 0) {
   constexpr int L = PD / 32;  // lanes per vector, 32 dims (16 code bytes) each
-  constexpr int VPB = 256 / L, NV = kVecsPerThread;
+  constexpr int VPB = 256 / L;
   const int lane = threadIdx.x % L;
   const uint8_t* slab = blockIdx.y ? p.v_slab : p.k_slab;
   const int64_t nvec = (int64_t)num_tokens * p.H;
@@ -355,7 +355,7 @@ __device__ __forceinline__ void copy_fresh(const ReadBackParams& p, const Gather
 // of them (a kernel of its own: the other two do without the places' shift)
 enum Read { kPaged, kGather, kWindow };
 
-template <int PD, int READ>
+template <int PD, int READ, int NV = kVecsPerThread>
 __global__ __launch_bounds__(256) void read_back_kernel(ReadBackParams p, int num_tokens) {
   __shared__ float cb[16];  // the codebook, indexed per lane
   __shared__ __attribute__((aligned(16))) _Float16 stage[4 * 64 * 32];
@@ -368,7 +368,7 @@ __global__ __launch_bounds__(256) void read_back_kernel(ReadBackParams p, int nu
     if (blk < 0) {
       const int i = find_request(p.nreq, (int)blockIdx.x, [&](int r) { return p.reqs[r].ctx_blk; });
       const GatherReq& r = p.reqs[i];
-      read_back<PD>(p, p.pages + (int64_t)r.bt_row * p.page_stride, r.ctx,
+      read_back<PD, NV>(p, p.pages + (int64_t)r.bt_row * p.page_stride, r.ctx,
                     (int)blockIdx.x - r.ctx_blk, out + (int64_t)r.dst_row * p.out_stride_tok, cb,
                     stage, READ == kWindow ? r.sinks : 0, READ == kWindow ? r.gap : 0);
     } else {
@@ -417,19 +417,19 @@ void fill_geometry(ReadBackParams& p, const uint8_t* k_slab, const uint8_t* v_sl
   p.nreq = p.ctx_blocks = 0;
 }
 
-template <int READ>
+template <int READ, int NV = kVecsPerThread>
 hipError_t launch_read_back(int pd, dim3 grid, hipStream_t s, const ReadBackParams& p, int tokens) {
   if (pd == 64)
-    hipLaunchKernelGGL((read_back_kernel<64, READ>), grid, dim3(256), 0, s, p, tokens);
+    hipLaunchKernelGGL((read_back_kernel<64, READ, NV>), grid, dim3(256), 0, s, p, tokens);
   else if (pd == 128)
-    hipLaunchKernelGGL((read_back_kernel<128, READ>), grid, dim3(256), 0, s, p, tokens);
+    hipLaunchKernelGGL((read_back_kernel<128, READ, NV>), grid, dim3(256), 0, s, p, tokens);
   else
-    hipLaunchKernelGGL((read_back_kernel<256, READ>), grid, dim3(256), 0, s, p, tokens);
+    hipLaunchKernelGGL((read_back_kernel<256, READ, NV>), grid, dim3(256), 0, s, p, tokens);
   return hipGetLastError();
 }
 
-int64_t ctx_block_count(int64_t tokens, int H, int pd) {
-  const int per = kVecsPerThread * (256 / (pd / 32));
+int64_t ctx_block_count(int64_t tokens, int H, int pd, int nv = kVecsPerThread) {
+  const int per = nv * (256 / (pd / 32));
   return (tokens * H + per - 1) / per;
 }
 
@@ -487,6 +487,15 @@ extern "C" int tq_dequant_paged(const uint8_t* k_slab, const uint8_t* v_slab,
 
 namespace tq {
 namespace {
+
+// Vectors per thread of a window's read-back: one, whose waves are four times as
+// many, up to 2^24 dims and at padded size 64, four above (us, one against four:
+// padded size 128, 16000 vectors 5.1 / 10.4, 98304 14.1 / 15.6, 196608 21.1 / 19.3,
+// 1048576 96.0 / 95.1; 256, 4000 5.0 / 11.1, 49152 14.0 / 16.7, 262144 55.4 / 54.4;
+// 64, 8000 4.3 / 9.2, 524288 25.2 / 27.1; two per thread lie behind both).
+int window_vecs(int64_t vectors, int pd) {
+  return pd == 64 || vectors * pd <= (1 << 24) ? 1 : kVecsPerThread;
+}
 
 // tq_prefill_gather, and (firsts given) tq_prefill_gather_window
 int gather(const char* what, const int32_t* firsts, int32_t sink, const uint8_t* k_slab,
@@ -551,6 +560,13 @@ int gather(const char* what, const int32_t* firsts, int32_t sink, const uint8_t*
   p.vec_load = in_dtype != TQ_F32 && head_dim % 8 == 0 && k_stride_tok % 8 == 0 &&
                k_stride_head % 8 == 0 && v_stride_tok % 8 == 0 && v_stride_head % 8 == 0 &&
                (((uintptr_t)key | (uintptr_t)value) & 15) == 0;
+  int nv = kVecsPerThread;  // vectors per thread
+  if (firsts) {
+    int64_t tokens = 0;
+    for (int i = 0; i < num_requests; i++)
+      tokens += ctx_lens[i] - firsts[i] + (sink < firsts[i] ? sink : firsts[i]);
+    nv = window_vecs(tokens * num_kv_heads, pd);
+  }
   for (int a = 0; a < num_requests; a += kMaxReqs) {
     p.nreq = num_requests - a < kMaxReqs ? num_requests - a : kMaxReqs;
     int64_t cblk = 0, fblk = 0;
@@ -570,7 +586,7 @@ int gather(const char* what, const int32_t* firsts, int32_t sink, const uint8_t*
       r.bt_row = table_rows[a + i];
       r.ctx_blk = (int)cblk;
       r.fresh_blk = (int)fblk;
-      cblk += ctx_block_count(r.ctx, num_kv_heads, pd);
+      cblk += ctx_block_count(r.ctx, num_kv_heads, pd, nv);
       fblk += ((int64_t)r.fresh * num_kv_heads * (pd / 8) + 256 * kFreshPieces - 1) /
               (256 * kFreshPieces);
       if (cblk + fblk > 0x7fffffffLL) {
@@ -582,8 +598,9 @@ int gather(const char* what, const int32_t* firsts, int32_t sink, const uint8_t*
     p.ctx_blocks = (int)cblk;
     const dim3 grid((unsigned)(cblk + fblk), 2);
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    const hipError_t e = firsts ? launch_read_back<kWindow>(pd, grid, st, p, 0)
-                                : launch_read_back<kGather>(pd, grid, st, p, 0);
+    const hipError_t e = !firsts   ? launch_read_back<kGather>(pd, grid, st, p, 0)
+                         : nv == 1 ? launch_read_back<kWindow, 1>(pd, grid, st, p, 0)
+                                   : launch_read_back<kWindow>(pd, grid, st, p, 0);
     if (e != hipSuccess) {
       set_error("%s: launch failed: %s", what, hipGetErrorString(e));
       return (int)e;
