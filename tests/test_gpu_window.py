@@ -107,9 +107,11 @@ def test_long(lens, window, sink):
 
 
 def test_a_window_beyond_the_sequence_is_full_attention():
-    """Bit for bit the decode over every token."""
+    """Within the same bounds as the decode over every token (whose split of the
+    work, and so its order of the sums, is another)."""
     c = C.make(12, [500, 33, 1, 0, 1200], 32, 8, 128)
     t, q, o = run(c, 2000, 7)
+    qx = q.double().cpu().numpy()
     rows = ops.balanced_rows(5, 32, 8, 128)
     full = torch.empty_like(o)
     ops.decode_paged_balanced(q, t["cache"], t["indices"], t["indptr"], t["seq"], 8, 128, 128,
@@ -117,7 +119,20 @@ def test_a_window_beyond_the_sequence_is_full_attention():
                               torch.empty((rows, 32, 128), device=DEV),
                               torch.empty((rows, 32), device=DEV),
                               torch.empty(7, dtype=torch.int32, device=DEV))
-    assert torch.equal(o, full)
+    ref = W.decode(c, qx, 2000, 7)
+    check_o(c, full, ref, qx, "fp16", 2000, 7)
+    check_o(c, o, ref, qx, "fp16", 2000, 7)
+
+
+@pytest.mark.parametrize("hq,hkv,hd", [(8, 1, 64), (16, 2, 96), (12, 6, 128), (8, 8, 256),
+                                       (16, 1, 128)])
+@pytest.mark.parametrize("window,sink", [(192, 16), (200, 9), (384, 16), (385, 16), (4, 396), (1, 400)])
+def test_where_one_launch_ends(hq, hkv, hd, window, sink):
+    """Windows on both sides of the sizes that one launch takes, few sequences
+    and more than workgroups of it would fit."""
+    lens = [1500, 0, window, window + 1, window + sink + 40, 7, 800]
+    run(C.make(hq + hd, lens, hq, hkv, hd), window, sink, "bf16")
+    run(C.make(hq + hd + 1, lens * 38, hq, hkv, hd), window, sink)
 
 
 def test_bad_pages_and_short_tables_are_empty():

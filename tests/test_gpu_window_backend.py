@@ -180,7 +180,12 @@ def test_without_a_window_nothing_changes():
     q = torch.randn((2, 8 * 128), device=DEV).half()
     out = impl.forward(None, q, None, None, cache, meta)
     wide = TurboQuantFusedImpl(8, 128, 0.09, 2, None, 1000, "fp8")
-    assert torch.equal(wide.forward(None, q, None, None, cache, meta), out)
+    # (a window beyond the sequences: the same sum in another order)
+    qx = q.view(2, 8, 128).double().cpu().numpy()
+    c.scale, c.signs = 0.09, impl._signs.cpu().numpy()
+    ref = W.decode(c, qx, 1000, 0)
+    for x in (out, wide.forward(None, q, None, None, cache, meta)):
+        check_o(c, x.view(2, 8, 128), ref, qx, "fp16", 1000, 0)
 
 
 def test_project_and_update():

@@ -633,19 +633,18 @@ constexpr bool kPvLo = TQ_PV_LO != 0;
 // The math of one step (two tiles, read into d): scores, softmax, PV.  whole():
 // whether every token of the step counts (uniform); counts(T, i): whether token i
 // of tile T does.
-template <int PD, int PACK, bool QC, int SH, bool PLO, class Whole, class Counts>
+template <int PD, int PACK, int SH, class Whole, class Counts>
 __device__ __forceinline__ void attend_step(const StepData<PD>& d, const half8_t* qb,
-                                            const half8_t* ql, uint32_t lanec, const uint32_t* lut,
-                                            Whole whole, Counts counts, int n, int q4, int ptile,
+                                            uint32_t lanec, const uint32_t* lut, Whole whole,
+                                            Counts counts, int n, int q4, int ptile,
                                             uint64_t hmask, float lpv, SoftmaxState<PD>& st) {
   // scores of both tiles (scheduling barriers keep the two tiles'
   // dequant temporaries from being live at the same time)
   float4_t acc[2];
   constexpr bool PM = PACK == 2;  // packed merge of the two tiles' unmerged sums
-  static_assert(PACK == 1 || QC, "two tiles per score set need the hi / lo columns");
-  acc[0] = tile_scores<PD, QC, SH, !PM>(d.k[0], qb, ql, lanec, lut);
+  acc[0] = tile_scores<PD, true, SH, !PM>(d.k[0], qb, qb, lanec, lut);
   __builtin_amdgcn_sched_barrier(0);
-  acc[1] = tile_scores<PD, QC, SH, !PM>(d.k[1], qb, ql, lanec, lut);
+  acc[1] = tile_scores<PD, true, SH, !PM>(d.k[1], qb, qb, lanec, lut);
   __builtin_amdgcn_sched_barrier(0);
   if constexpr (PM) acc[0] = pack_merge(acc[0], acc[1]);
   constexpr int NV = 4 * (2 / PACK);  // score values per lane
@@ -661,8 +660,7 @@ __device__ __forceinline__ void attend_step(const StepData<PD>& d, const half8_t
     for (int r = 0; r < 4; r++) {
       // tile 0's scores in lanes 0..7 of each row and tile 1's in 8..15
       // (PACK 2), times the K norm straight from its fp16 half
-      const float a = PACK == 2 ? acc[0][r] : acc[g][r];
-      sc[4 * g + r] = mul_lo_half(a, nr[r]);
+      sc[4 * g + r] = mul_lo_half(acc[g][r], nr[r]);
       nvr[4 * g + r] = nr[r];
     }
   }
@@ -676,21 +674,17 @@ __device__ __forceinline__ void attend_step(const StepData<PD>& d, const half8_t
     }
   }
   uint32_t pw[NV / 2], pl[NV / 2];
-  softmax_step<PD, NV, PLO>(sc, nvr, full, valid, PACK == 2, hmask, lpv, st, pw, pl);
+  softmax_step<PD, NV, true>(sc, nvr, full, valid, PACK == 2, hmask, lpv, st, pw, pl);
+  // columns n >= 8 take the lo parts of head n - 8's probabilities
+  const bool up = n >= 8;
   half8_t p8;
-  if constexpr (PACK == 2 && PLO) {
+  if constexpr (PACK == 2) {
     // lanes n < 8: hi parts of tile 0 (own) and tile 1 (lane n + 8);
     // lanes n >= 8: lo parts of tile 0 (lane n - 8) and tile 1 (own)
-    const bool up = n >= 8;
     const uint32_t r0 = ror8u(up ? pw[0] : pl[0]), r1 = ror8u(up ? pw[1] : pl[1]);
     p8 = up ? as_half8(r0, r1, pl[0], pl[1]) : as_half8(pw[0], pw[1], r0, r1);
-  } else if constexpr (PACK == 2) {
-    p8 = as_half8(pw[0], pw[1], shl8(pw[0]), shl8(pw[1]));
-  } else if constexpr (PLO) {
-    // lanes n >= 8 hold the same scores as lane n - 8: their lo parts
-    p8 = n >= 8 ? as_half8(pl[0], pl[1], pl[2], pl[3]) : as_half8(pw[0], pw[1], pw[2], pw[3]);
   } else {
-    p8 = as_half8(pw[0], pw[1], pw[2], pw[3]);
+    p8 = up ? as_half8(pl[0], pl[1], pl[2], pl[3]) : as_half8(pw[0], pw[1], pw[2], pw[3]);
   }
   step_pv<PD, SH>(d.v[0], d.v[1], p8, st, lanec, lut);
 }
@@ -753,7 +747,8 @@ void decode_partials_kernel(DecodeParams p) {
   constexpr int ECH = RG::ECH;
   constexpr int CPT = RG::CPT;
   constexpr int NI = RG::NI;
-  constexpr bool PLO = QC && kPvLo && MATH >= 2;  // PV probabilities as hi + lo
+  // PV probabilities as hi + lo (windowed: always; 1 .. 2% of a launch)
+  constexpr bool PLO = QC && (kPvLo || WIN) && MATH >= 2;
   // LDS: the dequant table at address 0 (the table reads rely on it), then
   // the ring of tile slots
   struct __attribute__((aligned(16))) Lds {
@@ -1394,7 +1389,9 @@ void decode_partials_kernel(DecodeParams p) {
   // rest between the row's lanes.  Rows are stored as fp16 (the combine
   // reads them so): half the bytes of fp32 rows, and their rounding
   // (relative 2^-11 on normalised outputs) is far inside the output
-  // tolerance.
+  // tolerance.  Windowed rows, of which window_plan makes few, stay fp32: with
+  // the lo parts of the probabilities that takes the rms error from 1.9 times
+  // that of the output's own rounding to 1.2.
   _Float16* const out = reinterpret_cast<_Float16*>(p.po) + orow0 * PD;
   for (int e = 8 * lane; e < ratio * PD; e += 512) {
     const float4_t a = *reinterpret_cast<const float4_t*>(stage + e);
@@ -1423,13 +1420,22 @@ void decode_partials_kernel(DecodeParams p) {
                                  (((sgnbits >> k) & 1u) << 31));
       }
     }
+    if constexpr (WIN) {
+      float4_t* const wide = reinterpret_cast<float4_t*>(p.po + orow0 * PD + e);
+      wide[0] = float4_t{x[0], x[1], x[2], x[3]};
+      wide[1] = float4_t{x[4], x[5], x[6], x[7]};
+      continue;
+    }
     const half8_t h = {(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3],
                        (_Float16)x[4], (_Float16)x[5], (_Float16)x[6], (_Float16)x[7]};
     *reinterpret_cast<half8_t*>(out + e) = h;
   }
 }
-// four fp16 partial-row values as fp32
-__device__ __forceinline__ float4_t load_half4(const _Float16* src) {
+// four partial-row values as fp32
+__device__ __forceinline__ float4_t load_row4(const float* src) {
+  return *reinterpret_cast<const float4_t*>(src);
+}
+__device__ __forceinline__ float4_t load_row4(const _Float16* src) {
   const half4_t h = *reinterpret_cast<const half4_t*>(src);
   return float4_t{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
 }
@@ -1445,8 +1451,9 @@ __device__ __forceinline__ float4_t load_half4(const _Float16* src) {
 // of group 0 store.
 //
 // ROWS: o rows of hd elements (hd % 4 == 0), fp16 or bf16 (else fp16 rows of PD).
-template <int PD, bool ROWS>
-__global__ __launch_bounds__(256) void combine_kernel(const _Float16* __restrict__ po,
+// T: the partial rows' type.
+template <int PD, bool ROWS, typename T = _Float16>
+__global__ __launch_bounds__(256) void combine_kernel(const T* __restrict__ po,
                                                       const float* __restrict__ plse, int S_fixed,
                                                       const int32_t* __restrict__ split_rows,
                                                       int Hq, int hd, int o_bf16,
@@ -1480,7 +1487,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const _Float16* __restrict
       if (sj < S) {
         const int64_t r = row0 + (int64_t)sj * Hq;
         l[j] = plse[r];
-        v[j] = load_half4(po + r * PD + col);
+        v[j] = load_row4(po + r * PD + col);
       }
     }
     float mr = m;
@@ -1535,6 +1542,342 @@ __global__ __launch_bounds__(256) void combine_kernel(const _Float16* __restrict
     }
     *reinterpret_cast<half4_t*>(o + ((int64_t)b * Hq + h) * (ROWS ? hd : PD) + col) = hv;
   }
+}
+
+// ---- a window in one launch ----------------------------------------------
+// Windowed decode where a workgroup takes all that one kv head of a sequence
+// sees, its waves the steps (32 tokens) round robin: no plan, no partial rows, no
+// second launch.  A wave loads codes and norms straight into the MFMA layout of
+// StepData (buffer loads, one step ahead of the math: two and four ahead measured
+// 0.5 and 1.1 us more at 1024 tokens, as did 16 waves, whose registers spill, and
+// four, 5 us), keeps its own softmax state, and the states meet in LDS once at the
+// end, in fp32, where the sum is rotated back and stored.  For short windows the
+// time is latencies (length, page ids, codes, table, merge), and the split form
+// pays two launches' worth; with more tokens to a workgroup the lookups that one
+// CU does alone (1.9 us for 256 tokens at head size 128) outlast that
+// (window_direct_pays).  Roundings are those of the split form: q' and the
+// probabilities times the V norms as fp16 hi + lo parts (22 bits), and the output.
+constexpr int kDirectWaves = 8;
+template <int PD>
+constexpr int direct_copies() {  // of the dequant table
+  return PD == 256 ? 16 : 32;
+}
+
+template <int PD, int NW = kDirectWaves>
+__global__ __launch_bounds__(64 * NW) void window_direct_kernel(DecodeParams p, void* out,
+                                                                int o_bf16) {
+  constexpr int KD = PD / 32, NO = PD / 16;
+  [[maybe_unused]] constexpr int VW = StepData<PD>::VW;
+  constexpr int PACK = PD <= 128 ? 2 : 1;
+  constexpr int EBS = PD == 64 ? 48 : (PD == 128 ? 80 : 144);
+  constexpr int LC = direct_copies<PD>(), SH = lut_shift(LC);
+  constexpr int HMAX = 8;  // q heads: hi and lo parts fill the 16 columns
+  struct __attribute__((aligned(16))) Work {
+    uint32_t klut[256 * LC];
+    _Float16 qhi[HMAX * PD], qlo[HMAX * PD];
+  };
+  struct __attribute__((aligned(16))) Merge {
+    float o[NW][HMAX * PD];
+    float mb[NW][HMAX], l[NW][HMAX];
+  };
+  union __attribute__((aligned(16))) Lds {
+    Work w;
+    Merge m;
+  };
+  __shared__ Lds sm;
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int q4 = lane >> 4, n = lane & 15;
+  const int kvh = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv;
+  const int ratio = p.ratio;
+  const int L = max(p.seq_lens[b], 0), ip = p.indptr[b];
+  const WindowSpan ws = window_span(L, p.window, p.sink);
+  const int steps = (ws.len + 2 * kTile - 1) / (2 * kTile);
+
+  // the page ids of this wave's tiles: lane i holds that of tile i % 2 of its
+  // step i / 2 (of 32, far more than window_direct_pays allows)
+  const int tpp = p.block_size / kTile;
+  const int64_t tokstride = (int64_t)p.Hkv * EBS;
+  const int rec = (int)(kTile * tokstride);
+  auto place = [&](int t) -> int { return t < ws.sinks ? t : t + ws.skip; };
+  [[maybe_unused]] int pages = -1;
+  {
+    const int t = 2 * (w + NW * (lane / 2)) + (lane & 1);
+    const int64_t e = (int64_t)ip + place(t) / tpp;
+    if (t * kTile < ws.len && e >= 0 && e < p.entries) pages = p.indices[e];
+  }
+
+  // s * q of this wave's share of the heads' elements (512 a wave): lane l holds 8
+  // consecutive ones
+  const int e0 = 512 * w + 8 * lane;
+  const bool qmine = e0 < ratio * PD;
+  float qx[8];
+  uint32_t sgn = 0;  // sign bits of dims e0 % PD .. + 7
+  {
+    u32x4 qv = {0u, 0u, 0u, 0u};
+    const int d = e0 % PD;
+    if (qmine && d < p.hd)
+      qv = *reinterpret_cast<const u32x4*>(p.q + (int64_t)b * p.q_sb +
+                                           (int64_t)(kvh * ratio + e0 / PD) * p.q_sh + d);
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const float xh = k & 1 ? hi_half(qv[k / 2]) : lo_half(qv[k / 2]);
+      const float xb = __uint_as_float(k & 1 ? qv[k / 2] & 0xffff0000u : qv[k / 2] << 16);
+      qx[k] = p.q_bf16 ? xb : xh;
+      if (p.signs) sgn |= (__float_as_uint(p.signs[d + k]) >> 31) << k;
+    }
+  }
+
+  // per-lane byte offsets inside a tile's slab
+  const uint32_t hoff = (uint32_t)kvh * EBS;
+  const uint32_t ko = (uint32_t)(n * tokstride) + hoff + q4 * (PD / 8);
+  const uint32_t vo = (uint32_t)(4 * q4 * tokstride) + hoff + n * (PD / 32);
+  const uint32_t no = (uint32_t)((4 * q4 + (lane & 3)) * tokstride) + hoff + PD / 2;
+  const int slotw = 16 / PACK;
+  const int ptile = n / slotw;  // tile of this lane's packed scores
+  // the codes and norms of the wave's i-th step; ok: its tiles' presence (bits)
+  auto load_step = [&](int i, StepData<PD>& d, int& ok) {
+    ok = 0;
+#if defined(__HIP_DEVICE_COMPILE__)
+    uint32_t nk[2], nv[2];
+#pragma unroll
+    for (int T = 0; T < 2; T++) {
+      const int t = 2 * (w + NW * i) + T;
+      const int pg = __builtin_amdgcn_readlane(pages, 2 * i + T);
+      const bool in = pg >= 0 && pg < p.num_blocks;
+      ok |= in ? 1 << T : 0;
+      const int64_t off =
+          in ? ((int64_t)pg * p.block_size + (place(t) % tpp) * kTile) * tokstride : 0;
+      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(p.ks + off), (short)0, in ? rec : 0, 0x00020000);
+      const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(p.vs + off), (short)0, in ? rec : 0, 0x00020000);
+      if constexpr (PD == 64) {
+        const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(rk, ko, 0, 0);
+        d.k[T][0] = x[0];
+        d.k[T][1] = x[1];
+      } else {
+#pragma unroll
+        for (int c = 0; c < KD / 4; c++) {
+          const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(rk, ko + 16 * c, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 4; e++) d.k[T][4 * c + e] = x[e];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const uint32_t o = vo + (uint32_t)(j * tokstride);
+        if constexpr (PD == 64) {
+          d.v[T][j][0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rv, o, 0, 0);
+        } else if constexpr (PD == 128) {
+          d.v[T][j][0] = __builtin_amdgcn_raw_buffer_load_b32(rv, o, 0, 0);
+        } else {
+          const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(rv, o, 0, 0);
+          d.v[T][j][0] = x[0];
+          d.v[T][j][VW - 1] = x[1];
+        }
+      }
+      nk[T] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rk, no, 0, 0);
+      nv[T] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rv, no, 0, 0);
+    }
+    if constexpr (PACK == 2) {
+      d.nkv[0] = ptile ? nk[1] | nv[1] << 16 : nk[0] | nv[0] << 16;
+      d.nkv[1] = 0;
+    } else {
+      d.nkv[0] = nk[0] | nv[0] << 16;
+      d.nkv[1] = nk[1] | nv[1] << 16;
+    }
+#else
+    (void)i;
+    (void)d;
+    (void)rec;
+    (void)ko;
+    (void)vo;
+    (void)no;
+#endif
+  };
+  const int mine = steps > w ? (steps - w + NW - 1) / NW : 0;  // this wave's steps
+  StepData<PD> d0, d1;
+  int ok0 = 0, ok1 = 0;
+  if (mine > 0) load_step(0, d0, ok0);
+
+  // ---- q' = FWHT(s q) / sqrt(pd) in log2 units as fp16 hi + lo, and the table
+  if (qmine) {
+    if (p.signs) {
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        qx[k] = __uint_as_float(__float_as_uint(qx[k]) ^ (((sgn >> k) & 1u) << 31));
+    }
+  }
+  if (p.signs) {  // (all lanes: the exchanges stay inside a head's PD / 8 lanes)
+#pragma unroll
+    for (int h = 1; h < 8; h <<= 1)
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        if (!(k & h)) {
+          const float a = qx[k], c = qx[k + h];
+          qx[k] = a + c;
+          qx[k + h] = a - c;
+        }
+#pragma unroll
+    for (int m = 1; m < PD / 8; m <<= 1) {
+      const float sg = (lane & m) ? -1.0f : 1.0f;
+#pragma unroll
+      for (int k = 0; k < 8; k++) qx[k] = __builtin_fmaf(sg, qx[k], xor_lane(qx[k], m));
+    }
+  }
+  if (qmine) {
+    const float qsc = (p.signs ? p.inv_sqrt_pd : 1.0f) * p.qk_scale;
+    half8_t hi, lo;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const float x = qx[k] * qsc;
+      hi[k] = (_Float16)x;
+      lo[k] = (_Float16)(x - (float)hi[k]);
+    }
+    *reinterpret_cast<half8_t*>(&sm.w.qhi[e0]) = hi;
+    *reinterpret_cast<half8_t*>(&sm.w.qlo[e0]) = lo;
+  }
+  build_table<LC>(sm.w.klut, 64 * NW);
+  __syncthreads();
+  half8_t qb[KD];
+  const int hq = n & 7;  // q head of this lane's B column
+#pragma unroll
+  for (int c = 0; c < KD; c++) {
+    const int e = hq * PD + q4 * (PD / 4) + 8 * c;
+    const half8_t none = {};
+    qb[c] = *reinterpret_cast<const half8_t*>(n < 8 ? &sm.w.qhi[e] : &sm.w.qlo[e]);
+    if (hq >= ratio) qb[c] = none;
+  }
+
+  SoftmaxState<PD> st;
+#pragma unroll
+  for (int i = 0; i < NO; i++) st.O[i] = float4_t{0.f, 0.f, 0.f, 0.f};
+  st.m = -INFINITY;
+  st.mb = -INFINITY;
+  st.lsum = 0.f;
+  const float lpv = -__log2f(p.pv_scale);
+  const uint64_t hmask = __builtin_amdgcn_ballot_w64(n % slotw < ratio);
+  const uint32_t lanec = (uint32_t)(lane & (LC - 1)) * 4u;
+  auto compute = [&](int i, const StepData<PD>& d, int have) {
+    const int t0 = 2 * kTile * (w + NW * i);  // the step's first token
+    attend_step<PD, PACK, SH>(
+        d, qb, lanec, sm.w.klut,
+        [&]() {
+          return have == 3 && t0 + 2 * kTile <= ws.len &&
+                 (t0 >= ws.h1 || t0 + 2 * kTile <= ws.h0);
+        },
+        [&](int T, int j) {
+          const int t = t0 + kTile * T + j;
+          return ((have >> T) & 1) && t < ws.len && (t >= ws.h1 || t < ws.h0);
+        },
+        n, q4, ptile, hmask, lpv, st);
+  };
+  // the next step's loads go out before a step's math
+  auto next = [&](int i, StepData<PD>& d, int& ok) {
+    if (i < mine) load_step(i, d, ok);
+  };
+  for (int i = 0; i < mine; i += 2) {
+    next(i + 1, d1, ok1);
+    compute(i, d0, ok0);
+    if (i + 1 >= mine) break;
+    next(i + 2, d0, ok0);
+    compute(i + 1, d1, ok1);
+  }
+
+  // ---- the waves' states meet
+  // (column n + 8 accumulated the lo parts of head n's probabilities)
+#pragma unroll
+  for (int i = 0; i < NO; i++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) st.O[i][r] = st.O[i][r] + ror8(st.O[i][r]);
+  float lt = st.lsum;
+  if constexpr (PACK == 2) lt += ror8(lt);
+  lt = xor32_sum(xor16_sum(lt));
+  __syncthreads();  // every wave is done with the table
+  if (n < ratio) {
+    float* dst = &sm.m.o[w][n * PD + q4 * (PD / 4)];
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+      for (int i = 0; i < NO; i += 4)
+        *reinterpret_cast<float4_t*>(dst + r * NO + i) =
+            float4_t{st.O[i][r], st.O[i + 1][r], st.O[i + 2][r], st.O[i + 3][r]};
+    if (q4 == 0) {
+      sm.m.mb[w][n] = st.mb;
+      sm.m.l[w][n] = lt;
+    }
+  }
+  __syncthreads();
+  // o = pv_scale sum_w 2^(mb_w - M) O_w / sum_w 2^(mb_w - M) l_w, rotated back: lane
+  // l of wave w the 8 dims it had of q
+  if (512 * w >= ratio * PD) return;  // uniform
+  const int h = min(e0 / PD, ratio - 1);
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < NW; i++) top = fmaxf(top, sm.m.mb[i][h]);
+  float den = 0.0f, x[8];
+#pragma unroll
+  for (int k = 0; k < 8; k++) x[k] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NW; i++) {
+    const float l = sm.m.l[i][h];
+    if (l == 0.0f) continue;  // a wave that saw nothing (a NaN sum stays)
+    const float f = __builtin_amdgcn_exp2f(sm.m.mb[i][h] - top);
+    const float* src = &sm.m.o[i][min(e0, ratio * PD - 8)];
+    const float4_t a = *reinterpret_cast<const float4_t*>(src);
+    const float4_t c = *reinterpret_cast<const float4_t*>(src + 4);
+    den = __builtin_fmaf(f, l, den);
+#pragma unroll
+    for (int k = 0; k < 8; k++) x[k] = __builtin_fmaf(f, k < 4 ? a[k] : c[k - 4], x[k]);
+  }
+  const float inv = den == 0.0f ? 0.0f : p.pv_scale / den;
+#pragma unroll
+  for (int k = 0; k < 8; k++) x[k] *= inv;
+  if (p.signs) {
+#pragma unroll
+    for (int hh = 1; hh < 8; hh <<= 1)
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        if (!(k & hh)) {
+          const float u = x[k], v = x[k + hh];
+          x[k] = u + v;
+          x[k + hh] = u - v;
+        }
+#pragma unroll
+    for (int m = 1; m < PD / 8; m <<= 1) {
+      const float sg = (lane & m) ? -1.0f : 1.0f;
+#pragma unroll
+      for (int k = 0; k < 8; k++) x[k] = __builtin_fmaf(sg, x[k], xor_lane(x[k], m));
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+      x[k] = __uint_as_float(__float_as_uint(x[k] * p.inv_sqrt_pd) ^ (((sgn >> k) & 1u) << 31));
+  }
+  const int d = e0 % PD;
+  if (!qmine || d >= p.hd) return;
+  u32x4 v;
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const f2 y = {x[2 * k], x[2 * k + 1]};
+    v[k] = o_bf16 ? __builtin_bit_cast(uint32_t, __builtin_convertvector(y, b2))
+                  : __builtin_bit_cast(uint32_t, __builtin_convertvector(y, h2));
+  }
+  u32x2* const o = reinterpret_cast<u32x2*>(static_cast<_Float16*>(out) +
+                                            ((int64_t)b * p.Hq + kvh * ratio + h) * p.hd + d);
+  o[0] = u32x2{v[0], v[1]};
+  o[1] = u32x2{v[2], v[3]};
+}
+
+typedef void (*DirectFn)(DecodeParams, void*, int);
+
+DirectFn direct_kernel(int pd) {
+  return pd == 64    ? &window_direct_kernel<64>
+         : pd == 128 ? &window_direct_kernel<128>
+                     : &window_direct_kernel<256>;
 }
 
 // LDS bytes of a partials workgroup of g kv heads (mirrors RingGeom).
@@ -1788,7 +2131,7 @@ static int combine_splits(const float* partition_o, const float* partition_lse,
                           int32_t batch, int32_t num_splits, const int32_t* split_rows,
                           int32_t max_rows, int32_t num_qo_heads, int32_t padded_dim,
                           const float* signs, void* o, tq_stream_t stream, int32_t row_dim = 0,
-                          bool o_bf16 = false) {
+                          bool o_bf16 = false, bool wide = false) {  // wide: fp32 rows
   if (row_dim == 0) row_dim = padded_dim;
   const int pd = padded_dim;
   if (pd != 64 && pd != 128 && pd != 256) {
@@ -1816,15 +2159,22 @@ static int combine_splits(const float* partition_o, const float* partition_lse,
   dim3 grid((unsigned)blocks), block(256);
   const _Float16* prow = reinterpret_cast<const _Float16*>(partition_o);
   const bool rows = row_dim != pd || o_bf16;
+#define TQ_WIDE(PDV)                                                                             \
+  hipLaunchKernelGGL((combine_kernel<PDV, true, float>), grid, block, 0, st, partition_o,        \
+                     partition_lse, num_splits, split_rows, num_qo_heads, row_dim, (int)o_bf16, out)
 #define TQ_COMBINE(PDV, R)                                                                       \
   hipLaunchKernelGGL((combine_kernel<PDV, R>), grid, block, 0, st, prow, partition_lse, num_splits, \
                      split_rows, num_qo_heads, row_dim, (int)o_bf16, out)
-  if (pd == 64 && rows) TQ_COMBINE(64, true);
+  if (wide && pd == 64) TQ_WIDE(64);
+  else if (wide && pd == 128) TQ_WIDE(128);
+  else if (wide) TQ_WIDE(256);
+  else if (pd == 64 && rows) TQ_COMBINE(64, true);
   else if (pd == 64) TQ_COMBINE(64, false);
   else if (pd == 128 && rows) TQ_COMBINE(128, true);
   else if (pd == 128) TQ_COMBINE(128, false);
   else if (rows) TQ_COMBINE(256, true);
   else TQ_COMBINE(256, false);
+#undef TQ_WIDE
 #undef TQ_COMBINE
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) {
@@ -2187,10 +2537,49 @@ extern "C" int tq_decode_balanced_rows(int32_t batch, int32_t num_qo_heads,
 namespace tq {
 namespace {
 
+// Whether one launch takes a windowed decode: at most 384 tokens in sight (192 at
+// head size 256) and a tile for the borders, and a CU for each workgroup.  us, split
+// form against this: 32 q / 8 kv heads, head size 128, window 128: 11.0 / 9.0 for one
+// sequence, 12.6 / 10.1 for 16, 18.2 / 21.3 for 64 (two workgroups to a CU); window
+// 384: 11.1 / 10.9 for one, 13.8 / 13.4 for 16; 512: 11.3 / 11.6 and 14.9 / 14.7.
+// Head size 64 (16 / 4): window 128 9.2 / 7.2, 12.3 / 9.1 for 64, 384 9.2 / 8.5, 512
+// 9.2 / 9.2.  256 (16 / 2): window 128 13.7 / 12.2, 18.5 / 13.6 for 64, 256 13.8 /
+// 14.9 and 20.4 / 16.9.
+bool window_direct_pays(const DecodeParams& p, int pd) {
+  static_assert(kDirectWaves * 512 >= 8 * 256, "q rows of a workgroup");
+  const int64_t seen = (int64_t)p.window + p.sink;
+  if (p.ratio > 8 || seen > (pd == 256 ? 192 : 384) + kTile) return false;
+  const Occupancy occ = occupancy(reinterpret_cast<const void*>(direct_kernel(pd)), 64 * kDirectWaves);
+  return (int64_t)p.B * p.Hkv <= occ.cus;
+}
+
+// The plan of a windowed decode: fewer units than a balanced plan would have where
+// the work of a window is small.  Merging 16 rows costs the combine about what a step
+// of 32 tokens costs a unit, so a unit takes at least sqrt(steps / 16) steps; a second
+// workgroup on a CU does not pay (of one wave, four do), nor do pairs; beyond a few
+// steps a unit the full, paired plan is ahead.  us, full / this: 32 q / 8 kv heads,
+// head size 128, window 1024: 14.9 / 12.6 for one sequence, 18.8 / 14.5 for 8, 18.9 /
+// 16.6 for 16, 23.9 / 21.0 for 32 (64: 30.4 / 31.1, full taken); 4096: 25.4 / 16.5 for
+// one, 24.0 / 20.6 for 8; 16384: 33.9 / 23.0 for one, 31.0 / 28.9 for 4.  Head size 64
+// (16 / 4): 1024 13.4 / 11.9 for 16, 4096 12.7 / 11.6 for one and 15.5 / 14.2 for 8;
+// 256 (16 / 2): 1024 22.2 / 19.0 for 16, 4096 26.0 / 21.5 for one.
+void window_plan(const DecodeParams& p, int pd, int max_rows, int cus, BalancedGrid& g) {
+  const int64_t steps =
+      ((int64_t)p.window + p.sink + 2 * kTile - 2 + kPlanAlign - 1) / kPlanAlign;  // of a sequence
+  const int64_t room = max((p.G == 1 ? 4 : 1) * cus / p.HG, 1);  // units
+  const int root = max((int)sqrt((double)steps / 16.0), 1);
+  const int64_t k = max((int64_t)root, (p.B * steps + room - 1) / room);
+  const int64_t units = p.B * ((steps + k - 1) / k);
+  if (k > root + (pd == 128 ? 6 : 4) || units > room || units > max_rows) return;
+  g.units = g.rows = (int)units;
+  g.pair_pct = 0;
+  g.blocks = units * p.HG;
+}
+
 // Workspace of a windowed decode of up to kPlanMaxBatch sequences: the row
-// table, the partial LSEs, the partial rows (fp16).
+// table, the partial LSEs, the partial rows (fp32).
 struct WindowWs {
-  int rows;
+  int rows, cus;
   int64_t lse, po, bytes;  // byte offsets, and the whole
 };
 int window_ws(int batch, int hq, int hkv, int pd, WindowWs& w) {
@@ -2212,10 +2601,11 @@ int window_ws(int batch, int hq, int hkv, int pd, WindowWs& w) {
       return kEinval;
     }
     w.rows = max(max(w.rows, occ.cus * occ.per_cu / hg), 2 * (occ.cus / hg));
+    w.cus = occ.cus;
   }
   w.lse = (int64_t)align256((size_t)(b + 2) * 4);
   w.po = w.lse + (int64_t)align256((size_t)w.rows * hq * 4);
-  w.bytes = w.po + (int64_t)w.rows * hq * pd * 2;
+  w.bytes = w.po + (int64_t)w.rows * hq * pd * 4;
   return 0;
 }
 
@@ -2266,6 +2656,17 @@ extern "C" int tq_decode_paged_window(
                         sm_scale, signs, static_cast<float*>(workspace),
                         static_cast<float*>(workspace), p, head_dim, q_dtype == TQ_BF16);
   if (rc || batch == 0) return rc;
+  p.window = window;
+  p.sink = sink;
+  p.entries = num_indices;
+  if (window_direct_pays(p, padded_dim)) {
+    hipLaunchKernelGGL(direct_kernel(padded_dim), dim3((unsigned)(batch * num_kv_heads)),
+                       dim3(64 * kDirectWaves), 0, reinterpret_cast<hipStream_t>(stream), p, o,
+                       (int)(o_dtype == TQ_BF16));
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) set_error("%s: launch failed: %s", who, hipGetErrorString(e));
+    return (int)e;
+  }
   WindowWs w;
   rc = window_ws(batch, num_qo_heads, num_kv_heads, padded_dim, w);
   if (rc) return rc;
@@ -2288,14 +2689,12 @@ extern "C" int tq_decode_paged_window(
     p.B = n;
     p.po = po;
     p.plse = lse;
-    p.window = window;
-    p.sink = sink;
-    p.entries = num_indices;
     const PartialsFn fn =
         window_kernel(padded_dim, p.G, p.ratio, head_dim != padded_dim || p.q_bf16 != 0);
     BalancedGrid g;
     rc = balanced_grid(fn, p, w.rows, g);
     if (rc) return rc;
+    window_plan(p, padded_dim, w.rows, w.cus, g);
     p.S = 1;
     p.cs = 1;
     p.units = g.units;
@@ -2305,7 +2704,7 @@ extern "C" int tq_decode_paged_window(
     if (rc) return rc;
     rc = combine_splits(po, lse, n, 1, table, g.rows, num_qo_heads, padded_dim, signs,
                         static_cast<_Float16*>(o) + (int64_t)a * num_qo_heads * head_dim, stream,
-                        head_dim, o_dtype == TQ_BF16);
+                        head_dim, o_dtype == TQ_BF16, true);
     if (rc) return rc;
   }
   return 0;
