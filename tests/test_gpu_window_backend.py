@@ -168,6 +168,44 @@ def test_more_decode_rows_than_a_plan_takes():
     check_o(c, out, W.decode(c, qx, 20, 0), qx, "fp16", 20, 0)
 
 
+def test_page_starts_of_a_capture_are_its_own():
+    """The first decode of a table's shape inside a capture, an eager one of the
+    same shape in front of any replay, and both on several streams."""
+    impl = TurboQuantFusedImpl(8, 128, 0.09, 2, None, 60, "fp8")
+    c = C.make(9, [300, 40, 111], 8, 2, 128, packed=False)
+    cache = torch.from_numpy(c.cache).to(DEV)
+    table = torch.from_numpy(c.indices.reshape(3, -1)).to(DEV)
+    lens = torch.from_numpy(c.lens).to(DEV)
+    q = torch.randn((3, 8 * 128), device=DEV).half()
+
+    def call(n, pad):
+        tab = torch.nn.functional.pad(table[:n], (0, pad), value=-1)
+        meta = e2e.Meta(1, n, tab, lens[:n], torch.arange(n + 1, dtype=torch.int32, device=DEV), None)
+        return impl.forward(None, q[:n], None, None, cache, meta)
+
+    call(2, 1)  # (what a first call sets up)
+    c.scale, c.signs = 0.09, impl._signs.cpu().numpy()
+    qx = q.view(3, 8, 128).double().cpu().numpy()
+    ref = W.decode(c, qx, 60, 0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            held = call(3, 0)
+        eager = call(3, 0)
+    other = call(3, 0)
+    torch.cuda.synchronize()
+    check_o(c, eager.view(3, 8, 128), ref, qx, "fp16", 60, 0)
+    assert torch.equal(other, eager)
+    for _ in range(3):
+        held.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, eager)
+        assert torch.equal(call(3, 0), eager)
+
+
 def test_without_a_window_nothing_changes():
     """sliding_window None: the calls that the backend made before."""
     impl = TurboQuantFusedImpl(8, 128, 0.09, 2, None, None, "fp8")

@@ -24,6 +24,7 @@ import traceback
 import torch
 import torch.nn.functional as F
 
+from .budget import STARTS_KEPT
 from .decoder_dispatch import KERNEL_NAME, STATIC_KERNEL_NAME
 from .decoder_dispatch import _op as _dispatch_op
 from .geometry import (BALANCED_MAX_BATCH, QUANT_BYTES_PER_CHUNK, TILE_DIMS, choose_splits,
@@ -179,6 +180,7 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
             raise ValueError(f"sliding_window {sliding_window} must be positive")
         self.sink = 0
         self._norm_write_op = self._window_op = None
+        self._starts: dict[tuple[int, int], torch.Tensor] = {}  # of page tables, by shape
 
     # ---------------------------------------------------------------- setup
     @staticmethod
@@ -439,14 +441,24 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
                 and q.stride(1) >= self.head_size and q.data_ptr() % 16 == 0
                 and o.is_contiguous() and o.data_ptr() % 8 == 0)
 
+    def _window_starts(self, table):
+        """Page-table starts of a strided table [n, pages].  Made on the host and
+        copied before the call returns, so that any stream may use them; kept for
+        good, as a graph may hold them, for at most STARTS_KEPT shapes.  A capture
+        makes its own (its memory is the graph's, filled by its replays)."""
+        n, pages = table.shape
+        key = ((n + BALANCED_MAX_BATCH) // BALANCED_MAX_BATCH * BALANCED_MAX_BATCH, pages)
+        starts = self._starts.get(key)
+        if starts is None:
+            if len(self._starts) >= STARTS_KEPT or (
+                    table.is_cuda and torch.cuda.is_current_stream_capturing()):
+                return torch.arange(n + 1, dtype=torch.int32, device=table.device) * pages
+            starts = torch.arange(key[0], dtype=torch.int32) * pages
+            starts = self._starts[key] = starts.to(table.device)
+        return starts[:n + 1]
+
     def _decode_window(self, q, kv_cache, table, seq_lens, out):
         """Windowed decode of one new token per row, q and out [n, Hq, head_size]."""
-        n, pages = q.shape[0], table.shape[1]
-        key = ("window", n, pages)
-        ws = self._v5_ws_cache.get(key)
-        if ws is None:
-            ws = self._v5_ws_cache[key] = {
-                "indptr": torch.arange(n + 1, dtype=torch.int32, device=q.device) * pages}
         half, d = (torch.float16, torch.bfloat16), self.head_size
         o = out
         if q.dtype not in half:
@@ -454,9 +466,9 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
         if d % 8:  # rows that the op does not take
             q, d = F.pad(q, (0, self._pd - d)), self._pd
         if o.dtype not in half or not o.is_contiguous() or d != self.head_size:
-            o = torch.empty((n, self.num_heads, d), dtype=q.dtype, device=q.device)
-        self._window_op(q, kv_cache, table.to(torch.int32).reshape(-1), ws["indptr"],
-                        seq_lens.to(torch.int32).contiguous(), self.num_kv_heads, d, self._pd,
+            o = torch.empty((q.shape[0], self.num_heads, d), dtype=q.dtype, device=q.device)
+        self._window_op(q, kv_cache, table.to(torch.int32).reshape(-1),
+                        self._window_starts(table), seq_lens.to(torch.int32).contiguous(), self.num_kv_heads, d, self._pd,
                         self.scale, self._signs, o, self.window, self.sink)
         if o is not out:
             out.copy_(o[:, :, :self.head_size])
