@@ -2554,10 +2554,12 @@ bool window_direct_pays(const DecodeParams& p, int pd) {
 }
 
 // The plan of a windowed decode: fewer units than a balanced plan would have where
-// the work of a window is small.  Merging 16 rows costs the combine about what a step
-// of 32 tokens costs a unit, so a unit takes at least sqrt(steps / 16) steps; a second
-// workgroup on a CU does not pay (of one wave, four do), nor do pairs; beyond a few
-// steps a unit the full, paired plan is ahead.  us, full / this: 32 q / 8 kv heads,
+// the work of a window is small (the kernel shares the real lengths out among them,
+// so short sequences make a unit smaller).  Merging 16 rows costs the combine about
+// what a step of 32 tokens costs a unit, so a unit takes at least sqrt(steps / 16)
+// steps; a second workgroup on a CU does not pay (of one wave, four do), nor do pairs
+// (16 ragged sequences, window 1000: 16.8 us with 192 units, 15.9 with 256 to 448,
+// 19.8 with 512); beyond a few steps a unit the full, paired plan is ahead.  us, full / this: 32 q / 8 kv heads,
 // head size 128, window 1024: 14.9 / 12.6 for one sequence, 18.8 / 14.5 for 8, 18.9 /
 // 16.6 for 16, 23.9 / 21.0 for 32 (64: 30.4 / 31.1, full taken); 4096: 25.4 / 16.5 for
 // one, 24.0 / 20.6 for 8; 16384: 33.9 / 23.0 for one, 31.0 / 28.9 for 4.  Head size 64
@@ -2568,9 +2570,9 @@ void window_plan(const DecodeParams& p, int pd, int max_rows, int cus, BalancedG
       ((int64_t)p.window + p.sink + 2 * kTile - 2 + kPlanAlign - 1) / kPlanAlign;  // of a sequence
   const int64_t room = max((p.G == 1 ? 4 : 1) * cus / p.HG, 1);  // units
   const int root = max((int)sqrt((double)steps / 16.0), 1);
-  const int64_t k = max((int64_t)root, (p.B * steps + room - 1) / room);
-  const int64_t units = p.B * ((steps + k - 1) / k);
-  if (k > root + (pd == 128 ? 6 : 4) || units > room || units > max_rows) return;
+  const int64_t k = max((int64_t)root, (p.B * steps + room - 1) / room);  // steps of a unit
+  const int64_t units = min(room, p.B * ((steps + root - 1) / root));
+  if (k > root + (pd == 128 ? 6 : 4) || units < p.B || units > max_rows) return;
   g.units = g.rows = (int)units;
   g.pair_pct = 0;
   g.blocks = units * p.HG;
