@@ -409,8 +409,11 @@ __device__ __forceinline__ void recompute_rows(const PP& p, const PrefillWork& w
         for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
         if (__builtin_amdgcn_ballot_w64(seen) == 0) continue;
         const float mn = fmaxf(m, top);
-        const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * p.c);
-        const float pr = seen ? __builtin_amdgcn_exp2f((sc - mn) * p.c) : 0.0f;
+        // (0 while every score so far is -inf, as in the tiles: such a key weighs
+        // nothing, where -inf from -inf would be NaN; a NaN score stays NaN)
+        const float base = mn == -INFINITY ? 0.0f : mn;
+        const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - base) * p.c);
+        const float pr = seen ? __builtin_amdgcn_exp2f((sc - base) * p.c) : 0.0f;
         float sum = pr;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
