@@ -2,12 +2,18 @@
 finite, against the formulas in 64 bits."""
 from __future__ import annotations
 
+import copy
 import math
 
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_window_prefill import DEV, call, check, make
+import budget_cases as C
+import test_gpu_window as D
+import window_cases as W
+from test_gpu_budget import queries, tensors
+from test_gpu_window_prefill import call, check, make
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +41,67 @@ def test_prefill_hidden_values_beside_scores_of_minus_infinity(hq, hkv, hd, n, c
     o = call(q, k, v, reqs, hd, window, sink)
     check(o, q, k, v, reqs, window, sink, 1 / math.sqrt(hd), hd)
     assert torch.isnan(o[:, 0, 3]).any() and torch.isfinite(o[:, 0, 4]).all()
+
+
+def norms(c, slab, value):
+    """A copy of the case with those K or V norms: value(norms fp16 [nb, page, H])."""
+    out = copy.copy(c)
+    out.cache = c.cache.copy()
+    at = out.cache[slab, ..., c.pd // 2:c.pd // 2 + 2 * (c.pd // 64)]
+    new = value(at[..., :2].copy().view(np.float16)[..., 0]).astype(np.float16)
+    at[:] = np.repeat(new[..., None], c.pd // 64, -1).view(np.uint8)
+    return out
+
+
+def decode_by_norms(c, q, window, sink):
+    """window_cases.decode with a score as the K norm times its unit row's product,
+    so that an infinite norm gives an infinite score."""
+    unit, r = norms(c, 0, np.ones_like), c.hq // c.hkv
+    o = np.zeros((len(c.lens), c.hq, c.pd))
+    for b, n in enumerate(c.lens):
+        pg, off, ok = C.places(c, b)
+        see = ok & W.sees(int(n) - 1, len(pg), window, sink)
+        pg, off = pg[see], off[see]
+        for h in range(c.hkv):
+            k = c.cache[0, pg, off, h, c.pd // 2:c.pd // 2 + 2].copy().view(np.float16)[:, 0]
+            s = C.rotated(c, q[b, h * r:(h + 1) * r], True) @ C.rows(unit, 0, pg, off, h).T \
+                * k.astype(np.float64) * c.scale
+            p = np.exp(s - s.max(-1, keepdims=True))
+            o[b, h * r:(h + 1) * r] = p / p.sum(-1, keepdims=True) @ C.rows(c, 1, pg, off, h)
+    return ((o @ C.hadamard(c.pd)) * c.signs)[..., :c.hd]
+
+
+@pytest.mark.parametrize("hq,hkv,hd", [(8, 2, 128), (16, 4, 64), (16, 2, 256), (16, 1, 128),
+                                       (32, 2, 128), (8, 8, 256), (16, 8, 64)])
+@pytest.mark.parametrize("lens,window,sink", [
+    ([193, 65, 333], 300, 4), ([161, 345], 130, 1),    # one launch (up to 8 q heads a kv head)
+    ([3009, 2500, 40], 2000, 4), ([193, 34, 353] * 14, 150, 0)])
+@pytest.mark.parametrize("tail", [False, True])
+def test_decode_scores_of_minus_infinity(hq, hkv, hd, lens, window, sink, tail):
+    """Keys with an infinite norm and a negative product weigh nothing, also where a
+    step, a wave's first one or a whole unit holds no others: the newest tokens
+    alone (tail), or all but the newest ones."""
+    c = C.make(hq + hd + len(lens), lens, hq, hkv, hd)
+    q, _ = queries(c, len(lens), "fp16")
+    qx = q.double().cpu().numpy()
+    bad = np.zeros((c.nb, c.page), bool)
+    for b, n in enumerate(c.lens):
+        # one entry of each head in all the places, that whose products are furthest from 0
+        pg, off, _ = C.places(c, b)
+        at = slice((int(n) - 1) // 32 * 32, None) if tail else slice(0, int(n) - 3)
+        bad[pg[at], off[at]] = True
+        r = hq // hkv
+        for h in range(hkv):
+            k = C.rows(c, 0, pg, off, h)
+            k /= np.linalg.norm(k, axis=-1, keepdims=True)
+            x = C.rotated(c, qx[b, h * r:(h + 1) * r], True)
+            dot = x / np.linalg.norm(x, axis=-1, keepdims=True) @ k.T
+            best = int(np.abs(dot).min(0).argmax())
+            assert np.abs(dot[:, best]).min() > 2e-3  # (far from what the kernel rounds)
+            c.cache[0, pg[at], off[at], h] = c.cache[0, pg[best], off[best], h]
+            q[b, h * r:(h + 1) * r] *= torch.from_numpy(-np.sign(dot[:, best]))[:, None].to(q)
+    qx = q.double().cpu().numpy()
+    c = norms(c, 0, lambda x: np.where(bad[..., None], np.inf, x))
+    o = D.call(c, tensors(c), q, torch.full_like(q, 7.0), window, sink)
+    D.check_o(norms(c, 0, lambda x: np.where(np.isfinite(x), x, 0)), o,
+              decode_by_norms(c, qx, window, sink), qx, "fp16", window, sink)

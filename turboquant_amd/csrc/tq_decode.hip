@@ -538,6 +538,13 @@ __device__ __forceinline__ uint32_t mix_pair_lo(float a, uint32_t na, float b, u
   return r;
 }
 
+// SoftmaxState::mb in front of the first score above -inf.  The lowest finite
+// value takes part in no sum: a score above -inf sets mb first.
+template <bool INF>
+__device__ __forceinline__ constexpr float no_reference() {
+  return INF ? -3.402823466e+38f : -INFINITY;
+}
+
 // Online softmax over the NV score values this lane holds for one step
 // (PACK 2: 4 values, tile (l%16)/8, head l%8; PACK 1: 8 values, tile 0 then
 // tile 1, head l%16; tokens 4*q4 + r), already scaled by the K norms.  nvr:
@@ -545,7 +552,10 @@ __device__ __forceinline__ uint32_t mix_pair_lo(float a, uint32_t na, float b, u
 // all are valid (uniform); hmask: the lanes of real heads (head < ratio).
 // Writes p * nv as fp16 pairs to pw; the running
 // max only moves when the step exceeds it by more than 2^3, so p <= 8.
-template <int PD, int NV, bool LO = false>
+// INF (windowed kernels, whose states start from no_reference<true>()): scores
+// of -inf (an infinite K norm) weigh nothing also while a head has no others;
+// otherwise -inf from a reference of -inf makes its sum NaN.
+template <int PD, int NV, bool LO = false, bool INF = false>
 __device__ __forceinline__ void softmax_step(float* sc, const uint32_t* nvr, bool full,
                                              const bool* valid, bool rot8, uint64_t hmask,
                                              float lpv, SoftmaxState<PD>& st, uint32_t* pw,
@@ -568,7 +578,7 @@ __device__ __forceinline__ void softmax_step(float* sc, const uint32_t* nvr, boo
     for (int i = 0; i < NO; i++) st.O[i] *= alpha;
     st.lsum *= alpha;
     st.m = m_new;
-    st.mb = m_new + lpv;
+    st.mb = INF ? fmaxf(m_new + lpv, no_reference<true>()) : m_new + lpv;
   }
   float pr[NV];
 #pragma unroll
@@ -674,7 +684,7 @@ __device__ __forceinline__ void attend_step(const StepData<PD>& d, const half8_t
     }
   }
   uint32_t pw[NV / 2], pl[NV / 2];
-  softmax_step<PD, NV, true>(sc, nvr, full, valid, PACK == 2, hmask, lpv, st, pw, pl);
+  softmax_step<PD, NV, true, true>(sc, nvr, full, valid, PACK == 2, hmask, lpv, st, pw, pl);
   // columns n >= 8 take the lo parts of head n - 8's probabilities
   const bool up = n >= 8;
   half8_t p8;
@@ -918,7 +928,7 @@ void decode_partials_kernel(DecodeParams p) {
 #pragma unroll
   for (int i = 0; i < NO; i++) st.O[i] = float4_t{0.f, 0.f, 0.f, 0.f};
   st.m = -INFINITY;
-  st.mb = -INFINITY;
+  st.mb = no_reference<WIN>();
   st.lsum = 0.f;
   const float lpv = -__log2f(p.pv_scale);
 
@@ -1275,7 +1285,7 @@ void decode_partials_kernel(DecodeParams p) {
         }
       }
       uint32_t pw[NV / 2], pl[NV / 2];
-      softmax_step<PD, NV, PLO>(sc, nvr, full, valid, PACK == 2, hmask, lpv, st, pw, pl);
+      softmax_step<PD, NV, PLO, WIN>(sc, nvr, full, valid, PACK == 2, hmask, lpv, st, pw, pl);
       half8_t p8;
       if constexpr (PACK == 2 && PLO) {
         // lanes n < 8: hi parts of tile 0 (own) and tile 1 (lane n + 8);
@@ -1754,7 +1764,7 @@ __global__ __launch_bounds__(64 * NW) void window_direct_kernel(DecodeParams p, 
 #pragma unroll
   for (int i = 0; i < NO; i++) st.O[i] = float4_t{0.f, 0.f, 0.f, 0.f};
   st.m = -INFINITY;
-  st.mb = -INFINITY;
+  st.mb = no_reference<true>();
   st.lsum = 0.f;
   const float lpv = -__log2f(p.pv_scale);
   const uint64_t hmask = __builtin_amdgcn_ballot_w64(n % slotw < ratio);
