@@ -422,6 +422,16 @@ def test_backend_windows():
             make(bad)
 
 
+@pytest.mark.parametrize("window", [None, 0, -1, 128, (127, 0)])
+@pytest.mark.parametrize("dtype", ["auto", "bfloat16"])
+def test_windows_of_an_unpacked_cache_are_the_parents(window, dtype):
+    """Such a layer takes whatever its parent takes; the window of the packed
+    cache's calls is not looked at."""
+    from turboquant_amd.vllm_backend_fused import TurboQuantFusedImpl
+    impl = TurboQuantFusedImpl(4, 64, 0.125, 2, None, window, dtype)
+    assert impl.window == 0 and impl.sliding_window == window
+
+
 def test_a_record_does_not_go_with_a_window():
     from turboquant_amd import e2e
     from turboquant_amd.budget import CacheRecord

@@ -175,9 +175,12 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
         # a budget.CacheRecord beside this layer's cache: forward fills it
         self.record = None
         # tokens a query sees (0: all), and first tokens that stay visible
-        self.window = 0 if sliding_window is None else int(sliding_window)
-        if sliding_window is not None and self.window < 1:
-            raise ValueError(f"sliding_window {sliding_window} must be positive")
+        # (an unpacked cache is the parent's, windows and all)
+        self.window = 0
+        if self._is_fp8 and sliding_window is not None:
+            self.window = int(sliding_window)
+            if self.window < 1:
+                raise ValueError(f"sliding_window {sliding_window} must be positive")
         self.sink = 0
         self._norm_write_op = self._window_op = None
         self._starts: dict[tuple[int, int], torch.Tensor] = {}  # of page tables, by shape
