@@ -432,6 +432,20 @@ def test_windows_of_an_unpacked_cache_are_the_parents(window, dtype):
     assert impl.window == 0 and impl.sliding_window == window
 
 
+def test_starts_of_a_traced_call_are_not_kept():
+    """A call over fake tensors leaves nothing that a later call would get."""
+    from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
+    from turboquant_amd.vllm_backend_fused import TurboQuantFusedImpl
+    impl = TurboQuantFusedImpl(4, 64, 0.125, 2, None, 8, "fp8")
+    with FakeTensorMode():
+        fake = impl._window_starts(torch.empty((3, 7), dtype=torch.int32))
+    assert isinstance(fake, FakeTensor) and fake.shape == (4,)
+    starts = impl._window_starts(torch.empty((3, 7), dtype=torch.int32))
+    assert type(starts) is torch.Tensor and starts.tolist() == [0, 7, 14, 21]
+    with FakeTensorMode():  # nor does it get theirs
+        assert isinstance(impl._window_starts(torch.empty((3, 7), dtype=torch.int32)), FakeTensor)
+
+
 def test_a_record_does_not_go_with_a_window():
     from turboquant_amd import e2e
     from turboquant_amd.budget import CacheRecord

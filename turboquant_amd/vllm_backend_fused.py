@@ -448,12 +448,14 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
         """Page-table starts of a strided table [n, pages].  Made on the host and
         copied before the call returns, so that any stream may use them; kept for
         good, as a graph may hold them, for at most STARTS_KEPT shapes.  A capture
-        makes its own (its memory is the graph's, filled by its replays)."""
+        makes its own (its memory is the graph's, filled by its replays), and so does
+        a traced call, whose tensors mean nothing to a later one."""
         n, pages = table.shape
         key = ((n + BALANCED_MAX_BATCH) // BALANCED_MAX_BATCH * BALANCED_MAX_BATCH, pages)
-        starts = self._starts.get(key)
+        traced = torch.compiler.is_compiling() or type(table) is not torch.Tensor
+        starts = None if traced else self._starts.get(key)
         if starts is None:
-            if len(self._starts) >= STARTS_KEPT or (
+            if traced or len(self._starts) >= STARTS_KEPT or (
                     table.is_cuda and torch.cuda.is_current_stream_capturing()):
                 return torch.arange(n + 1, dtype=torch.int32, device=table.device) * pages
             starts = torch.arange(key[0], dtype=torch.int32) * pages
