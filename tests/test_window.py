@@ -446,6 +446,17 @@ def test_starts_of_a_traced_call_are_not_kept():
         assert isinstance(impl._window_starts(torch.empty((3, 7), dtype=torch.int32)), FakeTensor)
 
 
+def test_starts_are_made_on_the_host_whatever_the_default_device():
+    """(a default device of "cuda" would make them on the current stream, which
+    another stream's first call does not wait for; "meta" shows it without a GPU)"""
+    from turboquant_amd.vllm_backend_fused import TurboQuantFusedImpl
+    impl = TurboQuantFusedImpl(4, 64, 0.125, 2, None, 8, "fp8")
+    table = torch.empty((3, 7), dtype=torch.int32)
+    with torch.device("meta"):
+        starts = impl._window_starts(table)
+    assert starts.device == table.device and starts.tolist() == [0, 7, 14, 21]
+
+
 def test_a_record_does_not_go_with_a_window():
     from turboquant_amd import e2e
     from turboquant_amd.budget import CacheRecord

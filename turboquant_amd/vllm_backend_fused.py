@@ -458,7 +458,7 @@ class TurboQuantFusedImpl(FlashAttentionImpl):
             if traced or len(self._starts) >= STARTS_KEPT or (
                     table.is_cuda and torch.cuda.is_current_stream_capturing()):
                 return torch.arange(n + 1, dtype=torch.int32, device=table.device) * pages
-            starts = torch.arange(key[0], dtype=torch.int32) * pages
+            starts = torch.arange(key[0], dtype=torch.int32, device="cpu") * pages
             starts = self._starts[key] = starts.to(table.device)
         return starts[:n + 1]
 
