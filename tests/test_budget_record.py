@@ -116,3 +116,16 @@ def test_a_batch_that_cannot_be_recorded_is_refused(missing, most):
         impl.forward(None, q, kv, kv, None if missing == "kv_cache" else cache, meta)
     # without metadata nothing is cached (a profiling pass): nothing to record
     assert torch.equal(impl.forward(None, q, kv, kv, None, None), torch.zeros_like(q))
+
+
+def test_starts_of_a_traced_call_are_not_kept():
+    """A call over fake tensors leaves nothing that a later call would get, and gets
+    nothing of an earlier one."""
+    from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
+    r, table = record(), torch.zeros((3, 7), dtype=torch.int32)
+    for _ in range(2):
+        with FakeTensorMode():
+            fake = r._tables(torch.empty((3, 7), dtype=torch.int32))[1]
+        assert isinstance(fake, FakeTensor) and fake.shape == (4,)
+        starts = r._tables(table)[1]
+        assert type(starts) is torch.Tensor and starts.tolist() == [0, 7, 14, 21]

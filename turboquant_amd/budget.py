@@ -59,8 +59,10 @@ class CacheRecord:
         if block_table.dtype != torch.int32 or not block_table.is_contiguous():
             block_table = block_table.to(torch.int32).contiguous()
         b, width = key = tuple(block_table.shape)
-        if self._last is None or self._last[0] != key:
-            starts = self._starts_of(width, b, block_table)
+        traced = torch.compiler.is_compiling() or type(block_table) is not torch.Tensor
+        if traced or self._last is None or self._last[0] != key:
+            # (a traced call's tensors mean nothing to a later one)
+            starts = None if traced else self._starts_of(width, b, block_table)
             if starts is None:  # this call's own, on its stream
                 return block_table.reshape(-1), torch.arange(
                     b + 1, dtype=torch.int32, device=block_table.device) * width
