@@ -129,3 +129,12 @@ def test_starts_of_a_traced_call_are_not_kept():
         assert isinstance(fake, FakeTensor) and fake.shape == (4,)
         starts = r._tables(table)[1]
         assert type(starts) is torch.Tensor and starts.tolist() == [0, 7, 14, 21]
+
+
+def test_starts_are_made_on_the_host_whatever_the_default_device():
+    """(a default device of "cuda" would make them on the current stream, which
+    another stream's first call does not wait for; "meta" shows it without a GPU)"""
+    r, table = record(), torch.zeros((3, 7), dtype=torch.int32)
+    with torch.device("meta"):
+        starts = r._tables(table)[1]
+    assert starts.device == table.device and starts.tolist() == [0, 7, 14, 21]

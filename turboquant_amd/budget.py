@@ -79,7 +79,8 @@ class CacheRecord:
         starts = self._starts.get(width)
         if starts is None and len(self._starts) < STARTS_KEPT and not (
                 block_table.is_cuda and torch.cuda.is_current_stream_capturing()):
-            starts = torch.arange(BALANCED_MAX_BATCH + 1, dtype=torch.int32) * width
+            starts = torch.arange(BALANCED_MAX_BATCH + 1, dtype=torch.int32,
+                                  device="cpu") * width
             starts = self._starts[width] = starts.to(block_table.device)
         return starts
 
