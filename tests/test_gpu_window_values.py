@@ -105,3 +105,32 @@ def test_decode_scores_of_minus_infinity(hq, hkv, hd, lens, window, sink, tail):
     o = D.call(c, tensors(c), q, torch.full_like(q, 7.0), window, sink)
     D.check_o(norms(c, 0, lambda x: np.where(np.isfinite(x), x, 0)), o,
               decode_by_norms(c, qx, window, sink), qx, "fp16", window, sink)
+
+
+@pytest.mark.parametrize("hq,hkv,hd", [(32, 8, 128), (16, 4, 64)])
+@pytest.mark.parametrize("where", ["q", "k"])
+def test_prefill_of_nan_scores_takes_its_usual_time(hq, hkv, hd, where):
+    """Rows that their own scores make NaN are not computed a second time, one by
+    one (which took 140 times as long)."""
+    n, window, sink = 4096, 1024, 4
+    q, k, v, reqs = make(1, [(n, n)], hq, hkv, hd)
+
+    def time():
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        o = call(q, k, v, reqs, hd, window, sink)
+        best = math.inf
+        for _ in range(5):
+            start.record()
+            call(q, k, v, reqs, hd, window, sink, o)
+            end.record()
+            torch.cuda.synchronize()
+            best = min(best, start.elapsed_time(end))
+        return best, o
+    usual, o = time()
+    assert torch.isfinite(o).all()
+    if where == "q":
+        q[:] = math.nan
+    else:
+        k[0], v[0] = math.nan, math.nan
+    spent, o = time()
+    assert torch.isnan(o).all() and spent < 5 * usual

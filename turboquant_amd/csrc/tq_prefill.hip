@@ -368,10 +368,14 @@ __device__ __forceinline__ bool behind_window(int kb, int wpos, int window, int 
 // cores.  A tile's V rows enter the MFMAs for all of the wave's rows, those that
 // a row does not see with probability 0, and 0 times a NaN or an infinity is
 // NaN; here a row takes the keys in its sight alone (over this workgroup's
-// tiles).  So a row is NaN only if what it sees makes it so.  Such rows are rare:
-// the check costs a sum over the outputs.  rows: bit i: row row0 + i of the
-// request; store(row, dims V lane .. + V - 1 of O / sum, reference max in log2
-// units, sum).
+// tiles).  So a row is NaN only if what it sees makes it so.  A row whose own sum
+// is NaN (hidden keys add nothing to that) is not among them: a score in its
+// sight is NaN, and so is all of it.  Such rows are rare: the check costs a sum
+// over the outputs.  One at a time they are slow, 64 keys about 10 us a wave: with
+// a value that is not finite among the first keys of 4096 tokens (32 / 8 heads of
+// 128, window 1024) 13 ms for 0.094; rows of NaN queries or keys were as slow
+// before they were left out.  rows: bit i: row row0 + i of the request; store(row,
+// dims V lane .. + V - 1 of O / sum, reference max in log2 units, sum).
 template <int kD, int kBN, class PP, class Store>
 __device__ __forceinline__ void recompute_rows(const PP& p, const PrefillWork& wk, int head, int g,
                                                int row0, uint32_t rows, Store store) {
@@ -745,7 +749,7 @@ void prefill_kernel(PP p) {
     for (int d = 0; d < kD / 32; d++)
 #pragma unroll
       for (int j = 0; j < 16; j++) z = __builtin_fmaf(oacc[d][j], 0.0f, z);
-    const uint64_t bad = __builtin_amdgcn_ballot_w64(z != z && qrow < wk.lq);
+    const uint64_t bad = __builtin_amdgcn_ballot_w64(z != z && lsum == lsum && qrow < wk.lq);
     again = (uint32_t)(bad | bad >> 32);
   }
   const bool mine = qrow < wk.lq && !(kWindowed<PP> && (again >> n & 1u));
@@ -1060,7 +1064,7 @@ void prefill_rb_kernel(PP p) {
       for (int d = 0; d < kD / 32; d++)
 #pragma unroll
         for (int j = 0; j < 16; j++) z = __builtin_fmaf(oacc[rb][d][j], 0.0f, z);
-      const uint64_t bad = __builtin_amdgcn_ballot_w64(z != z && qrow < wk.lq);
+      const uint64_t bad = __builtin_amdgcn_ballot_w64(z != z && ls == ls && qrow < wk.lq);
       again = (uint32_t)(bad | bad >> 32);
     }
     if (qrow < wk.lq && !(kWindowed<PP> && (again >> n & 1u))) {
