@@ -134,3 +134,32 @@ def test_prefill_of_nan_scores_takes_its_usual_time(hq, hkv, hd, where):
         k[0], v[0] = math.nan, math.nan
     spent, o = time()
     assert torch.isnan(o).all() and spent < 5 * usual
+
+
+# the levels as the decode's table holds them: fp16 of 1.48098 times each, read as
+# multiples of that
+TABLE = (C.LEVELS * 1.4809800386428833).astype(np.float16).astype(np.float64) / 1.4809800386428833
+
+
+@pytest.mark.parametrize("hq,hkv,hd", [(8, 2, 128), (16, 2, 64), (16, 2, 256), (8, 8, 128),
+                                       (12, 6, 96)])
+@pytest.mark.parametrize("many", [False, True])
+def test_decode_of_one_token_is_its_value(monkeypatch, hq, hkv, hd, many):
+    """Up to 8 q heads a kv head a probability enters as an fp16 pair and partial
+    rows are fp32: a window of one token gives its V row (of the table's levels) to
+    the output's rounding, 2^-11, and in front of it the pair's 2^-22 and fp32
+    sums, 64 u, relative to the row, which the rotation back keeps.  One launch,
+    and the split form for more workgroups than it takes (many)."""
+    monkeypatch.setattr(C, "LEVELS", TABLE)
+    lens = [(37 * i) % 90 + 1 for i in range(300 if many else 3)]
+    c = C.make(hq + hd, lens, hq, hkv, hd)
+    q, qx = queries(c, len(lens), "fp16")
+    o = D.call(c, tensors(c), q, torch.full_like(q, 7.0), 1, 0).double().cpu().numpy()
+    ref = W.decode(c, qx, 1, 0)
+    at = [(C.places(c, b)[0][-1], C.places(c, b)[1][-1]) for b in range(len(lens))]
+    size = np.stack([[np.linalg.norm(C.rows(c, 1, [pg], [off], h)) for h in range(hkv)]
+                     for pg, off in at])
+    tol = 2.0 ** -11 * np.abs(ref) + 2.0 ** -25 + \
+        (2.0 ** -22 + 64 * 2.0 ** -24) * np.repeat(size, hq // hkv, 1)[..., None]
+    err = np.abs(o - ref)
+    assert (err <= tol).all(), f"off by {err.max():.3e}, {(err / tol).max():.2f} x bound"
