@@ -163,3 +163,26 @@ def test_decode_of_one_token_is_its_value(monkeypatch, hq, hkv, hd, many):
         (2.0 ** -22 + 64 * 2.0 ** -24) * np.repeat(size, hq // hkv, 1)[..., None]
     err = np.abs(o - ref)
     assert (err <= tol).all(), f"off by {err.max():.3e}, {(err / tol).max():.2f} x bound"
+
+
+@pytest.mark.parametrize("hq,hkv,hd", [(8, 2, 128), (16, 1, 64), (16, 2, 256)])
+@pytest.mark.parametrize("lens,window", [([70, 200], 300), ([3000, 40], 2000)])
+def test_rows_whose_every_score_is_minus_infinity_are_zeros(hq, hkv, hd, lens, window):
+    """As the plain kernels leave them (their softmax has no value)."""
+    c = C.make(5, lens, hq, hkv, hd)
+    c.cache[0] = c.cache[0, :1, :1]  # (one entry a head, and so one sign of its products)
+    c = norms(c, 0, lambda x: np.full_like(x, np.inf))
+    unit = norms(c, 0, np.ones_like)
+    q, qx = queries(c, len(lens), "fp16")
+    for h in range(hkv):
+        dot = C.rotated(c, qx[:, h * hq // hkv:(h + 1) * hq // hkv], True) @ \
+            C.rows(unit, 0, [0], [0], h)[0]
+        q[:, h * hq // hkv:(h + 1) * hq // hkv] *= torch.from_numpy(-np.sign(dot))[..., None].to(q)
+    o = D.call(c, tensors(c), q, torch.full_like(q, 7.0), window, 2)
+    assert (o == 0).all()
+    # prefill: the first rows see the keys of the infinity alone
+    q, k, v, reqs = make(3, [(lens[0], lens[0]), (3, 9000)], hq, hkv, hd)
+    scores_of_minus_infinity(q, k, [0, 1, 2, *range(len(k) - 9000, len(k))])
+    v[40, :, 1] = math.nan
+    o = call(q, k, v, reqs, hd, window, 2)
+    assert (o[:3] == 0).all() and (o[-3:] == 0).all() and torch.isfinite(o[3:40]).all()
