@@ -260,6 +260,19 @@ def test_prefill_workspace_follows_the_window():
         lib.tq_prefill_batch_workspace_bytes(_ints(100), _ints(20000), 1, 4, 128)
 
 
+def test_abi_names_the_workspace_that_is_too_small():
+    """(refused in front of the launch; the addresses are never read)"""
+    lib = _lib.load()
+    buf, p = _buffer()
+    size = lib.tq_prefill_window_workspace_bytes(_ints(100), _ints(20000), 1, 4, 128, 19000, 0)
+    assert size > 0
+    rc = lib.tq_prefill_attention_window(
+        p, 512, 128, 1, p, 256, 128, p, 256, 128, None, None, 0, 0, p, 512, 128, 1, _ints(0),
+        _ints(100), _ints(0), _ints(20000), _ints(0), 1, 4, 2, 128, 128, 0.1, 19000, 0, p, size - 1,
+        None)
+    assert rc == -22 and b"tq_prefill_window_workspace_bytes" in lib.tq_last_error()
+
+
 @pytest.mark.parametrize("bad,match", [
     (dict(sink=-1), b"negative"), (dict(first=None), b"null"), (dict(first=(41,)), b"bad request"),
     (dict(first=(-1,)), b"bad request"), (dict(ctx=(-1,), first=(-1,)), b"bad request"),

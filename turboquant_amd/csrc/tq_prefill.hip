@@ -1650,7 +1650,8 @@ int attention_batch(
       const BatchPlan bp = plan_batch(q_lens + a, kv_lens + a, n, num_qo_heads, padded_dim,
                                       window, sink);
       if (batch_ws_bytes(bp, num_qo_heads, padded_dim) > (workspace ? workspace_bytes : 0)) {
-        set_error("%s: workspace smaller than tq_prefill_batch_workspace_bytes", what);
+        set_error("%s: workspace smaller than tq_prefill_%s_workspace_bytes", what,
+                  window > 0 ? "window" : "batch");
         return kEinval;
       }
       p.ws_o = static_cast<float*>(workspace);
