@@ -231,7 +231,8 @@ int tq_decode_balanced_rows(int32_t batch, int32_t num_qo_heads, int32_t num_kv_
  * hold anything; num_indices is the length of `indices`, and tokens whose
  * entry lies outside [0, num_indices), or names a page outside [0,
  * num_blocks), count as absent.  A sequence without a token in sight gets a row
- * of zeros.  The tokens in sight of any 1024 consecutive sequences add up to
+ * of zeros, and so does a head whose every score is -inf (K norms that are
+ * infinite); a single such token weighs nothing.  The tokens in sight of any 1024 consecutive sequences add up to
  * less than 2^30.  The workspace (any device memory of the given size, 16-byte
  * aligned) serves one call at a time and holds nothing between calls; equal
  * inputs give equal bits.
@@ -515,9 +516,11 @@ int tq_prefill_attention_batch(
  * stand, so the rows that tq_prefill_gather_window closes up serve as they are:
  * behind the sinks a key's distance from a query does not change.  Key tiles
  * out of sight are not read, and a key that a query does not see does not
- * touch its row, whatever its K and V hold (NaN and infinities too).  window
- * >= 1, sink >= 0, sm_scale > 0; bf16 queries in fp16's range.  The workspace
- * must hold tq_prefill_window_workspace_bytes.
+ * touch its row, whatever its K and V hold (NaN and infinities too).  Rows with a
+ * value that is not finite in V among their key tiles, hidden or seen, are
+ * computed one by one, more than a hundred times as slowly.  A row whose every
+ * score is -inf is zeros.  window >= 1, sink >= 0, sm_scale > 0; bf16 queries in fp16's range.  The
+ * workspace must hold tq_prefill_window_workspace_bytes.
  */
 int64_t tq_prefill_window_workspace_bytes(const int32_t* q_lens, const int32_t* kv_lens,
                                           int32_t num_requests, int32_t num_qo_heads,

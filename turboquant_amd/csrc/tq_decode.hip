@@ -757,7 +757,8 @@ void decode_partials_kernel(DecodeParams p) {
   constexpr int ECH = RG::ECH;
   constexpr int CPT = RG::CPT;
   constexpr int NI = RG::NI;
-  // PV probabilities as hi + lo (windowed: always; 1 .. 2% of a launch)
+  // PV probabilities as hi + lo (windowed, up to 8 q heads a kv head: 1 .. 2% of a
+  // launch; more heads leave no free columns, and theirs are single fp16 values)
   constexpr bool PLO = QC && (kPvLo || WIN) && MATH >= 2;
   // LDS: the dequant table at address 0 (the table reads rely on it), then
   // the ring of tile slots
@@ -1401,7 +1402,8 @@ void decode_partials_kernel(DecodeParams p) {
   // (relative 2^-11 on normalised outputs) is far inside the output
   // tolerance.  Windowed rows, of which window_plan makes few, stay fp32: with
   // the lo parts of the probabilities that takes the rms error from 1.9 times
-  // that of the output's own rounding to 1.2.
+  // that of the output's own rounding to 1.2 (1.4 without them, above 8 q heads a
+  // kv head).
   _Float16* const out = reinterpret_cast<_Float16*>(p.po) + orow0 * PD;
   for (int e = 8 * lane; e < ratio * PD; e += 512) {
     const float4_t a = *reinterpret_cast<const float4_t*>(stage + e);
@@ -2549,12 +2551,14 @@ namespace {
 
 // Whether one launch takes a windowed decode: at most 384 tokens in sight (192 at
 // head size 256) and a tile for the borders, and a CU for each workgroup.  us, split
-// form against this: 32 q / 8 kv heads, head size 128, window 128: 11.0 / 9.0 for one
-// sequence, 12.6 / 10.1 for 16, 18.2 / 21.3 for 64 (two workgroups to a CU); window
-// 384: 11.1 / 10.9 for one, 13.8 / 13.4 for 16; 512: 11.3 / 11.6 and 14.9 / 14.7.
-// Head size 64 (16 / 4): window 128 9.2 / 7.2, 12.3 / 9.1 for 64, 384 9.2 / 8.5, 512
-// 9.2 / 9.2.  256 (16 / 2): window 128 13.7 / 12.2, 18.5 / 13.6 for 64, 256 13.8 /
-// 14.9 and 20.4 / 16.9.
+// form against this: 32 q / 8 kv heads, head size 128, window 128: 10.8 / 8.8 for one
+// sequence, 12.0 / 9.0 for 16, 18.2 / 21.3 for 64 (two workgroups to a CU); window
+// 384: 11.0 / 10.6 for one, 13.3 / 12.1 for 16; 512: 11.0 / 11.3 and 14.3 / 13.4.
+// Head size 64 (16 / 4): window 128 9.0 / 6.8, 11.6 / 7.3 for 64, 384 9.0 / 8.1, 512
+// 9.1 / 8.7.  256 (16 / 2): window 128 13.4 / 12.1, 18.0 / 12.4 for 64, 256 13.5 /
+// 14.4 for one, 14.7 / 14.5 for 16, 20.0 / 15.3 for 64, 27.7 / 17.0 for 128.  The
+// limits are those of a single sequence: with many, one launch stays ahead further
+// (the last figures), which the rule does not ask for yet.
 bool window_direct_pays(const DecodeParams& p, int pd) {
   static_assert(kDirectWaves * 512 >= 8 * 256, "q rows of a workgroup");
   const int64_t seen = (int64_t)p.window + p.sink;
@@ -2569,12 +2573,12 @@ bool window_direct_pays(const DecodeParams& p, int pd) {
 // what a step of 32 tokens costs a unit, so a unit takes at least sqrt(steps / 16)
 // steps; a second workgroup on a CU does not pay (of one wave, four do), nor do pairs
 // (16 ragged sequences, window 1000: 16.8 us with 192 units, 15.9 with 256 to 448,
-// 19.8 with 512); beyond a few steps a unit the full, paired plan is ahead.  us, full / this: 32 q / 8 kv heads,
-// head size 128, window 1024: 14.9 / 12.6 for one sequence, 18.8 / 14.5 for 8, 18.9 /
-// 16.6 for 16, 23.9 / 21.0 for 32 (64: 30.4 / 31.1, full taken); 4096: 25.4 / 16.5 for
-// one, 24.0 / 20.6 for 8; 16384: 33.9 / 23.0 for one, 31.0 / 28.9 for 4.  Head size 64
-// (16 / 4): 1024 13.4 / 11.9 for 16, 4096 12.7 / 11.6 for one and 15.5 / 14.2 for 8;
-// 256 (16 / 2): 1024 22.2 / 19.0 for 16, 4096 26.0 / 21.5 for one.
+// 19.8 with 512); beyond a few steps a unit the full, paired plan is ahead.  us, full /
+// this: 32 q / 8 kv heads, head size 128, window 1024: 12.4 / 11.2 for one sequence,
+// 18.1 / 13.6 for 8, 19.2 / 16.4 for 16, 24.6 / 21.0 for 32 (64: 30.4, full taken);
+// 4096: 16.9 / 13.6 for one, 23.6 / 19.9 for 8; 16384: 23.5 / 19.6 for one, 28.8 / 27.3
+// for 4.  Head size 64 (16 / 4): 1024 12.8 / 11.3 for 16, 4096 10.2 / 10.3 for one and
+// 14.1 / 13.4 for 8; 256 (16 / 2): 1024 22.2 / 18.8 for 16, 4096 17.8 / 17.2 for one.
 void window_plan(const DecodeParams& p, int pd, int max_rows, int cus, BalancedGrid& g) {
   const int64_t steps =
       ((int64_t)p.window + p.sink + 2 * kTile - 2 + kPlanAlign - 1) / kPlanAlign;  // of a sequence

@@ -1170,7 +1170,8 @@ def prefill_attention_window(q: torch.Tensor, o: torch.Tensor, requests, num_kv_
     request's keys sees the keys j with P - window < j <= P, and j < sink.  The
     keys may be closed up as prefill_gather_window leaves them.  What K and V
     hold for a key that a query does not see (NaN too) does not reach it.
-    sm_scale > 0.  tq_prefill_attention_window."""
+    sm_scale > 0; bf16 queries enter as fp16 (beyond 65504 they are infinite).
+    tq_prefill_attention_window."""
     if (_nat or _native()).prefill_window(q, o, requests, num_kv_heads, head_dim, padded_dim,
                                           sm_scale, window, sink, k, v, k2, v2):
         return o
@@ -1227,8 +1228,9 @@ def norm_rope_write(qkv: torch.Tensor, q_weight: torch.Tensor | None,
     rotated / 2] turn dims (i, i + rotated / 2) by the row of the token's position:
     positions int32 or int64 [tokens], or [axes, tokens] with `sections`, the
     number of pairs that follow each axis, in order.  A position outside the
-    tables gives NaN rows.  rotated must be a multiple of 16, head_dim of 8.
-    tq_norm_rope_write."""
+    tables gives NaN rows.  rotated must be a multiple of 16, head_dim of 8.  What
+    is not contiguous and 16-byte aligned is copied first, whole, on every call:
+    tables kept as halves of one tensor are better split once.  tq_norm_rope_write."""
     if (_nat or _native()).norm_rope_write(qkv, q_weight, k_weight, cos, sin, positions, kv_cache,
                                            signs, slot_mapping, num_qo_heads, head_dim, padded_dim,
                                            q, k, eps, sections):
